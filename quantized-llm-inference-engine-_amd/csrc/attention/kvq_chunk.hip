@@ -1,0 +1,69 @@
+// Attention of a chunk of query tokens per sequence over the 8-bit KV cache: the tile kernel of tile_attention.hpp
+// over codes that it dequantizes exactly to bf16. fp16 queries: query and probabilities in two bf16 pieces each.
+#include "tile_attention.hpp"
+
+namespace llmopt {
+namespace {
+
+using namespace tile;
+
+template <int FMT, bool QF16, int HD>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QF16 ? 1 : 2, QF16 ? 1 : 2)))
+    kvq_chunk_kernel(const KvqAttnArgs a) {
+  constexpr int kRows = 128;
+  __shared__ __align__(16) uint8_t lds[4 * kKeys * HD * 2];
+  // Workgroups in the order (KV head, row block, sequence), a sequence's last blocks (the longest walks) first.
+  const uint32_t kv_heads = uint32_t(a.c.kv_heads);
+  const int rows = a.group * int(a.q_len);
+  const uint32_t blocks = uint32_t((rows + kRows - 1) / kRows);
+  const uint32_t rest = blockIdx.x / kv_heads;
+  const uint32_t kvh = blockIdx.x - rest * kv_heads;
+  const int64_t s = rest / blocks;
+  const int row0 = int(blocks - 1 - rest % blocks) * kRows;
+  Work w{};
+  const int64_t h0 = int64_t(kvh) * a.group;
+  w.query = static_cast<const uint16_t*>(a.query) + s * a.q_seq_stride + h0 * a.q_head_stride;
+  w.q_tok_stride = a.q_tok_stride;
+  w.q_head_stride = a.q_head_stride;
+  w.out = static_cast<uint16_t*>(a.out) + s * a.o_seq_stride + h0 * a.o_head_stride;
+  w.o_tok_stride = a.o_tok_stride;
+  w.o_head_stride = a.o_head_stride;
+  w.group = a.group;
+  w.rows = rows;
+  w.row0 = row0;
+  w.base = a.context_lens[s] - int(a.q_len);
+  const int last = int(uint32_t(min(row0 + kRows, rows) - 1) / uint32_t(a.group));
+  w.t_end = max(0, min(w.base + last + 1, int(a.c.ldb * a.c.block_size)));
+  w.scale = a.scale;
+  w.softcap = a.softcap;
+  for (int k = 0; k < 2; ++k) w.codes[k] = a.c.codes[k], w.scales[k] = a.c.scales[k];
+  w.table = a.c.block_ids + s * a.c.ldb;
+  w.kv_heads = kv_heads;
+  w.kvh = kvh;
+  w.block_size = uint32_t(a.c.block_size);
+  w.ldb = uint32_t(a.c.ldb);
+  w.num_blocks = uint32_t(a.c.num_blocks);
+  attend<kSrcCodes, FMT, false, QF16, HD, QF16 ? 2 : 1, QF16 ? 2 : 1, 1>(w, lds);
+}
+
+template <int FMT, bool QF16>
+hipError_t launch_hd(const KvqAttnArgs& a, hipStream_t stream) {
+  const int64_t blocks = (a.group * a.q_len + 127) / 128;
+  const int64_t grid = blocks * a.c.kv_heads * a.num_seqs;
+  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (a.c.head_dim == 128)
+    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 128>), dim3(unsigned(grid)), dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 64>), dim3(unsigned(grid)), dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_kvq_chunk(const KvqAttnArgs& a, int fmt, int q_dtype, hipStream_t stream) {
+  if (a.num_seqs == 0 || a.q_len == 0) return hipSuccess;
+  if (q_dtype == kDtF16) return fmt == kFmtInt8 ? launch_hd<kFmtInt8, true>(a, stream) : launch_hd<kFmtE4m3, true>(a, stream);
+  return fmt == kFmtInt8 ? launch_hd<kFmtInt8, false>(a, stream) : launch_hd<kFmtE4m3, false>(a, stream);
+}
+
+}  // namespace llmopt

@@ -1,0 +1,84 @@
+// Causal attention over packed prompts (PackedAttention.forward): sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1]
+// - 1 of query [total, heads, d] and key / value [total, kv_heads, d]; a token sees its sequence's tokens up to itself.
+// The tile kernel of tile_attention.hpp over 16-bit rows.
+#include "tile_attention.hpp"
+
+namespace llmopt {
+namespace {
+
+using namespace tile;
+
+template <bool F16, int HD, int RB>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(RB == 1 ? 2 : 1, RB == 1 ? 2 : 1)))
+    packed_attention_kernel(const PackedAttnArgs a) {
+  constexpr int kRows = 128 * RB;
+  __shared__ __align__(16) uint8_t lds[4 * kKeys * HD * 2];
+  const uint32_t kv_heads = uint32_t(a.kv_heads);
+  const uint32_t unit = blockIdx.x / kv_heads, kvh = blockIdx.x - unit * kv_heads;
+  auto cu = [&](int64_t i) -> int64_t {
+    const int64_t v = a.cu_seqlens[i];
+    return v < 0 ? 0 : v > a.total_tokens ? a.total_tokens : v;
+  };
+  if (unit >= a.blocks) {
+    // Rows in front of the first sequence (there are none in a proper call) and behind the last one: zeros.
+    const int64_t lo = a.num_seqs > 0 ? cu(0) : a.total_tokens, hi = a.num_seqs > 0 ? cu(a.num_seqs) : a.total_tokens;
+    const int64_t per_row = a.group * (HD / 8);
+    for (int64_t i = (unit - a.blocks) * kThreads + threadIdx.x; i < (lo + a.total_tokens - hi) * per_row;
+         i += a.tail_blocks * kThreads) {
+      const int64_t r = i / per_row, x = i - r * per_row;
+      const int64_t tok = r < lo ? r : hi + r - lo;
+      uint16_t* dst = static_cast<uint16_t*>(a.out) + tok * a.o_tok_stride + (kvh * int64_t(a.group) + x / (HD / 8)) * a.o_head_stride;
+      *reinterpret_cast<u32x4*>(dst + 8 * (x % (HD / 8))) = u32x4{0u, 0u, 0u, 0u};
+    }
+    return;
+  }
+  // Sequence i's row blocks start at floor(cu[i] group / kRows) + i: room for the ceil(len group / kRows) it has.
+  auto start = [&](int64_t i) -> int64_t { return cu(i) * a.group / kRows + i; };
+  const int64_t s = last_at_most(a.num_seqs, int64_t(unit), start);
+  const int64_t first = cu(s), len = cu(s + 1) - first;
+  const int64_t block = int64_t(unit) - start(s), count = (len * a.group + kRows - 1) / kRows;
+  if (block < 0 || block >= count) return;
+  Work w{};
+  const int64_t h0 = int64_t(kvh) * a.group;
+  w.query = static_cast<const uint16_t*>(a.query) + first * a.q_tok_stride + h0 * a.q_head_stride;
+  w.q_tok_stride = a.q_tok_stride;
+  w.q_head_stride = a.q_head_stride;
+  w.out = static_cast<uint16_t*>(a.out) + first * a.o_tok_stride + h0 * a.o_head_stride;
+  w.o_tok_stride = a.o_tok_stride;
+  w.o_head_stride = a.o_head_stride;
+  w.group = a.group;
+  w.rows = int(len * a.group);
+  w.row0 = int(count - 1 - block) * kRows;  // the longest walks first
+  w.base = 0;
+  w.t_end = int(uint32_t(min(w.row0 + kRows, w.rows) - 1) / uint32_t(a.group)) + 1;
+  w.scale = a.scale;
+  w.softcap = a.softcap;
+  w.key = static_cast<const uint16_t*>(a.key) + first * a.k_tok_stride + int64_t(kvh) * a.k_head_stride;
+  w.value = static_cast<const uint16_t*>(a.value) + first * a.v_tok_stride + int64_t(kvh) * a.v_head_stride;
+  w.k_tok_stride = a.k_tok_stride;
+  w.v_tok_stride = a.v_tok_stride;
+  w.len = int(len);
+  attend<kSrcPacked, 0, F16, F16, HD, 1, 1, RB>(w, lds);
+}
+
+template <bool F16, int HD, int RB>
+hipError_t launch(PackedAttnArgs a, hipStream_t stream) {
+  constexpr int kRows = 128 * RB;
+  a.blocks = a.num_seqs > 0 ? a.total_tokens * a.group / kRows + a.num_seqs : 0;
+  a.tail_blocks = a.zero_tail ? 32 : 0;
+  const int64_t grid = (a.blocks + a.tail_blocks) * a.kv_heads;
+  if (grid <= 0) return hipSuccess;
+  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((packed_attention_kernel<F16, HD, RB>), dim3(unsigned(grid)), dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_packed_attention(const PackedAttnArgs& a, int dtype, int64_t head_dim, hipStream_t stream) {
+  if (a.total_tokens == 0) return hipSuccess;
+  if (dtype == kDtBf16) return head_dim == 128 ? launch<false, 128, 1>(a, stream) : launch<false, 64, 1>(a, stream);
+  return head_dim == 128 ? launch<true, 128, 1>(a, stream) : launch<true, 64, 1>(a, stream);
+}
+
+}  // namespace llmopt

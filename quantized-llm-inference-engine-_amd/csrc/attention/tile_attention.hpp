@@ -1,0 +1,505 @@
+// Causal attention of many query rows, for packed prompts (16-bit keys and values, rows of a tensor) and for chunks
+// over the 8-bit cache (codes by block table). One kernel, two sources of key tiles.
+//
+// A workgroup of four waves owns kRows = 128 RB query rows of one (sequence, KV head): the sequence's rows are its
+// tokens x the `group` query heads that share the KV head, token-major, 32 RB rows per wave. It walks the keys in
+// tiles of 64, held as 16-bit rows in a double buffer in LDS that all rows read:
+//   * packed: by direct loads, one tile ahead;
+//   * codes: loaded into registers one tile ahead, dequantized exactly to bf16 (code x power of two) behind the
+//     tile's products, and stored.
+// Per tile and wave, on v_mfma_f32_32x32x16:
+//   * S^T = K Q^T (A: 32 keys x 16 dims from LDS, B: 16 dims x 32 rows, in registers): lane l holds row l % 32
+//     against 16 keys of each block of 32 -- keys 8 q + 4 (l / 32) + r --, so a row's softmax takes one exchange
+//     between the lane halves;
+//   * online softmax in fp32, in powers of two;
+//   * O^T += V^T P^T with the probabilities as they lie (slot 4 a + r of lane half h is key 8 a + 4 h + r), V^T by
+//     transposing LDS reads of the row-major V tile.
+// A key that is masked for some rows of a tile only has probability 0 for them, but 0 x infinity would still reach
+// their output: a wave whose rows come out with anything that is not finite computes those rows once more, key by
+// key (never for finite inputs).
+#pragma once
+
+#include "attn_common.hpp"
+
+namespace llmopt {
+namespace tile {
+
+enum : int { kSrcPacked = 0, kSrcCodes = 1 };
+
+constexpr int kThreads = 256;
+constexpr int kKeys = 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <bool F16>
+struct Op {
+  __device__ static f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (F16)
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  __device__ static uint32_t pack(float lo, float hi) {
+    if constexpr (F16)
+      return uint32_t(__builtin_bit_cast(uint16_t, _Float16(lo))) | (uint32_t(__builtin_bit_cast(uint16_t, _Float16(hi))) << 16);
+    else
+      return pack_bf16(lo, hi);
+  }
+  __device__ static float add_pair(uint32_t pair, float sum) {  // sum + both halves, in fp32
+    if constexpr (F16)
+      return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, pair), __builtin_bit_cast(f16x2_t, 0x3C003C00u), sum, false);
+    else
+      return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), __builtin_bit_cast(bf16x2_t, 0x3F803F80u), sum, false);
+  }
+};
+
+// Four 16-bit elements of one column of four rows: of 16 lanes, lane 4 r + c reads dims 4 c .. of row r and lane i
+// receives dim i of rows 0 .. 3.
+__device__ __forceinline__ u32x2 read_transposed(const uint8_t* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+
+__device__ __forceinline__ float other_half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float other_half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Place of 16-byte chunk c within row r of a K or V tile: 16 rows of one K chunk, and the four rows of a transposing
+// read of V, fall on distinct banks.
+template <int HD>
+__device__ __forceinline__ int k_chunk(int r, int c) {
+  return HD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
+}
+template <int HD>
+__device__ __forceinline__ int v_chunk(int r, int c) {
+  return HD == 128 ? c ^ ((r & 3) << 2) : c ^ ((r & 2) << 1);
+}
+
+// What a workgroup works on, the same for both sources.
+struct Work {
+  const void* query;  // its sequence's token 0, its KV head's first query head
+  int64_t q_tok_stride, q_head_stride;
+  void* out;          // likewise
+  int64_t o_tok_stride, o_head_stride;
+  int group;
+  int rows;   // query rows of the (sequence, KV head)
+  int row0;   // the workgroup's first
+  int base;   // position of query token 0
+  int t_end;  // its keys: t < t_end
+  float scale, softcap;
+  // packed: key and value rows of the sequence's token 0
+  const uint16_t* key;
+  const uint16_t* value;
+  int64_t k_tok_stride, v_tok_stride;
+  int len;
+  // codes
+  const uint8_t* codes[2];
+  const float* scales[2];
+  const int32_t* table;
+  uint32_t kv_heads, kvh, block_size, ldb, num_blocks;
+};
+
+// KQ, KP: 16-bit pieces of the query and of a probability. F16: fp16 operands (packed fp16), else bf16.
+// QF16: the query's and output's type is fp16 (else bf16).
+template <int SRC, int FMT, bool F16, bool QF16, int HD, int KQ, int KP, int RB>
+__device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
+  constexpr int kCh = HD / 8;               // 16-byte chunks per 16-bit row
+  constexpr int kRowBytes = HD * 2;
+  constexpr int kTile = kKeys * kRowBytes;  // one K (or V) tile
+  constexpr int kRpl = 64 / kCh;            // 16-bit rows per wave load (1 KB)
+  constexpr int kLoads = 16 / kRpl;         // packed: wave loads per tile, of K and of V: 16 rows
+  constexpr int kCpr = HD / 16;             // codes: 16-byte loads per row
+  constexpr int kCrl = 64 / kCpr;           // codes: rows per wave load
+  constexpr int kCLoads = 16 / kCrl > 0 ? 16 / kCrl : 1;
+  constexpr int kS = HD / 16;               // 16-dim slices of the scores
+  constexpr int kD = HD / 32;               // 32-dim blocks of the output
+  constexpr int kWaveRows = 32 * RB;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const uint32_t group = uint32_t(a.group);
+  const int wrow = a.row0 + kWaveRows * wave;  // the wave's first row
+  auto tok_of = [&](int row) -> int { return int(uint32_t(row) / group); };
+  int q_pos[RB], tok[RB], head[RB];
+  bool row_ok[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int row = wrow + 32 * b + col;
+    row_ok[b] = row < a.rows;
+    tok[b] = tok_of(row_ok[b] ? row : a.rows - 1);
+    head[b] = (row_ok[b] ? row : a.rows - 1) - tok[b] * a.group;
+    q_pos[b] = row_ok[b] ? a.base + tok[b] : -1;
+  }
+  const int first_pos = a.base + tok_of(wrow);
+  const int wave_last = wrow < a.rows ? a.base + tok_of(min(wrow + kWaveRows, a.rows) - 1) : -1;
+  const int n_tiles = (a.t_end + kKeys - 1) / kKeys;
+
+  // ---- the wave's query rows: the B operand, dims 16 m + 8 half .. of row col ----
+  u32x4 qf[RB][KQ][kS];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const uint16_t* q = static_cast<const uint16_t*>(a.query) + tok[b] * a.q_tok_stride + head[b] * a.q_head_stride + 8 * half;
+#pragma unroll
+    for (int m = 0; m < kS; ++m) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(q + 16 * m);
+      if constexpr (KQ == 1) {
+        qf[b][0][m] = w;
+      } else {  // fp16 = two bf16 pieces, exactly (8 + 3 significant bits)
+        u32x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = f16_to_f32(uint16_t(w[e])), y = f16_to_f32(uint16_t(w[e] >> 16));
+          hi[e] = pack_bf16(x, y);
+          lo[e] = pack_bf16(x - __uint_as_float(hi[e] << 16), y - __uint_as_float(hi[e] & 0xFFFF0000u));
+        }
+        qf[b][0][m] = hi;
+        qf[b][1][m] = lo;
+      }
+    }
+  }
+
+  const float neg_inf = -__int_as_float(0x7F800000);
+  // Probabilities are 2^(score c - m c), one fma and one exponential per score. c has to be positive for the maximum
+  // of the scores to be that of the exponents: a negative scale moves into the query rows, a zero one becomes too
+  // small to matter.
+  const bool capped = a.softcap > 0.0f;
+  const float magnitude = __builtin_fabsf(a.scale) * kLog2e;
+  const float c2 = capped ? kLog2e : magnitude > 0.0f ? magnitude : 1e-30f;
+  const uint32_t q_sign = !capped && a.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int p = 0; p < KQ; ++p)
+#pragma unroll
+      for (int m = 0; m < kS; ++m) qf[b][p][m] ^= q_sign;
+  float m_run[RB], mc[RB], l_run[RB];  // per row: running maximum, m_run c2 (0 without keys), this lane's share of the sum
+  f32x16 o[RB][kD];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    m_run[b] = neg_inf, mc[b] = 0.0f, l_run[b] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kD; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[b][d][v] = 0.0f;
+  }
+
+  // ---- key tiles ----
+  uint8_t* const buf[2] = {lds, lds + 2 * kTile};
+  // Packed: rows past the sequence repeat its last one; no row sees them.
+  auto fetch_packed = [&](int t0, int b) {
+    const int last = min(kKeys, a.len - t0) - 1;
+    const auto krs = make_rsrc(a.key + t0 * a.k_tok_stride, uint32_t(last * a.k_tok_stride * 2 + kRowBytes));
+    const auto vrs = make_rsrc(a.value + t0 * a.v_tok_stride, uint32_t(last * a.v_tok_stride * 2 + kRowBytes));
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = wave * 16 + kRpl * i + lane / kCh;
+      const uint32_t row = uint32_t(min(r, last));
+      uint8_t* dst = buf[b] + (wave * 16 + kRpl * i) * kRowBytes;
+      load_lds16_cached(krs, dst, row * uint32_t(a.k_tok_stride * 2) + 16 * k_chunk<HD>(r, lane % kCh), 0);
+      load_lds16_cached(vrs, dst + kTile, row * uint32_t(a.v_tok_stride * 2) + 16 * v_chunk<HD>(r, lane % kCh), 0);
+    }
+  };
+  // Codes: lane l looks up key t0 + l, the entry a tile ahead of its use.
+  auto fetch_entry = [&](int t0) -> int32_t {
+    const uint32_t t = uint32_t(t0 + lane);
+    const uint32_t bi = t / a.block_size;
+    return int(t) < a.t_end && bi < a.ldb ? a.table[bi] : -1;
+  };
+  u32x4 held[2][kCLoads];
+  float held_scale[2][kCLoads];
+  uint64_t held_mask = 0;
+  auto fetch_codes = [&](int t0, int32_t entry) {
+    const uint32_t t = uint32_t(t0 + lane);
+    const bool ok = entry >= 0 && uint32_t(entry) < a.num_blocks;
+    held_mask = __builtin_amdgcn_ballot_w64(ok);
+    const uint32_t block = ok ? uint32_t(entry) * a.kv_heads + a.kvh : a.kvh;  // no key: some row of the cache
+    const uint32_t slot = ok ? t % a.block_size : 0u;
+#pragma unroll
+    for (int i = 0; i < kCLoads; ++i) {
+      const int r = wave * 16 + kCrl * i + lane / kCpr;
+      const int64_t bl = uint32_t(__shfl(int(block), r & 63, 64));
+      const int64_t row = bl * a.block_size + __shfl(int(slot), r & 63, 64);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        held[k][i] = *reinterpret_cast<const u32x4*>(a.codes[k] + row * HD + 16 * (lane % kCpr));
+        held_scale[k][i] = a.scales[k][bl];
+      }
+    }
+  };
+  auto store_codes = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < kCLoads; ++i) {
+      const int r = wave * 16 + kCrl * i + lane / kCpr, c = 2 * (lane % kCpr);
+      const bool ok = (held_mask >> (r & 63)) & 1u;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        u32x4 codes = held[k][i];
+        asm("" : "+v"(codes));  // whole words until here
+        const float s = held_scale[k][i];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          u32x4 w;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t x = codes[2 * j + e];
+            w[2 * e] = pack_bf16(code_to_f32<FMT>(x, 0) * s, code_to_f32<FMT>(x, 1) * s);
+            w[2 * e + 1] = pack_bf16(code_to_f32<FMT>(x, 2) * s, code_to_f32<FMT>(x, 3) * s);
+          }
+          if (!ok) w = u32x4{0u, 0u, 0u, 0u};  // its scores are masked; its value must not be anything but finite
+          const int at = k == 0 ? k_chunk<HD>(r, c + j) : v_chunk<HD>(r, c + j);
+          *reinterpret_cast<u32x4*>(buf[b] + k * kTile + r * kRowBytes + 16 * at) = w;
+        }
+      }
+    }
+  };
+
+  // Per-lane LDS addresses of V: key 4 half + (lane % 16) / 4, dims 16 ((lane / 16) % 2) + 4 (lane % 4) of a block.
+  const int vkey = 4 * half + ((lane & 15) >> 2);
+  const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const int v_off = vkey * kRowBytes + 8 * (lane & 1);
+
+  auto compute = [&](const uint8_t* kt, int t0, uint64_t mask) {
+    const uint8_t* vt = kt + kTile;
+    f32x16 sc[RB][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sc[b][kb][v] = 0.0f;
+#pragma unroll
+      for (int m = 0; m < kS; ++m) {
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + (32 * kb + col) * kRowBytes + 16 * k_chunk<HD>(col, 2 * m + half));
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int p = 0; p < KQ; ++p) sc[b][kb] = Op<F16>::mfma(kf, qf[b][p][m], sc[b][kb]);
+      }
+    }
+    u32x4 pf[RB][KP][4];
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      if (capped) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sc[b][kb][v] = tanhf(sc[b][kb][v] * a.scale / a.softcap) * a.softcap;
+      }
+      if (mask != ~uint64_t(0) || t0 + kKeys - 1 > first_pos) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          // Bit 8 q + r: key 8 q + 4 half + r of the block is a key at or before this row's token.
+          const int room = q_pos[b] - t0 - 32 * kb - 4 * half;
+          const uint32_t bits = (uint32_t(mask >> (32 * kb)) >> (4 * half)) & (room >= 31 ? ~0u : room < 0 ? 0u : (2u << room) - 1u);
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const uint32_t keep = uint32_t(int32_t(bits << (31 - (8 * (v / 4) + v % 4))) >> 31);
+            sc[b][kb][v] = __uint_as_float((__float_as_uint(sc[b][kb][v]) & keep) | (__float_as_uint(neg_inf) & ~keep));
+          }
+        }
+      }
+      float top = neg_inf;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) top = fmaxf(top, sc[b][kb][v]);
+      const float m_new = fmaxf(m_run[b], other_half_max(top));
+      if (__builtin_amdgcn_ballot_w64(m_new > m_run[b])) {
+        const float mc_new = m_new == neg_inf ? 0.0f : m_new * c2;
+        const float alpha = m_run[b] == neg_inf ? 0.0f : __builtin_amdgcn_exp2f(mc[b] - mc_new);
+        m_run[b] = m_new;
+        mc[b] = mc_new;
+        if (t0 > 0) {
+          l_run[b] *= alpha;
+#pragma unroll
+          for (int d = 0; d < kD; ++d)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[b][d][v] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float p[8];
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i / 2][8 * (i % 2) + v], c2, -mc[b]));
+        // The sum adds the probabilities as rounded (KP = 2: to 16 bits), so that a row's weights add up to one.
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t hi = Op<F16>::pack(p[2 * e], p[2 * e + 1]);
+          pf[b][0][i][e] = hi;
+          l_run[b] = Op<F16>::add_pair(hi, l_run[b]);
+          if constexpr (KP == 2) {
+            const uint32_t lo = Op<F16>::pack(p[2 * e] - __uint_as_float(hi << 16), p[2 * e + 1] - __uint_as_float(hi & 0xFFFF0000u));
+            pf[b][1][i][e] = lo;
+            l_run[b] = Op<F16>::add_pair(lo, l_run[b]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < kD; ++d) {
+        // Keys 16 i + vkey and 8 further: both have vkey's low bits, so one swizzle.
+        const uint8_t* p0 = vt + 16 * i * kRowBytes + v_off + 16 * v_chunk<HD>(vkey, 4 * d + vc);
+        const u32x2 lo = read_transposed(p0), hi = read_transposed(p0 + 8 * kRowBytes);
+        const u32x4 vf = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int p = 0; p < KP; ++p) o[b][d] = Op<F16>::mfma(vf, pf[b][p][i], o[b][d]);
+      }
+  };
+
+  if (n_tiles > 0) {
+    if constexpr (SRC == kSrcPacked) {
+      fetch_packed(0, 0);
+      for (int i = 0; i < n_tiles; ++i) {
+        const int t0 = i * kKeys;
+        wait_vmcnt<0>();    // this wave's rows of tile i
+        wait_lgkmcnt0();    // its reads of the buffer that is refilled next
+        __builtin_amdgcn_s_barrier();
+        if (i + 1 < n_tiles) fetch_packed(t0 + kKeys, (i + 1) & 1);
+        if (t0 <= wave_last) compute(buf[i & 1], t0, ~uint64_t(0));
+      }
+    } else {
+      int32_t entry = fetch_entry(0);
+      fetch_codes(0, entry);
+      entry = fetch_entry(kKeys);
+      uint64_t mask = held_mask;
+      store_codes(0);
+      for (int i = 0; i < n_tiles; ++i) {
+        const int t0 = i * kKeys;
+        wait_lgkmcnt0();    // its stores of tile i, and its reads of the buffer that is refilled next
+        __builtin_amdgcn_s_barrier();
+        const uint64_t now = mask;
+        if (i + 1 < n_tiles) {
+          const int32_t e = entry;
+          entry = fetch_entry(t0 + 2 * kKeys);
+          fetch_codes(t0 + kKeys, e);
+          mask = held_mask;
+        }
+        if (t0 <= wave_last) compute(buf[i & 1], t0, now);
+        if (i + 1 < n_tiles) store_codes((i + 1) & 1);
+      }
+    }
+  }
+
+  // ---- output: row col, dims 32 d + 8 q + 4 half + r, through LDS so that the stores are whole rows ----
+  wait_lgkmcnt0();
+  __builtin_amdgcn_s_barrier();  // every wave is past its last tile
+  uint8_t* const stage = lds + wave * 32 * kRowBytes;
+  auto narrow = [&](float lo, float hi) -> uint32_t {
+    if constexpr (QF16)
+      return uint32_t(f32_to_f16_rne(lo)) | (uint32_t(f32_to_f16_rne(hi)) << 16);
+    else
+      return pack_bf16(lo, hi);
+  };
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const float l = other_half_sum(l_run[b]);
+    // Zeros without keys; over the cache also for a sum that is no number (as the torch sequence's nan_to_num gives).
+    const bool none = SRC == kSrcPacked ? l == 0.0f : !(l > 0.0f);
+    const float inv = 1.0f / l;
+    bool odd = false;
+#pragma unroll
+    for (int d = 0; d < kD; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          v[r] = none ? 0.0f : o[b][d][4 * q + r] * inv;
+          odd |= !(__builtin_fabsf(v[r]) < __int_as_float(0x7F800000));
+        }
+        *reinterpret_cast<u32x2*>(stage + col * kRowBytes + 16 * k_chunk<HD>(col, 4 * d + q) + 8 * half) =
+            u32x2{narrow(v[0], v[1]), narrow(v[2], v[3])};
+      }
+    wait_lgkmcnt0();  // the wave's own rows: no barrier
+#pragma unroll
+    for (int i = 0; i < 32 / kRpl; ++i) {
+      const int r = kRpl * i + lane / kCh, c = lane % kCh;
+      const int row = wrow + 32 * b + r;
+      if (row >= a.rows) continue;
+      const int t = tok_of(row);
+      const u32x4 w = *reinterpret_cast<const u32x4*>(stage + r * kRowBytes + 16 * k_chunk<HD>(r, c));
+      uint16_t* dst = static_cast<uint16_t*>(a.out) + t * a.o_tok_stride + (row - t * a.group) * a.o_head_stride + 8 * c;
+      *reinterpret_cast<u32x4*>(dst) = w;
+    }
+    wait_lgkmcnt0();
+
+    // ---- rows with anything that is not finite: once more, key by key, masked keys left out ----
+    uint64_t bad64 = __builtin_amdgcn_ballot_w64(odd && row_ok[b]);
+    if (bad64) {
+      wait_vmcnt<0>();  // the stores above
+      uint32_t bad = uint32_t(bad64) | uint32_t(bad64 >> 32);
+      constexpr int kE = HD / 64;  // dims per lane
+      for (; bad; bad &= bad - 1) {
+        const int row = wrow + 32 * b + __builtin_ctz(bad);
+        const int t_row = tok_of(row), g = row - t_row * a.group;
+        const int pos = a.base + t_row;
+        const uint16_t* q = static_cast<const uint16_t*>(a.query) + t_row * a.q_tok_stride + g * a.q_head_stride;
+        auto element = [&](int k, int t, int d, bool& key) -> float {  // dim d of key (value) t
+          if constexpr (SRC == kSrcPacked) {
+            const uint16_t x = k == 0 ? a.key[t * a.k_tok_stride + d] : a.value[t * a.v_tok_stride + d];
+            return F16 ? f16_to_f32(x) : bf16_to_f32(x);
+          } else {
+            const uint32_t bi = uint32_t(t) / a.block_size;
+            const int32_t entry = bi < a.ldb ? a.table[bi] : -1;
+            key = key && entry >= 0 && uint32_t(entry) < a.num_blocks;
+            const int64_t bl = (key ? int64_t(entry) : 0) * a.kv_heads + a.kvh;
+            return code_to_f32<FMT>(a.codes[k][(bl * a.block_size + uint32_t(t) % a.block_size) * HD + d], 0) * a.scales[k][bl];
+          }
+        };
+        float m = neg_inf, sum = 0.0f, acc[kE] = {};
+        for (int t0 = 0; t0 <= pos && t0 < a.t_end; t0 += 64) {
+          const int t = t0 + lane;
+          bool key = t <= pos && t < a.t_end;
+          float dot = 0.0f;
+          for (int d = 0; d < HD; ++d) {
+            const float x = QF16 ? f16_to_f32(q[d]) : bf16_to_f32(q[d]);
+            dot = __builtin_fmaf(x, element(0, key ? t : 0, d, key), dot);
+          }
+          float sc = dot * a.scale;
+          if (capped) sc = tanhf(sc / a.softcap) * a.softcap;
+          sc = key ? sc * kLog2e : neg_inf;
+          float top = sc;
+#pragma unroll
+          for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+          const float m_new = fmaxf(m, top), ref = m_new == neg_inf ? 0.0f : m_new;
+          const float alpha = m == neg_inf ? 0.0f : __builtin_amdgcn_exp2f(m - ref);
+          m = m_new;
+          const float p = key ? __builtin_amdgcn_exp2f(sc - ref) : 0.0f;
+          sum *= alpha;
+#pragma unroll
+          for (int e = 0; e < kE; ++e) acc[e] *= alpha;
+          uint64_t keys = __builtin_amdgcn_ballot_w64(key);
+          for (; keys; keys &= keys - 1) {
+            const int from = __builtin_ctzll(keys);
+            const float pt = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), from));
+            sum += pt;
+            bool yes = true;
+#pragma unroll
+            for (int e = 0; e < kE; ++e) acc[e] = __builtin_fmaf(pt, element(1, t0 + from, kE * lane + e, yes), acc[e]);
+          }
+        }
+        const bool no = SRC == kSrcPacked ? sum == 0.0f : !(sum > 0.0f);
+        uint16_t* dst = static_cast<uint16_t*>(a.out) + t_row * a.o_tok_stride + g * a.o_head_stride + kE * lane;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+          const float v = no ? 0.0f : acc[e] / sum;
+          dst[e] = QF16 ? f32_to_f16_rne(v) : f32_to_bf16_rne(v);
+        }
+      }
+    }
+  }
+}
+
+}  // namespace tile
+}  // namespace llmopt

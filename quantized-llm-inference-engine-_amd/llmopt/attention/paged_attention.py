@@ -6,8 +6,9 @@ log-sum-exp when the context is long). Here, on a HIP device, :meth:`PagedAttent
 calls ``llmopt_paged_attention_decode`` for one query token per sequence (the decode step) and
 ``llmopt_paged_attention_prefill`` for more (a prefill chunk, with the causal mask): both read
 K/V from the cache blocks in place, once per KV head for all the query heads that share it, with
-an online softmax. Other calls (host tensors, shapes the kernels do not take) run the
-reference's sequence in torch.
+an online softmax. Over a :class:`llmopt.cache.QuantizedPagedKVCache` both kinds of call run
+``llmopt_kvq_attention``, which reads its 8-bit codes in place. Other calls (host tensors, shapes the
+kernels do not take) run the reference's sequence in torch.
 """
 
 from __future__ import annotations
@@ -16,6 +17,7 @@ from dataclasses import dataclass
 
 import torch
 
+from llmopt.cache.quantized_cache import QuantizedPagedKVCache
 from llmopt.utils.logging import get_logger
 
 __all__ = ["AttentionBackend", "PagedAttention", "PagedAttentionConfig", "merge_states"]
@@ -116,7 +118,8 @@ class PagedAttention:
 
         ``block_ids`` is ``[seq, max_blocks]`` (``-1`` padded); ``context_lens`` is ``[seq]``, the
         context length after this step's K/V were written. Returns ``[seq, heads, q_len, head_dim]``
-        in the query's dtype. Query position ``i`` of a sequence sits at ``ctx - q_len + i`` and
+        in the query's dtype. ``cache`` is a :class:`PagedKVCache` or a :class:`QuantizedPagedKVCache`.
+        Query position ``i`` of a sequence sits at ``ctx - q_len + i`` and
         sees keys up to and including its own position.
         """
         seqs = int(query.shape[0])
@@ -127,6 +130,9 @@ class PagedAttention:
             from llmopt.kernels import ops
 
             try:
+                if isinstance(cache, QuantizedPagedKVCache):
+                    return ops.kvq_attention(query[:, :, :q_len], *cache.layer(layer_idx), block_ids, context_lens,
+                                             self.scale, self.config.softcap)
                 if q_len == 1:
                     out = ops.paged_decode_attention(
                         query[:, :, 0, :], cache.key_cache[layer_idx], cache.value_cache[layer_idx], block_ids,

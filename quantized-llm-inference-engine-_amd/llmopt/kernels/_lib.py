@@ -1,4 +1,4 @@
-"""ctypes binding of ``libllmopt_qlinear.so`` (C ABI in ``include/llmopt_qlinear.h``).
+"""ctypes binding of ``libllmopt_qlinear.so`` (C ABI in ``include/*.h``).
 
 The library is loaded after ``torch`` so that both share torch's HIP runtime (the
 library's own run path points at the same copy). A missing library raises: the HIP
@@ -25,6 +25,7 @@ __all__ = [
     "ALGO_DENSE",
     "DTYPE_CODES",
     "EXPORTED_SYMBOLS",
+    "KVQ_FORMATS",
     "binding_path",
     "call",
     "library_path",
@@ -33,6 +34,7 @@ __all__ = [
 ]
 
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+KVQ_FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}  # the 8-bit KV cache's codes
 
 ALGO_AUTO = 0
 ALGO_GENERIC = 1
@@ -48,7 +50,7 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _size = ctypes.c_size_t
 
-# name -> (restype, argtypes); mirrors include/llmopt_qlinear.h.
+# name -> (restype, argtypes); mirrors include/*.h.
 _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "llmopt_q_abi_version": (_int, []),
     "llmopt_q_last_error": (ctypes.c_char_p, []),
@@ -133,6 +135,23 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _int, _int, _int, _int, _int,
          _p, _size, _p, _int],
     ),
+    "llmopt_kvq_last_error": (ctypes.c_char_p, []),
+    "llmopt_kvq_write": (
+        _int,
+        [_p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64,
+         _i64, _int, _i64, _i64, _i64, _p],
+    ),
+    "llmopt_kvq_attention_workspace": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "llmopt_kvq_attention": (
+        _int,
+        [_p, _int, _i64, _i64, _i64, _p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64,
+         ctypes.c_float, ctypes.c_float, _p, _i64, _i64, _i64, _p, _size, _p],
+    ),
+    "llmopt_packed_attention": (
+        _int,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _int, _p, _i64, _i64, _i64, _i64, _i64, ctypes.c_float,
+         ctypes.c_float, _p, _i64, _i64, _int, _p],
+    ),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 ABI_VERSION = 1
@@ -216,7 +235,9 @@ def call(rc: int, what: str) -> None:
     """Raise the Python exception matching a negative status code."""
     if rc == 0:
         return
-    message = load_library().llmopt_q_last_error().decode(errors="replace")
+    lib = load_library()
+    kvq = what.startswith(("llmopt_kvq", "llmopt_packed"))  # include/llmopt_kvq.h keeps its own message
+    message = (lib.llmopt_kvq_last_error() if kvq else lib.llmopt_q_last_error()).decode(errors="replace")
     if rc == ERR_INVALID_ARG:
         raise ValueError(f"{what}: {message}")
     if rc == ERR_UNSUPPORTED:

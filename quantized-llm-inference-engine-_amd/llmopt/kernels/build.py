@@ -1,4 +1,4 @@
-"""Build ``libllmopt_qlinear.so`` from ``csrc/*.hip`` with hipcc for gfx950, and the torch binding of
+"""Build ``libllmopt_qlinear.so`` from ``csrc/*.hip`` and ``csrc/attention/*.hip`` with hipcc for gfx950, and the torch binding of
 the linears' host path, ``_llmopt_torch.so``, from ``csrc/torch_binding.cpp`` with g++.
 
 Usage: ``python -m llmopt.kernels.build`` (or :func:`build_library`). Objects go to
@@ -60,11 +60,11 @@ def _torch_lib_dir() -> str | None:
 
 
 def sources() -> list[Path]:
-    return sorted(CSRC.glob("*.hip"))
+    return sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("attention/*.hip"))
 
 
 def build_library(verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compile every ``csrc/*.hip`` and link the shared library. Always rebuilds."""
+    """Compile every ``csrc/*.hip`` and ``csrc/attention/*.hip`` and link the shared library. Always rebuilds."""
     hipcc = _hipcc()
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
     srcs = sources()

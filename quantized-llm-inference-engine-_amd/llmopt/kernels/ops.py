@@ -11,7 +11,10 @@ These are the only entry points the quantization layer uses on HIP devices:
 * :func:`kv_write_decode` / :func:`kv_write` replace ``PagedKVCache.write_decode`` / ``write``
   (``src/llmopt/cache/paged_cache.py:187-277``),
 * :func:`paged_decode_attention` replaces ``PagedAttention.forward`` for one query token per
-  sequence (``src/llmopt/attention/paged_attention.py:145-290``), reading the cache in place.
+  sequence (``src/llmopt/attention/paged_attention.py:145-290``), reading the cache in place,
+* :func:`kvq_write` and :func:`kvq_attention` are those steps over the 8-bit cache
+  (:class:`llmopt.cache.QuantizedPagedKVCache`), and :func:`packed_attention` is causal attention
+  over packed prompts.
 
 Each wrapper checks what torch would check (dtypes, devices, shapes), passes raw
 device pointers and the current HIP stream to the library, and raises if the
@@ -20,17 +23,21 @@ library is missing or reports an error. Nothing here computes on the host.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
 
-from llmopt.kernels._lib import ALGO_AUTO, ALGO_DENSE, DTYPE_CODES, call, load_binding, load_library
+from llmopt.kernels._lib import ALGO_AUTO, ALGO_DENSE, DTYPE_CODES, KVQ_FORMATS, call, load_binding, load_library
 
 __all__ = [
     "dequantize",
     "kv_write",
     "kv_write_decode",
+    "kvq_attention",
+    "kvq_write",
     "module_linear",
+    "packed_attention",
     "paged_decode_attention",
     "quant_linear",
     "quant_linear_swiglu",
@@ -644,6 +651,179 @@ def paged_decode_attention_rope(
         "llmopt_paged_attention_decode_rope",
     )
     return out
+
+
+# ---- the 8-bit KV cache and packed prompts -----------------------------------------------------
+
+
+def _launching_on(device: torch.device):  # noqa: ANN202 - a context manager
+    """Kernels are launched on the tensors' device, whichever is current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _kvq_cache(key_codes, key_scales, value_codes, value_scales) -> tuple[int, int, int, int, int]:  # noqa: ANN001
+    """(num_blocks, block_size, kv_heads, head_dim, format) of one layer's 8-bit cache: codes ``[num_blocks, kv_heads,
+    block_size, head_dim]``, scales fp32 ``[num_blocks, kv_heads]``."""
+    if key_codes.dim() != 4 or key_codes.shape != value_codes.shape:
+        raise ValueError(f"expected two [blocks, kv_heads, block_size, head_dim] code tensors, got "
+                         f"{tuple(key_codes.shape)} and {tuple(value_codes.shape)}")
+    if key_codes.dtype != value_codes.dtype or key_codes.dtype not in KVQ_FORMATS:
+        raise TypeError(f"cache codes must be int8 or float8_e4m3fn, got {key_codes.dtype}, {value_codes.dtype}")
+    if key_scales.shape != key_codes.shape[:2] or value_scales.shape != key_codes.shape[:2]:
+        raise ValueError(f"expected scales of shape {tuple(key_codes.shape[:2])}, got {tuple(key_scales.shape)} and "
+                         f"{tuple(value_scales.shape)}")
+    if key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32:
+        raise TypeError(f"cache scales must be float32, got {key_scales.dtype}, {value_scales.dtype}")
+    if not (key_codes.is_contiguous() and value_codes.is_contiguous() and key_scales.is_contiguous()
+            and value_scales.is_contiguous()):
+        raise ValueError("the cache's codes and scales must be contiguous")
+    _same_device(key_codes, key_scales, value_codes, value_scales)
+    nb, kvh, bs, hd = (int(d) for d in key_codes.shape)
+    return nb, bs, kvh, hd, KVQ_FORMATS[key_codes.dtype]
+
+
+def kvq_write(key_codes, key_scales, value_codes, value_scales, block_ids, token_offsets, keys, values,  # noqa: ANN001
+              cu_seqlens: torch.Tensor | None = None, query_lens: torch.Tensor | None = None) -> None:
+    """Quantize new keys and values into one layer of an 8-bit cache (``llmopt_kvq_write``): ``keys``/``values``
+    ``[seq, q_len, kv_heads, head_dim]`` (of which sequence ``s`` keeps the first ``query_lens[s]``), or with
+    ``cu_seqlens [seq + 1]`` packed ``[tokens, kv_heads, head_dim]``; any strides with a unit inner one."""
+    nb, bs, kvh, hd, fmt = _kvq_cache(key_codes, key_scales, value_codes, value_scales)
+    packed = cu_seqlens is not None
+    if keys.dim() != (3 if packed else 4) or tuple(keys.shape[-2:]) != (kvh, hd) or keys.shape != values.shape:
+        raise ValueError(f"kvq_write: keys and values must be [{'tokens' if packed else 'seq, q_len'}, {kvh}, {hd}], got "
+                         f"{tuple(keys.shape)} and {tuple(values.shape)}")
+    if packed and (cu_seqlens.dim() != 1 or query_lens is not None or cu_seqlens.numel() < 1):
+        raise ValueError("kvq_write: cu_seqlens must be [seq + 1], without query_lens")
+    seqs = int(cu_seqlens.shape[0]) - 1 if packed else int(keys.shape[0])
+    if seqs == 0 or keys.numel() == 0:
+        return
+    if block_ids.dim() != 2:
+        raise ValueError("kvq_write: block_ids must be [seqs, blocks]")
+    _check_rows("kvq_write", seqs, block_ids=block_ids, token_offsets=token_offsets.reshape(-1))
+    if not (keys.is_floating_point() and values.is_floating_point()):
+        raise TypeError(f"kvq_write: keys and values must be floating-point, got {keys.dtype}, {values.dtype}")
+    dev = key_codes.device
+    _same_device(key_codes, keys, values)
+    if keys.dtype != values.dtype or keys.dtype not in DTYPE_CODES:
+        keys, values = keys.float(), values.float()
+    keys = keys if keys.stride(-1) == 1 else keys.contiguous()
+    values = values if values.stride(-1) == 1 else values.contiguous()
+    table, offsets = _int32(block_ids, dev), _int32(token_offsets.reshape(-1), dev)
+    cu = _int32(cu_seqlens, dev) if packed else None
+    lens = None
+    if query_lens is not None:
+        _check_rows("kvq_write", seqs, query_lens=query_lens.reshape(-1))
+        lens = _int32(query_lens.reshape(-1), dev)
+    ks, vs = ((0,) * packed + t.stride() for t in (keys, values))
+    with _launching_on(dev):
+        call(
+            load_library().llmopt_kvq_write(
+                key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(), value_scales.data_ptr(), fmt,
+                nb, bs, kvh, hd, table.data_ptr(), int(table.shape[1]), offsets.data_ptr(),
+                None if cu is None else cu.data_ptr(), None if lens is None else lens.data_ptr(), keys.data_ptr(),
+                ks[0], ks[1], ks[2], values.data_ptr(), vs[0], vs[1], vs[2], DTYPE_CODES[keys.dtype], seqs,
+                0 if packed else int(keys.shape[1]), int(keys.shape[0]) if packed else 0, _stream_handle(dev),
+            ),
+            "llmopt_kvq_write",
+        )
+
+
+def kvq_attention(query: torch.Tensor, key_codes: torch.Tensor, key_scales: torch.Tensor, value_codes: torch.Tensor,
+                  value_scales: torch.Tensor, block_ids: torch.Tensor, context_lens: torch.Tensor, scale: float,
+                  softcap: float = 0.0) -> torch.Tensor:
+    """Attention of ``query [seq, heads, q_len, head_dim]`` (fp32 / fp16 / bf16, any strides with a unit inner one) over
+    one layer of an 8-bit cache, read in place: query token j sits at ``context_lens - q_len + j`` and sees the keys up
+    to its own position. Returns ``[seq, heads, q_len, head_dim]`` in the query's dtype, a view of a ``[seq, q_len,
+    heads, head_dim]`` buffer. Raises ``NotImplementedError`` for head dims other than 64 and 128."""
+    nb, bs, kvh, hd, fmt = _kvq_cache(key_codes, key_scales, value_codes, value_scales)
+    if query.dim() != 4 or int(query.shape[3]) != hd:
+        raise ValueError(f"query of shape {tuple(query.shape)} does not match head_dim {hd}")
+    if query.dtype not in DTYPE_CODES:
+        raise TypeError(f"unsupported query dtype {query.dtype}")
+    seqs, heads, q_len = (int(d) for d in query.shape[:3])
+    dev = key_codes.device
+    _same_device(key_codes, query)
+    if block_ids.dim() != 2:
+        raise ValueError("kvq_attention: block_ids must be [seqs, blocks]")
+    _check_rows("kvq_attention", seqs, block_ids=block_ids, context_lens=context_lens.reshape(-1))
+    out = torch.empty(seqs, q_len, heads, hd, dtype=query.dtype, device=dev)
+    view = out.permute(0, 2, 1, 3)
+    if out.numel() == 0:
+        return view
+    dt = DTYPE_CODES[query.dtype]
+    q = query if query.stride(3) == 1 else query.contiguous()
+    if dt and q_len > 1 and (q.data_ptr() % 16 or any(st % 8 for st in q.stride()[:3])):
+        q = q.clone(memory_format=torch.contiguous_format)  # the chunk kernel reads whole 16-byte pieces
+    table, lens = _int32(block_ids, dev), _int32(context_lens.reshape(-1), dev)
+    ldb = int(table.shape[1])
+    lib = load_library()
+    with _launching_on(dev):
+        ws_bytes = lib.llmopt_kvq_attention_workspace(seqs, heads, kvh, hd, q_len, ldb, bs, dt)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        call(
+            lib.llmopt_kvq_attention(
+                q.data_ptr(), dt, q.stride(0), q.stride(1), q.stride(2), key_codes.data_ptr(), key_scales.data_ptr(),
+                value_codes.data_ptr(), value_scales.data_ptr(), fmt, nb, bs, kvh, hd, table.data_ptr(), ldb,
+                lens.data_ptr(), seqs, heads, q_len, float(scale), float(softcap), out.data_ptr(), q_len * heads * hd,
+                hd, heads * hd, None if ws is None else ws.data_ptr(), ws_bytes, _stream_handle(dev),
+            ),
+            "llmopt_kvq_attention",
+        )
+    return view
+
+
+def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tensor,
+                     scale: float, softcap: float = 0.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention over packed prompts: ``query [tokens, heads, head_dim]``, ``key``/``value`` ``[tokens, kv_heads,
+    head_dim]`` (fp16 or bf16, any token and head strides), sequence ``s`` the rows ``cu_seqlens[s]`` up to
+    ``cu_seqlens[s + 1]``. Rows behind the last sequence are zeros, in a given ``out`` left as they were. Raises
+    ``NotImplementedError`` for fp32 and for head dims other than 64 and 128."""
+    if query.dim() != 3 or key.dim() != 3 or key.shape != value.shape or query.shape[0] != key.shape[0] \
+            or query.shape[2] != key.shape[2]:
+        raise ValueError(f"packed_attention: query [tokens, heads, d], key and value [tokens, kv_heads, d] expected, got "
+                         f"{tuple(query.shape)}, {tuple(key.shape)}, {tuple(value.shape)}")
+    if not query.dtype == key.dtype == value.dtype or query.dtype not in DTYPE_CODES:
+        raise TypeError(f"packed_attention: unsupported dtypes {query.dtype}, {key.dtype}, {value.dtype}")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError("packed_attention: cu_seqlens must be [sequences + 1]")
+    tokens, heads, hd = (int(d) for d in query.shape)
+    kvh = int(key.shape[1])
+    dev = query.device
+    _same_device(query, key, value, out)
+    if kvh == 0 or heads % kvh:
+        raise ValueError(f"packed_attention: {heads} heads are not a multiple of {kvh} KV heads")
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype):
+        raise ValueError(f"packed_attention: out must be {tuple(query.shape)} {query.dtype}")
+    if query.dtype == torch.float32 or hd not in (64, 128):
+        raise NotImplementedError(f"packed_attention: {query.dtype}, head_dim {hd}")
+
+    def rows16(t: torch.Tensor) -> bool:
+        return (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
+                and 0 <= t.stride(0) <= 1 << 24)
+
+    query, key, value = (t if rows16(t) else t.clone(memory_format=torch.contiguous_format) for t in (query, key, value))
+    result = out
+    if out is None:
+        result = torch.empty(tokens, heads, hd, dtype=query.dtype, device=dev)
+    elif not rows16(out):
+        result = out.clone(memory_format=torch.contiguous_format)
+    if tokens:
+        cu = _int32(cu_seqlens, dev)
+        with _launching_on(dev):
+            call(
+                load_library().llmopt_packed_attention(
+                    query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(), key.stride(0), key.stride(1),
+                    value.data_ptr(), value.stride(0), value.stride(1), DTYPE_CODES[query.dtype], cu.data_ptr(),
+                    int(cu.shape[0]) - 1, tokens, heads, kvh, hd, float(scale), float(softcap), result.data_ptr(),
+                    result.stride(0), result.stride(1), int(out is None), _stream_handle(dev),
+                ),
+                "llmopt_packed_attention",
+            )
+    if out is not None and result is not out:
+        out.copy_(result)
+    return result if out is None else out
 
 
 def argmax_rows(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:

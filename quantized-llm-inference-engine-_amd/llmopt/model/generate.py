@@ -53,7 +53,8 @@ class GreedyGenerator:
     Args:
         model: a :class:`DecoderOnlyModel` (any device).
         block_size: cache block size in tokens.
-        cache_dtype: KV cache dtype (default: the embedding's dtype).
+        cache_dtype: KV cache dtype (default: the embedding's dtype); ``torch.int8`` or
+            ``torch.float8_e4m3fn`` for a :class:`llmopt.cache.QuantizedPagedKVCache`.
         use_graph: capture the decode step as a HIP graph (HIP devices only).
     """
 

@@ -91,10 +91,12 @@ class DecoderOnlyModel(nn.Module):
         return ModelOutput(logits=logits.view(seqs, 1 if last_only else q_len, -1))
 
     def allocate_cache(self, num_blocks: int, block_size: int, dtype: torch.dtype, device: torch.device | str) -> object:
-        """A :class:`PagedKVCache` for this model (``modeling.py:132-145``)."""
-        from llmopt.cache.paged_cache import PagedKVCache
+        """A :class:`PagedKVCache` for this model (``modeling.py:132-145``), for ``torch.int8`` and
+        ``torch.float8_e4m3fn`` a :class:`QuantizedPagedKVCache`."""
+        from llmopt.cache import PagedKVCache, QuantizedPagedKVCache
 
-        return PagedKVCache(self.config.num_hidden_layers, num_blocks, block_size, self.config.num_key_value_heads,
+        kind = QuantizedPagedKVCache if dtype in QuantizedPagedKVCache.FORMATS else PagedKVCache
+        return kind(self.config.num_hidden_layers, num_blocks, block_size, self.config.num_key_value_heads,
                             self.config.head_dim, dtype=dtype, device=device)
 
 
