@@ -130,6 +130,16 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
   }
 }
 
+// Bytes 2 HI and 2 HI + 1 of a word times their scale as a bf16 pair, exactly. The e4m3 conversion takes a power of
+// two with it (by its exponent alone: NaN gives NaN, and 0, whose codes are zeros, 2^-127).
+template <int FMT, bool HI>
+__device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float scale) {
+  if constexpr (FMT == kFmtE4m3)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+  else
+    return pack_bf16(float(int8_t(w >> (HI ? 16 : 0))) * scale, float(int8_t(w >> (HI ? 24 : 8))) * scale);
+}
+
 // Eight codes in order as one MFMA operand.
 template <int FMT, bool F16>
 __device__ __forceinline__ u32x4 code_operand(uint32_t lo, uint32_t hi) {
@@ -166,23 +176,36 @@ __device__ __forceinline__ float sum_across_rows(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Among `count` strictly increasing starts, the last i with start(i) <= x (start(0) <= x), by all 64 lanes of a
-// wave: each round asks 64 of them at even distances and keeps one gap.
+// The packed sequence that owns grid unit `unit`, found by all 64 lanes of a wave. Sequence i's units begin at
+// start(cu[i], i), strictly increasing; cu_seqlens is read within [0, total]. Each round asks 64 sequences at even distances
+// and keeps one gap; the last round's lanes hold what the caller needs next (the sequence's rows, and its entry of
+// `more`, if given), so that up to 64 sequences cost one round trip to memory.
+struct Packed {
+  int64_t s;           // the last sequence whose units begin at or before `unit` (0 if none does)
+  int32_t first, end;  // its rows
+  int32_t more;
+};
 template <class F>
-__device__ __forceinline__ int64_t last_at_most(int64_t count, int64_t x, F start) {
+__device__ __forceinline__ Packed find_packed(const int32_t* cu_seqlens, int64_t count, int64_t total, int64_t unit,
+                                              const int32_t* more, F start) {
   const int lane = threadIdx.x & 63;
+  auto clamped = [&](int32_t v) -> int32_t { return v < 0 ? 0 : v > total ? int32_t(total) : v; };
   int64_t lo = 0, n = count;  // the answer is in [lo, lo + n)
-  while (n > 1) {
+  for (;;) {
     const int64_t step = (n + 63) / 64;
-    const int64_t i = lo + lane * step;
-    const bool ok = lane * step < n && start(i) <= x;
-    const uint64_t votes = __builtin_amdgcn_ballot_w64(ok);
+    const bool in = lane * step < n;
+    const int64_t i = lo + (in ? lane * step : 0);
+    const int32_t first = clamped(cu_seqlens[i]), end = clamped(cu_seqlens[i + 1]);
+    const int32_t extra = more ? more[i] : 0;
+    const uint64_t votes = __builtin_amdgcn_ballot_w64(in && start(int64_t(first), i) <= unit);
     const int last = votes ? 63 - __builtin_clzll(votes) : 0;
     lo += last * step;
+    if (step == 1)
+      return Packed{lo, __builtin_amdgcn_readlane(first, last), __builtin_amdgcn_readlane(end, last),
+                    __builtin_amdgcn_readlane(extra, last)};
     const int64_t left = n - last * step;
     n = left < step ? left : step;
   }
-  return lo;
 }
 
 }  // namespace llmopt

@@ -80,6 +80,11 @@ Plan plan_decode(int64_t num_seqs, int64_t kv_heads, int64_t group, int64_t q_le
   return Plan{int((tiles + per - 1) / per), waves, per};
 }
 
+// A workgroup of the tile kernel reads its query rows (128 tokens, one KV head's query heads) at 32-bit offsets.
+bool near_rows(int64_t group, int64_t tok_stride, int64_t head_stride) {
+  return tok_stride >= 0 && tok_stride <= (int64_t(1) << 22) && head_stride >= 0 && head_stride <= (int64_t(1) << 29) / group;
+}
+
 // Whether the tile kernel takes the chunk: 16-bit queries, more than 32 rows per KV head.
 bool takes_tiles(int64_t group, int64_t q_len, int q_dtype) { return q_dtype != LLMOPT_DTYPE_F32 && group * q_len > 32; }
 
@@ -185,7 +190,8 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
     return aligned(p, 16) && (x * esize) % 16 == 0 && (y * esize) % 16 == 0 && (z * esize) % 16 == 0;
   };
   a.q_vec = rows16(query, q_seq_stride, q_head_stride, q_tok_stride);
-  if (takes_tiles(group, q_len, q_dtype) && a.q_vec && rows16(out, o_seq_stride, o_head_stride, o_tok_stride))
+  if (takes_tiles(group, q_len, q_dtype) && a.q_vec && near_rows(group, q_tok_stride, q_head_stride) &&
+      rows16(out, o_seq_stride, o_head_stride, o_tok_stride))
     return hip_status(llmopt::launch_kvq_chunk(a, format, q_dtype, static_cast<hipStream_t>(stream)),
                       "chunk attention launch");
   const Plan plan = plan_decode(num_seqs, kv_heads, group, q_len, ldb, block_size);
@@ -224,9 +230,11 @@ int llmopt_packed_attention(const void* query, int64_t q_tok_stride, int64_t q_h
   const int64_t group = num_heads / kv_heads;
   constexpr int64_t kStride = int64_t(1) << 24;  // a tile's 64 rows at 32-bit offsets
   if (total_tokens > kMaxInt / 4 / group || num_seqs > kMaxInt / 4 || k_tok_stride < 0 || k_tok_stride > kStride ||
-      v_tok_stride < 0 || v_tok_stride > kStride || ((total_tokens * group + 127) / 128 + num_seqs + 64) > kMaxInt / kv_heads)
-    return fail(LLMOPT_ERR_UNSUPPORTED, "packed attention: %lld tokens, %lld sequences, row strides %lld / %lld",
-                (long long)total_tokens, (long long)num_seqs, (long long)k_tok_stride, (long long)v_tok_stride);
+      v_tok_stride < 0 || v_tok_stride > kStride ||
+      !near_rows(group, q_tok_stride, q_head_stride) || ((total_tokens * group + 127) / 128 + num_seqs + 64) > kMaxInt / kv_heads)
+    return fail(LLMOPT_ERR_UNSUPPORTED, "packed attention: %lld tokens, %lld sequences, token strides %lld / %lld / %lld",
+                (long long)total_tokens, (long long)num_seqs, (long long)q_tok_stride, (long long)k_tok_stride,
+                (long long)v_tok_stride);
   const int64_t strides[] = {q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride,
                              v_head_stride, o_tok_stride, o_head_stride};
   bool rows16 = aligned(query, 16) && aligned(key, 16) && aligned(value, 16) && aligned(out, 16);

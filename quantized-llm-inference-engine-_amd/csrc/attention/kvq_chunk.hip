@@ -7,8 +7,10 @@ namespace {
 
 using namespace tile;
 
-template <int FMT, bool QF16, int HD>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(QF16 ? 1 : 2, QF16 ? 1 : 2)))
+constexpr int kThreads = 256;
+
+template <int FMT, bool QF16, int HD, bool CAP>
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 ? (QF16 ? 2 : 3) : QF16 ? 1 : 2, HD == 64 ? (QF16 ? 2 : 3) : QF16 ? 1 : 2)))
     kvq_chunk_kernel(const KvqAttnArgs a) {
   constexpr int kRows = 128;
   __shared__ __align__(16) uint8_t lds[4 * kKeys * HD * 2];
@@ -31,6 +33,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(Q
   w.group = a.group;
   w.rows = rows;
   w.row0 = row0;
+  w.row0_tok = int(uint32_t(row0) / uint32_t(a.group));
   w.base = a.context_lens[s] - int(a.q_len);
   const int last = int(uint32_t(min(row0 + kRows, rows) - 1) / uint32_t(a.group));
   w.t_end = max(0, min(w.base + last + 1, int(a.c.ldb * a.c.block_size)));
@@ -43,27 +46,33 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(Q
   w.block_size = uint32_t(a.c.block_size);
   w.ldb = uint32_t(a.c.ldb);
   w.num_blocks = uint32_t(a.c.num_blocks);
-  attend<kSrcCodes, FMT, false, QF16, HD, QF16 ? 2 : 1, QF16 ? 2 : 1, 1>(w, lds);
+  attend<kSrcCodes, FMT, false, QF16, HD, QF16 ? 2 : 1, QF16 ? 2 : 1, 4, CAP>(w, lds);
 }
 
-template <int FMT, bool QF16>
+template <int FMT, bool QF16, bool CAP>
 hipError_t launch_hd(const KvqAttnArgs& a, hipStream_t stream) {
   const int64_t blocks = (a.group * a.q_len + 127) / 128;
   const int64_t grid = blocks * a.c.kv_heads * a.num_seqs;
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
   if (a.c.head_dim == 128)
-    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 128>), dim3(unsigned(grid)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 128, CAP>), dim3(unsigned(grid)), dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 64>), dim3(unsigned(grid)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 64, CAP>), dim3(unsigned(grid)), dim3(kThreads), 0, stream, a);
   return hipGetLastError();
+}
+
+template <int FMT>
+hipError_t launch_type(const KvqAttnArgs& a, int q_dtype, hipStream_t stream) {
+  const bool cap = a.softcap > 0.0f;
+  if (q_dtype == kDtF16) return cap ? launch_hd<FMT, true, true>(a, stream) : launch_hd<FMT, true, false>(a, stream);
+  return cap ? launch_hd<FMT, false, true>(a, stream) : launch_hd<FMT, false, false>(a, stream);
 }
 
 }  // namespace
 
 hipError_t launch_kvq_chunk(const KvqAttnArgs& a, int fmt, int q_dtype, hipStream_t stream) {
   if (a.num_seqs == 0 || a.q_len == 0) return hipSuccess;
-  if (q_dtype == kDtF16) return fmt == kFmtInt8 ? launch_hd<kFmtInt8, true>(a, stream) : launch_hd<kFmtE4m3, true>(a, stream);
-  return fmt == kFmtInt8 ? launch_hd<kFmtInt8, false>(a, stream) : launch_hd<kFmtE4m3, false>(a, stream);
+  return fmt == kFmtInt8 ? launch_type<kFmtInt8>(a, q_dtype, stream) : launch_type<kFmtE4m3>(a, q_dtype, stream);
 }
 
 }  // namespace llmopt

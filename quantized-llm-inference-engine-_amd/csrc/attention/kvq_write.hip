@@ -72,26 +72,24 @@ __global__ void __launch_bounds__(64 * kWaves) kvq_write_kernel(const KvqWriteAr
   const int64_t bs = a.c.block_size, hd = a.c.head_dim;
 
   // ---- the unit's sequence, block and rows ----
-  int64_t s, j, row0, len;  // block j of the sequence's new ones; the source row and count of its new tokens
+  int64_t s, j, row0, len, off;  // block j of the sequence's new ones; their source row, count and position
   if (a.cu_seqlens) {
-    auto cu = [&](int64_t i) -> int64_t {
-      const int64_t v = a.cu_seqlens[i];
-      return v < 0 ? 0 : v > a.total_tokens ? a.total_tokens : v;
-    };
     // Sequence i's units start at floor(cu[i] / bs) + 2 i: room for the len / bs + 2 blocks it can touch.
-    auto start = [&](int64_t i) -> int64_t { return uint32_t(cu(i)) / uint32_t(bs) + 2 * i; };
-    s = last_at_most(a.num_seqs, unit, start);
-    j = unit - start(s);
-    row0 = cu(s);
-    len = cu(s + 1) - row0;
+    auto start = [&](int64_t at, int64_t i) -> int64_t { return uint32_t(at) / uint32_t(bs) + 2 * i; };
+    const Packed p = find_packed(a.cu_seqlens, a.num_seqs, a.total_tokens, unit, a.offsets, start);
+    s = p.s;
+    j = unit - start(p.first, s);
+    row0 = p.first;
+    len = p.end - p.first;
+    off = p.more;
   } else {
     s = unit / uint32_t(a.units_per_seq);
     j = unit - s * a.units_per_seq;
     row0 = 0;
     len = a.query_lens ? a.query_lens[s] : a.q_len;
     if (len > a.q_len) len = a.q_len;
+    off = a.offsets[s];
   }
-  const int64_t off = a.offsets[s];
   if (off < 0 || j < 0) return;
   const int64_t first = uint32_t(off) / uint32_t(bs), jb = first + j;  // 32 bits: checked on the host
   const int64_t p0 = j == 0 ? off : jb * bs;

@@ -8,23 +8,23 @@ namespace {
 
 using namespace tile;
 
-template <bool F16, int HD, int RB>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(RB == 1 ? 2 : 1, RB == 1 ? 2 : 1)))
+template <bool F16, int HD, int W, bool CAP>
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : 4, HD == 128 ? 2 : 4)))
     packed_attention_kernel(const PackedAttnArgs a) {
-  constexpr int kRows = 128 * RB;
+  constexpr int kRows = 32 * W;
   __shared__ __align__(16) uint8_t lds[4 * kKeys * HD * 2];
   const uint32_t kv_heads = uint32_t(a.kv_heads);
   const uint32_t unit = blockIdx.x / kv_heads, kvh = blockIdx.x - unit * kv_heads;
-  auto cu = [&](int64_t i) -> int64_t {
-    const int64_t v = a.cu_seqlens[i];
-    return v < 0 ? 0 : v > a.total_tokens ? a.total_tokens : v;
-  };
   if (unit >= a.blocks) {
+    auto cu = [&](int64_t i) -> int64_t {
+      const int64_t v = a.cu_seqlens[i];
+      return v < 0 ? 0 : v > a.total_tokens ? a.total_tokens : v;
+    };
     // Rows in front of the first sequence (there are none in a proper call) and behind the last one: zeros.
     const int64_t lo = a.num_seqs > 0 ? cu(0) : a.total_tokens, hi = a.num_seqs > 0 ? cu(a.num_seqs) : a.total_tokens;
     const int64_t per_row = a.group * (HD / 8);
-    for (int64_t i = (unit - a.blocks) * kThreads + threadIdx.x; i < (lo + a.total_tokens - hi) * per_row;
-         i += a.tail_blocks * kThreads) {
+    for (int64_t i = (unit - a.blocks) * (64 * W) + threadIdx.x; i < (lo + a.total_tokens - hi) * per_row;
+         i += a.tail_blocks * (64 * W)) {
       const int64_t r = i / per_row, x = i - r * per_row;
       const int64_t tok = r < lo ? r : hi + r - lo;
       uint16_t* dst = static_cast<uint16_t*>(a.out) + tok * a.o_tok_stride + (kvh * int64_t(a.group) + x / (HD / 8)) * a.o_head_stride;
@@ -33,10 +33,10 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(R
     return;
   }
   // Sequence i's row blocks start at floor(cu[i] group / kRows) + i: room for the ceil(len group / kRows) it has.
-  auto start = [&](int64_t i) -> int64_t { return cu(i) * a.group / kRows + i; };
-  const int64_t s = last_at_most(a.num_seqs, int64_t(unit), start);
-  const int64_t first = cu(s), len = cu(s + 1) - first;
-  const int64_t block = int64_t(unit) - start(s), count = (len * a.group + kRows - 1) / kRows;
+  auto start = [&](int64_t first, int64_t i) -> int64_t { return uint32_t(first) * uint32_t(a.group) / uint32_t(kRows) + i; };
+  const Packed p = find_packed(a.cu_seqlens, a.num_seqs, a.total_tokens, int64_t(unit), nullptr, start);
+  const int64_t first = p.first, len = p.end - p.first;
+  const int64_t block = int64_t(unit) - start(first, p.s), count = (len * a.group + kRows - 1) / kRows;
   if (block < 0 || block >= count) return;
   Work w{};
   const int64_t h0 = int64_t(kvh) * a.group;
@@ -49,6 +49,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(R
   w.group = a.group;
   w.rows = int(len * a.group);
   w.row0 = int(count - 1 - block) * kRows;  // the longest walks first
+  w.row0_tok = int(uint32_t(w.row0) / uint32_t(a.group));
   w.base = 0;
   w.t_end = int(uint32_t(min(w.row0 + kRows, w.rows) - 1) / uint32_t(a.group)) + 1;
   w.scale = a.scale;
@@ -58,18 +59,21 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(R
   w.k_tok_stride = a.k_tok_stride;
   w.v_tok_stride = a.v_tok_stride;
   w.len = int(len);
-  attend<kSrcPacked, 0, F16, F16, HD, 1, 1, RB>(w, lds);
+  attend<kSrcPacked, 0, F16, F16, HD, 1, 1, W, CAP>(w, lds);
 }
 
-template <bool F16, int HD, int RB>
+template <bool F16, int HD, int W>
 hipError_t launch(PackedAttnArgs a, hipStream_t stream) {
-  constexpr int kRows = 128 * RB;
+  constexpr int kRows = 32 * W;
   a.blocks = a.num_seqs > 0 ? a.total_tokens * a.group / kRows + a.num_seqs : 0;
   a.tail_blocks = a.zero_tail ? 32 : 0;
   const int64_t grid = (a.blocks + a.tail_blocks) * a.kv_heads;
   if (grid <= 0) return hipSuccess;
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((packed_attention_kernel<F16, HD, RB>), dim3(unsigned(grid)), dim3(kThreads), 0, stream, a);
+  if (a.softcap > 0.0f)
+    hipLaunchKernelGGL((packed_attention_kernel<F16, HD, W, true>), dim3(unsigned(grid)), dim3(64 * W), 0, stream, a);
+  else
+    hipLaunchKernelGGL((packed_attention_kernel<F16, HD, W, false>), dim3(unsigned(grid)), dim3(64 * W), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -77,8 +81,8 @@ hipError_t launch(PackedAttnArgs a, hipStream_t stream) {
 
 hipError_t launch_packed_attention(const PackedAttnArgs& a, int dtype, int64_t head_dim, hipStream_t stream) {
   if (a.total_tokens == 0) return hipSuccess;
-  if (dtype == kDtBf16) return head_dim == 128 ? launch<false, 128, 1>(a, stream) : launch<false, 64, 1>(a, stream);
-  return head_dim == 128 ? launch<true, 128, 1>(a, stream) : launch<true, 64, 1>(a, stream);
+  if (dtype == kDtBf16) return head_dim == 128 ? launch<false, 128, 4>(a, stream) : launch<false, 64, 4>(a, stream);
+  return head_dim == 128 ? launch<true, 128, 4>(a, stream) : launch<true, 64, 4>(a, stream);
 }
 
 }  // namespace llmopt

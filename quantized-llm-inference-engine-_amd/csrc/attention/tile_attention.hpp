@@ -26,7 +26,6 @@ namespace tile {
 
 enum : int { kSrcPacked = 0, kSrcCodes = 1 };
 
-constexpr int kThreads = 256;
 constexpr int kKeys = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -41,8 +40,11 @@ struct Op {
       return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   __device__ static uint32_t pack(float lo, float hi) {
+    // fp16 by the pair conversion that cuts: the sum below adds the probabilities as cut, so what they have in common
+    // cancels, and they spread over one step (2^-10), as rounded ones do. Three instructions for two numbers rounded:
+    // 183 us against 167 for 4 prompts of 2048.
     if constexpr (F16)
-      return uint32_t(__builtin_bit_cast(uint16_t, _Float16(lo))) | (uint32_t(__builtin_bit_cast(uint16_t, _Float16(hi))) << 16);
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
     else
       return pack_bf16(lo, hi);
   }
@@ -88,7 +90,8 @@ struct Work {
   int64_t o_tok_stride, o_head_stride;
   int group;
   int rows;   // query rows of the (sequence, KV head)
-  int row0;   // the workgroup's first
+  int row0;   // the workgroup's first, and its token
+  int row0_tok;
   int base;   // position of query token 0
   int t_end;  // its keys: t < t_end
   float scale, softcap;
@@ -104,51 +107,74 @@ struct Work {
   uint32_t kv_heads, kvh, block_size, ldb, num_blocks;
 };
 
-// KQ, KP: 16-bit pieces of the query and of a probability. F16: fp16 operands (packed fp16), else bf16.
-// QF16: the query's and output's type is fp16 (else bf16).
-template <int SRC, int FMT, bool F16, bool QF16, int HD, int KQ, int KP, int RB>
+// KQ, KP: 16-bit pieces of the query and of a probability. F16: fp16 operands (packed fp16), else bf16. QF16: the
+// query's and output's type is fp16 (else bf16). W: waves. CAP: the scores are soft-capped.
+template <int SRC, int FMT, bool F16, bool QF16, int HD, int KQ, int KP, int W, bool CAP>
 __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   constexpr int kCh = HD / 8;               // 16-byte chunks per 16-bit row
   constexpr int kRowBytes = HD * 2;
   constexpr int kTile = kKeys * kRowBytes;  // one K (or V) tile
   constexpr int kRpl = 64 / kCh;            // 16-bit rows per wave load (1 KB)
-  constexpr int kLoads = 16 / kRpl;         // packed: wave loads per tile, of K and of V: 16 rows
+  constexpr int kTr = kKeys / W;            // rows of a tile that a wave brings in
+  constexpr int kLoads = kTr / kRpl;        // packed: in wave loads of K and of V
   constexpr int kCpr = HD / 16;             // codes: 16-byte loads per row
   constexpr int kCrl = 64 / kCpr;           // codes: rows per wave load
-  constexpr int kCLoads = 16 / kCrl > 0 ? 16 / kCrl : 1;
+  constexpr int kCLoads = kTr / kCrl;
   constexpr int kS = HD / 16;               // 16-dim slices of the scores
   constexpr int kD = HD / 32;               // 32-dim blocks of the output
-  constexpr int kWaveRows = 32 * RB;
+  static_assert(kLoads > 0 && (SRC == kSrcPacked || kCLoads > 0), "a wave brings in whole loads");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const uint32_t group = uint32_t(a.group);
-  const int wrow = a.row0 + kWaveRows * wave;  // the wave's first row
   auto tok_of = [&](int row) -> int { return int(uint32_t(row) / group); };
-  int q_pos[RB], tok[RB], head[RB];
-  bool row_ok[RB];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int row = wrow + 32 * b + col;
-    row_ok[b] = row < a.rows;
-    tok[b] = tok_of(row_ok[b] ? row : a.rows - 1);
-    head[b] = (row_ok[b] ? row : a.rows - 1) - tok[b] * a.group;
-    q_pos[b] = row_ok[b] ? a.base + tok[b] : -1;
-  }
+  const int wrow = a.row0 + 32 * wave;  // the wave's first row
+  const bool row_ok = wrow + col < a.rows;
+  const int own_row = row_ok ? wrow + col : a.rows - 1;
+  const int tok = tok_of(own_row), head = own_row - tok * a.group;
+  const int q_pos = row_ok ? a.base + tok : -1;
   const int first_pos = a.base + tok_of(wrow);
-  const int wave_last = wrow < a.rows ? a.base + tok_of(min(wrow + kWaveRows, a.rows) - 1) : -1;
+  const int wave_last = wrow < a.rows ? a.base + tok_of(min(wrow + 32, a.rows) - 1) : -1;
   const int n_tiles = (a.t_end + kKeys - 1) / kKeys;
 
-  // ---- the wave's query rows: the B operand, dims 16 m + 8 half .. of row col ----
-  u32x4 qf[RB][KQ][kS];
+  const float neg_inf = -__int_as_float(0x7F800000);
+  // Probabilities are 2^(score c - m c), one fma and one exponential per score. c has to be positive for the maximum
+  // of the scores to be that of the exponents: a negative scale moves into the query rows, a zero one becomes too
+  // small to matter.
+  const float magnitude = __builtin_fabsf(a.scale) * kLog2e;
+  const float c2 = CAP ? kLog2e : magnitude > 0.0f ? magnitude : 1e-30f;
+  const uint32_t q_sign = !CAP && a.scale < 0.0f ? 0x80008000u : 0u;
+  float m_run = neg_inf, mc = 0.0f, l_run = 0.0f;  // the row's running maximum, m_run c2 (0 without keys), this lane's
+                                                   // share of the sum
+  f32x16 o[kD];
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const uint16_t* q = static_cast<const uint16_t*>(a.query) + tok[b] * a.q_tok_stride + head[b] * a.q_head_stride + 8 * half;
+  for (int d = 0; d < kD; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[d][v] = 0.0f;
+
+  // ---- the wave's query rows: the B operand, dims 16 m + 8 half .. of row col ----
+  // The rows come in whole, by direct loads into the second tile buffers (a lane's 16-byte pieces straight from memory
+  // would touch each line four times).
+  u32x4 qf[KQ][kS];
+  uint8_t* const q_lds = lds + (wave & 1) * (32 * kRowBytes) + kTile + (wave >> 1) * (2 * kTile);
+  auto fetch_query = [&]() {
+    const auto rs = make_rsrc(static_cast<const uint16_t*>(a.query) + a.row0_tok * a.q_tok_stride, 0x7FFFFFFFu);
+#pragma unroll
+    for (int j = 0; j < 32 / kRpl; ++j) {
+      const int r = kRpl * j + lane / kCh;
+      const int row = min(wrow + r, a.rows - 1);  // rows past the end repeat the last one
+      const int t = tok_of(row);
+      load_lds16_cached(rs, q_lds + kRpl * j * kRowBytes,
+                        uint32_t(((t - a.row0_tok) * a.q_tok_stride + (row - t * a.group) * a.q_head_stride) * 2) +
+                            16 * k_chunk<HD>(r, lane % kCh), 0);
+    }
+  };
+  auto load_query = [&]() {
 #pragma unroll
     for (int m = 0; m < kS; ++m) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(q + 16 * m);
+      const u32x4 w = *reinterpret_cast<const u32x4*>(q_lds + col * kRowBytes + 16 * k_chunk<HD>(col, 2 * m + half));
       if constexpr (KQ == 1) {
-        qf[b][0][m] = w;
+        qf[0][m] = w ^ q_sign;
       } else {  // fp16 = two bf16 pieces, exactly (8 + 3 significant bits)
         u32x4 hi, lo;
 #pragma unroll
@@ -157,103 +183,78 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
           hi[e] = pack_bf16(x, y);
           lo[e] = pack_bf16(x - __uint_as_float(hi[e] << 16), y - __uint_as_float(hi[e] & 0xFFFF0000u));
         }
-        qf[b][0][m] = hi;
-        qf[b][1][m] = lo;
+        qf[0][m] = hi ^ q_sign;
+        qf[1][m] = lo ^ q_sign;
       }
     }
-  }
+  };
 
-  const float neg_inf = -__int_as_float(0x7F800000);
-  // Probabilities are 2^(score c - m c), one fma and one exponential per score. c has to be positive for the maximum
-  // of the scores to be that of the exponents: a negative scale moves into the query rows, a zero one becomes too
-  // small to matter.
-  const bool capped = a.softcap > 0.0f;
-  const float magnitude = __builtin_fabsf(a.scale) * kLog2e;
-  const float c2 = capped ? kLog2e : magnitude > 0.0f ? magnitude : 1e-30f;
-  const uint32_t q_sign = !capped && a.scale < 0.0f ? 0x80008000u : 0u;
-#pragma unroll
-  for (int b = 0; b < RB; ++b)
-#pragma unroll
-    for (int p = 0; p < KQ; ++p)
-#pragma unroll
-      for (int m = 0; m < kS; ++m) qf[b][p][m] ^= q_sign;
-  float m_run[RB], mc[RB], l_run[RB];  // per row: running maximum, m_run c2 (0 without keys), this lane's share of the sum
-  f32x16 o[RB][kD];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    m_run[b] = neg_inf, mc[b] = 0.0f, l_run[b] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < kD; ++d)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) o[b][d][v] = 0.0f;
-  }
-
-  // ---- key tiles ----
-  uint8_t* const buf[2] = {lds, lds + 2 * kTile};
+  // ---- key tiles: two buffers of K and two of V; tile i in buffer i % 2 (offsets: they stay LDS addresses) ----
+  auto k_buf = [&](int i) -> uint8_t* { return lds + (i & 1) * kTile; };
+  auto v_buf = [&](int i) -> uint8_t* { return lds + 2 * kTile + (i & 1) * kTile; };
   // Packed: rows past the sequence repeat its last one; no row sees them.
-  auto fetch_packed = [&](int t0, int b) {
-    const int last = min(kKeys, a.len - t0) - 1;
-    const auto krs = make_rsrc(a.key + t0 * a.k_tok_stride, uint32_t(last * a.k_tok_stride * 2 + kRowBytes));
-    const auto vrs = make_rsrc(a.value + t0 * a.v_tok_stride, uint32_t(last * a.v_tok_stride * 2 + kRowBytes));
+  auto fetch_packed = [&](int k, int i) {
+    const int t0 = i * kKeys, last = min(kKeys, a.len - t0) - 1;
+    const int64_t stride = k ? a.v_tok_stride : a.k_tok_stride;
+    const auto rs = make_rsrc((k ? a.value : a.key) + t0 * stride, uint32_t(last * stride * 2 + kRowBytes));
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int r = wave * 16 + kRpl * i + lane / kCh;
-      const uint32_t row = uint32_t(min(r, last));
-      uint8_t* dst = buf[b] + (wave * 16 + kRpl * i) * kRowBytes;
-      load_lds16_cached(krs, dst, row * uint32_t(a.k_tok_stride * 2) + 16 * k_chunk<HD>(r, lane % kCh), 0);
-      load_lds16_cached(vrs, dst + kTile, row * uint32_t(a.v_tok_stride * 2) + 16 * v_chunk<HD>(r, lane % kCh), 0);
+    for (int j = 0; j < kLoads; ++j) {
+      const int r = wave * kTr + kRpl * j + lane / kCh;
+      const int c = k ? v_chunk<HD>(r, lane % kCh) : k_chunk<HD>(r, lane % kCh);
+      load_lds16_cached(rs, (k ? v_buf(i) : k_buf(i)) + (wave * kTr + kRpl * j) * kRowBytes,
+                        uint32_t(min(r, last)) * uint32_t(stride * 2) + 16 * c, 0);
     }
   };
-  // Codes: lane l looks up key t0 + l, the entry a tile ahead of its use.
-  auto fetch_entry = [&](int t0) -> int32_t {
-    const uint32_t t = uint32_t(t0 + lane);
+  // Codes: lane l looks up key l of a tile, the table entry some tiles ahead of its use.
+  struct Place {
+    uint32_t block, slot;  // (block, KV head) and slot of the lane's key; no key: some row of the cache
+    uint64_t mask;         // which keys there are
+  };
+  struct Held {
+    u32x4 codes[kCLoads > 0 ? kCLoads : 1];
+    float scale[kCLoads > 0 ? kCLoads : 1];
+  };
+  auto entry_of = [&](int i) -> int32_t {
+    const uint32_t t = uint32_t(i * kKeys + lane);
     const uint32_t bi = t / a.block_size;
     return int(t) < a.t_end && bi < a.ldb ? a.table[bi] : -1;
   };
-  u32x4 held[2][kCLoads];
-  float held_scale[2][kCLoads];
-  uint64_t held_mask = 0;
-  auto fetch_codes = [&](int t0, int32_t entry) {
-    const uint32_t t = uint32_t(t0 + lane);
+  auto place_of = [&](int i, int32_t entry) -> Place {
     const bool ok = entry >= 0 && uint32_t(entry) < a.num_blocks;
-    held_mask = __builtin_amdgcn_ballot_w64(ok);
-    const uint32_t block = ok ? uint32_t(entry) * a.kv_heads + a.kvh : a.kvh;  // no key: some row of the cache
-    const uint32_t slot = ok ? t % a.block_size : 0u;
-#pragma unroll
-    for (int i = 0; i < kCLoads; ++i) {
-      const int r = wave * 16 + kCrl * i + lane / kCpr;
-      const int64_t bl = uint32_t(__shfl(int(block), r & 63, 64));
-      const int64_t row = bl * a.block_size + __shfl(int(slot), r & 63, 64);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        held[k][i] = *reinterpret_cast<const u32x4*>(a.codes[k] + row * HD + 16 * (lane % kCpr));
-        held_scale[k][i] = a.scales[k][bl];
-      }
-    }
+    return Place{ok ? uint32_t(entry) * a.kv_heads + a.kvh : a.kvh, ok ? uint32_t(i * kKeys + lane) % a.block_size : 0u,
+                 __builtin_amdgcn_ballot_w64(ok)};
   };
-  auto store_codes = [&](int b) {
+  auto fetch_codes = [&](int k, const Place& p) -> Held {
+    Held h;
 #pragma unroll
-    for (int i = 0; i < kCLoads; ++i) {
-      const int r = wave * 16 + kCrl * i + lane / kCpr, c = 2 * (lane % kCpr);
-      const bool ok = (held_mask >> (r & 63)) & 1u;
+    for (int j = 0; j < kCLoads; ++j) {
+      const int r = wave * kTr + kCrl * j + lane / kCpr;
+      const int64_t block = uint32_t(__shfl(int(p.block), r, 64));
+      const int64_t row = block * a.block_size + __shfl(int(p.slot), r, 64);
+      h.codes[j] = *reinterpret_cast<const u32x4*>(a.codes[k] + row * HD + 16 * (lane % kCpr));
+      h.scale[j] = a.scales[k][block];
+    }
+    return h;
+  };
+  auto store_codes = [&](int k, int i, Held& h, uint64_t mask) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        u32x4 codes = held[k][i];
-        asm("" : "+v"(codes));  // whole words until here
-        const float s = held_scale[k][i];
+    for (int j = 0; j < kCLoads; ++j) {
+      const int r = wave * kTr + kCrl * j + lane / kCpr, c = 2 * (lane % kCpr);
+      const bool ok = k == 0 || ((mask >> r) & 1u);
+      asm("" : "+v"(h.codes[j]));  // whole words until here
+      const float s = h.scale[j];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          u32x4 w;
+      for (int q = 0; q < 2; ++q) {
+        u32x4 w;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t x = codes[2 * j + e];
-            w[2 * e] = pack_bf16(code_to_f32<FMT>(x, 0) * s, code_to_f32<FMT>(x, 1) * s);
-            w[2 * e + 1] = pack_bf16(code_to_f32<FMT>(x, 2) * s, code_to_f32<FMT>(x, 3) * s);
-          }
-          if (!ok) w = u32x4{0u, 0u, 0u, 0u};  // its scores are masked; its value must not be anything but finite
-          const int at = k == 0 ? k_chunk<HD>(r, c + j) : v_chunk<HD>(r, c + j);
-          *reinterpret_cast<u32x4*>(buf[b] + k * kTile + r * kRowBytes + 16 * at) = w;
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t x = h.codes[j][2 * q + e];
+          w[2 * e] = scaled_pair<FMT, false>(x, s);
+          w[2 * e + 1] = scaled_pair<FMT, true>(x, s);
         }
+        if (!ok) w = u32x4{0u, 0u, 0u, 0u};  // its probability is 0: its value must not be anything but finite
+        const int at = k == 0 ? k_chunk<HD>(r, c + q) : v_chunk<HD>(r, c + q);
+        *reinterpret_cast<u32x4*>((k == 0 ? k_buf(i) : v_buf(i)) + r * kRowBytes + 16 * at) = w;
       }
     }
   };
@@ -263,130 +264,143 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
   const int v_off = vkey * kRowBytes + 8 * (lane & 1);
 
-  auto compute = [&](const uint8_t* kt, int t0, uint64_t mask) {
-    const uint8_t* vt = kt + kTile;
-    f32x16 sc[RB][2];
+  struct Scores {
+    f32x16 s[2];
+  };
+  auto scores = [&](Scores& sc, int i) {
+    const uint8_t* kt = k_buf(i);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-      for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) sc[b][kb][v] = 0.0f;
+      for (int v = 0; v < 16; ++v) sc.s[kb][v] = 0.0f;
 #pragma unroll
       for (int m = 0; m < kS; ++m) {
         const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + (32 * kb + col) * kRowBytes + 16 * k_chunk<HD>(col, 2 * m + half));
 #pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-          for (int p = 0; p < KQ; ++p) sc[b][kb] = Op<F16>::mfma(kf, qf[b][p][m], sc[b][kb]);
+        for (int p = 0; p < KQ; ++p) sc.s[kb] = Op<F16>::mfma(kf, qf[p][m], sc.s[kb]);
       }
     }
-    u32x4 pf[RB][KP][4];
+  };
+  u32x4 pf[KP][4];
+  auto probabilities = [&](const Scores& sc) {
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      if (capped) {
+    for (int i = 0; i < 4; ++i) {
+      float p[8];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+      for (int v = 0; v < 8; ++v) p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc.s[i / 2][8 * (i % 2) + v], c2, -mc));
+      // The sum adds the probabilities as rounded (KP = 2: to 16 bits), so that a row's weights add up to one.
 #pragma unroll
-          for (int v = 0; v < 16; ++v) sc[b][kb][v] = tanhf(sc[b][kb][v] * a.scale / a.softcap) * a.softcap;
-      }
-      if (mask != ~uint64_t(0) || t0 + kKeys - 1 > first_pos) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          // Bit 8 q + r: key 8 q + 4 half + r of the block is a key at or before this row's token.
-          const int room = q_pos[b] - t0 - 32 * kb - 4 * half;
-          const uint32_t bits = (uint32_t(mask >> (32 * kb)) >> (4 * half)) & (room >= 31 ? ~0u : room < 0 ? 0u : (2u << room) - 1u);
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const uint32_t keep = uint32_t(int32_t(bits << (31 - (8 * (v / 4) + v % 4))) >> 31);
-            sc[b][kb][v] = __uint_as_float((__float_as_uint(sc[b][kb][v]) & keep) | (__float_as_uint(neg_inf) & ~keep));
-          }
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t hi = Op<F16>::pack(p[2 * e], p[2 * e + 1]);
+        pf[0][i][e] = hi;
+        l_run = Op<F16>::add_pair(hi, l_run);
+        if constexpr (KP == 2) {
+          const uint32_t lo = Op<F16>::pack(p[2 * e] - __uint_as_float(hi << 16), p[2 * e + 1] - __uint_as_float(hi & 0xFFFF0000u));
+          pf[1][i][e] = lo;
+          l_run = Op<F16>::add_pair(lo, l_run);
         }
       }
-      float top = neg_inf;
+    }
+  };
+  // Tile i: its scores, their softmax, and its part of the output.
+  auto step = [&](int i, uint64_t mask) {
+    Scores sc;
+    scores(sc, i);
+    const int t0 = i * kKeys;
+    if constexpr (CAP) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) top = fmaxf(top, sc[b][kb][v]);
-      const float m_new = fmaxf(m_run[b], other_half_max(top));
-      if (__builtin_amdgcn_ballot_w64(m_new > m_run[b])) {
-        const float mc_new = m_new == neg_inf ? 0.0f : m_new * c2;
-        const float alpha = m_run[b] == neg_inf ? 0.0f : __builtin_amdgcn_exp2f(mc[b] - mc_new);
-        m_run[b] = m_new;
-        mc[b] = mc_new;
-        if (t0 > 0) {
-          l_run[b] *= alpha;
+        for (int v = 0; v < 16; ++v) sc.s[kb][v] = tanhf(sc.s[kb][v] * a.scale / a.softcap) * a.softcap;
+    }
+    if (mask != ~uint64_t(0) || t0 + kKeys - 1 > first_pos) {
 #pragma unroll
-          for (int d = 0; d < kD; ++d)
+      for (int kb = 0; kb < 2; ++kb) {
+        // Bit 8 q + r: key 8 q + 4 half + r of the block is a key at or before this row's token.
+        const int room = q_pos - t0 - 32 * kb - 4 * half;
+        const uint32_t bits = (uint32_t(mask >> (32 * kb)) >> (4 * half)) & (room >= 31 ? ~0u : room < 0 ? 0u : (2u << room) - 1u);
 #pragma unroll
-            for (int v = 0; v < 16; ++v) o[b][d][v] *= alpha;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float p[8];
-#pragma unroll
-        for (int v = 0; v < 8; ++v)
-          p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i / 2][8 * (i % 2) + v], c2, -mc[b]));
-        // The sum adds the probabilities as rounded (KP = 2: to 16 bits), so that a row's weights add up to one.
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t hi = Op<F16>::pack(p[2 * e], p[2 * e + 1]);
-          pf[b][0][i][e] = hi;
-          l_run[b] = Op<F16>::add_pair(hi, l_run[b]);
-          if constexpr (KP == 2) {
-            const uint32_t lo = Op<F16>::pack(p[2 * e] - __uint_as_float(hi << 16), p[2 * e + 1] - __uint_as_float(hi & 0xFFFF0000u));
-            pf[b][1][i][e] = lo;
-            l_run[b] = Op<F16>::add_pair(lo, l_run[b]);
-          }
+        for (int v = 0; v < 16; ++v) {
+          const uint32_t keep = uint32_t(int32_t(bits << (31 - (8 * (v / 4) + v % 4))) >> 31);
+          sc.s[kb][v] = __uint_as_float((__float_as_uint(sc.s[kb][v]) & keep) | (__float_as_uint(neg_inf) & ~keep));
         }
       }
     }
+    float top = neg_inf;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) top = fmaxf(top, sc.s[kb][v]);
+    const float m_new = fmaxf(m_run, other_half_max(top));
+    if (__builtin_amdgcn_ballot_w64(m_new > m_run)) {
+      const float mc_new = m_new == neg_inf ? 0.0f : m_new * c2;
+      const float alpha = m_run == neg_inf ? 0.0f : __builtin_amdgcn_exp2f(mc - mc_new);
+      m_run = m_new;
+      mc = mc_new;
+      if (t0 > 0) {
+        l_run *= alpha;
+#pragma unroll
+        for (int d = 0; d < kD; ++d)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
+      }
+    }
+    probabilities(sc);
+    const uint8_t* vt = v_buf(i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int d = 0; d < kD; ++d) {
-        // Keys 16 i + vkey and 8 further: both have vkey's low bits, so one swizzle.
-        const uint8_t* p0 = vt + 16 * i * kRowBytes + v_off + 16 * v_chunk<HD>(vkey, 4 * d + vc);
+        // Keys 16 j + vkey and 8 further: both have vkey's low bits, so one swizzle.
+        const uint8_t* p0 = vt + 16 * j * kRowBytes + v_off + 16 * v_chunk<HD>(vkey, 4 * d + vc);
         const u32x2 lo = read_transposed(p0), hi = read_transposed(p0 + 8 * kRowBytes);
         const u32x4 vf = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-          for (int p = 0; p < KP; ++p) o[b][d] = Op<F16>::mfma(vf, pf[b][p][i], o[b][d]);
+        for (int p = 0; p < KP; ++p) o[d] = Op<F16>::mfma(vf, pf[p][j], o[d]);
       }
   };
 
   if (n_tiles > 0) {
     if constexpr (SRC == kSrcPacked) {
       fetch_packed(0, 0);
+      fetch_packed(1, 0);
+      fetch_query();
+      wait_vmcnt<0>();
+      load_query();
       for (int i = 0; i < n_tiles; ++i) {
-        const int t0 = i * kKeys;
-        wait_vmcnt<0>();    // this wave's rows of tile i
-        wait_lgkmcnt0();    // its reads of the buffer that is refilled next
+        wait_vmcnt<0>();  // this wave's rows of tile i
+        wait_lgkmcnt0();  // its reads of the buffers that are refilled next
         __builtin_amdgcn_s_barrier();
-        if (i + 1 < n_tiles) fetch_packed(t0 + kKeys, (i + 1) & 1);
-        if (t0 <= wave_last) compute(buf[i & 1], t0, ~uint64_t(0));
+        if (i + 1 < n_tiles) {
+          fetch_packed(0, i + 1);
+          fetch_packed(1, i + 1);
+        }
+        if (i * kKeys <= wave_last) step(i, ~uint64_t(0));
       }
     } else {
-      int32_t entry = fetch_entry(0);
-      fetch_codes(0, entry);
-      entry = fetch_entry(kKeys);
-      uint64_t mask = held_mask;
-      store_codes(0);
+      Place place = place_of(0, entry_of(0));
+      int32_t entry = entry_of(1);
+      Held hk = fetch_codes(0, place), hv = fetch_codes(1, place);
+      fetch_query();
+      store_codes(0, 0, hk, place.mask);
+      store_codes(1, 0, hv, place.mask);
+      wait_vmcnt<0>();
+      load_query();
       for (int i = 0; i < n_tiles; ++i) {
-        const int t0 = i * kKeys;
-        wait_lgkmcnt0();    // its stores of tile i, and its reads of the buffer that is refilled next
+        wait_lgkmcnt0();  // its stores of tile i, and its reads of the buffers that are refilled next
         __builtin_amdgcn_s_barrier();
-        const uint64_t now = mask;
+        const uint64_t mask = place.mask;
         if (i + 1 < n_tiles) {
-          const int32_t e = entry;
-          entry = fetch_entry(t0 + 2 * kKeys);
-          fetch_codes(t0 + kKeys, e);
-          mask = held_mask;
+          place = place_of(i + 1, entry);
+          hk = fetch_codes(0, place);
+          hv = fetch_codes(1, place);
+          entry = entry_of(i + 2);
         }
-        if (t0 <= wave_last) compute(buf[i & 1], t0, now);
-        if (i + 1 < n_tiles) store_codes((i + 1) & 1);
+        if (i * kKeys <= wave_last) step(i, mask);
+        if (i + 1 < n_tiles) {
+          store_codes(0, i + 1, hk, place.mask);
+          store_codes(1, i + 1, hv, place.mask);
+        }
       }
     }
   }
@@ -401,13 +415,12 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
     else
       return pack_bf16(lo, hi);
   };
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const float l = other_half_sum(l_run[b]);
+  {
+    const float l = other_half_sum(l_run);
     // Zeros without keys; over the cache also for a sum that is no number (as the torch sequence's nan_to_num gives).
     const bool none = SRC == kSrcPacked ? l == 0.0f : !(l > 0.0f);
     const float inv = 1.0f / l;
-    bool odd = false;
+    bool bad_value = false;
 #pragma unroll
     for (int d = 0; d < kD; ++d)
 #pragma unroll
@@ -415,8 +428,8 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
         float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          v[r] = none ? 0.0f : o[b][d][4 * q + r] * inv;
-          odd |= !(__builtin_fabsf(v[r]) < __int_as_float(0x7F800000));
+          v[r] = none ? 0.0f : o[d][4 * q + r] * inv;
+          bad_value |= !(__builtin_fabsf(v[r]) < __int_as_float(0x7F800000));
         }
         *reinterpret_cast<u32x2*>(stage + col * kRowBytes + 16 * k_chunk<HD>(col, 4 * d + q) + 8 * half) =
             u32x2{narrow(v[0], v[1]), narrow(v[2], v[3])};
@@ -425,7 +438,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
 #pragma unroll
     for (int i = 0; i < 32 / kRpl; ++i) {
       const int r = kRpl * i + lane / kCh, c = lane % kCh;
-      const int row = wrow + 32 * b + r;
+      const int row = wrow + r;
       if (row >= a.rows) continue;
       const int t = tok_of(row);
       const u32x4 w = *reinterpret_cast<const u32x4*>(stage + r * kRowBytes + 16 * k_chunk<HD>(r, c));
@@ -435,13 +448,13 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
     wait_lgkmcnt0();
 
     // ---- rows with anything that is not finite: once more, key by key, masked keys left out ----
-    uint64_t bad64 = __builtin_amdgcn_ballot_w64(odd && row_ok[b]);
+    uint64_t bad64 = __builtin_amdgcn_ballot_w64(bad_value && row_ok);
     if (bad64) {
       wait_vmcnt<0>();  // the stores above
       uint32_t bad = uint32_t(bad64) | uint32_t(bad64 >> 32);
       constexpr int kE = HD / 64;  // dims per lane
       for (; bad; bad &= bad - 1) {
-        const int row = wrow + 32 * b + __builtin_ctz(bad);
+        const int row = wrow + __builtin_ctz(bad);
         const int t_row = tok_of(row), g = row - t_row * a.group;
         const int pos = a.base + t_row;
         const uint16_t* q = static_cast<const uint16_t*>(a.query) + t_row * a.q_tok_stride + g * a.q_head_stride;
@@ -467,7 +480,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
             dot = __builtin_fmaf(x, element(0, key ? t : 0, d, key), dot);
           }
           float sc = dot * a.scale;
-          if (capped) sc = tanhf(sc / a.softcap) * a.softcap;
+          if (CAP) sc = tanhf(sc / a.softcap) * a.softcap;
           sc = key ? sc * kLog2e : neg_inf;
           float top = sc;
 #pragma unroll

@@ -131,8 +131,8 @@ class PagedAttention:
 
             try:
                 if isinstance(cache, QuantizedPagedKVCache):
-                    return ops.kvq_attention(query[:, :, :q_len], *cache.layer(layer_idx), block_ids, context_lens,
-                                             self.scale, self.config.softcap)
+                    return ops.cache_attention(query, cache, layer_idx, block_ids, context_lens, q_len, self.scale,
+                                               self.config.softcap)
                 if q_len == 1:
                     out = ops.paged_decode_attention(
                         query[:, :, 0, :], cache.key_cache[layer_idx], cache.value_cache[layer_idx], block_ids,

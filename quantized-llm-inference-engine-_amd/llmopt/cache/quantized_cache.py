@@ -71,8 +71,7 @@ class QuantizedPagedKVCache:
     def _adopt(self, key_codes, key_scales, value_codes, value_scales) -> None:  # noqa: ANN001
         self.key_codes, self.key_scales = key_codes, key_scales
         self.value_codes, self.value_scales = value_codes, value_scales
-        self.num_layers, self.num_blocks, self.num_kv_heads, self.block_size, self.head_dim = (
-            int(d) for d in key_codes.shape)
+        self.num_layers, self.num_blocks, self.num_kv_heads, self.block_size, self.head_dim = key_codes.shape
         self.dtype = key_codes.dtype
         self.device = key_codes.device
 
@@ -87,12 +86,15 @@ class QuantizedPagedKVCache:
         if key_codes.dtype not in cls.FORMATS or value_codes.dtype != key_codes.dtype:
             raise TypeError(f"the 8-bit cache holds int8 or float8_e4m3fn codes, not {key_codes.dtype}, "
                             f"{value_codes.dtype}")
-        for scales in (key_scales, value_scales):
-            if scales.shape != key_codes.shape[:3] or scales.dtype != torch.float32:
-                raise ValueError(f"expected float32 scales {tuple(key_codes.shape[:3])}, got {tuple(scales.shape)} "
-                                 f"{scales.dtype}")
+        shape, device = key_codes.shape[:3], key_codes.device
+        if key_scales.shape != shape or value_scales.shape != shape or key_scales.dtype != torch.float32 \
+                or value_scales.dtype != torch.float32:
+            raise ValueError(f"expected float32 scales {tuple(shape)}, got {tuple(key_scales.shape)} "
+                             f"{key_scales.dtype} and {tuple(value_scales.shape)} {value_scales.dtype}")
         tensors = (key_codes, key_scales, value_codes, value_scales)
-        if not all(t.is_contiguous() and t.device == key_codes.device for t in tensors):
+        if not (key_codes.is_contiguous() and key_scales.is_contiguous() and value_codes.is_contiguous()
+                and value_scales.is_contiguous()) or not key_scales.device == value_codes.device \
+                == value_scales.device == device:
             raise ValueError("the cache's tensors must be contiguous and on one device")
         cache = cls.__new__(cls)
         cache._adopt(*tensors)
@@ -122,6 +124,9 @@ class QuantizedPagedKVCache:
         first negative block or at the end of the row; a block id past the cache and a negative offset write nothing.
         No block may belong to two sequences of one call.
         """
+        if keys.dim() != 4 or values.dim() != 4:
+            raise ValueError(f"write takes [seq, q_len, kv_heads, head_dim], got {tuple(keys.shape)} and "
+                             f"{tuple(values.shape)}")
         self._write(layer_idx, block_ids, token_offsets, keys, values, None, query_lens)
 
     def write_decode(
@@ -135,7 +140,10 @@ class QuantizedPagedKVCache:
         """Quantize one token per sequence, ``keys``/``values`` ``[seq, kv_heads, head_dim]``, at ``token_offsets[s]``.
         A token whose block id is not one of the cache's is not written (:class:`PagedKVCache` puts it into block 0,
         whose scale it would spoil here), so ``-1`` rows pad a batch."""
-        self._write(layer_idx, block_ids, token_offsets, keys.unsqueeze(1), values.unsqueeze(1), None, None)
+        if keys.dim() != 3 or values.dim() != 3:
+            raise ValueError(f"write_decode takes [seq, kv_heads, head_dim], got {tuple(keys.shape)} and "
+                             f"{tuple(values.shape)}")
+        self._write(layer_idx, block_ids, token_offsets, keys, values, None, None)
 
     def write_packed(
         self,
@@ -155,8 +163,10 @@ class QuantizedPagedKVCache:
         if self.key_codes.device.type == "cuda":
             from llmopt.kernels import ops
 
-            ops.kvq_write(*self.layer(layer_idx), block_ids, token_offsets, keys, values, cu_seqlens, query_lens)
+            ops.cache_write(self, layer_idx, block_ids, token_offsets, keys, values, cu_seqlens, query_lens)
             return
+        if cu_seqlens is None and keys.dim() == 3:
+            keys, values = keys.unsqueeze(1), values.unsqueeze(1)
         if keys.shape != values.shape or keys.dim() != (4 if cu_seqlens is None else 3) \
                 or tuple(keys.shape[-2:]) != (self.num_kv_heads, self.head_dim):
             raise ValueError(f"keys and values of shape {tuple(keys.shape)} and {tuple(values.shape)} do not match the "

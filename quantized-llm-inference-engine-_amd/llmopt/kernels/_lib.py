@@ -201,7 +201,8 @@ def binding_path() -> Path:
 
 
 def load_binding():  # noqa: ANN201 - the extension module, or None
-    """Load (once) and return the native host path of the linears (``csrc/torch_binding.cpp``), with
+    """Load (once) and return the native host path of the linears, of the 8-bit KV cache and of packed
+    attention (``csrc/torch_binding.cpp``), with
     the kernel library's entry points attached. None, with one warning, where it is not built or does not
     load into this torch: calls then take the general path, the same kernels through ctypes."""
     global _binding, _binding_tried
@@ -222,6 +223,9 @@ def load_binding():  # noqa: ANN201 - the extension module, or None
                 module.attach(*(ctypes.cast(getattr(lib, name), _p).value for name in (
                     "llmopt_q_linear_ex", "llmopt_q_linear_workspace_ex", "llmopt_q_linear_swiglu",
                     "llmopt_q_linear_swiglu_workspace_ex")))
+                module.attach_kvq(*(ctypes.cast(getattr(lib, name), _p).value for name in (
+                    "llmopt_kvq_write", "llmopt_kvq_attention_workspace", "llmopt_kvq_attention",
+                    "llmopt_packed_attention")))
                 _binding = module
             except (ImportError, OSError) as exc:
                 warnings.warn(f"the linears' native host path is not available ({exc}); calls go through ctypes, "

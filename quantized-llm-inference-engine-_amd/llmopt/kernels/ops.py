@@ -48,6 +48,8 @@ __all__ = [
     "rope_kv_write_decode",
     "paged_decode_attention_rope",
     "argmax_rows",
+    "cache_attention",
+    "cache_write",
     "paged_prefill_attention",
     "unpack_nibbles",
 ]
@@ -730,6 +732,35 @@ def kvq_write(key_codes, key_scales, value_codes, value_scales, block_ids, token
         )
 
 
+def cache_write(cache, layer_idx: int, block_ids: torch.Tensor, token_offsets: torch.Tensor,  # noqa: ANN001
+                keys: torch.Tensor, values: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
+                query_lens: torch.Tensor | None = None) -> None:
+    """:func:`kvq_write` into a layer of a :class:`QuantizedPagedKVCache`, also of ``keys``/``values`` ``[seq, kv_heads,
+    head_dim]`` (one token each). The plain form of a call (int32 metadata, everything on the current device) has its
+    checks and launch in native code; any other takes :func:`kvq_write`."""
+    binding = load_binding()
+    if binding is not None and binding.kvq_write(
+            cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, layer_idx, block_ids,
+            token_offsets, keys, values, cu_seqlens, query_lens):
+        return
+    if cu_seqlens is None and keys.dim() == 3:
+        keys, values = keys.unsqueeze(1), values.unsqueeze(1)
+    kvq_write(*cache.layer(layer_idx), block_ids, token_offsets, keys, values, cu_seqlens, query_lens)
+
+
+def cache_attention(query: torch.Tensor, cache, layer_idx: int, block_ids: torch.Tensor,  # noqa: ANN001
+                    context_lens: torch.Tensor, q_len: int, scale: float, softcap: float = 0.0) -> torch.Tensor:
+    """:func:`kvq_attention` of the first ``q_len`` tokens of ``query`` over a layer of a
+    :class:`QuantizedPagedKVCache`, the plain form of a call in native code as in :func:`cache_write`."""
+    binding = load_binding()
+    if binding is not None:
+        out = binding.kvq_attention(cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, layer_idx,
+                                    block_ids, context_lens, query, q_len, scale, softcap)
+        if out is not None:
+            return out
+    return kvq_attention(query[:, :, :q_len], *cache.layer(layer_idx), block_ids, context_lens, scale, softcap)
+
+
 def kvq_attention(query: torch.Tensor, key_codes: torch.Tensor, key_scales: torch.Tensor, value_codes: torch.Tensor,
                   value_scales: torch.Tensor, block_ids: torch.Tensor, context_lens: torch.Tensor, scale: float,
                   softcap: float = 0.0) -> torch.Tensor:
@@ -780,6 +811,11 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     head_dim]`` (fp16 or bf16, any token and head strides), sequence ``s`` the rows ``cu_seqlens[s]`` up to
     ``cu_seqlens[s + 1]``. Rows behind the last sequence are zeros, in a given ``out`` left as they were. Raises
     ``NotImplementedError`` for fp32 and for head dims other than 64 and 128."""
+    binding = load_binding() if out is None and query.is_cuda else None
+    if binding is not None:  # the plain form of a call, in native code
+        result = binding.packed_attention(query, key, value, cu_seqlens, scale, softcap)
+        if result is not None:
+            return result
     if query.dim() != 3 or key.dim() != 3 or key.shape != value.shape or query.shape[0] != key.shape[0] \
             or query.shape[2] != key.shape[2]:
         raise ValueError(f"packed_attention: query [tokens, heads, d], key and value [tokens, kv_heads, d] expected, got "
@@ -801,7 +837,7 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
 
     def rows16(t: torch.Tensor) -> bool:
         return (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
-                and 0 <= t.stride(0) <= 1 << 24)
+                and 0 <= t.stride(0) <= 1 << 22 and 0 <= t.stride(1) <= 1 << 22)
 
     query, key, value = (t if rows16(t) else t.clone(memory_format=torch.contiguous_format) for t in (query, key, value))
     result = out

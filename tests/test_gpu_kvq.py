@@ -246,11 +246,12 @@ def test_scale_and_softcap(q_len, scale, softcap):
     _check(attention.forward(q, cache, 0, table, lens), q, cache, table, lens, scale, softcap)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("q_len", [1, 48])
-def test_scales_far_apart(dtype, q_len):
-    """Blocks whose scales are up to 2^60 apart: neither a probability nor a product may vanish or overflow."""
-    cache, table = _filled(2, 300, 16, 2, 64, torch.int8, seed=9, spread=0.0)
+def test_scales_far_apart(fmt, dtype, q_len):
+    """Blocks whose scales are up to 2^34 apart: neither a probability nor a product may vanish or overflow."""
+    cache, table = _filled(2, 300, 16, 2, 64, FORMATS[fmt], seed=9, spread=0.0)
     cache.value_scales.copy_(torch.exp2(torch.randint(-30, 4, cache.value_scales.shape, device="cuda").float()))
     cache.value_scales[0, table[0].long()] = 2.0**-30  # a sequence of nothing but small values
     lens = torch.tensor([300, 290], dtype=torch.int32, device="cuda")
@@ -278,9 +279,10 @@ def test_what_lies_behind_the_context_does_not_matter(q_len):
     assert torch.equal(attention.forward(q, cache, 0, table, lens), want)
 
 
-def test_a_later_block_that_is_not_finite_leaves_earlier_queries_alone():
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_later_block_that_is_not_finite_leaves_earlier_queries_alone(fmt):
     """A chunk's last tokens are in a block marked NaN: queries before that block do not see it."""
-    cache, table = _filled(1, 128, 16, 2, 64, torch.int8, seed=13)
+    cache, table = _filled(1, 128, 16, 2, 64, FORMATS[fmt], seed=13)
     lens = torch.tensor([128], dtype=torch.int32, device="cuda")
     q = torch.randn(1, 8, 100, 64, device="cuda").bfloat16()
     attention = PagedAttention(8, 2, 64)
