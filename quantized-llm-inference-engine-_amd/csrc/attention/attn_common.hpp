@@ -51,7 +51,7 @@ struct KvqAttnArgs {
   int group;          // query heads per KV head
   float scale, softcap;
   int q_vec;          // query rows 16-byte aligned
-  // decode: splits of tiles_per_split 32-token tiles; partial results when splits > 1
+  // splits of tiles_per_split 32-token tiles (the chunk kernel: an even number); partial results when splits > 1
   int splits, waves;
   int64_t tiles_per_split;
   float* part_out;  // [splits, num_seqs, kv_heads, group * q_len, head_dim], each normalized
@@ -77,6 +77,8 @@ struct PackedAttnArgs {
 hipError_t launch_kvq_write(const KvqWriteArgs& a, int fmt, int src_dtype, bool vec, hipStream_t stream);
 hipError_t launch_kvq_decode(const KvqAttnArgs& a, int fmt, int q_dtype, hipStream_t stream);
 hipError_t launch_kvq_chunk(const KvqAttnArgs& a, int fmt, int q_dtype, hipStream_t stream);
+// Merges the parts of a.splits > 1 splits into a.out.
+hipError_t launch_kvq_merge(const KvqAttnArgs& a, int q_dtype, hipStream_t stream);
 hipError_t launch_packed_attention(const PackedAttnArgs& a, int dtype, int64_t head_dim, hipStream_t stream);
 
 // ---- conversions ---------------------------------------------------------------------------------

@@ -61,32 +61,51 @@ int describe_cache(llmopt::KvqCache& c, const void* key_codes, const float* key_
   return LLMOPT_OK;
 }
 
-// How the decode kernel's work is cut: `waves` per workgroup, `splits` of the context of `tiles_per_split` 32-token
-// tiles each.
+// How the attention's work is cut: on the tile kernel or the decode kernel (`waves` per workgroup), in `splits` of the
+// context of `tiles_per_split` 32-token tiles each. The context lengths are on the device, so the table's width stands for
+// them. Measured (MI355X, bf16, 32 / 8 heads of 128, int8, ragged contexts of half to the whole width; us):
+//   * Tile or decode kernel: the decode kernel reads the keys once per 16 query rows, the tile kernel once per 128, but it
+//     starts slower and its workgroups are fewer. Level where (16-row blocks x 32-token tiles) is about 28000 at heads of
+//     128 (half the work each at 64): 1 sequence of 8000, 32 / 64 / 512 new tokens 26.6 / 39.6 / 219 against 30.9 / 33.3 /
+//     112; 8 of 2000, 24 / 64 tokens 34.2 / 55 against 32.9 / 46; 32 of 1000, 9 / 24 tokens 34.4 / 51 against 34.7 / 43.
+//   * Workgroups of eight waves, one per CU, in one round: 1 sequence of 8000 in 32 splits 14.2 (4 splits 23.5), 8 of 4096
+//     in 4 splits 19.6 (1 33, 8 23.3), 32 of 640 in 1 split 12.5 (2 19.2); past 256 pairs none (64 of 8192: 147 - 165; 2
+//     splits 176). A split has a tile per wave at least, and up to 24 tiles stay whole but for a few pairs: the merge costs 3.
+//   * Four waves, two workgroups per CU, from 512 pairs over tables of up to 2048 tokens: 64 of 640 18.0 (eight waves 21.4),
+//     128 of 1024 47 (57), 64 of 2048 45.7 (46.3); longer ones 162 (147).
+//   * Tables much wider than their contexts: a split is at most 1024 tokens for a few pairs, 8192 for many.
+//   * The tile kernel's row blocks fill two workgroups per CU with splits of 512 tokens at least: 1 sequence of 8000, 512
+//     tokens 224 without splits, 112 with.
 struct Plan {
+  bool tile;
   int splits, waves;
   int64_t tiles_per_split;
 };
 
-Plan plan_decode(int64_t num_seqs, int64_t kv_heads, int64_t group, int64_t q_len, int64_t ldb, int64_t block_size) {
-  const int64_t tiles = std::max<int64_t>(1, (ldb * block_size + 31) / 32);
-  const int64_t pairs = std::max<int64_t>(1, num_seqs * kv_heads * ((group * q_len + 15) / 16));
-  constexpr int waves = 4;
-  // About four workgroups per CU, each wave with two tiles at least.
-  int64_t splits = std::max<int64_t>(1, 1024 / pairs);
-  splits = std::min(splits, (tiles + 2 * waves - 1) / (2 * waves));
+Plan plan_attention(int64_t num_seqs, int64_t kv_heads, int64_t group, int64_t head_dim, int64_t q_len, int64_t ldb,
+                    int64_t block_size, int q_dtype, bool tile_rows) {
+  const int64_t tiles = std::max<int64_t>(1, (ldb * block_size + 31) / 32), rows = group * q_len;
+  const int64_t pairs = std::max<int64_t>(1, num_seqs * kv_heads * ((rows + 15) / 16));
+  bool tile = tile_rows && q_dtype != LLMOPT_DTYPE_F32 && rows > 32 && pairs * tiles * head_dim > 3600000;
+  if (tile) {
+    const int64_t blocks = num_seqs * kv_heads * ((rows + 127) / 128);
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / blocks, tiles / 16, 16}));
+    const int64_t per = ((tiles + splits - 1) / splits + 1) / 2 * 2;
+    return Plan{true, int((tiles + per - 1) / per), 4, per};
+  }
+  const int waves = pairs >= 512 && tiles <= 64 ? 4 : 8;
+  int64_t splits = 1;
+  if (pairs < 256 && (tiles > 24 || pairs < 32)) splits = std::max<int64_t>(1, std::min(256 / pairs, (tiles + 7) / 8));
+  splits = std::max(splits, tiles / (pairs <= 32 ? 32 : pairs < 256 ? 128 : 256));
   splits = std::min<int64_t>(splits, 256);
   const int64_t per = (tiles + splits - 1) / splits;
-  return Plan{int((tiles + per - 1) / per), waves, per};
+  return Plan{false, int((tiles + per - 1) / per), waves, per};
 }
 
 // A workgroup of the tile kernel reads its query rows (128 tokens, one KV head's query heads) at 32-bit offsets.
 bool near_rows(int64_t group, int64_t tok_stride, int64_t head_stride) {
   return tok_stride >= 0 && tok_stride <= (int64_t(1) << 22) && head_stride >= 0 && head_stride <= (int64_t(1) << 29) / group;
 }
-
-// Whether the tile kernel takes the chunk: 16-bit queries, more than 32 rows per KV head.
-bool takes_tiles(int64_t group, int64_t q_len, int q_dtype) { return q_dtype != LLMOPT_DTYPE_F32 && group * q_len > 32; }
 
 }  // namespace
 
@@ -141,8 +160,8 @@ size_t llmopt_kvq_attention_workspace(int64_t num_seqs, int64_t num_heads, int64
                                       int64_t q_len, int64_t ldb, int64_t block_size, int q_dtype) {
   if (num_seqs <= 0 || num_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_len <= 0 || ldb <= 0 || block_size <= 0)
     return 0;
-  if (num_heads % kv_heads != 0 || takes_tiles(num_heads / kv_heads, q_len, q_dtype)) return 0;
-  const Plan plan = plan_decode(num_seqs, kv_heads, num_heads / kv_heads, q_len, ldb, block_size);
+  if (num_heads % kv_heads != 0) return 0;
+  const Plan plan = plan_attention(num_seqs, kv_heads, num_heads / kv_heads, head_dim, q_len, ldb, block_size, q_dtype, true);
   if (plan.splits <= 1) return 0;
   return size_t(plan.splits) * size_t(num_seqs) * size_t(num_heads) * size_t(q_len) * size_t(head_dim + 1) * sizeof(float);
 }
@@ -190,11 +209,9 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
     return aligned(p, 16) && (x * esize) % 16 == 0 && (y * esize) % 16 == 0 && (z * esize) % 16 == 0;
   };
   a.q_vec = rows16(query, q_seq_stride, q_head_stride, q_tok_stride);
-  if (takes_tiles(group, q_len, q_dtype) && a.q_vec && near_rows(group, q_tok_stride, q_head_stride) &&
-      rows16(out, o_seq_stride, o_head_stride, o_tok_stride))
-    return hip_status(llmopt::launch_kvq_chunk(a, format, q_dtype, static_cast<hipStream_t>(stream)),
-                      "chunk attention launch");
-  const Plan plan = plan_decode(num_seqs, kv_heads, group, q_len, ldb, block_size);
+  const bool tile_rows = a.q_vec && near_rows(group, q_tok_stride, q_head_stride) &&
+                         rows16(out, o_seq_stride, o_head_stride, o_tok_stride);
+  const Plan plan = plan_attention(num_seqs, kv_heads, group, head_dim, q_len, ldb, block_size, q_dtype, tile_rows);
   a.waves = plan.waves;
   a.splits = plan.splits;
   a.tiles_per_split = plan.tiles_per_split;
@@ -208,6 +225,9 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
     a.part_out = static_cast<float*>(workspace);
     a.part_lse = a.part_out + rows * size_t(head_dim);
   }
+  if (plan.tile)
+    return hip_status(llmopt::launch_kvq_chunk(a, format, q_dtype, static_cast<hipStream_t>(stream)),
+                      "chunk attention launch");
   return hip_status(llmopt::launch_kvq_decode(a, format, q_dtype, static_cast<hipStream_t>(stream)),
                     "attention launch");
 }

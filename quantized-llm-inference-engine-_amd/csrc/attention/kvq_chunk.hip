@@ -1,5 +1,6 @@
 // Attention of a chunk of query tokens per sequence over the 8-bit KV cache: the tile kernel of tile_attention.hpp
-// over codes that it dequantizes exactly to bf16. fp16 queries: query and probabilities in two bf16 pieces each.
+// over codes that it dequantizes exactly to bf16. fp16 queries: query and probabilities in two bf16 pieces each. Few row
+// blocks (one long prompt's next chunk) are cut along the keys as well, and the parts merged as the decode kernel's are.
 #include "tile_attention.hpp"
 
 namespace llmopt {
@@ -37,6 +38,15 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(H
   w.base = a.context_lens[s] - int(a.q_len);
   const int last = int(uint32_t(min(row0 + kRows, rows) - 1) / uint32_t(a.group));
   w.t_end = max(0, min(w.base + last + 1, int(a.c.ldb * a.c.block_size)));
+  if (a.splits > 1) {
+    const int span = int(a.tiles_per_split) * 32;  // a multiple of 64
+    w.t_begin = int(blockIdx.y) * span;
+    if (w.t_begin >= w.t_end) return;  // the merge does not read this part
+    w.t_end = min(w.t_end, w.t_begin + span);
+    const int64_t part = ((int64_t(blockIdx.y) * a.num_seqs + s) * kv_heads + kvh) * rows;
+    w.part_out = a.part_out + part * HD;
+    w.part_lse = a.part_lse + part;
+  }
   w.scale = a.scale;
   w.softcap = a.softcap;
   for (int k = 0; k < 2; ++k) w.codes[k] = a.c.codes[k], w.scales[k] = a.c.scales[k];
@@ -54,10 +64,12 @@ hipError_t launch_hd(const KvqAttnArgs& a, hipStream_t stream) {
   const int64_t blocks = (a.group * a.q_len + 127) / 128;
   const int64_t grid = blocks * a.c.kv_heads * a.num_seqs;
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const dim3 grid3(unsigned(grid), unsigned(a.splits));
   if (a.c.head_dim == 128)
-    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 128, CAP>), dim3(unsigned(grid)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 128, CAP>), grid3, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 64, CAP>), dim3(unsigned(grid)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 64, CAP>), grid3, dim3(kThreads), 0, stream, a);
+  if (a.splits > 1) return launch_kvq_merge(a, QF16 ? kDtF16 : kDtBf16, stream);
   return hipGetLastError();
 }
 

@@ -47,7 +47,7 @@ struct Pieces {
 };
 
 template <int QT, int FMT, int HD, int W, bool UNI>
-__global__ void __launch_bounds__(64 * W) kvq_decode_kernel(const KvqAttnArgs a) {
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) kvq_decode_kernel(const KvqAttnArgs a) {
   constexpr int kJ = HD / 64;      // 16-byte loads of a key row per lane
   constexpr int kNm = 2 * kJ;      // score MFMAs per half (32 dims each)
   constexpr int kNv = HD / 16;     // P V MFMAs per tile, dims per lane and token
@@ -67,16 +67,23 @@ __global__ void __launch_bounds__(64 * W) kvq_decode_kernel(const KvqAttnArgs a)
   const int tok = int(uint32_t(row) / uint32_t(a.group));
   const int last_tok = int(uint32_t(min(16 * rb + 15, rows - 1)) / uint32_t(a.group));
   const uint32_t bs = uint32_t(a.c.block_size), ldb = uint32_t(a.c.ldb), nblk = uint32_t(a.c.num_blocks);
+  const int32_t* const table = a.c.block_ids + s * a.c.ldb;
+  const int t_begin = int(split * a.tiles_per_split) * 32;
+  auto tile_t0 = [&](int i) -> int { return t_begin + 32 * (wave + W * i); };
+  // The first table entries do not wait for the context's length.
+  int32_t first_entry = -1;
+  if constexpr (UNI) {
+    const uint32_t bi = uint32_t(tile_t0(lane / 2) + 16 * (lane & 1)) / bs;
+    if (bi < ldb) first_entry = table[bi];
+  }
   const int base = a.context_lens[s] - q_len;  // position of query token 0
   const int q_pos = row_ok ? base + tok : -1;
   const int first_pos = base + int(uint32_t(16 * rb) / uint32_t(a.group));
   // The rows' keys: t < t_end, within the table (its width in tokens is below 2^31, checked on the host).
   const int t_end = max(0, min(base + last_tok + 1, int(ldb * bs)));
-  const int t_begin = int(split * a.tiles_per_split) * 32;
   const int n_all = min(int(a.tiles_per_split), (t_end - t_begin + 31) / 32);
   const int n_tiles = n_all > wave ? (n_all - wave + W - 1) / W : 0;
   if (a.splits > 1 && n_all <= 0) return;  // the merge does not read this part
-  auto tile_t0 = [&](int i) -> int { return t_begin + 32 * (wave + W * i); };
 
   // ---- the query row col: dims 64 j + 16 kb + 8 h .. + 8 are operand 2 j + h ----
   u32x4 qf[kQ][kNm];
@@ -123,7 +130,6 @@ __global__ void __launch_bounds__(64 * W) kvq_decode_kernel(const KvqAttnArgs a)
     }
   }
 
-  const int32_t* const table = a.c.block_ids + s * a.c.ldb;
   const uint8_t* const kcodes = a.c.codes[0];
   const uint8_t* const vcodes = a.c.codes[1];
   // Row of token slot `slot` of `block` in the codes; below 2^31 (checked on the host).
@@ -263,7 +269,7 @@ __global__ void __launch_bounds__(64 * W) kvq_decode_kernel(const KvqAttnArgs a)
     }
   };
 
-  constexpr int kDepth = 2;
+  constexpr int kDepth = 2;  // tiles in flight behind the one that is computed
   Tile ring[kDepth];
   if constexpr (UNI) {
     const uint32_t k_lane = uint32_t(col * HD + 16 * kb), v_lane = uint32_t(4 * kb * HD + kNv * col);
@@ -275,8 +281,9 @@ __global__ void __launch_bounds__(64 * W) kvq_decode_kernel(const KvqAttnArgs a)
       {
         const uint32_t t = uint32_t(tile_t0(g0 + lane / 2) + 16 * (lane & 1));
         const uint32_t bi = t / bs;
+        if (g0 > 0) first_entry = bi < ldb ? table[bi] : -1;
         if (lane < 2 * n && int(t) < t_end) {
-          const int32_t entry = table[bi];
+          const int32_t entry = first_entry;
           if (entry >= 0 && uint32_t(entry) < nblk) {
             my_row = row_at(uint32_t(entry), t - bi * bs);
             const int64_t at = int64_t(entry) * kv_heads + kvh;
@@ -357,18 +364,20 @@ __global__ void __launch_bounds__(64 * W) kvq_decode_kernel(const KvqAttnArgs a)
 
   // ---- the waves' parts: lane (col, kb) holds row col, dims kNv (4 kb + r) + i ----
   l_run = sum_across_rows(l_run);
-  __shared__ float m_lds[W][16];
-  __shared__ float l_lds[W][16];
-  __shared__ __align__(16) float o_lds[W][16][HD + 4];
+  extern __shared__ __align__(16) float merge_lds[];  // [W][16] maxima, sums; [W][rows][HD + 4]: launch_waves sizes it
+  const int here = min(16, rows - 16 * rb);
+  float(*const m_lds)[16] = reinterpret_cast<float(*)[16]>(merge_lds);
+  float(*const l_lds)[16] = m_lds + W;
+  float* const o_lds = merge_lds + 2 * W * 16;
   if (kb == 0) m_lds[wave][col] = m_run, l_lds[wave][col] = l_run;
   if (row_ok) {
+    float* const at = o_lds + (wave * here + col) * (HD + 4);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int i = 0; i < kNv; ++i) o_lds[wave][col][kNv * (4 * kb + r) + i] = o[i][r];
+      for (int i = 0; i < kNv; ++i) at[kNv * (4 * kb + r) + i] = o[i][r];
   }
   __syncthreads();
-  const int here = min(16, rows - 16 * rb);
   for (int e = int(threadIdx.x); e < here * HD; e += 64 * W) {
     const int rr = e / HD, d = e % HD;
     float top = neg_inf;
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(64 * W) kvq_decode_kernel(const KvqAttnArgs a)
       const float mw = m_lds[w][rr];
       const float f = mw == neg_inf ? 0.0f : __builtin_amdgcn_exp2f(mw - top);
       lsum = __builtin_fmaf(f, l_lds[w][rr], lsum);
-      acc = __builtin_fmaf(f, o_lds[w][rr][d], acc);
+      acc = __builtin_fmaf(f, o_lds[(w * here + rr) * (HD + 4) + d], acc);
     }
     // Zeros without keys, and for a sum that is no number (as the torch sequence's nan_to_num gives).
     const float val = lsum > 0.0f ? acc / lsum : 0.0f;
@@ -395,7 +404,7 @@ __global__ void __launch_bounds__(64 * W) kvq_decode_kernel(const KvqAttnArgs a)
     } else {
       const int64_t at = ((int64_t(split) * a.num_seqs + s) * kv_heads + kvh) * rows + r;
       a.part_out[at * HD + d] = val;
-      if (d == 0) a.part_lse[at] = lsum > 0.0f ? top + __builtin_amdgcn_logf(lsum) : neg_inf;
+      if (d == 0) a.part_lse[at] = lsum == 0.0f ? neg_inf : top + __builtin_amdgcn_logf(lsum);  // NaN stays
     }
   }
 }
@@ -449,15 +458,13 @@ template <int QT, int FMT, int HD, bool UNI>
 hipError_t launch_waves(const KvqAttnArgs& a, hipStream_t stream) {
   const int64_t rows = a.group * a.q_len, blocks = (rows + 15) / 16;
   const dim3 grid(unsigned(a.splits), unsigned(a.c.kv_heads * blocks), unsigned(a.num_seqs));
+  const size_t lds = size_t(a.waves) * (2 * 16 + size_t(rows < 16 ? rows : 16) * (HD + 4)) * sizeof(float);
   switch (a.waves) {
-    case 4: hipLaunchKernelGGL((kvq_decode_kernel<QT, FMT, HD, 4, UNI>), grid, dim3(256), 0, stream, a); break;
-    case 8: hipLaunchKernelGGL((kvq_decode_kernel<QT, FMT, HD, 8, UNI>), grid, dim3(512), 0, stream, a); break;
+    case 4: hipLaunchKernelGGL((kvq_decode_kernel<QT, FMT, HD, 4, UNI>), grid, dim3(256), lds, stream, a); break;
+    case 8: hipLaunchKernelGGL((kvq_decode_kernel<QT, FMT, HD, 8, UNI>), grid, dim3(512), lds, stream, a); break;
     default: return hipErrorInvalidValue;
   }
-  if (a.splits > 1) {
-    const dim3 merge(unsigned((rows + 3) / 4), unsigned(a.c.kv_heads), unsigned(a.num_seqs));
-    hipLaunchKernelGGL((kvq_merge_kernel<QT, HD>), merge, dim3(256), 0, stream, a);
-  }
+  if (a.splits > 1) return launch_kvq_merge(a, QT, stream);
   return hipGetLastError();
 }
 
@@ -474,7 +481,26 @@ hipError_t launch_fmt(const KvqAttnArgs& a, int fmt, hipStream_t stream) {
   return fmt == kFmtInt8 ? launch_hd<QT, kFmtInt8>(a, stream) : launch_hd<QT, kFmtE4m3>(a, stream);
 }
 
+template <int QT>
+void launch_merge(const KvqAttnArgs& a, hipStream_t stream) {
+  const int64_t rows = a.group * a.q_len;
+  const dim3 grid(unsigned((rows + 3) / 4), unsigned(a.c.kv_heads), unsigned(a.num_seqs));
+  if (a.c.head_dim == 128)
+    hipLaunchKernelGGL((kvq_merge_kernel<QT, 128>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((kvq_merge_kernel<QT, 64>), grid, dim3(256), 0, stream, a);
+}
+
 }  // namespace
+
+hipError_t launch_kvq_merge(const KvqAttnArgs& a, int q_dtype, hipStream_t stream) {
+  switch (q_dtype) {
+    case kDtF32: launch_merge<kDtF32>(a, stream); break;
+    case kDtF16: launch_merge<kDtF16>(a, stream); break;
+    default: launch_merge<kDtBf16>(a, stream); break;
+  }
+  return hipGetLastError();
+}
 
 hipError_t launch_kvq_decode(const KvqAttnArgs& a, int fmt, int q_dtype, hipStream_t stream) {
   if (a.num_seqs == 0 || a.q_len == 0) return hipSuccess;

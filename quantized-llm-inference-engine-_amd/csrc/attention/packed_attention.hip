@@ -51,6 +51,7 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(HD 
   w.row0 = int(count - 1 - block) * kRows;  // the longest walks first
   w.row0_tok = int(uint32_t(w.row0) / uint32_t(a.group));
   w.base = 0;
+  w.t_begin = 0;
   w.t_end = int(uint32_t(min(w.row0 + kRows, w.rows) - 1) / uint32_t(a.group)) + 1;
   w.scale = a.scale;
   w.softcap = a.softcap;

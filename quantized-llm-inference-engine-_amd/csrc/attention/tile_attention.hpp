@@ -93,7 +93,8 @@ struct Work {
   int row0;   // the workgroup's first, and its token
   int row0_tok;
   int base;   // position of query token 0
-  int t_end;  // its keys: t < t_end
+  int t_begin;  // its keys: t_begin (a multiple of 64) <= t < t_end
+  int t_end;
   float scale, softcap;
   // packed: key and value rows of the sequence's token 0
   const uint16_t* key;
@@ -105,6 +106,9 @@ struct Work {
   const float* scales[2];
   const int32_t* table;
   uint32_t kv_heads, kvh, block_size, ldb, num_blocks;
+  // codes: with part_out, the split's normalized rows [rows, HD] and log-sum-exps (powers of two) go there, in fp32
+  float* part_out;
+  float* part_lse;
 };
 
 // KQ, KP: 16-bit pieces of the query and of a probability. F16: fp16 operands (packed fp16), else bf16. QF16: the
@@ -135,7 +139,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   const int q_pos = row_ok ? a.base + tok : -1;
   const int first_pos = a.base + tok_of(wrow);
   const int wave_last = wrow < a.rows ? a.base + tok_of(min(wrow + 32, a.rows) - 1) : -1;
-  const int n_tiles = (a.t_end + kKeys - 1) / kKeys;
+  const int first_tile = a.t_begin / kKeys, n_tiles = (a.t_end + kKeys - 1) / kKeys;
 
   const float neg_inf = -__int_as_float(0x7F800000);
   // Probabilities are 2^(score c - m c), one fma and one exponential per score. c has to be positive for the maximum
@@ -156,7 +160,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   // The rows come in whole, by direct loads into the second tile buffers (a lane's 16-byte pieces straight from memory
   // would touch each line four times).
   u32x4 qf[KQ][kS];
-  uint8_t* const q_lds = lds + (wave & 1) * (32 * kRowBytes) + kTile + (wave >> 1) * (2 * kTile);
+  uint8_t* const q_lds = lds + (wave & 1) * (32 * kRowBytes) + (first_tile & 1 ? 0 : kTile) + (wave >> 1) * (2 * kTile);
   auto fetch_query = [&]() {
     const auto rs = make_rsrc(static_cast<const uint16_t*>(a.query) + a.row0_tok * a.q_tok_stride, 0x7FFFFFFFu);
 #pragma unroll
@@ -337,7 +341,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
       const float alpha = m_run == neg_inf ? 0.0f : __builtin_amdgcn_exp2f(mc - mc_new);
       m_run = m_new;
       mc = mc_new;
-      if (t0 > 0) {
+      if (i > first_tile) {
         l_run *= alpha;
 #pragma unroll
         for (int d = 0; d < kD; ++d)
@@ -360,7 +364,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
       }
   };
 
-  if (n_tiles > 0) {
+  if (n_tiles > first_tile) {
     if constexpr (SRC == kSrcPacked) {
       fetch_packed(0, 0);
       fetch_packed(1, 0);
@@ -378,15 +382,15 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
         if (i * kKeys <= wave_last) step(i, ~uint64_t(0));
       }
     } else {
-      Place place = place_of(0, entry_of(0));
-      int32_t entry = entry_of(1);
+      Place place = place_of(first_tile, entry_of(first_tile));
+      int32_t entry = entry_of(first_tile + 1);
       Held hk = fetch_codes(0, place), hv = fetch_codes(1, place);
       fetch_query();
-      store_codes(0, 0, hk, place.mask);
-      store_codes(1, 0, hv, place.mask);
+      store_codes(0, first_tile, hk, place.mask);
+      store_codes(1, first_tile, hv, place.mask);
       wait_vmcnt<0>();
       load_query();
-      for (int i = 0; i < n_tiles; ++i) {
+      for (int i = first_tile; i < n_tiles; ++i) {
         wait_lgkmcnt0();  // its stores of tile i, and its reads of the buffers that are refilled next
         __builtin_amdgcn_s_barrier();
         const uint64_t mask = place.mask;
@@ -402,6 +406,105 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
           store_codes(1, i + 1, hv, place.mask);
         }
       }
+    }
+  }
+
+  // ---- rows with anything that is not finite: once more, key by key, masked keys left out ----
+  auto again = [&](uint64_t lanes) {
+    if (lanes) {
+      wait_vmcnt<0>();  // the rows' own stores
+      uint32_t bad = uint32_t(lanes) | uint32_t(lanes >> 32);
+      constexpr int kE = HD / 64;  // dims per lane
+      for (; bad; bad &= bad - 1) {
+        const int row = wrow + __builtin_ctz(bad);
+        const int t_row = tok_of(row), g = row - t_row * a.group;
+        const int pos = a.base + t_row;
+        const uint16_t* q = static_cast<const uint16_t*>(a.query) + t_row * a.q_tok_stride + g * a.q_head_stride;
+        auto element = [&](int k, int t, int d, bool& key) -> float {  // dim d of key (value) t
+          if constexpr (SRC == kSrcPacked) {
+            const uint16_t x = k == 0 ? a.key[t * a.k_tok_stride + d] : a.value[t * a.v_tok_stride + d];
+            return F16 ? f16_to_f32(x) : bf16_to_f32(x);
+          } else {
+            const uint32_t bi = uint32_t(t) / a.block_size;
+            const int32_t entry = bi < a.ldb ? a.table[bi] : -1;
+            key = key && entry >= 0 && uint32_t(entry) < a.num_blocks;
+            const int64_t bl = (key ? int64_t(entry) : 0) * a.kv_heads + a.kvh;
+            return code_to_f32<FMT>(a.codes[k][(bl * a.block_size + uint32_t(t) % a.block_size) * HD + d], 0) * a.scales[k][bl];
+          }
+        };
+        float m = neg_inf, sum = 0.0f, acc[kE] = {};
+        for (int t0 = a.t_begin; t0 <= pos && t0 < a.t_end; t0 += 64) {
+          const int t = t0 + lane;
+          bool key = t <= pos && t < a.t_end;
+          float dot = 0.0f;
+          for (int d = 0; d < HD; ++d) {
+            const float x = QF16 ? f16_to_f32(q[d]) : bf16_to_f32(q[d]);
+            dot = __builtin_fmaf(x, element(0, key ? t : 0, d, key), dot);
+          }
+          float sc = dot * a.scale;
+          if (CAP) sc = tanhf(sc / a.softcap) * a.softcap;
+          sc = key ? sc * kLog2e : neg_inf;
+          float top = sc;
+#pragma unroll
+          for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+          const float m_new = fmaxf(m, top), ref = m_new == neg_inf ? 0.0f : m_new;
+          const float alpha = m == neg_inf ? 0.0f : __builtin_amdgcn_exp2f(m - ref);
+          m = m_new;
+          const float p = key ? __builtin_amdgcn_exp2f(sc - ref) : 0.0f;
+          sum *= alpha;
+#pragma unroll
+          for (int e = 0; e < kE; ++e) acc[e] *= alpha;
+          uint64_t keys = __builtin_amdgcn_ballot_w64(key);
+          for (; keys; keys &= keys - 1) {
+            const int from = __builtin_ctzll(keys);
+            const float pt = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), from));
+            sum += pt;
+            bool yes = true;
+#pragma unroll
+            for (int e = 0; e < kE; ++e) acc[e] = __builtin_fmaf(pt, element(1, t0 + from, kE * lane + e, yes), acc[e]);
+          }
+        }
+        const bool no = SRC == kSrcPacked ? sum == 0.0f : !(sum > 0.0f);
+        if constexpr (SRC == kSrcCodes) {
+          if (a.part_out) {
+#pragma unroll
+            for (int e = 0; e < kE; ++e) a.part_out[int64_t(row) * HD + kE * lane + e] = no ? 0.0f : acc[e] / sum;
+            if (lane == 0) a.part_lse[row] = sum == 0.0f ? neg_inf : m + __builtin_amdgcn_logf(sum);
+            continue;
+          }
+        }
+        uint16_t* dst = static_cast<uint16_t*>(a.out) + t_row * a.o_tok_stride + g * a.o_head_stride + kE * lane;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+          const float v = no ? 0.0f : acc[e] / sum;
+          dst[e] = QF16 ? f32_to_f16_rne(v) : f32_to_bf16_rne(v);
+        }
+      }
+    }
+  };
+
+  if constexpr (SRC == kSrcCodes) {
+    if (a.part_out) {
+      // ---- a part of the keys: fp32 rows and their log-sum-exps, for the merge kernel ----
+      const float l = other_half_sum(l_run);
+      const float inv = 1.0f / l;
+      bool bad_value = false;
+      float* const dst = a.part_out + int64_t(own_row) * HD + 4 * half;
+#pragma unroll
+      for (int d = 0; d < kD; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            v[r] = l > 0.0f ? o[d][4 * q + r] * inv : 0.0f;
+            bad_value |= !(__builtin_fabsf(v[r]) < __int_as_float(0x7F800000));
+          }
+          if (row_ok) *reinterpret_cast<f32x4*>(dst + 32 * d + 8 * q) = v;
+        }
+      if (row_ok && half == 0) a.part_lse[own_row] = l == 0.0f ? neg_inf : mc + __builtin_amdgcn_logf(l);  // NaN stays
+      again(__builtin_amdgcn_ballot_w64(bad_value && row_ok));
+      return;
     }
   }
 
@@ -445,72 +548,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
       uint16_t* dst = static_cast<uint16_t*>(a.out) + t * a.o_tok_stride + (row - t * a.group) * a.o_head_stride + 8 * c;
       *reinterpret_cast<u32x4*>(dst) = w;
     }
-    wait_lgkmcnt0();
-
-    // ---- rows with anything that is not finite: once more, key by key, masked keys left out ----
-    uint64_t bad64 = __builtin_amdgcn_ballot_w64(bad_value && row_ok);
-    if (bad64) {
-      wait_vmcnt<0>();  // the stores above
-      uint32_t bad = uint32_t(bad64) | uint32_t(bad64 >> 32);
-      constexpr int kE = HD / 64;  // dims per lane
-      for (; bad; bad &= bad - 1) {
-        const int row = wrow + __builtin_ctz(bad);
-        const int t_row = tok_of(row), g = row - t_row * a.group;
-        const int pos = a.base + t_row;
-        const uint16_t* q = static_cast<const uint16_t*>(a.query) + t_row * a.q_tok_stride + g * a.q_head_stride;
-        auto element = [&](int k, int t, int d, bool& key) -> float {  // dim d of key (value) t
-          if constexpr (SRC == kSrcPacked) {
-            const uint16_t x = k == 0 ? a.key[t * a.k_tok_stride + d] : a.value[t * a.v_tok_stride + d];
-            return F16 ? f16_to_f32(x) : bf16_to_f32(x);
-          } else {
-            const uint32_t bi = uint32_t(t) / a.block_size;
-            const int32_t entry = bi < a.ldb ? a.table[bi] : -1;
-            key = key && entry >= 0 && uint32_t(entry) < a.num_blocks;
-            const int64_t bl = (key ? int64_t(entry) : 0) * a.kv_heads + a.kvh;
-            return code_to_f32<FMT>(a.codes[k][(bl * a.block_size + uint32_t(t) % a.block_size) * HD + d], 0) * a.scales[k][bl];
-          }
-        };
-        float m = neg_inf, sum = 0.0f, acc[kE] = {};
-        for (int t0 = 0; t0 <= pos && t0 < a.t_end; t0 += 64) {
-          const int t = t0 + lane;
-          bool key = t <= pos && t < a.t_end;
-          float dot = 0.0f;
-          for (int d = 0; d < HD; ++d) {
-            const float x = QF16 ? f16_to_f32(q[d]) : bf16_to_f32(q[d]);
-            dot = __builtin_fmaf(x, element(0, key ? t : 0, d, key), dot);
-          }
-          float sc = dot * a.scale;
-          if (CAP) sc = tanhf(sc / a.softcap) * a.softcap;
-          sc = key ? sc * kLog2e : neg_inf;
-          float top = sc;
-#pragma unroll
-          for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-          const float m_new = fmaxf(m, top), ref = m_new == neg_inf ? 0.0f : m_new;
-          const float alpha = m == neg_inf ? 0.0f : __builtin_amdgcn_exp2f(m - ref);
-          m = m_new;
-          const float p = key ? __builtin_amdgcn_exp2f(sc - ref) : 0.0f;
-          sum *= alpha;
-#pragma unroll
-          for (int e = 0; e < kE; ++e) acc[e] *= alpha;
-          uint64_t keys = __builtin_amdgcn_ballot_w64(key);
-          for (; keys; keys &= keys - 1) {
-            const int from = __builtin_ctzll(keys);
-            const float pt = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), from));
-            sum += pt;
-            bool yes = true;
-#pragma unroll
-            for (int e = 0; e < kE; ++e) acc[e] = __builtin_fmaf(pt, element(1, t0 + from, kE * lane + e, yes), acc[e]);
-          }
-        }
-        const bool no = SRC == kSrcPacked ? sum == 0.0f : !(sum > 0.0f);
-        uint16_t* dst = static_cast<uint16_t*>(a.out) + t_row * a.o_tok_stride + g * a.o_head_stride + kE * lane;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          const float v = no ? 0.0f : acc[e] / sum;
-          dst[e] = QF16 ? f32_to_f16_rne(v) : f32_to_bf16_rne(v);
-        }
-      }
-    }
+    again(__builtin_amdgcn_ballot_w64(bad_value && row_ok));
   }
 }
 
