@@ -1,5 +1,5 @@
 // Attention of a chunk of query tokens per sequence over the 8-bit KV cache: the tile kernel of tile_attention.hpp
-// over codes that it dequantizes exactly to bf16. fp16 queries: query and probabilities in two bf16 pieces each. Few row
+// over codes that it dequantizes exactly to bf16. fp16 queries: keys as fp16 operands, probabilities in two bf16 pieces. Few row
 // blocks (one long prompt's next chunk) are cut along the keys as well, and the parts merged as the decode kernel's are.
 #include "tile_attention.hpp"
 
@@ -11,10 +11,10 @@ using namespace tile;
 constexpr int kThreads = 256;
 
 template <int FMT, bool QF16, int HD, bool CAP>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 ? (QF16 ? 2 : 3) : QF16 ? 1 : 2, HD == 64 ? (QF16 ? 2 : 3) : QF16 ? 1 : 2)))
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : 2, HD == 64 ? 3 : 2)))
     kvq_chunk_kernel(const KvqAttnArgs a) {
   constexpr int kRows = 128;
-  __shared__ __align__(16) uint8_t lds[4 * kKeys * HD * 2];
+  __shared__ __align__(16) uint8_t lds[4 * kKeys * HD * 2 + (QF16 ? 2 * kKeys * 4 : 0)];
   // Workgroups in the order (KV head, row block, sequence), a sequence's last blocks (the longest walks) first.
   const uint32_t kv_heads = uint32_t(a.c.kv_heads);
   const int rows = a.group * int(a.q_len);
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(H
   w.block_size = uint32_t(a.c.block_size);
   w.ldb = uint32_t(a.c.ldb);
   w.num_blocks = uint32_t(a.c.num_blocks);
-  attend<kSrcCodes, FMT, false, QF16, HD, QF16 ? 2 : 1, QF16 ? 2 : 1, 4, CAP>(w, lds);
+  attend<kSrcCodes, FMT, false, QF16, HD, QF16 ? 2 : 1, 4, CAP>(w, lds);
 }
 
 template <int FMT, bool QF16, bool CAP>

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(HD 
   w.k_tok_stride = a.k_tok_stride;
   w.v_tok_stride = a.v_tok_stride;
   w.len = int(len);
-  attend<kSrcPacked, 0, F16, F16, HD, 1, 1, W, CAP>(w, lds);
+  attend<kSrcPacked, 0, F16, F16, HD, 1, W, CAP>(w, lds);
 }
 
 template <bool F16, int HD, int W>

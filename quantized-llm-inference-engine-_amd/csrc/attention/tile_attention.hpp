@@ -28,6 +28,11 @@ enum : int { kSrcPacked = 0, kSrcCodes = 1 };
 
 constexpr int kKeys = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
+// Probabilities that are cut to fp16 lose 0.721 2^-11 of their value on average (half a step over a mantissa spread evenly
+// in its logarithm), the largest, 1, nothing. They are raised by that much first, as a part of the exponent: log2(1 +
+// 0.721 2^-11). 2-norm error of 32 prompts of up to 1024 tokens against float64: cut 2.85e-4, raised and cut 2.40e-4; the
+// output's own rounding alone makes 2.02e-4.
+constexpr float kCut = 5.08e-4f;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -40,9 +45,8 @@ struct Op {
       return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   __device__ static uint32_t pack(float lo, float hi) {
-    // fp16 by the pair conversion that cuts: the sum below adds the probabilities as cut, so what they have in common
-    // cancels, and they spread over one step (2^-10), as rounded ones do. Three instructions for two numbers rounded:
-    // 183 us against 167 for 4 prompts of 2048.
+    // fp16 by the pair conversion that cuts (see kCut). Rounding takes three instructions for two numbers: 183 us against
+    // 167 for 4 prompts of 2048.
     if constexpr (F16)
       return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
     else
@@ -111,9 +115,9 @@ struct Work {
   float* part_lse;
 };
 
-// KQ, KP: 16-bit pieces of the query and of a probability. F16: fp16 operands (packed fp16), else bf16. QF16: the
+// KP: 16-bit pieces of a probability. F16: fp16 operands (packed fp16), else bf16. QF16: the
 // query's and output's type is fp16 (else bf16). W: waves. CAP: the scores are soft-capped.
-template <int SRC, int FMT, bool F16, bool QF16, int HD, int KQ, int KP, int W, bool CAP>
+template <int SRC, int FMT, bool F16, bool QF16, int HD, int KP, int W, bool CAP>
 __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   constexpr int kCh = HD / 8;               // 16-byte chunks per 16-bit row
   constexpr int kRowBytes = HD * 2;
@@ -126,6 +130,9 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   constexpr int kCLoads = kTr / kCrl;
   constexpr int kS = HD / 16;               // 16-dim slices of the scores
   constexpr int kD = HD / 32;               // 32-dim blocks of the output
+  // fp16 queries over codes: the keys are the codes themselves, exact in fp16, and their scales, by key in LDS behind
+  // the tiles, multiply the scores (two bf16 pieces of the query instead: 287 us against 193 for a chunk of 4 x 512 after up to 3500).
+  constexpr bool kRawKeys = SRC == kSrcCodes && QF16;
   static_assert(kLoads > 0 && (SRC == kSrcPacked || kCLoads > 0), "a wave brings in whole loads");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -159,7 +166,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   // ---- the wave's query rows: the B operand, dims 16 m + 8 half .. of row col ----
   // The rows come in whole, by direct loads into the second tile buffers (a lane's 16-byte pieces straight from memory
   // would touch each line four times).
-  u32x4 qf[KQ][kS];
+  u32x4 qf[kS];
   uint8_t* const q_lds = lds + (wave & 1) * (32 * kRowBytes) + (first_tile & 1 ? 0 : kTile) + (wave >> 1) * (2 * kTile);
   auto fetch_query = [&]() {
     const auto rs = make_rsrc(static_cast<const uint16_t*>(a.query) + a.row0_tok * a.q_tok_stride, 0x7FFFFFFFu);
@@ -177,25 +184,14 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
 #pragma unroll
     for (int m = 0; m < kS; ++m) {
       const u32x4 w = *reinterpret_cast<const u32x4*>(q_lds + col * kRowBytes + 16 * k_chunk<HD>(col, 2 * m + half));
-      if constexpr (KQ == 1) {
-        qf[0][m] = w ^ q_sign;
-      } else {  // fp16 = two bf16 pieces, exactly (8 + 3 significant bits)
-        u32x4 hi, lo;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = f16_to_f32(uint16_t(w[e])), y = f16_to_f32(uint16_t(w[e] >> 16));
-          hi[e] = pack_bf16(x, y);
-          lo[e] = pack_bf16(x - __uint_as_float(hi[e] << 16), y - __uint_as_float(hi[e] & 0xFFFF0000u));
-        }
-        qf[0][m] = hi ^ q_sign;
-        qf[1][m] = lo ^ q_sign;
-      }
+      qf[m] = w ^ q_sign;
     }
   };
 
   // ---- key tiles: two buffers of K and two of V; tile i in buffer i % 2 (offsets: they stay LDS addresses) ----
   auto k_buf = [&](int i) -> uint8_t* { return lds + (i & 1) * kTile; };
   auto v_buf = [&](int i) -> uint8_t* { return lds + 2 * kTile + (i & 1) * kTile; };
+  float* const k_scales = reinterpret_cast<float*>(lds + 4 * kTile);  // [2][kKeys], only for kRawKeys
   // Packed: rows past the sequence repeat its last one; no row sees them.
   auto fetch_packed = [&](int k, int i) {
     const int t0 = i * kKeys, last = min(kKeys, a.len - t0) - 1;
@@ -247,14 +243,20 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
       const bool ok = k == 0 || ((mask >> r) & 1u);
       asm("" : "+v"(h.codes[j]));  // whole words until here
       const float s = h.scale[j];
+      if (kRawKeys && k == 0 && lane % kCpr == 0) k_scales[(i & 1) * kKeys + r] = s;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         u32x4 w;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t x = h.codes[j][2 * q + e];
-          w[2 * e] = scaled_pair<FMT, false>(x, s);
-          w[2 * e + 1] = scaled_pair<FMT, true>(x, s);
+          if (kRawKeys && k == 0) {
+            w[2 * e] = code_pair<FMT, true, false>(x);
+            w[2 * e + 1] = code_pair<FMT, true, true>(x);
+          } else {
+            w[2 * e] = scaled_pair<FMT, false>(x, s);
+            w[2 * e + 1] = scaled_pair<FMT, true>(x, s);
+          }
         }
         if (!ok) w = u32x4{0u, 0u, 0u, 0u};  // its probability is 0: its value must not be anything but finite
         const int at = k == 0 ? k_chunk<HD>(r, c + q) : v_chunk<HD>(r, c + q);
@@ -280,18 +282,18 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
 #pragma unroll
       for (int m = 0; m < kS; ++m) {
         const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + (32 * kb + col) * kRowBytes + 16 * k_chunk<HD>(col, 2 * m + half));
-#pragma unroll
-        for (int p = 0; p < KQ; ++p) sc.s[kb] = Op<F16>::mfma(kf, qf[p][m], sc.s[kb]);
+        sc.s[kb] = Op<F16 || kRawKeys>::mfma(kf, qf[m], sc.s[kb]);
       }
     }
   };
   u32x4 pf[KP][4];
   auto probabilities = [&](const Scores& sc) {
+    const float shift = F16 ? kCut - mc : -mc;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float p[8];
 #pragma unroll
-      for (int v = 0; v < 8; ++v) p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc.s[i / 2][8 * (i % 2) + v], c2, -mc));
+      for (int v = 0; v < 8; ++v) p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc.s[i / 2][8 * (i % 2) + v], c2, shift));
       // The sum adds the probabilities as rounded (KP = 2: to 16 bits), so that a row's weights add up to one.
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -310,6 +312,16 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   auto step = [&](int i, uint64_t mask) {
     Scores sc;
     scores(sc, i);
+    if constexpr (kRawKeys) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 s = *reinterpret_cast<const f32x4*>(k_scales + (i & 1) * kKeys + 32 * kb + 8 * q + 4 * half);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc.s[kb][4 * q + r] *= s[r];
+        }
+    }
     const int t0 = i * kKeys;
     if constexpr (CAP) {
 #pragma unroll

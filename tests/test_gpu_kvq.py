@@ -280,11 +280,12 @@ def test_what_lies_behind_the_context_does_not_matter(q_len):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-def test_a_later_block_that_is_not_finite_leaves_earlier_queries_alone(fmt):
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_later_block_that_is_not_finite_leaves_earlier_queries_alone(fmt, dtype):
     """A chunk's last tokens are in a block marked NaN: queries before that block do not see it."""
     cache, table = _filled(1, 128, 16, 2, 64, FORMATS[fmt], seed=13)
     lens = torch.tensor([128], dtype=torch.int32, device="cuda")
-    q = torch.randn(1, 8, 100, 64, device="cuda").bfloat16()
+    q = torch.randn(1, 8, 100, 64, device="cuda").to(dtype)
     attention = PagedAttention(8, 2, 64)
     want = attention.forward(q, cache, 0, table, lens).clone()
     cache.value_scales[0, int(table[0, 7])] = float("nan")
