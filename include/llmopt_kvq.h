@@ -25,6 +25,11 @@ extern "C" {
 #define LLMOPT_KVQ_INT8 0
 #define LLMOPT_KVQ_E4M3 1
 
+/* The kernel of an attention call: chosen by a rule on the sizes, or one of them. */
+#define LLMOPT_KVQ_ALGO_AUTO 0
+#define LLMOPT_KVQ_ALGO_ROWS 1  /* 16 query rows per workgroup, keys from memory into registers */
+#define LLMOPT_KVQ_ALGO_TILES 2 /* 128 query rows per workgroup, keys in LDS; fp16 and bf16, 16-byte aligned rows */
+
 const char* llmopt_kvq_last_error(void);
 
 /*
@@ -53,7 +58,7 @@ int llmopt_kvq_write(void* key_codes, float* key_scales, void* value_codes, floa
 
 /* Bytes of workspace llmopt_kvq_attention uses to split the context (0: no split). */
 size_t llmopt_kvq_attention_workspace(int64_t num_seqs, int64_t num_heads, int64_t kv_heads, int64_t head_dim,
-                                      int64_t q_len, int64_t ldb, int64_t block_size, int q_dtype);
+                                      int64_t q_len, int64_t ldb, int64_t block_size, int q_dtype, int algo);
 
 /*
  * Attention of q_len query tokens per sequence over the cache, with the rules of llmopt_paged_attention_decode / _prefill
@@ -61,8 +66,9 @@ size_t llmopt_kvq_attention_workspace(int64_t num_seqs, int64_t num_heads, int64
  * t <= that position, t < context_lens[s], whose block id names a block; query head h reads KV head h / (num_heads /
  * kv_heads); zeros without keys; softcap > 0 applies tanh(x / softcap) * softcap to the scaled scores. query
  * element (s, h, j, d) at s * q_seq_stride + h * q_head_stride + j * q_tok_stride + d, out likewise with the o_*
- * strides, in q_dtype (F32, F16 or BF16). Supported: head_dim 64 or 128, any number of heads per KV head. With less workspace
- * than llmopt_kvq_attention_workspace asks for, the context is not split (correct, slower for few sequences).
+ * strides, in q_dtype (F32, F16 or BF16). Supported: head_dim 64 or 128, any number of heads per KV head, and for
+ * LLMOPT_KVQ_ALGO_TILES what it names; otherwise LLMOPT_ERR_UNSUPPORTED. With less workspace than
+ * llmopt_kvq_attention_workspace asks for, the context is not split (correct, slower for few sequences).
  */
 int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, int64_t q_head_stride,
                          int64_t q_tok_stride, const void* key_codes, const float* key_scales, const void* value_codes,
@@ -70,7 +76,7 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
                          int64_t kv_heads, int64_t head_dim, const int32_t* block_ids, int64_t ldb,
                          const int32_t* context_lens, int64_t num_seqs, int64_t num_heads, int64_t q_len, float scale,
                          float softcap, void* out, int64_t o_seq_stride, int64_t o_head_stride, int64_t o_tok_stride,
-                         void* workspace, size_t workspace_bytes, void* stream);
+                         int algo, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Causal attention over packed prompts: sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 of query

@@ -83,10 +83,12 @@ struct Plan {
 };
 
 Plan plan_attention(int64_t num_seqs, int64_t kv_heads, int64_t group, int64_t head_dim, int64_t q_len, int64_t ldb,
-                    int64_t block_size, int q_dtype, bool tile_rows) {
+                    int64_t block_size, int q_dtype, bool tile_rows, int algo) {
   const int64_t tiles = std::max<int64_t>(1, (ldb * block_size + 31) / 32), rows = group * q_len;
   const int64_t pairs = std::max<int64_t>(1, num_seqs * kv_heads * ((rows + 15) / 16));
-  bool tile = tile_rows && q_dtype != LLMOPT_DTYPE_F32 && rows > 32 && pairs * tiles * head_dim > 3600000;
+  const bool tile = algo == LLMOPT_KVQ_ALGO_TILES ||
+                    (algo == LLMOPT_KVQ_ALGO_AUTO && tile_rows && q_dtype != LLMOPT_DTYPE_F32 && rows > 32 &&
+                     pairs * tiles * head_dim > 3600000);
   if (tile) {
     const int64_t blocks = num_seqs * kv_heads * ((rows + 127) / 128);
     int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / blocks, tiles / 16, 16}));
@@ -157,11 +159,11 @@ int llmopt_kvq_write(void* key_codes, float* key_scales, void* value_codes, floa
 }
 
 size_t llmopt_kvq_attention_workspace(int64_t num_seqs, int64_t num_heads, int64_t kv_heads, int64_t head_dim,
-                                      int64_t q_len, int64_t ldb, int64_t block_size, int q_dtype) {
+                                      int64_t q_len, int64_t ldb, int64_t block_size, int q_dtype, int algo) {
   if (num_seqs <= 0 || num_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_len <= 0 || ldb <= 0 || block_size <= 0)
     return 0;
   if (num_heads % kv_heads != 0) return 0;
-  const Plan plan = plan_attention(num_seqs, kv_heads, num_heads / kv_heads, head_dim, q_len, ldb, block_size, q_dtype, true);
+  const Plan plan = plan_attention(num_seqs, kv_heads, num_heads / kv_heads, head_dim, q_len, ldb, block_size, q_dtype, true, algo);
   if (plan.splits <= 1) return 0;
   return size_t(plan.splits) * size_t(num_seqs) * size_t(num_heads) * size_t(q_len) * size_t(head_dim + 1) * sizeof(float);
 }
@@ -172,12 +174,14 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
                          int64_t kv_heads, int64_t head_dim, const int32_t* block_ids, int64_t ldb,
                          const int32_t* context_lens, int64_t num_seqs, int64_t num_heads, int64_t q_len, float scale,
                          float softcap, void* out, int64_t o_seq_stride, int64_t o_head_stride, int64_t o_tok_stride,
-                         void* workspace, size_t workspace_bytes, void* stream) {
+                         int algo, void* workspace, size_t workspace_bytes, void* stream) {
   llmopt::KvqAttnArgs a{};
   const int rc = describe_cache(a.c, key_codes, key_scales, value_codes, value_scales, format, num_blocks, block_size,
                                 kv_heads, head_dim, block_ids, ldb);
   if (rc != LLMOPT_OK) return rc;
   if (!valid_dtype(q_dtype)) return fail(LLMOPT_ERR_INVALID_ARG, "bad dtype code %d", q_dtype);
+  if (algo < LLMOPT_KVQ_ALGO_AUTO || algo > LLMOPT_KVQ_ALGO_TILES)
+    return fail(LLMOPT_ERR_INVALID_ARG, "bad algorithm code %d", algo);
   if (num_seqs < 0 || q_len < 0 || num_heads < 1 || num_heads % kv_heads != 0)
     return fail(LLMOPT_ERR_INVALID_ARG, "num_heads %lld must be a positive multiple of kv_heads %lld, sequences and "
                 "q_len not negative", (long long)num_heads, (long long)kv_heads);
@@ -211,7 +215,9 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
   a.q_vec = rows16(query, q_seq_stride, q_head_stride, q_tok_stride);
   const bool tile_rows = a.q_vec && near_rows(group, q_tok_stride, q_head_stride) &&
                          rows16(out, o_seq_stride, o_head_stride, o_tok_stride);
-  const Plan plan = plan_attention(num_seqs, kv_heads, group, head_dim, q_len, ldb, block_size, q_dtype, tile_rows);
+  if (algo == LLMOPT_KVQ_ALGO_TILES && (q_dtype == LLMOPT_DTYPE_F32 || !tile_rows))
+    return fail(LLMOPT_ERR_UNSUPPORTED, "the tile kernel takes fp16 and bf16 rows aligned to 16 bytes");
+  const Plan plan = plan_attention(num_seqs, kv_heads, group, head_dim, q_len, ldb, block_size, q_dtype, tile_rows, algo);
   a.waves = plan.waves;
   a.splits = plan.splits;
   a.tiles_per_split = plan.tiles_per_split;

@@ -6,7 +6,8 @@
 //
 // Why: at one token the kernel takes 4.8 us, and the same steps in Python (attribute look-ups, checks,
 // two ctypes calls) held a 4096 x 4096 call at 18.9 us; 6.9 us with this path. An append to the 8-bit cache, a decode
-// step's attention over it and a short packed prompt: KVQ_FIGURES.
+// step's attention over it and a short packed prompt: 28 / 36 / 17 us in Python, 8.8 / 13.6 / 7.3 here, the kernels 4.2 /
+// 9.7 / 8.0 (calls in a row overlap).
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -130,11 +131,11 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
 using KvqWriteFn = int (*)(void*, float*, void*, float*, int, int64_t, int64_t, int64_t, int64_t, const int32_t*, int64_t,
                            const int32_t*, const int32_t*, const int32_t*, const void*, int64_t, int64_t, int64_t,
                            const void*, int64_t, int64_t, int64_t, int, int64_t, int64_t, int64_t, void*);
-using KvqWorkspaceFn = size_t (*)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int);
+using KvqWorkspaceFn = size_t (*)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int, int);
 using KvqAttentionFn = int (*)(const void*, int, int64_t, int64_t, int64_t, const void*, const float*, const void*,
                                const float*, int, int64_t, int64_t, int64_t, int64_t, const int32_t*, int64_t,
                                const int32_t*, int64_t, int64_t, int64_t, float, float, void*, int64_t, int64_t, int64_t,
-                               void*, size_t, void*);
+                               int, void*, size_t, void*);
 using PackedFn = int (*)(const void*, int64_t, int64_t, const void*, int64_t, int64_t, const void*, int64_t, int64_t, int,
                          const int32_t*, int64_t, int64_t, int64_t, int64_t, int64_t, float, float, void*, int64_t,
                          int64_t, int, void*);
@@ -288,7 +289,7 @@ PyObject* kvq_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (dtype && q_len > 1 && (reinterpret_cast<uintptr_t>(qp) % 16 || q->stride(0) % 8 || q->stride(1) % 8 || q->stride(2) % 8))
     Py_RETURN_NONE;
   const int64_t ldb = table->size(1), d = c.head_dim;
-  const size_t ws_bytes = g_kvq.workspace(seqs, heads, c.heads, d, q_len, ldb, c.block_size, dtype);
+  const size_t ws_bytes = g_kvq.workspace(seqs, heads, c.heads, d, q_len, ldb, c.block_size, dtype, 0);
   const auto options = at::TensorOptions().device(c.device);
   at::Tensor ws;
   at::Tensor out = at::empty_strided({seqs, heads, q_len, d}, {q_len * heads * d, d, heads * d, 1}, options.dtype(q->scalar_type()));
@@ -303,7 +304,7 @@ PyObject* kvq_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     pybind11::gil_scoped_release released;
     rc = g_kvq.attention(qp, dtype, q0, q1, q2, c.codes[0], c.scales[0], c.codes[1], c.scales[1], c.format, c.blocks,
                          c.block_size, c.heads, d, tp, ldb, lp, seqs, heads, q_len, float(scale), float(softcap), op,
-                         q_len * heads * d, d, heads * d, wp, ws_bytes, stream);
+                         q_len * heads * d, d, heads * d, 0, wp, ws_bytes, stream);
   }
   if (rc != 0) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));

@@ -42,6 +42,10 @@ ALGO_DECODE = 2
 ALGO_PREFILL = 3
 ALGO_DENSE = 4
 
+KVQ_ALGO_AUTO = 0
+KVQ_ALGO_ROWS = 1
+KVQ_ALGO_TILES = 2
+
 ERR_INVALID_ARG = -1
 ERR_UNSUPPORTED = -2
 
@@ -141,11 +145,11 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64,
          _i64, _int, _i64, _i64, _i64, _p],
     ),
-    "llmopt_kvq_attention_workspace": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "llmopt_kvq_attention_workspace": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int]),
     "llmopt_kvq_attention": (
         _int,
         [_p, _int, _i64, _i64, _i64, _p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64,
-         ctypes.c_float, ctypes.c_float, _p, _i64, _i64, _i64, _p, _size, _p],
+         ctypes.c_float, ctypes.c_float, _p, _i64, _i64, _i64, _int, _p, _size, _p],
     ),
     "llmopt_packed_attention": (
         _int,

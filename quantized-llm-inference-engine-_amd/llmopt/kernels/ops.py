@@ -28,7 +28,8 @@ import ctypes
 
 import torch
 
-from llmopt.kernels._lib import ALGO_AUTO, ALGO_DENSE, DTYPE_CODES, KVQ_FORMATS, call, load_binding, load_library
+from llmopt.kernels._lib import (ALGO_AUTO, ALGO_DENSE, DTYPE_CODES, KVQ_ALGO_AUTO, KVQ_ALGO_ROWS, KVQ_FORMATS, call,
+                                 load_binding, load_library)
 
 __all__ = [
     "dequantize",
@@ -763,11 +764,12 @@ def cache_attention(query: torch.Tensor, cache, layer_idx: int, block_ids: torch
 
 def kvq_attention(query: torch.Tensor, key_codes: torch.Tensor, key_scales: torch.Tensor, value_codes: torch.Tensor,
                   value_scales: torch.Tensor, block_ids: torch.Tensor, context_lens: torch.Tensor, scale: float,
-                  softcap: float = 0.0) -> torch.Tensor:
+                  softcap: float = 0.0, algo: int = KVQ_ALGO_AUTO) -> torch.Tensor:
     """Attention of ``query [seq, heads, q_len, head_dim]`` (fp32 / fp16 / bf16, any strides with a unit inner one) over
     one layer of an 8-bit cache, read in place: query token j sits at ``context_lens - q_len + j`` and sees the keys up
     to its own position. Returns ``[seq, heads, q_len, head_dim]`` in the query's dtype, a view of a ``[seq, q_len,
-    heads, head_dim]`` buffer. Raises ``NotImplementedError`` for head dims other than 64 and 128."""
+    heads, head_dim]`` buffer. ``algo``: the kernel, by default chosen by the sizes (``include/llmopt_kvq.h``). Raises
+    ``NotImplementedError`` for head dims other than 64 and 128."""
     nb, bs, kvh, hd, fmt = _kvq_cache(key_codes, key_scales, value_codes, value_scales)
     if query.dim() != 4 or int(query.shape[3]) != hd:
         raise ValueError(f"query of shape {tuple(query.shape)} does not match head_dim {hd}")
@@ -785,20 +787,20 @@ def kvq_attention(query: torch.Tensor, key_codes: torch.Tensor, key_scales: torc
         return view
     dt = DTYPE_CODES[query.dtype]
     q = query if query.stride(3) == 1 else query.contiguous()
-    if dt and q_len > 1 and (q.data_ptr() % 16 or any(st % 8 for st in q.stride()[:3])):
+    if dt and (q_len > 1 or algo) and algo != KVQ_ALGO_ROWS and (q.data_ptr() % 16 or any(st % 8 for st in q.stride()[:3])):
         q = q.clone(memory_format=torch.contiguous_format)  # the chunk kernel reads whole 16-byte pieces
     table, lens = _int32(block_ids, dev), _int32(context_lens.reshape(-1), dev)
     ldb = int(table.shape[1])
     lib = load_library()
     with _launching_on(dev):
-        ws_bytes = lib.llmopt_kvq_attention_workspace(seqs, heads, kvh, hd, q_len, ldb, bs, dt)
+        ws_bytes = lib.llmopt_kvq_attention_workspace(seqs, heads, kvh, hd, q_len, ldb, bs, dt, int(algo))
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         call(
             lib.llmopt_kvq_attention(
                 q.data_ptr(), dt, q.stride(0), q.stride(1), q.stride(2), key_codes.data_ptr(), key_scales.data_ptr(),
                 value_codes.data_ptr(), value_scales.data_ptr(), fmt, nb, bs, kvh, hd, table.data_ptr(), ldb,
                 lens.data_ptr(), seqs, heads, q_len, float(scale), float(softcap), out.data_ptr(), q_len * heads * hd,
-                hd, heads * hd, None if ws is None else ws.data_ptr(), ws_bytes, _stream_handle(dev),
+                hd, heads * hd, int(algo), None if ws is None else ws.data_ptr(), ws_bytes, _stream_handle(dev),
             ),
             "llmopt_kvq_attention",
         )

@@ -15,6 +15,7 @@ import torch
 from llmopt.attention import PagedAttention, PagedAttentionConfig
 from llmopt.cache import PagedKVCache, QuantizedPagedKVCache
 from llmopt.kernels import ops
+from llmopt.kernels._lib import KVQ_ALGO_ROWS, KVQ_ALGO_TILES
 from llmopt.model import GreedyGenerator, ModelConfig, random_quantized_model
 from oracle import kvq_oracle as ko
 
@@ -157,14 +158,14 @@ def _filled(seqs, longest, block, kvh, hd, dtype, seed, spread=1.0):
     return QuantizedPagedKVCache.from_tensors(*parts), table
 
 
-def _check(out, q, cache, table, lens, scale, softcap=0.0):
-    """`out` against the oracle over what the cache holds, within the bounds of this module's docstring."""
+def _check(outs, q, cache, table, lens, scale, softcap=0.0):
+    """Each of `outs` against the oracle over what the cache holds, within the bounds of this module's docstring."""
     seqs, heads, q_len, hd = q.shape
     group = heads // cache.num_kv_heads
     keys, values, valid = (t.cpu() for t in cache.gather(0, table, lens))
     u, step = HALF_P[q.dtype], torch.finfo(q.dtype).eps / 2
-    got = out.double().cpu().numpy()
-    assert np.isfinite(got).all()
+    outs = [out.double().cpu().numpy() for out in outs]
+    assert all(np.isfinite(got).all() for got in outs)
     for s in range(seqs):
         ctx = int(lens[s])
         t = np.arange(keys.shape[1])
@@ -176,8 +177,20 @@ def _check(out, q, cache, table, lens, scale, softcap=0.0):
             bound = 2 * (u + fp32) * spread + step * np.abs(want) + 1e-30
             if q.dtype == torch.float16:
                 bound = bound + 2.0**-25  # half a step of the smallest fp16 numbers
-            worst = np.max(np.abs(got[s, h] - want) / bound)
-            assert worst <= 1.0, (s, h, worst)
+            for i, got in enumerate(outs):
+                worst = np.max(np.abs(got[s, h] - want) / bound)
+                assert worst <= 1.0, (i, s, h, worst)
+
+
+def _each(q, cache, table, lens, scale, softcap=0.0):
+    """The attention by PagedAttention and by every kernel that takes the query: [(output)]."""
+    attention = PagedAttention(q.shape[1], cache.num_kv_heads, q.shape[3], scale=scale, config=PagedAttentionConfig(softcap=softcap))
+    outs = [attention.forward(q, cache, 0, table, lens)]
+    for algo in (KVQ_ALGO_ROWS, KVQ_ALGO_TILES)[: 1 if q.dtype == torch.float32 else 2]:
+        outs.append(ops.kvq_attention(q, *cache.layer(0), table, lens, scale, softcap, algo))
+    for out in outs:
+        assert out.dtype == q.dtype and out.shape == q.shape
+    return outs
 
 
 SHAPES = [  # seqs, heads, kv_heads, head_dim, block, lengths
@@ -200,9 +213,7 @@ def test_decode_attention(fmt, dtype, shape):
     cache, table = _filled(seqs, max(lens), block, kvh, hd, FORMATS[fmt], seed=hd + block)
     lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
     q = torch.randn(seqs, heads, 1, hd, device="cuda").to(dtype)
-    out = PagedAttention(heads, kvh, hd).forward(q, cache, 0, table, lens)
-    assert out.dtype == dtype and out.shape == q.shape
-    _check(out, q, cache, table, lens, hd**-0.5)
+    _check(_each(q, cache, table, lens, hd**-0.5), q, cache, table, lens, hd**-0.5)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -217,9 +228,24 @@ def test_chunk_attention(fmt, dtype, q_len, shape):
     # token-major rows of a wider tensor: strides that are not contiguous
     wide = torch.randn(seqs, q_len, heads + 1, hd, device="cuda").to(dtype)
     q = wide[:, :, :heads].permute(0, 2, 1, 3)
-    out = PagedAttention(heads, kvh, hd).forward(q, cache, 0, table, lens)
-    assert out.dtype == dtype and out.shape == q.shape
-    _check(out, q, cache, table, lens, hd**-0.5)
+    _check(_each(q, cache, table, lens, hd**-0.5), q, cache, table, lens, hd**-0.5)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("seqs,heads,kvh,hd,block,q_len,longest", [(4, 32, 8, 128, 16, 200, 900), (1, 32, 8, 128, 16, 300, 3000),
+                                                                  (2, 24, 8, 64, 48, 700, 2500), (3, 5, 5, 128, 7, 1100, 1500)])
+def test_chunks_that_the_rule_gives_to_the_tile_kernel(fmt, dtype, seqs, heads, kvh, hd, block, q_len, longest):
+    """Whole and split over the keys; the same numbers as when the kernel is asked for."""
+    cache, table = _filled(seqs, longest, block, kvh, hd, FORMATS[fmt], seed=q_len)
+    lens = torch.tensor([longest - 31 * s for s in range(seqs)], dtype=torch.int32, device="cuda")
+    q = torch.randn(seqs, q_len, heads, hd, device="cuda").to(dtype).permute(0, 2, 1, 3)
+    auto, _, tiles = _each(q, cache, table, lens, hd**-0.5)
+    assert torch.equal(auto, tiles)
+    some = torch.tensor([0, heads // kvh], device="cuda")  # a head of the first and of the second KV head
+    part = QuantizedPagedKVCache.from_tensors(*(t[:, :, :2].contiguous() for t in (cache.key_codes, cache.key_scales, cache.value_codes,
+                                                                                  cache.value_scales)))
+    _check([auto[:, some]], q[:, some], part, table, lens, hd**-0.5)
 
 
 @pytest.mark.parametrize("q_len", [1, 3, 70])
@@ -229,11 +255,12 @@ def test_rows_without_keys_and_missing_blocks(q_len):
     table[0, 1], table[1, 0], table[2, :], table[3, 2] = -1, -1, -1, 10**6
     lens = torch.tensor([100, 100, 100, 100, 0, max(0, q_len - 2)], dtype=torch.int32, device="cuda")
     q = torch.randn(6, heads, q_len, hd, device="cuda").bfloat16()
-    out = PagedAttention(heads, kvh, hd).forward(q, cache, 0, table, lens)
-    _check(out, q, cache, table, lens, hd**-0.5)
-    assert not bool(out[2].any()) and not bool(out[4].any())
-    if q_len > 2:
-        assert not bool(out[5, :, :2].any()) and bool(out[5, :, 2:].any())
+    outs = _each(q, cache, table, lens, hd**-0.5)
+    _check(outs, q, cache, table, lens, hd**-0.5)
+    for out in outs:
+        assert not bool(out[2].any()) and not bool(out[4].any())
+        if q_len > 2:
+            assert not bool(out[5, :, :2].any()) and bool(out[5, :, 2:].any())
 
 
 @pytest.mark.parametrize("q_len", [1, 4, 80])
@@ -242,8 +269,8 @@ def test_scale_and_softcap(q_len, scale, softcap):
     cache, table = _filled(2, 150, 16, 2, 128, torch.float8_e4m3fn, seed=6, spread=0.5)
     lens = torch.tensor([150, 81], dtype=torch.int32, device="cuda")
     q = torch.randn(2, 4, q_len, 128, device="cuda").bfloat16()
-    attention = PagedAttention(4, 2, 128, scale=scale, config=PagedAttentionConfig(softcap=softcap))
-    _check(attention.forward(q, cache, 0, table, lens), q, cache, table, lens, scale, softcap)
+    for dtype in (torch.bfloat16, torch.float16):
+        _check(_each(q.to(dtype), cache, table, lens, scale, softcap), q.to(dtype), cache, table, lens, scale, softcap)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -256,7 +283,7 @@ def test_scales_far_apart(fmt, dtype, q_len):
     cache.value_scales[0, table[0].long()] = 2.0**-30  # a sequence of nothing but small values
     lens = torch.tensor([300, 290], dtype=torch.int32, device="cuda")
     q = torch.randn(2, 8, q_len, 64, device="cuda").to(dtype)
-    _check(PagedAttention(8, 2, 64).forward(q, cache, 0, table, lens), q, cache, table, lens, 0.125)
+    _check(_each(q, cache, table, lens, 0.125), q, cache, table, lens, 0.125)
 
 
 @pytest.mark.parametrize("q_len", [1, 6, 70])
@@ -264,8 +291,7 @@ def test_what_lies_behind_the_context_does_not_matter(q_len):
     cache, table = _filled(3, 200, 16, 2, 128, torch.float8_e4m3fn, seed=12)
     lens = torch.tensor([100, 97, 128], dtype=torch.int32, device="cuda")
     q = torch.randn(3, 8, q_len, 128, device="cuda").bfloat16()
-    attention = PagedAttention(8, 2, 128)
-    want = attention.forward(q, cache, 0, table, lens).clone()
+    want = _each(q, cache, table, lens, 0.1)
     for s in range(3):
         first = -(-int(lens[s]) // 16)
         later = table[s, first:].long()
@@ -276,7 +302,8 @@ def test_what_lies_behind_the_context_does_not_matter(q_len):
             codes.view(torch.uint8)[0, later] = 0x7F
             if slot:
                 codes.view(torch.uint8)[0, block, :, slot:] = 0x7F  # NaN codes of another request
-    assert torch.equal(attention.forward(q, cache, 0, table, lens), want)
+    for a, b in zip(_each(q, cache, table, lens, 0.1), want):
+        assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -286,13 +313,16 @@ def test_a_later_block_that_is_not_finite_leaves_earlier_queries_alone(fmt, dtyp
     cache, table = _filled(1, 128, 16, 2, 64, FORMATS[fmt], seed=13)
     lens = torch.tensor([128], dtype=torch.int32, device="cuda")
     q = torch.randn(1, 8, 100, 64, device="cuda").to(dtype)
-    attention = PagedAttention(8, 2, 64)
-    want = attention.forward(q, cache, 0, table, lens).clone()
+    want = _each(q, cache, table, lens, 0.125)
     cache.value_scales[0, int(table[0, 7])] = float("nan")
-    got = attention.forward(q, cache, 0, table, lens)
-    assert bool(got[:, :, 84:].isnan().all()) and bool(got[:, :, :84].isfinite().all())
-    # Recomputed key by key without the probabilities' rounding to bf16.
-    assert float((got[:, :, :84] - want[:, :, :84]).abs().max()) <= 4 * 2.0**-8 * float(want[:, :, :84].abs().max())
+    for got, was in zip(_each(q, cache, table, lens, 0.125), want):
+        assert bool(got[:, :, 84:].isnan().all()) and bool(got[:, :, :84].isfinite().all())
+        # Where they are computed once more, key by key, it is without the probabilities' rounding to bf16.
+        assert float((got[:, :, :84] - was[:, :, :84]).abs().max()) <= 4 * 2.0**-8 * float(was[:, :, :84].abs().max())
+    cache.value_scales[0, int(table[0, 7])] = 1.0
+    cache.key_scales[0, int(table[0, 7])] = float("nan")
+    for got, was in zip(_each(q, cache, table, lens, 0.125), want):
+        assert not bool(got[:, :, 84:].any()) and torch.equal(got[:, :, :84], was[:, :, :84])  # no sum: zeros
 
 
 def test_decode_without_a_workspace_and_at_every_split():
@@ -305,7 +335,7 @@ def test_decode_without_a_workspace_and_at_every_split():
         q = torch.randn(seqs, heads, 1, hd, device="cuda").bfloat16()
         out = PagedAttention(heads, kvh, hd).forward(q, cache, 0, table, lens)
         some = torch.unique(torch.cat([torch.tensor([0, seqs - 1]), torch.randint(0, seqs, (2,))])).cuda()
-        _check(out[some], q[some], cache, table[some], lens[some], hd**-0.5)
+        _check([out[some]], q[some], cache, table[some], lens[some], hd**-0.5)
 
 
 def test_a_cache_past_32_bits():
@@ -328,7 +358,7 @@ def test_a_cache_past_32_bits():
         assert torch.equal(a.cpu(), b)
     for q_len in (1, 40):
         q = torch.randn(1, 32, q_len, hd, device="cuda").bfloat16()
-        _check(PagedAttention(32, kvh, hd).forward(q, cache, 0, table, lens.cuda()), q, cache, table, lens, hd**-0.5)
+        _check(_each(q, cache, table, lens.cuda(), hd**-0.5), q, cache, table, lens, hd**-0.5)
 
 
 # ---- as it is used ---------------------------------------------------------------------------------
@@ -421,7 +451,7 @@ def test_other_head_dims_take_the_torch_sequence():
     q = torch.randn(2, 4, 3, 96, device="cuda")
     with pytest.raises(NotImplementedError):
         ops.kvq_attention(q, *cache.layer(0), table, lens, 0.1)
-    _check(PagedAttention(4, 2, 96).forward(q, cache, 0, table, lens), q, cache, table, lens, 96**-0.5)
+    _check([PagedAttention(4, 2, 96).forward(q, cache, 0, table, lens)], q, cache, table, lens, 96**-0.5)
 
 
 def test_refusals_on_the_device():

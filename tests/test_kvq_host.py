@@ -293,11 +293,12 @@ def test_c_entry_points_validate_on_the_host():
     assert kv(nb=1 << 28) == -2 and kv(ldb=1 << 27) == -2 and kv(seqs=1 << 30) == -2 and kv(q=1 << 31) == -2
     assert kv(seqs=0) == 0 and kv(q=0) == 0 and kv(ldb=0) == 0  # nothing to write: no launch
 
-    def at(fmt=0, hd=64, kvh=2, heads=4, seqs=1, q=1, dt=2, ptr=16, codes=16):
-        return attend(ptr, dt, 0, 0, 0, codes, ptr, codes, ptr, fmt, 4, 16, kvh, hd, ptr, 1, ptr, seqs, heads, q, 1.0, 0.0, ptr, 0, 0, 0, None, 0, None)
+    def at(fmt=0, hd=64, kvh=2, heads=4, seqs=1, q=1, dt=2, ptr=16, codes=16, algo=0, stride=0):
+        return attend(ptr, dt, stride, 0, 0, codes, ptr, codes, ptr, fmt, 4, 16, kvh, hd, ptr, 1, ptr, seqs, heads, q, 1.0, 0.0, ptr, 0, 0, 0, algo, None, 0, None)
 
     assert at(fmt=5) == -1 and at(dt=9) == -1 and at(heads=3) == -1 and at(heads=0) == -1 and at(seqs=-1) == -1 and at(ptr=None) == -1
     assert at(hd=96) == -2 and at(seqs=65536) == -2 and at(q=1 << 30) == -2 and at(codes=24) == -2
+    assert at(algo=3) == -1 and at(algo=-1) == -1 and at(algo=2, dt=0) == -2 and at(algo=2, stride=4) == -2
     assert at(seqs=0) == 0 and at(q=0) == 0
 
     def pk(dt=2, seqs=1, tokens=4, heads=4, kvh=2, hd=64, ptr=16, stride=64):
@@ -306,7 +307,7 @@ def test_c_entry_points_validate_on_the_host():
     assert pk(dt=7) == -1 and pk(seqs=-1) == -1 and pk(tokens=-1) == -1 and pk(heads=3) == -1 and pk(ptr=None) == -1
     assert pk(dt=0) == -2 and pk(hd=80) == -2 and pk(ptr=8) == -2 and pk(stride=65) == -2 and pk(stride=1 << 25) == -2 and pk(tokens=1 << 30) == -2
     assert pk(tokens=0) == 0
-    assert lib.llmopt_kvq_attention_workspace(1, 32, 8, 128, 1, 512, 16, 2) > 0
-    assert lib.llmopt_kvq_attention_workspace(1, 32, 7, 128, 1, 512, 16, 2) == 0 and lib.llmopt_kvq_attention_workspace(0, 32, 8, 128, 1, 512, 16, 2) == 0
+    assert lib.llmopt_kvq_attention_workspace(1, 32, 8, 128, 1, 512, 16, 2, 0) > 0
+    assert lib.llmopt_kvq_attention_workspace(1, 32, 7, 128, 1, 512, 16, 2, 0) == 0 and lib.llmopt_kvq_attention_workspace(0, 32, 8, 128, 1, 512, 16, 2, 0) == 0
     with pytest.raises(NotImplementedError, match="16-byte"):
         _lib.call(at(codes=24), "llmopt_kvq_attention")
