@@ -191,8 +191,7 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
   if (!query || !key_codes || !value_codes || !key_scales || !value_scales || !block_ids || !context_lens || !out)
     return fail(LLMOPT_ERR_INVALID_ARG, "null pointer argument");
   const int64_t group = num_heads / kv_heads;
-  if (num_seqs > 65535 || q_len > kMaxInt / 4 || group * q_len > kMaxInt / 4 ||
-      kv_heads * ((group * q_len + 15) / 16) > 65535)
+  if (num_seqs > 65535 || q_len > kMaxInt / 4 || group * q_len > kMaxInt / 4)
     return fail(LLMOPT_ERR_UNSUPPORTED, "batch of %lld sequences x %lld tokens too large for one launch",
                 (long long)num_seqs, (long long)q_len);
   if (!aligned(key_codes, 16) || !aligned(value_codes, 16))
@@ -218,6 +217,10 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
   if (algo == LLMOPT_KVQ_ALGO_TILES && (q_dtype == LLMOPT_DTYPE_F32 || !tile_rows))
     return fail(LLMOPT_ERR_UNSUPPORTED, "the tile kernel takes fp16 and bf16 rows aligned to 16 bytes");
   const Plan plan = plan_attention(num_seqs, kv_heads, group, head_dim, q_len, ldb, block_size, q_dtype, tile_rows, algo);
+  const int64_t blocks = kv_heads * ((group * q_len + (plan.tile ? 127 : 15)) / (plan.tile ? 128 : 16));
+  if (plan.tile ? blocks > kMaxInt / num_seqs : blocks > 65535)
+    return fail(LLMOPT_ERR_UNSUPPORTED, "batch of %lld sequences x %lld tokens too large for one launch",
+                (long long)num_seqs, (long long)q_len);
   a.waves = plan.waves;
   a.splits = plan.splits;
   a.tiles_per_split = plan.tiles_per_split;

@@ -9,7 +9,7 @@ namespace {
 using namespace tile;
 
 template <bool F16, int HD, int W, bool CAP>
-__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : 4, HD == 128 ? 2 : 4)))
+__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : CAP ? 3 : 4, HD == 128 ? 2 : CAP ? 3 : 4)))
     packed_attention_kernel(const PackedAttnArgs a) {
   constexpr int kRows = 32 * W;
   __shared__ __align__(16) uint8_t lds[4 * kKeys * HD * 2];

@@ -15,6 +15,7 @@ GPU time of its kernels and not their host launch overhead.
 from __future__ import annotations
 
 import time
+from collections.abc import Sequence
 from dataclasses import dataclass
 
 import torch
@@ -48,7 +49,8 @@ def _argmax(logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tens
 
 
 class GreedyGenerator:
-    """Greedy decoding of a batch of equal-length prompts with ``model``.
+    """Greedy decoding of a batch of prompts with ``model``: of equal length, or over an 8-bit cache of any
+    lengths, which are prefilled packed.
 
     Args:
         model: a :class:`DecoderOnlyModel` (any device).
@@ -72,28 +74,45 @@ class GreedyGenerator:
             torch.cuda.synchronize(self.device)
 
     @torch.no_grad()
-    def generate(self, prompts: torch.Tensor, steps: int, forced: torch.Tensor | None = None) -> GenerationResult:
-        """Generate ``steps`` tokens per prompt (``prompts [seq, prompt_len]``). With ``forced
-        [seq, steps]`` the step inputs are those tokens instead of the argmax (teacher forcing);
+    def generate(self, prompts: torch.Tensor | Sequence[torch.Tensor], steps: int,
+                 forced: torch.Tensor | None = None) -> GenerationResult:
+        """Generate ``steps`` tokens per prompt (``prompts [seq, prompt_len]``, or a list of prompts ``[n]``
+        of any lengths from 1, for a ``cache_dtype`` of 8 bits). With ``forced [seq, steps]`` the step inputs are those tokens instead of the argmax (teacher forcing);
         ``tokens`` then still holds the argmax of every step."""
         if steps < 1:
             raise ValueError("steps must be >= 1")
         dev = self.device
-        seqs, plen = int(prompts.shape[0]), int(prompts.shape[1])
+        ragged = not isinstance(prompts, torch.Tensor)
+        if ragged:
+            if not prompts or any(p.dim() != 1 or p.shape[0] < 1 for p in prompts):
+                raise ValueError("a list of prompts needs one-dimensional ones of at least one token")
+            lengths = [int(p.shape[0]) for p in prompts]
+            seqs, plen = len(lengths), max(lengths)
+        else:
+            seqs, plen = int(prompts.shape[0]), int(prompts.shape[1])
         per_seq = -(-(plen + steps) // self.block_size)
         cache = self.model.allocate_cache(seqs * per_seq, self.block_size, self.cache_dtype, dev)
         table = torch.arange(seqs * per_seq, dtype=torch.int32, device=dev).view(seqs, per_seq)
         out = torch.empty(seqs, steps, dtype=torch.long, device=dev)
 
         # ---- prefill ----
-        ids = prompts.to(dev).reshape(-1)
-        pos = torch.arange(plen, device=dev).repeat(seqs)
-        lens = torch.full((seqs,), plen, dtype=torch.int32, device=dev)
+        offsets = torch.zeros(seqs, dtype=torch.int32, device=dev)
+        if ragged:
+            ids = torch.cat([p.to(dev) for p in prompts])
+            pos = torch.cat([torch.arange(n, device=dev) for n in lengths])
+            lens = torch.tensor(lengths, dtype=torch.int32, device=dev)
+            cu = torch.zeros(seqs + 1, dtype=torch.int32, device=dev)
+            cu[1:] = torch.cumsum(lens, 0)
+            shape = {"cu_seqlens": cu}
+        else:
+            ids = prompts.to(dev).reshape(-1)
+            pos = torch.arange(plen, device=dev).repeat(seqs)
+            lens = torch.full((seqs,), plen, dtype=torch.int32, device=dev)
+            shape = {"q_len": plen}
         self._sync()
         t0 = time.perf_counter()
-        logits = self.model(ids, pos, cache=cache, block_ids=table, context_lens=lens,
-                            token_offsets=torch.zeros(seqs, dtype=torch.int32, device=dev), q_len=plen,
-                            last_only=True).last_logits()
+        logits = self.model(ids, pos, cache=cache, block_ids=table, context_lens=lens, token_offsets=offsets,
+                            last_only=True, **shape).last_logits()
         out[:, 0] = _argmax(logits)
         self._sync()
         prefill_s = time.perf_counter() - t0
@@ -101,8 +120,8 @@ class GreedyGenerator:
 
         # ---- decode: static buffers advanced in place ----
         tok = (forced[:, 0].to(dev) if forced is not None else out[:, 0]).contiguous().clone()
-        pos = torch.full((seqs,), plen, dtype=torch.long, device=dev)
-        lens = torch.full((seqs,), plen + 1, dtype=torch.int32, device=dev)
+        pos = lens.to(torch.long)
+        lens = lens + 1
         nxt = torch.empty(seqs, dtype=torch.long, device=dev)
 
         # Without teacher forcing the step's argmax is the next step's input: written straight

@@ -17,6 +17,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from llmopt.attention.packed_attention import PackedAttention
 from llmopt.attention.paged_attention import PagedAttention, PagedAttentionConfig
 from llmopt.model.rotary import RotaryEmbedding, apply_rotary_pos_emb
 from llmopt.quantization.fused import FusedQuantLinear, QuantSwiGLU
@@ -109,6 +110,11 @@ class PagedAttentionLayer(nn.Module):
     K/V at ``token_offsets`` (default ``context_lens - q_len``), attends over the cached context
     and projects the result. Without a cache, each sequence attends causally over its own
     ``q_len`` tokens.
+
+    With ``cu_seqlens [seq + 1]`` the rows are whole prompts of different lengths, packed one after the other
+    (:class:`PackedAttention`): each attends causally over its own keys and values as they are computed, which go
+    into the cache, if there is one, from ``token_offsets`` (default 0); the cache is a
+    :class:`llmopt.cache.QuantizedPagedKVCache`, and ``context_lens`` and ``q_len`` are not used.
     """
 
     def __init__(self, config: object, layer_idx: int, backend: str = "auto") -> None:
@@ -128,6 +134,7 @@ class PagedAttentionLayer(nn.Module):
         self.fused_ops = True  # False: the torch rotary sequence even on HIP devices
         self.attn = PagedAttention(self.num_heads, self.num_kv_heads, self.head_dim,
                                    config=PagedAttentionConfig(block_size=16), backend=backend)
+        self.packed = PackedAttention(self.num_heads, self.num_kv_heads, self.head_dim)
 
     def fuse_qkv(self) -> bool:
         """Merge quantized q, k and v projections into one :class:`FusedQuantLinear`."""
@@ -156,7 +163,10 @@ class PagedAttentionLayer(nn.Module):
 
     def forward(self, hidden: torch.Tensor, positions: torch.Tensor, cache: object | None = None,
                 block_ids: torch.Tensor | None = None, context_lens: torch.Tensor | None = None,
-                token_offsets: torch.Tensor | None = None, q_len: int = 1) -> torch.Tensor:
+                token_offsets: torch.Tensor | None = None, q_len: int = 1,
+                cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
+        if cu_seqlens is not None:
+            return self._packed_forward(hidden, positions, cache, block_ids, token_offsets, cu_seqlens)
         total = int(hidden.shape[0])
         seqs = total // max(1, q_len)
         q, k, v = self._project(hidden)
@@ -226,6 +236,32 @@ class PagedAttentionLayer(nn.Module):
         out = out.permute(0, 2, 1, 3).reshape(total, self.num_heads * self.head_dim)
         return self.o_proj(out)
 
+    def _packed_forward(self, hidden: torch.Tensor, positions: torch.Tensor, cache: object | None,
+                        block_ids: torch.Tensor | None, token_offsets: torch.Tensor | None,
+                        cu_seqlens: torch.Tensor) -> torch.Tensor:
+        """Packed prompts (see the class): ``hidden [tokens, hidden]``, ``positions [tokens]``."""
+        total = int(hidden.shape[0])
+        q, k, v = self._project(hidden)
+        q = q.reshape(total, self.num_heads, self.head_dim)
+        k = k.reshape(total, self.num_kv_heads, self.head_dim)
+        v = v.reshape(total, self.num_kv_heads, self.head_dim)
+        if self.fused_ops and _hip(q):
+            from llmopt.kernels import ops
+
+            self.rotary.check(positions)
+            q, k = ops.rope(q, k, positions, self.rotary.cos_cached, self.rotary.sin_cached)
+        else:
+            cos, sin = self.rotary(positions, dtype=q.dtype)
+            q, k = apply_rotary_pos_emb(q, k, cos.view(total, 1, self.head_dim), sin.view(total, 1, self.head_dim))
+        if cache is not None and block_ids is not None:
+            if not hasattr(cache, "write_packed"):
+                raise TypeError(f"packed prompts need a QuantizedPagedKVCache, not a {type(cache).__name__}")
+            if token_offsets is None:
+                token_offsets = torch.zeros(int(cu_seqlens.shape[0]) - 1, dtype=torch.int32, device=q.device)
+            cache.write_packed(self.layer_idx, block_ids, token_offsets, cu_seqlens, k, v)
+        out = self.packed.forward(q, k, v, cu_seqlens)
+        return self.o_proj(out.reshape(total, self.num_heads * self.head_dim))
+
     def _causal_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """Cache-free path: ``[seq, heads, q_len, d]`` attending causally over its own tokens
         (the reference's ``_dense_attention``, ``layers.py:145-163``), computed in fp32."""
@@ -251,15 +287,17 @@ class DecoderLayer(nn.Module):
 
     def forward(self, hidden: torch.Tensor, positions: torch.Tensor, cache: object | None = None,
                 block_ids: torch.Tensor | None = None, context_lens: torch.Tensor | None = None,
-                token_offsets: torch.Tensor | None = None, q_len: int = 1) -> torch.Tensor:
+                token_offsets: torch.Tensor | None = None, q_len: int = 1,
+                cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
         hidden, mlp_out = self.forward_chained(hidden, None, positions, cache, block_ids, context_lens,
-                                               token_offsets, q_len)
+                                               token_offsets, q_len, cu_seqlens=cu_seqlens)
         return hidden + mlp_out
 
     def forward_chained(self, hidden: torch.Tensor, pending, positions: torch.Tensor,  # noqa: ANN001
                         cache: object | None = None, block_ids: torch.Tensor | None = None,
                         context_lens: torch.Tensor | None = None, token_offsets: torch.Tensor | None = None,
-                        q_len: int = 1, defer_mlp: bool = False) -> tuple[torch.Tensor, object]:
+                        q_len: int = 1, defer_mlp: bool = False,
+                        cu_seqlens: torch.Tensor | None = None) -> tuple[torch.Tensor, object]:
         """The layer with its final residual add left to the caller: takes ``hidden`` plus the
         previous layer's not-yet-added MLP output ``pending`` (or None) and returns ``(hidden,
         mlp_out)``. The input stream is ``hidden + pending``, formed inside the first norm's
@@ -270,6 +308,6 @@ class DecoderLayer(nn.Module):
             normed = self.input_layernorm(hidden)
         else:
             normed, hidden = self.input_layernorm.add_forward(pending, hidden)
-        attn = self.self_attn(normed, positions, cache, block_ids, context_lens, token_offsets, q_len)
+        attn = self.self_attn(normed, positions, cache, block_ids, context_lens, token_offsets, q_len, cu_seqlens)
         normed, hidden = self.post_attention_layernorm.add_forward(attn, hidden)
         return hidden, self.mlp(normed, defer=defer_mlp)

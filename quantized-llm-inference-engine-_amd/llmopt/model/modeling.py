@@ -59,28 +59,38 @@ class DecoderOnlyModel(nn.Module):
 
     def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, cache: object | None = None,
                 block_ids: torch.Tensor | None = None, context_lens: torch.Tensor | None = None,
-                token_offsets: torch.Tensor | None = None, q_len: int = 1, last_only: bool = False) -> ModelOutput:
+                token_offsets: torch.Tensor | None = None, q_len: int = 1, last_only: bool = False,
+                cu_seqlens: torch.Tensor | None = None) -> ModelOutput:
         """One engine step: ``input_ids``/``positions`` ``[seq * q_len]`` (or ``[seq, q_len]``),
-        per-sequence cache metadata as in :class:`PagedAttentionLayer`."""
+        per-sequence cache metadata as in :class:`PagedAttentionLayer`. With ``cu_seqlens [seq + 1]``
+        a prefill of packed prompts of different lengths (none empty): ids and positions ``[tokens]``,
+        logits ``[1, tokens, vocab]``, with ``last_only`` ``[seq, 1, vocab]``."""
         input_ids = input_ids.reshape(-1)
         positions = positions.reshape(-1)
         hidden = self.embed_tokens(input_ids)
-        if token_offsets is None and context_lens is not None and block_ids is not None:
+        if token_offsets is None and context_lens is not None and block_ids is not None and cu_seqlens is None:
             # Where this step's tokens go in the cache: computed once here, not in every layer.
             token_offsets = context_lens - q_len
         pending = None  # each layer's MLP output, added inside the next norm's kernel
         last = len(self.layers) - 1
         # The final norm takes the last layer's partial sums too unless it first keeps only each
         # sequence's last row (last_only with several tokens per sequence).
-        defer_last = not last_only or q_len == 1
+        defer_last = not last_only or (q_len == 1 and cu_seqlens is None)
         for i, layer in enumerate(self.layers):
             # A layer may hand its down projection's partial sums to the next norm.
             hidden, pending = layer.forward_chained(hidden, pending, positions, cache=cache, block_ids=block_ids,
                                                     context_lens=context_lens, token_offsets=token_offsets,
-                                                    q_len=q_len,
+                                                    q_len=q_len, cu_seqlens=cu_seqlens,
                                                     defer_mlp=self.defer_reductions and (i < last or defer_last))
         seqs = int(hidden.shape[0]) // max(1, q_len)
-        if last_only and q_len > 1:
+        if cu_seqlens is not None:
+            seqs, q_len = 1, int(hidden.shape[0])
+            if last_only:
+                seqs = int(cu_seqlens.shape[0]) - 1
+                last_rows = cu_seqlens[1:].to(device=hidden.device, dtype=torch.long) - 1
+                hidden = hidden[last_rows]
+                pending = pending[last_rows] if pending is not None else None
+        elif last_only and q_len > 1:
             # The residual add, RMSNorm and lm_head act row by row, so keeping only the last rows
             # first is exact.
             hidden = last_token_hidden(hidden, q_len).contiguous()

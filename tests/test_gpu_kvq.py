@@ -463,3 +463,45 @@ def test_refusals_on_the_device():
         ops.kvq_attention(torch.zeros(2, 4, 1, 64), *cache.layer(0), table, lens, 0.1)
     with pytest.raises(ValueError):
         PagedAttention(4, 2, 64).forward(torch.zeros(2, 3, 1, 64, device="cuda").half(), cache, 0, table, lens)
+
+
+def test_generation_from_prompts_of_different_lengths():
+    """Packed prefill, quantized cache and graph-replayed decode steps of a ragged batch, against each prompt alone."""
+    config = ModelConfig.tiny()
+    model = random_quantized_model(config, device="cuda", dtype=torch.bfloat16, seed=4)
+    gen = torch.Generator().manual_seed(5)
+    prompts = [torch.randint(0, config.vocab_size, (n,), generator=gen) for n in (3, 130, 64, 1)]
+    forced = torch.randint(0, config.vocab_size, (4, 20), generator=gen)
+    generator = GreedyGenerator(model, cache_dtype=torch.int8)
+    together = generator.generate(prompts, 20, forced=forced)
+    eager = GreedyGenerator(model, cache_dtype=torch.int8, use_graph=False).generate(prompts, 20, forced=forced)
+    assert torch.equal(together.tokens, eager.tokens)
+    for s, p in enumerate(prompts):
+        alone = generator.generate([p], 20, forced=forced[s : s + 1])
+        # bf16 activations through two layers: other kernels for other batch sizes round differently, by 2^-8 a step
+        far = (together.prefill_logits[s] - alone.prefill_logits[0]).norm() / alone.prefill_logits[0].norm()
+        assert float(far) < 0.03, (s, float(far))
+
+
+def test_any_form_of_the_metadata_and_without_the_native_path(monkeypatch):
+    cache, table = _filled(3, 600, 16, 2, 128, torch.int8, seed=30)
+    twin = QuantizedPagedKVCache.from_tensors(*(t.clone() for t in (cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales)))
+    lens = torch.tensor([599, 200, 17], dtype=torch.int32, device="cuda")
+    q = torch.randn(3, 8, 1, 128, device="cuda").half()
+    k, v = torch.randn(3, 2, 128, device="cuda").half(), torch.randn(3, 2, 128, device="cuda").half()
+    attention = PagedAttention(8, 2, 128)
+    cache.write_decode(0, table, lens, k, v)
+    want = attention.forward(q, cache, 0, table, lens + 1)
+    wide = torch.cat([table, table], dim=1).to(torch.int64)[:, : table.shape[1]]
+    flat = torch.empty(q.numel() + 1, dtype=q.dtype, device="cuda")
+    flat[1:] = q.reshape(-1)
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(ops, "load_binding", lambda: None)
+        twin.write_decode(0, wide, lens.cpu().long()[:, None], k.double(), v.double())
+        assert torch.equal(twin.key_codes, cache.key_codes) and torch.equal(twin.value_scales, cache.value_scales)
+        for layer in (0, -1):
+            got = attention.forward(flat[1:].view(q.shape), twin, layer, wide, (lens + 1).long()[:, None])
+            assert torch.equal(got, want)
+        with pytest.raises(IndexError):
+            attention.forward(q, twin, 1, table, lens)

@@ -13,7 +13,7 @@ import torch
 from llmopt.attention import PackedAttention, PagedAttention
 from llmopt.cache import PagedKVCache, QuantizedPagedKVCache
 from llmopt.kernels import _lib, ops
-from llmopt.model import DecoderOnlyModel, ModelConfig
+from llmopt.model import DecoderOnlyModel, GreedyGenerator, ModelConfig
 from oracle import kvq_oracle as ko
 
 FORMATS = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
@@ -311,3 +311,50 @@ def test_c_entry_points_validate_on_the_host():
     assert lib.llmopt_kvq_attention_workspace(1, 32, 7, 128, 1, 512, 16, 2, 0) == 0 and lib.llmopt_kvq_attention_workspace(0, 32, 8, 128, 1, 512, 16, 2, 0) == 0
     with pytest.raises(NotImplementedError, match="16-byte"):
         _lib.call(at(codes=24), "llmopt_kvq_attention")
+
+
+# ---- packed prompts in the model --------------------------------------------------------------------
+
+
+def test_packed_prefill_of_a_model():
+    """Packed prompts against each prompt alone without a cache, and what the cache holds afterwards."""
+    torch.manual_seed(0)
+    model = DecoderOnlyModel(ModelConfig.tiny())
+    lens = [7, 1, 20]
+    prompts = [torch.randint(0, 512, (n,)) for n in lens]
+    cu = torch.tensor([0, *np.cumsum(lens)], dtype=torch.int32)
+    positions = torch.cat([torch.arange(n) for n in lens])
+    cache = model.allocate_cache(9, 8, torch.int8, "cpu")
+    table = torch.arange(9, dtype=torch.int32).view(3, 3)
+    with torch.no_grad():
+        every = model(torch.cat(prompts), positions, cu_seqlens=cu).logits
+        last = model(torch.cat(prompts), positions, cache=cache, block_ids=table, cu_seqlens=cu, last_only=True).logits
+        assert every.shape == (1, 28, 512) and last.shape == (3, 1, 512)
+        for s, p in enumerate(prompts):
+            alone = model(p, torch.arange(lens[s]), q_len=lens[s]).logits[0]
+            torch.testing.assert_close(every[0, cu[s] : cu[s + 1]], alone, atol=1e-5, rtol=1e-4)
+            torch.testing.assert_close(last[s, 0], alone[-1], atol=1e-5, rtol=1e-4)
+            again = model.allocate_cache(9, 8, torch.int8, "cpu")
+            model(p, torch.arange(lens[s]), cache=again, block_ids=table[s : s + 1], cu_seqlens=torch.tensor([0, lens[s]]))
+            for a, b in zip(cache.gather(1, table[s : s + 1], torch.tensor(lens[s : s + 1])),
+                            again.gather(1, table[s : s + 1], torch.tensor(lens[s : s + 1]))):
+                assert float((a.float() - b.float()).abs().max()) < 0.05  # a code at most where fp32 sums differ in their last bits
+        with pytest.raises(TypeError, match="QuantizedPagedKVCache"):
+            model(torch.cat(prompts), positions, cache=model.allocate_cache(9, 8, torch.float32, "cpu"), block_ids=table, cu_seqlens=cu)
+
+
+def test_generation_from_prompts_of_different_lengths():
+    torch.manual_seed(1)
+    model = DecoderOnlyModel(ModelConfig.tiny())
+    prompts = [torch.randint(0, 512, (n,)) for n in (3, 17, 9)]
+    generator = GreedyGenerator(model, block_size=8, cache_dtype=torch.int8)
+    together = generator.generate(prompts, 6)
+    for s, p in enumerate(prompts):
+        alone = generator.generate([p], 6)
+        torch.testing.assert_close(together.prefill_logits[s], alone.prefill_logits[0], atol=1e-5, rtol=1e-4)
+        assert torch.equal(together.tokens[s], alone.tokens[0])
+    for bad in ([], [torch.zeros(0, dtype=torch.long)], [torch.zeros(1, 2, dtype=torch.long)]):
+        with pytest.raises(ValueError):
+            generator.generate(bad, 2)
+    with pytest.raises(TypeError, match="QuantizedPagedKVCache"):
+        GreedyGenerator(model).generate(prompts, 2)
