@@ -4,7 +4,7 @@
 // them in registers (blocks of more than 8 x 64 chunks of 8 numbers are read twice), takes their largest magnitude, fixes
 // the scale and writes the codes. Bound by HBM (3 bytes per 16-bit number) and, one wave's work being 4 KB, by its chain of
 // loads: lengths and offsets, then the rows and the table entry together. Measured (MI355X, bf16, 8 heads of 128, blocks of
-// 16): 32 prompts of 1 - 1024 tokens 27.5 us (104 MB, 3.8 TB/s; 36 with the table before the rows and numbers held as fp32),
+// 16): 32 prompts of 1 - 1024 tokens 23.1 us (104 MB, 4.5 TB/s; 36 with the table before the rows and numbers held as fp32),
 // one token of 256 sequences 6.0, of one sequence 4.8.
 //   need  = 2^e, the smallest e >= -126 with amax <= top 2^e (top = 127 or 448), 0 for amax = 0, NaN for a row
 //           that holds an infinity or a NaN
@@ -202,8 +202,9 @@ __global__ void __launch_bounds__(64 * kWaves) kvq_write_kernel(const KvqWriteAr
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] = finite ? x[i].get(e) * inv : 0.0f;
       if constexpr (VEC)
-        *reinterpret_cast<u32x2*>(dst + int64_t(c) * 8) =
-            u32x2{f32_to_codes<FMT>(v[0], v[1], v[2], v[3]), f32_to_codes<FMT>(v[4], v[5], v[6], v[7])};
+        __builtin_nontemporal_store(
+            u32x2{f32_to_codes<FMT>(v[0], v[1], v[2], v[3]), f32_to_codes<FMT>(v[4], v[5], v[6], v[7])},
+            reinterpret_cast<u32x2*>(dst + int64_t(c) * 8));  // 32 prompts: 27.8 -> 23.1 us
       else
         dst[c] = uint8_t(f32_to_codes<FMT>(v[0], 0.f, 0.f, 0.f));
     }

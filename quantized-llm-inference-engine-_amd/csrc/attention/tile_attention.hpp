@@ -558,7 +558,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
       const int t = tok_of(row);
       const u32x4 w = *reinterpret_cast<const u32x4*>(stage + r * kRowBytes + 16 * k_chunk<HD>(r, c));
       uint16_t* dst = static_cast<uint16_t*>(a.out) + t * a.o_tok_stride + (row - t * a.group) * a.o_head_stride + 8 * c;
-      *reinterpret_cast<u32x4*>(dst) = w;
+      __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(dst));  // 128 prompts of 128: 84 -> 68 us
     }
     again(__builtin_amdgcn_ballot_w64(bad_value && row_ok));
   }
