@@ -6,8 +6,8 @@
 //
 // Why: at one token the kernel takes 4.8 us, and the same steps in Python (attribute look-ups, checks,
 // two ctypes calls) held a 4096 x 4096 call at 18.9 us; 6.9 us with this path. An append to the 8-bit cache, a decode
-// step's attention over it and a short packed prompt: 28 / 36 / 17 us in Python, 8.8 / 13.6 / 7.3 here, the kernels 4.2 /
-// 9.7 / 8.0 (calls in a row overlap).
+// step's attention over it and a short packed prompt: 28 / 36 / 17 us in Python, 8.0 / 12.1 / 7.3 here, a replayed graph
+// of them 4.8 / 9.2 / 7.3.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -184,19 +184,15 @@ struct Layer {
   int64_t blocks, heads, block_size, head_dim;
   at::Device device = at::kCPU;
 
-  bool from(PyObject* const* args) {
-    const at::Tensor* t[4];
+  const at::Tensor* t[4];
+
+  // Whether the four tensors are a cache (whole, all layers) on one HIP device.
+  bool check(PyObject* const* args) {
     for (int i = 0; i < 4; ++i)
       if (!(t[i] = tensor_of(args[i]))) return false;
-    const int64_t layer = PyLong_AsLongLong(args[4]);
-    if (layer == -1 && PyErr_Occurred()) {
-      PyErr_Clear();
-      return false;
-    }
     device = t[0]->device();
     const auto type = t[0]->scalar_type();
     if (!device.is_cuda() || (type != at::kChar && type != at::kFloat8_e4m3fn) || t[0]->dim() != 5) return false;
-    if (layer < 0 || layer >= t[0]->size(0)) return false;
     for (int k = 0; k < 2; ++k) {
       const at::Tensor &c = *t[2 * k], &s = *t[2 * k + 1];
       if (c.device() != device || c.scalar_type() != type || c.sizes() != t[0]->sizes() || !c.is_contiguous() ||
@@ -205,6 +201,17 @@ struct Layer {
         return false;
     }
     format = type == at::kChar ? 0 : 1;
+    return true;
+  }
+
+  bool from(PyObject* const* args) {
+    if (!check(args)) return false;
+    const int64_t layer = PyLong_AsLongLong(args[4]);
+    if (layer == -1 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return false;
+    }
+    if (layer < 0 || layer >= t[0]->size(0)) return false;
     blocks = t[0]->size(1), heads = t[0]->size(2), block_size = t[0]->size(3), head_dim = t[0]->size(4);
     for (int k = 0; k < 2; ++k) {
       codes[k] = static_cast<char*>(t[2 * k]->mutable_data_ptr()) + layer * blocks * heads * block_size * head_dim;
@@ -213,6 +220,21 @@ struct Layer {
     return true;
   }
 };
+
+// kvq_cache_shape(key_codes, key_scales, value_codes, value_scales) -> (layers, blocks, kv_heads, block_size, head_dim), or
+// None where the general checks have to look.
+PyObject* kvq_cache_shape(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "kvq_cache_shape takes four tensors");
+    return nullptr;
+  }
+  HANDLE_TH_ERRORS
+  Layer c;
+  if (!c.check(args) || c.t[0]->numel() == 0) Py_RETURN_NONE;
+  const auto s = c.t[0]->sizes();
+  return Py_BuildValue("(LLLLL)", (long long)s[0], (long long)s[1], (long long)s[2], (long long)s[3], (long long)s[4]);
+  END_HANDLE_TH_ERRORS
+}
 
 bool on_current_device(const at::Device& dev) { return dev.index() == c10::hip::current_device(); }
 
@@ -356,6 +378,7 @@ PyMethodDef methods[] = {
     {"attach", reinterpret_cast<PyCFunction>(attach), METH_FASTCALL, nullptr},
     {"attach_kvq", reinterpret_cast<PyCFunction>(attach_kvq), METH_FASTCALL, nullptr},
     {"linear", reinterpret_cast<PyCFunction>(linear), METH_FASTCALL, nullptr},
+    {"kvq_cache_shape", reinterpret_cast<PyCFunction>(kvq_cache_shape), METH_FASTCALL, nullptr},
     {"kvq_write", reinterpret_cast<PyCFunction>(kvq_write), METH_FASTCALL, nullptr},
     {"kvq_attention", reinterpret_cast<PyCFunction>(kvq_attention), METH_FASTCALL, nullptr},
     {"packed_attention", reinterpret_cast<PyCFunction>(packed_attention), METH_FASTCALL, nullptr},

@@ -66,12 +66,12 @@ class QuantizedPagedKVCache:
         shape = (num_layers, num_blocks, num_kv_heads, block_size, head_dim)
         codes = [torch.zeros(shape, dtype=torch.int8, device=device).view(dtype) for _ in range(2)]
         scales = [torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)]
-        self._adopt(codes[0], scales[0], codes[1], scales[1])
+        self._adopt(codes[0], scales[0], codes[1], scales[1], shape)
 
-    def _adopt(self, key_codes, key_scales, value_codes, value_scales) -> None:  # noqa: ANN001
+    def _adopt(self, key_codes, key_scales, value_codes, value_scales, shape) -> None:  # noqa: ANN001
         self.key_codes, self.key_scales = key_codes, key_scales
         self.value_codes, self.value_scales = value_codes, value_scales
-        self.num_layers, self.num_blocks, self.num_kv_heads, self.block_size, self.head_dim = key_codes.shape
+        self.num_layers, self.num_blocks, self.num_kv_heads, self.block_size, self.head_dim = shape
         self.dtype = key_codes.dtype
         self.device = key_codes.device
 
@@ -80,6 +80,14 @@ class QuantizedPagedKVCache:
                      value_scales: torch.Tensor) -> QuantizedPagedKVCache:
         """A cache over tensors that exist already (shapes as the attributes; shared, not copied). The scales must
         be powers of two, 0 or NaN, and the codes finite."""
+        cache = cls.__new__(cls)
+        if key_codes.is_cuda:  # the checks below in native code: 0.6 us instead of 4
+            from llmopt.kernels import ops
+
+            shape = ops.cache_shape(key_codes, key_scales, value_codes, value_scales)
+            if shape is not None:
+                cache._adopt(key_codes, key_scales, value_codes, value_scales, shape)
+                return cache
         if key_codes.dim() != 5 or key_codes.shape != value_codes.shape or 0 in key_codes.shape:
             raise ValueError(f"expected two [layers, blocks, kv_heads, block_size, head_dim] code tensors, got "
                              f"{tuple(key_codes.shape)} and {tuple(value_codes.shape)}")
@@ -96,8 +104,7 @@ class QuantizedPagedKVCache:
                 and value_scales.is_contiguous()) or not key_scales.device == value_codes.device \
                 == value_scales.device == device:
             raise ValueError("the cache's tensors must be contiguous and on one device")
-        cache = cls.__new__(cls)
-        cache._adopt(*tensors)
+        cache._adopt(*tensors, key_codes.shape)
         return cache
 
     def layer(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:

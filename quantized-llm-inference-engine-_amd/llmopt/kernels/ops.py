@@ -50,6 +50,7 @@ __all__ = [
     "paged_decode_attention_rope",
     "argmax_rows",
     "cache_attention",
+    "cache_shape",
     "cache_write",
     "paged_prefill_attention",
     "unpack_nibbles",
@@ -731,6 +732,14 @@ def kvq_write(key_codes, key_scales, value_codes, value_scales, block_ids, token
             ),
             "llmopt_kvq_write",
         )
+
+
+def cache_shape(key_codes: torch.Tensor, key_scales: torch.Tensor, value_codes: torch.Tensor,
+                value_scales: torch.Tensor) -> tuple[int, ...] | None:
+    """The shape of a :class:`QuantizedPagedKVCache`'s codes if the four tensors are one on a HIP device, checked in
+    native code; None where that is not built or says no."""
+    binding = load_binding()
+    return None if binding is None else binding.kvq_cache_shape(key_codes, key_scales, value_codes, value_scales)
 
 
 def cache_write(cache, layer_idx: int, block_ids: torch.Tensor, token_offsets: torch.Tensor,  # noqa: ANN001
