@@ -419,27 +419,50 @@ __global__ void __launch_bounds__(256) kvq_merge_kernel(const KvqAttnArgs a) {
   const int r = int(blockIdx.x) * 4 + int(threadIdx.x >> 6);
   const int64_t kvh = blockIdx.y, s = blockIdx.z;
   if (r >= rows) return;
+  const float neg_inf = -__int_as_float(0x7F800000);
+  const int64_t stride = a.num_seqs * int64_t(kv_heads) * rows;  // between two splits
+  const float* const lse_at = a.part_lse + (s * kv_heads + kvh) * rows + r;
+  const float* const part = a.part_out + ((s * kv_heads + kvh) * rows + r) * HD + kD * lane;
+  // The log-sum-exps, a split per lane, and the first parts are on their way before the context's length, which says
+  // how many there are, is known: parts past it were not written and are not used.
+  constexpr int kAhead = 4;
+  float ahead[kAhead][kD];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+    for (int d = 0; d < kD; ++d) ahead[i][d] = i < a.splits ? part[i * stride * HD + d] : 0.0f;
+  float lse = lane < a.splits ? lse_at[lane * stride] : neg_inf;
   // The splits that the row's block of 16 ran.
   const int base = a.context_lens[s] - int(a.q_len);
   const int last_tok = int(uint32_t(min((r & ~15) + 15, rows - 1)) / uint32_t(a.group));
   const int t_end = max(0, min(base + last_tok + 1, int(a.c.ldb * a.c.block_size)));
   const int span = int(a.tiles_per_split) * 32;
   const int n = min(a.splits, (t_end + span - 1) / span);
-  const float neg_inf = -__int_as_float(0x7F800000);
-  auto at = [&](int i) { return ((int64_t(i) * a.num_seqs + s) * kv_heads + kvh) * rows + r; };
-  float top = neg_inf;
-  for (int i = lane; i < n; i += 64) top = fmaxf(top, a.part_lse[at(i)]);
+  lse = lane < n ? lse : neg_inf;
+  float top = lse;
+  for (int i = 64 + lane; i < n; i += 64) top = fmaxf(top, lse_at[i * stride]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   float acc[kD] = {}, sum = 0.0f;
   if (top != neg_inf) {
+    auto weight = [&](float x) { return x == neg_inf ? 0.0f : __builtin_amdgcn_exp2f(x - top); };
+    const float w_lane = weight(lse);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_lane), i));
+      if (i < n) {
+        sum += w;
+#pragma unroll
+        for (int d = 0; d < kD; ++d) acc[d] = __builtin_fmaf(w, ahead[i][d], acc[d]);
+      }
+    }
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float lse = a.part_lse[at(i)];
-      const float w = lse == neg_inf ? 0.0f : __builtin_amdgcn_exp2f(lse - top);
+    for (int i = kAhead; i < n; ++i) {
+      const float w = i < 64 ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w_lane), i & 63))
+                             : weight(lse_at[i * stride]);
       sum += w;
 #pragma unroll
-      for (int d = 0; d < kD; ++d) acc[d] = __builtin_fmaf(w, a.part_out[at(i) * HD + kD * lane + d], acc[d]);
+      for (int d = 0; d < kD; ++d) acc[d] = __builtin_fmaf(w, part[i * stride * HD + d], acc[d]);
     }
   }
   const int tok = int(uint32_t(r) / uint32_t(a.group));
