@@ -104,9 +104,10 @@ Plan plan_attention(int64_t num_seqs, int64_t kv_heads, int64_t group, int64_t h
   return Plan{false, int((tiles + per - 1) / per), waves, per};
 }
 
-// A workgroup of the tile kernel reads its query rows (128 tokens, one KV head's query heads) at 32-bit offsets.
+// A workgroup of the tile kernel reads its query rows (128 tokens, one KV head's query heads) and writes its output at
+// 32-bit offsets, and finds a row's token in fp32.
 bool near_rows(int64_t group, int64_t tok_stride, int64_t head_stride) {
-  return tok_stride >= 0 && tok_stride <= (int64_t(1) << 22) && head_stride >= 0 && head_stride <= (int64_t(1) << 29) / group;
+  return group < (int64_t(1) << 19) && tok_stride >= 0 && tok_stride <= (int64_t(1) << 22) && head_stride >= 0 && head_stride <= (int64_t(1) << 29) / group;
 }
 
 }  // namespace
@@ -213,7 +214,7 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
   };
   a.q_vec = rows16(query, q_seq_stride, q_head_stride, q_tok_stride);
   const bool tile_rows = a.q_vec && near_rows(group, q_tok_stride, q_head_stride) &&
-                         rows16(out, o_seq_stride, o_head_stride, o_tok_stride);
+                         near_rows(group, o_tok_stride, o_head_stride) && rows16(out, o_seq_stride, o_head_stride, o_tok_stride);
   if (algo == LLMOPT_KVQ_ALGO_TILES && (q_dtype == LLMOPT_DTYPE_F32 || !tile_rows))
     return fail(LLMOPT_ERR_UNSUPPORTED, "the tile kernel takes fp16 and bf16 rows aligned to 16 bytes");
   const Plan plan = plan_attention(num_seqs, kv_heads, group, head_dim, q_len, ldb, block_size, q_dtype, tile_rows, algo);
@@ -260,7 +261,8 @@ int llmopt_packed_attention(const void* query, int64_t q_tok_stride, int64_t q_h
   constexpr int64_t kStride = int64_t(1) << 24;  // a tile's 64 rows at 32-bit offsets
   if (total_tokens > kMaxInt / 4 / group || num_seqs > kMaxInt / 4 || k_tok_stride < 0 || k_tok_stride > kStride ||
       v_tok_stride < 0 || v_tok_stride > kStride ||
-      !near_rows(group, q_tok_stride, q_head_stride) || ((total_tokens * group + 127) / 128 + num_seqs + 64) > kMaxInt / kv_heads)
+      !near_rows(group, q_tok_stride, q_head_stride) || !near_rows(group, o_tok_stride, o_head_stride) ||
+      ((total_tokens * group + 127) / 128 + num_seqs + 64) > kMaxInt / kv_heads)
     return fail(LLMOPT_ERR_UNSUPPORTED, "packed attention: %lld tokens, %lld sequences, token strides %lld / %lld / %lld",
                 (long long)total_tokens, (long long)num_seqs, (long long)q_tok_stride, (long long)k_tok_stride,
                 (long long)v_tok_stride);

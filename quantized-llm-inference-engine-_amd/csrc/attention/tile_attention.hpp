@@ -1,9 +1,9 @@
 // Causal attention of many query rows, for packed prompts (16-bit keys and values, rows of a tensor) and for chunks
 // over the 8-bit cache (codes by block table). One kernel, two sources of key tiles.
 //
-// A workgroup of four waves owns kRows = 128 RB query rows of one (sequence, KV head): the sequence's rows are its
-// tokens x the `group` query heads that share the KV head, token-major, 32 RB rows per wave. It walks the keys in
-// tiles of 64, held as 16-bit rows in a double buffer in LDS that all rows read:
+// A workgroup of four waves owns 128 query rows of one (sequence, KV head): the sequence's rows are its tokens x the
+// `group` query heads that share the KV head, token-major, 32 rows per wave. It walks the keys in tiles of 64, held as
+// 16-bit rows in a double buffer in LDS that all rows read:
 //   * packed: by direct loads, one tile ahead;
 //   * codes: loaded into registers one tile ahead, dequantized exactly to bf16 (code x power of two) behind the
 //     tile's products, and stored.
@@ -14,10 +14,21 @@
 //   * online softmax in fp32, in powers of two;
 //   * O^T += V^T P^T with the probabilities as they lie (slot 4 a + r of lane half h is key 8 a + 4 h + r), V^T by
 //     transposing LDS reads of the row-major V tile.
+// Bound by the matrix units and the power they draw: the clock falls to 1.65 - 1.94 GHz under it (1.5 - 1.9 under a large
+// library product of 1206 TFLOP/s), and MFMAs are under way in half of the cycles, VALU work (32 exponentials, 32 fused
+// multiply-adds, 32 roundings and sums per 32 MFMAs) beside them from the SIMD's other wave. Measured (MI355X, heads
+// of 128, 32 query and 8 KV heads): one prompt of 8192 in bf16 534 us (1030 TFLOP/s), 4 of 2048 162 (850), 32 of 512 115
+// (601). Short prompts: rows, tokens and finiteness by few instructions at a walk's ends (32 of 1 - 1024 tokens in fp16 175 ->
+// 165, 512 of 32 106 -> 85), half a tile where the last one has up to 32 keys (165 -> 162). Measured and not taken: 64
+// rows per wave (733 against 560 for 8192), eight waves per workgroup (533 against 547, but 199 against 188 for
+// 32 prompts), three buffers (575), the next tile's products between the softmax of this one (545 - 576 against 542), three
+// workgroups per CU with one V buffer (552 against 545).
 // A key that is masked for some rows of a tile only has probability 0 for them, but 0 x infinity would still reach
 // their output: a wave whose rows come out with anything that is not finite computes those rows once more, key by
 // key (never for finite inputs).
 #pragma once
+
+#include <type_traits>
 
 #include "attn_common.hpp"
 
@@ -28,13 +39,11 @@ enum : int { kSrcPacked = 0, kSrcCodes = 1 };
 
 constexpr int kKeys = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
-// Probabilities that are cut to fp16 lose 0.721 2^-11 of their value on average (half a step over a mantissa spread evenly
-// in its logarithm), the largest, 1, nothing. They are raised by that much first, as a part of the exponent: log2(1 +
-// 0.721 2^-11). 2-norm error of 32 prompts of up to 1024 tokens against float64: cut 2.85e-4, raised and cut 2.40e-4; the
-// output's own rounding alone makes 2.02e-4.
-constexpr float kCut = 5.08e-4f;
-
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+template <int N>
+using Blocks = std::integral_constant<int, N>;
 
 template <bool F16>
 struct Op {
@@ -45,10 +54,8 @@ struct Op {
       return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   __device__ static uint32_t pack(float lo, float hi) {
-    // fp16 by the pair conversion that cuts (see kCut). Rounding takes three instructions for two numbers: 183 us against
-    // 167 for 4 prompts of 2048.
     if constexpr (F16)
-      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+      return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo, hi}), f16x2_t));  // one instruction
     else
       return pack_bf16(lo, hi);
   }
@@ -140,12 +147,18 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   const uint32_t group = uint32_t(a.group);
   auto tok_of = [&](int row) -> int { return int(uint32_t(row) / group); };
   const int wrow = a.row0 + 32 * wave;  // the wave's first row
-  const bool row_ok = wrow + col < a.rows;
-  const int own_row = row_ok ? wrow + col : a.rows - 1;
-  const int tok = tok_of(own_row), head = own_row - tok * a.group;
-  const int q_pos = row_ok ? a.base + tok : -1;
-  const int first_pos = a.base + tok_of(wrow);
-  const int wave_last = wrow < a.rows ? a.base + tok_of(min(wrow + 32, a.rows) - 1) : -1;
+  const int own_row = wrow + col;
+  const bool row_ok = own_row < a.rows;
+  // The token, counted from row0_tok, of the row n rows behind that token's first: (n + 1/2) / group is at least 1 / (2
+  // group) away from a whole number, and its three roundings in fp32 are off by less for n < 2^20 (n < group + 128, checked
+  // on the host). Integer divisions, here and per row that is loaded or stored, were a third of a short walk's VALU work.
+  const float inv_group = __builtin_amdgcn_rcpf(float(a.group));
+  const int rem0 = a.row0 - a.row0_tok * a.group + 32 * wave;  // wrow's n
+  auto tok_at = [&](int n) -> int { return int((float(n) + 0.5f) * inv_group); };
+  const int pos0 = a.base + a.row0_tok;
+  const int q_pos = row_ok ? pos0 + tok_at(rem0 + col) : -1;
+  const int first_pos = pos0 + __builtin_amdgcn_readfirstlane(tok_at(rem0));
+  const int wave_last = wrow < a.rows ? pos0 + __builtin_amdgcn_readfirstlane(tok_at(rem0 + min(31, a.rows - 1 - wrow))) : -1;
   const int first_tile = a.t_begin / kKeys, n_tiles = (a.t_end + kKeys - 1) / kKeys;
 
   const float neg_inf = -__int_as_float(0x7F800000);
@@ -167,17 +180,20 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   // The rows come in whole, by direct loads into the second tile buffers (a lane's 16-byte pieces straight from memory
   // would touch each line four times).
   u32x4 qf[kS];
+  // Byte offset from row0_tok's first head of row wrow + r; below 2^31 (strides checked on the host).
+  auto row_offset = [&](int r, int64_t tok_stride, int64_t head_stride) -> uint32_t {
+    const uint32_t n = uint32_t(rem0 + r), t = uint32_t(tok_at(rem0 + r));
+    return (n * uint32_t(head_stride) + t * uint32_t(tok_stride - head_stride * a.group)) * 2;
+  };
   uint8_t* const q_lds = lds + (wave & 1) * (32 * kRowBytes) + (first_tile & 1 ? 0 : kTile) + (wave >> 1) * (2 * kTile);
   auto fetch_query = [&]() {
     const auto rs = make_rsrc(static_cast<const uint16_t*>(a.query) + a.row0_tok * a.q_tok_stride, 0x7FFFFFFFu);
 #pragma unroll
     for (int j = 0; j < 32 / kRpl; ++j) {
       const int r = kRpl * j + lane / kCh;
-      const int row = min(wrow + r, a.rows - 1);  // rows past the end repeat the last one
-      const int t = tok_of(row);
-      load_lds16_cached(rs, q_lds + kRpl * j * kRowBytes,
-                        uint32_t(((t - a.row0_tok) * a.q_tok_stride + (row - t * a.group) * a.q_head_stride) * 2) +
-                            16 * k_chunk<HD>(r, lane % kCh), 0);
+      // Rows past the end repeat the last one.
+      const uint32_t at = row_offset(min(r, a.rows - 1 - wrow), a.q_tok_stride, a.q_head_stride);
+      load_lds16_cached(rs, q_lds + kRpl * j * kRowBytes, at + 16 * k_chunk<HD>(r, lane % kCh), 0);
     }
   };
   auto load_query = [&]() {
@@ -273,10 +289,11 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   struct Scores {
     f32x16 s[2];
   };
-  auto scores = [&](Scores& sc, int i) {
+  auto scores = [&](auto nb, Scores& sc, int i) {
+    constexpr int NB = decltype(nb)::value;
     const uint8_t* kt = k_buf(i);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int kb = 0; kb < NB; ++kb) {
 #pragma unroll
       for (int v = 0; v < 16; ++v) sc.s[kb][v] = 0.0f;
 #pragma unroll
@@ -287,13 +304,13 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
     }
   };
   u32x4 pf[KP][4];
-  auto probabilities = [&](const Scores& sc) {
-    const float shift = F16 ? kCut - mc : -mc;
+  auto probabilities = [&](auto nb, const Scores& sc) {
+    constexpr int NB = decltype(nb)::value;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2 * NB; ++i) {
       float p[8];
 #pragma unroll
-      for (int v = 0; v < 8; ++v) p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc.s[i / 2][8 * (i % 2) + v], c2, shift));
+      for (int v = 0; v < 8; ++v) p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc.s[i / 2][8 * (i % 2) + v], c2, -mc));
       // The sum adds the probabilities as rounded (KP = 2: to 16 bits), so that a row's weights add up to one.
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -309,12 +326,14 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
     }
   };
   // Tile i: its scores, their softmax, and its part of the output.
-  auto step = [&](int i, uint64_t mask) {
+  // Its first NB blocks of 32 keys: the others are behind all of the wave's rows.
+  auto step = [&](auto nb, int i, uint64_t mask) {
+    constexpr int NB = decltype(nb)::value;
     Scores sc;
-    scores(sc, i);
+    scores(nb, sc, i);
     if constexpr (kRawKeys) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f32x4 s = *reinterpret_cast<const f32x4*>(k_scales + (i & 1) * kKeys + 32 * kb + 8 * q + 4 * half);
@@ -325,13 +344,13 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
     const int t0 = i * kKeys;
     if constexpr (CAP) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int v = 0; v < 16; ++v) sc.s[kb][v] = tanhf(sc.s[kb][v] * a.scale / a.softcap) * a.softcap;
     }
     if (mask != ~uint64_t(0) || t0 + kKeys - 1 > first_pos) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+      for (int kb = 0; kb < NB; ++kb) {
         // Bit 8 q + r: key 8 q + 4 half + r of the block is a key at or before this row's token.
         const int room = q_pos - t0 - 32 * kb - 4 * half;
         const uint32_t bits = (uint32_t(mask >> (32 * kb)) >> (4 * half)) & (room >= 31 ? ~0u : room < 0 ? 0u : (2u << room) - 1u);
@@ -344,7 +363,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
     }
     float top = neg_inf;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int v = 0; v < 16; ++v) top = fmaxf(top, sc.s[kb][v]);
     const float m_new = fmaxf(m_run, other_half_max(top));
@@ -361,10 +380,10 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
           for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
       }
     }
-    probabilities(sc);
+    probabilities(nb, sc);
     const uint8_t* vt = v_buf(i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 2 * NB; ++j)
 #pragma unroll
       for (int d = 0; d < kD; ++d) {
         // Keys 16 j + vkey and 8 further: both have vkey's low bits, so one swizzle.
@@ -383,15 +402,23 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
       fetch_query();
       wait_vmcnt<0>();
       load_query();
-      for (int i = 0; i < n_tiles; ++i) {
-        wait_vmcnt<0>();  // this wave's rows of tile i
+      auto arrived = [&]() {
+        wait_vmcnt<0>();  // this wave's rows of the tile
         wait_lgkmcnt0();  // its reads of the buffers that are refilled next
         __builtin_amdgcn_s_barrier();
+      };
+      const int whole = a.t_end % kKeys != 0 && a.t_end % kKeys <= 32 ? n_tiles - 1 : n_tiles;
+      for (int i = 0; i < whole; ++i) {
+        arrived();
         if (i + 1 < n_tiles) {
           fetch_packed(0, i + 1);
           fetch_packed(1, i + 1);
         }
-        if (i * kKeys <= wave_last) step(i, ~uint64_t(0));
+        if (i * kKeys <= wave_last) step(Blocks<2>{}, i, ~uint64_t(0));
+      }
+      if (whole < n_tiles) {
+        arrived();
+        if (whole * kKeys <= wave_last) step(Blocks<1>{}, whole, ~uint64_t(0));
       }
     } else {
       Place place = place_of(first_tile, entry_of(first_tile));
@@ -412,7 +439,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
           hv = fetch_codes(1, place);
           entry = entry_of(i + 2);
         }
-        if (i * kKeys <= wave_last) step(i, mask);
+        if (i * kKeys <= wave_last) step(Blocks<2>{}, i, mask);
         if (i + 1 < n_tiles) {
           store_codes(0, i + 1, hk, place.mask);
           store_codes(1, i + 1, hv, place.mask);
@@ -524,18 +551,18 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   wait_lgkmcnt0();
   __builtin_amdgcn_s_barrier();  // every wave is past its last tile
   uint8_t* const stage = lds + wave * 32 * kRowBytes;
-  auto narrow = [&](float lo, float hi) -> uint32_t {
-    if constexpr (QF16)
-      return uint32_t(f32_to_f16_rne(lo)) | (uint32_t(f32_to_f16_rne(hi)) << 16);
-    else
-      return pack_bf16(lo, hi);
-  };
   {
     const float l = other_half_sum(l_run);
     // Zeros without keys; over the cache also for a sum that is no number (as the torch sequence's nan_to_num gives).
     const bool none = SRC == kSrcPacked ? l == 0.0f : !(l > 0.0f);
     const float inv = 1.0f / l;
-    bool bad_value = false;
+    if (__builtin_amdgcn_ballot_w64(none))
+#pragma unroll
+      for (int d = 0; d < kD; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] = none ? 0.0f : o[d][v];
+    const float scale = none ? 1.0f : inv;
+    float bad[2] = {0.0f, 0.0f};  // 0 x a number is 0, 0 x anything else is not
 #pragma unroll
     for (int d = 0; d < kD; ++d)
 #pragma unroll
@@ -543,23 +570,23 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
         float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          v[r] = none ? 0.0f : o[d][4 * q + r] * inv;
-          bad_value |= !(__builtin_fabsf(v[r]) < __int_as_float(0x7F800000));
+          v[r] = o[d][4 * q + r] * scale;
+          bad[r % 2] = __builtin_fmaf(v[r], 0.0f, bad[r % 2]);
         }
         *reinterpret_cast<u32x2*>(stage + col * kRowBytes + 16 * k_chunk<HD>(col, 4 * d + q) + 8 * half) =
-            u32x2{narrow(v[0], v[1]), narrow(v[2], v[3])};
+            u32x2{Op<QF16>::pack(v[0], v[1]), Op<QF16>::pack(v[2], v[3])};
       }
     wait_lgkmcnt0();  // the wave's own rows: no barrier
+    char* const out = static_cast<char*>(a.out) + a.row0_tok * a.o_tok_stride * 2;
 #pragma unroll
     for (int i = 0; i < 32 / kRpl; ++i) {
       const int r = kRpl * i + lane / kCh, c = lane % kCh;
-      const int row = wrow + r;
-      if (row >= a.rows) continue;
-      const int t = tok_of(row);
+      if (wrow + r >= a.rows) continue;
       const u32x4 w = *reinterpret_cast<const u32x4*>(stage + r * kRowBytes + 16 * k_chunk<HD>(r, c));
-      uint16_t* dst = static_cast<uint16_t*>(a.out) + t * a.o_tok_stride + (row - t * a.group) * a.o_head_stride + 8 * c;
-      __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(dst));  // 128 prompts of 128: 84 -> 68 us
+      // Non-temporal: 128 prompts of 128 84 -> 68 us.
+      __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(out + (row_offset(r, a.o_tok_stride, a.o_head_stride) + 16 * c)));
     }
+    const bool bad_value = bad[0] != 0.0f || bad[1] != 0.0f;
     again(__builtin_amdgcn_ballot_w64(bad_value && row_ok));
   }
 }
