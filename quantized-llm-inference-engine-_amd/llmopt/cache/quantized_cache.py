@@ -180,6 +180,7 @@ class QuantizedPagedKVCache:
                              f"cache's {self.num_kv_heads} heads of {self.head_dim}")
         if not (keys.is_floating_point() and values.is_floating_point()):
             raise TypeError(f"keys and values must be floating-point, got {keys.dtype}, {values.dtype}")
+        keys, values = keys.detach(), values.detach()  # the cache is no part of a graph
         table = block_ids.to("cpu", torch.long).tolist()
         starts = token_offsets.reshape(-1).tolist()
         if cu_seqlens is not None:

@@ -246,6 +246,16 @@ def test_write_refusals():
         ops.kvq_write(codes.transpose(1, 2), scales[:, :1].expand(2, 4), codes.transpose(1, 2), scales[:, :1].expand(2, 4), table, off, good, good)
 
 
+@pytest.mark.parametrize("fmt", [torch.int8, torch.float8_e4m3fn])
+def test_a_write_keeps_no_graph(fmt):
+    cache = QuantizedPagedKVCache(1, 2, 4, 2, 64, dtype=fmt)
+    k = torch.randn(1, 3, 2, 64, requires_grad=True)
+    for offset in (1, 1):
+        cache.write(0, torch.tensor([[0]]), torch.tensor([offset]), k * 2, k * 3)
+    for t in (cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales):
+        assert not t.requires_grad
+
+
 def test_attention_refusals():
     cache = QuantizedPagedKVCache(1, 2, 4, 2, 64)
     table, lens = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
