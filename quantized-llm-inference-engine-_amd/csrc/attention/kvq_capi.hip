@@ -189,7 +189,8 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
   if (head_dim != 64 && head_dim != 128)
     return fail(LLMOPT_ERR_UNSUPPORTED, "attention over the 8-bit cache: head_dim %lld", (long long)head_dim);
   if (num_seqs == 0 || q_len == 0) return LLMOPT_OK;
-  if (!query || !key_codes || !value_codes || !key_scales || !value_scales || !block_ids || !context_lens || !out)
+  if (!query || !key_codes || !value_codes || !key_scales || !value_scales || (!block_ids && ldb > 0) || !context_lens ||
+      !out)
     return fail(LLMOPT_ERR_INVALID_ARG, "null pointer argument");
   const int64_t group = num_heads / kv_heads;
   if (num_seqs > 65535 || q_len > kMaxInt / 4 || group * q_len > kMaxInt / 4)

@@ -263,6 +263,24 @@ def test_rows_without_keys_and_missing_blocks(q_len):
             assert not bool(out[5, :, :2].any()) and bool(out[5, :, 2:].any())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kvh,hd", [(71, 1, 64), (131, 1, 128), (600, 2, 64)])
+def test_wide_groups(dtype, heads, kvh, hd):
+    cache, table = _filled(2, 70, 16, kvh, hd, torch.int8, seed=11)
+    lens = torch.tensor([70, 5], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, heads, 3, hd, generator=torch.Generator(device="cuda").manual_seed(12), device="cuda").to(dtype)
+    _check(_each(q, cache, table, lens, hd**-0.5), q, cache, table, lens, hd**-0.5)
+
+
+@pytest.mark.parametrize("q_len", [1, 3, 70])
+def test_a_table_without_columns(q_len):
+    cache, _ = _filled(2, 50, 16, 2, 64, torch.int8, seed=2)
+    table = torch.zeros(2, 0, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([3, 0], dtype=torch.int32, device="cuda")
+    for out in _each(torch.ones(2, 4, q_len, 64, dtype=torch.bfloat16, device="cuda"), cache, table, lens, 0.1):
+        assert not bool(out.any())
+
+
 @pytest.mark.parametrize("q_len", [1, 4, 80])
 @pytest.mark.parametrize("scale,softcap", [(0.3, 5.0), (-0.1, 0.0), (0.0, 0.0)])
 def test_scale_and_softcap(q_len, scale, softcap):

@@ -61,6 +61,19 @@ def test_packed_attention(dtype, heads, kvh, hd, lens):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kvh,hd", [(4, 4, 128), (8, 2, 128), (11, 1, 64), (71, 1, 64), (131, 1, 128), (600, 2, 64)])
+@pytest.mark.parametrize("lens", [[32, 33, 31, 1], [96, 97, 95, 160]])
+def test_last_tiles_and_wide_groups(dtype, heads, kvh, hd, lens):
+    q, k, v, cu = _inputs(lens, heads, kvh, hd, dtype, seed=9)
+    some = sorted({0, 1, heads // 2 - 1, heads // 2, heads - 1})
+    _check(PackedAttention(heads, kvh, hd).forward(q, k, v, cu), q, k, v, cu, hd**-0.5, heads=some)
+    first, *_ = heads_first = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    out = torch.zeros_like(first)
+    assert PackedAttention(heads, kvh, hd).forward(*heads_first, cu, out=out) is out
+    _check(out, q, k, v, cu, hd**-0.5, heads=some)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_a_long_prompt(dtype):
     q, k, v, cu = _inputs([4001, 30], 8, 2, 128, dtype, seed=5)
     _check(PackedAttention(8, 2, 128).forward(q, k, v, cu), q, k, v, cu, 128**-0.5, heads=[0, 5])

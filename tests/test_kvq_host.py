@@ -256,6 +256,15 @@ def test_a_write_keeps_no_graph(fmt):
         assert not t.requires_grad
 
 
+def test_packed_out_whose_rows_overlap_is_refused():
+    q, k = torch.zeros(6, 4, 64, dtype=torch.float16), torch.zeros(6, 2, 64, dtype=torch.float16)
+    cu = torch.tensor([0, 6], dtype=torch.int32)
+    flat = torch.zeros(6 * 4 * 64, dtype=torch.float16)
+    for strides in ((0, 64, 1), (256, 0, 1), (128, 64, 1), (64, 128, 1), (256, 32, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.packed_attention(q, k, k, cu, 0.125, out=flat.as_strided((6, 4, 64), strides))
+
+
 def test_attention_refusals():
     cache = QuantizedPagedKVCache(1, 2, 4, 2, 64)
     table, lens = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
