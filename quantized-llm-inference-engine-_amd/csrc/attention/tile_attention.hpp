@@ -223,30 +223,43 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   };
   // Codes: lane l looks up key l of a tile, the table entry some tiles ahead of its use.
   struct Place {
-    uint32_t block, slot;  // (block, KV head) and slot of the lane's key; no key: some row of the cache
-    uint64_t mask;         // which keys there are
+    uint32_t block, row;  // the lane's key: its (block, KV head) and its row of the codes; no key: some row of the cache
+    uint64_t mask;        // which keys there are
   };
   struct Held {
     u32x4 codes[kCLoads > 0 ? kCLoads : 1];
     float scale[kCLoads > 0 ? kCLoads : 1];
   };
-  auto entry_of = [&](int i) -> int32_t {
-    const uint32_t t = uint32_t(i * kKeys + lane);
-    const uint32_t bi = t / a.block_size;
-    return int(t) < a.t_end && bi < a.ldb ? a.table[bi] : -1;
+  struct Look {
+    uint32_t bi, slot;  // the key's column in the table, and its slot
   };
-  auto place_of = [&](int i, int32_t entry) -> Place {
+  // Tile by tile without dividing again: a tile is tile_blocks blocks and tile_slots slots.
+  const uint32_t tile_blocks = SRC == kSrcCodes ? kKeys / a.block_size : 0u;
+  const uint32_t tile_slots = kKeys - tile_blocks * a.block_size;
+  auto look_at = [&](int i) -> Look {
+    const uint32_t t = uint32_t(i * kKeys + lane), bi = t / a.block_size;
+    return Look{bi, t - bi * a.block_size};
+  };
+  auto advance = [&](Look& l) {
+    l.slot += tile_slots;
+    const bool over = l.slot >= a.block_size;
+    l.slot -= over ? a.block_size : 0u;
+    l.bi += tile_blocks + (over ? 1u : 0u);
+  };
+  auto entry_of = [&](int i, const Look& l) -> int32_t {  // t_end is within the table
+    return i * kKeys + lane < a.t_end ? a.table[l.bi] : -1;
+  };
+  auto place_of = [&](const Look& l, int32_t entry) -> Place {
     const bool ok = entry >= 0 && uint32_t(entry) < a.num_blocks;
-    return Place{ok ? uint32_t(entry) * a.kv_heads + a.kvh : a.kvh, ok ? uint32_t(i * kKeys + lane) % a.block_size : 0u,
-                 __builtin_amdgcn_ballot_w64(ok)};
+    const uint32_t block = (ok ? uint32_t(entry) : 0u) * a.kv_heads + a.kvh;
+    return Place{block, block * a.block_size + l.slot, __builtin_amdgcn_ballot_w64(ok)};  // below 2^31: checked on the host
   };
   auto fetch_codes = [&](int k, const Place& p) -> Held {
     Held h;
 #pragma unroll
     for (int j = 0; j < kCLoads; ++j) {
       const int r = wave * kTr + kCrl * j + lane / kCpr;
-      const int64_t block = uint32_t(__shfl(int(p.block), r, 64));
-      const int64_t row = block * a.block_size + __shfl(int(p.slot), r, 64);
+      const int64_t block = uint32_t(__shfl(int(p.block), r, 64)), row = uint32_t(__shfl(int(p.row), r, 64));
       h.codes[j] = *reinterpret_cast<const u32x4*>(a.codes[k] + row * HD + 16 * (lane % kCpr));
       h.scale[j] = a.scales[k][block];
     }
@@ -256,8 +269,11 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
 #pragma unroll
     for (int j = 0; j < kCLoads; ++j) {
       const int r = wave * kTr + kCrl * j + lane / kCpr, c = 2 * (lane % kCpr);
-      const bool ok = k == 0 || ((mask >> r) & 1u);
       asm("" : "+v"(h.codes[j]));  // whole words until here
+      if (k == 1 && mask != ~uint64_t(0) && !((mask >> r) & 1u)) {  // no key: its probability is 0, its value must be finite
+        h.codes[j] = u32x4{0u, 0u, 0u, 0u};
+        h.scale[j] = 0.0f;
+      }
       const float s = h.scale[j];
       if (kRawKeys && k == 0 && lane % kCpr == 0) k_scales[(i & 1) * kKeys + r] = s;
 #pragma unroll
@@ -274,7 +290,6 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
             w[2 * e + 1] = scaled_pair<FMT, true>(x, s);
           }
         }
-        if (!ok) w = u32x4{0u, 0u, 0u, 0u};  // its probability is 0: its value must not be anything but finite
         const int at = k == 0 ? k_chunk<HD>(r, c + q) : v_chunk<HD>(r, c + q);
         *reinterpret_cast<u32x4*>((k == 0 ? k_buf(i) : v_buf(i)) + r * kRowBytes + 16 * at) = w;
       }
@@ -421,8 +436,10 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
         if (whole * kKeys <= wave_last) step(Blocks<1>{}, whole, ~uint64_t(0));
       }
     } else {
-      Place place = place_of(first_tile, entry_of(first_tile));
-      int32_t entry = entry_of(first_tile + 1);
+      Look look = look_at(first_tile);
+      Place place = place_of(look, entry_of(first_tile, look));
+      advance(look);
+      int32_t entry = entry_of(first_tile + 1, look);
       Held hk = fetch_codes(0, place), hv = fetch_codes(1, place);
       fetch_query();
       store_codes(0, first_tile, hk, place.mask);
@@ -434,10 +451,11 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
         __builtin_amdgcn_s_barrier();
         const uint64_t mask = place.mask;
         if (i + 1 < n_tiles) {
-          place = place_of(i + 1, entry);
+          place = place_of(look, entry);
           hk = fetch_codes(0, place);
           hv = fetch_codes(1, place);
-          entry = entry_of(i + 2);
+          advance(look);
+          entry = entry_of(i + 2, look);
         }
         if (i * kKeys <= wave_last) step(Blocks<2>{}, i, mask);
         if (i + 1 < n_tiles) {
