@@ -17,7 +17,7 @@ using namespace tile;
 constexpr int kThreads = 256;
 
 template <int FMT, bool QF16, int HD, bool CAP>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 && !CAP ? 3 : 2, HD == 64 && !CAP ? 3 : 2)))
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : 2, HD == 64 ? 3 : 2)))
     kvq_chunk_kernel(const KvqAttnArgs a) {
   constexpr int kRows = 128;
   __shared__ __align__(16) uint8_t lds[4 * kKeys * HD * 2 + (QF16 ? 2 * kKeys * 4 : 0)];
