@@ -2,11 +2,11 @@
 // over codes that it dequantizes exactly to bf16. fp16 queries: keys as fp16 operands, probabilities in two bf16 pieces. Few row
 // blocks (one long prompt's next chunk) are cut along the keys as well, and the parts merged as the decode kernel's are.
 //
-// Bound by issue: each of a CU's workgroups dequantizes its own tiles (a conversion per two codes and as many scalings, then
+// Bound by issue: each of a CU's workgroups dequantizes its own tiles (a conversion per two codes, for int8 as many scalings, then
 // 16-byte LDS stores), beside the softmax and the MFMAs. Measured (MI355X, 32 query and 8 KV heads of 128, e4m3 codes,
-// bf16): the next 512 tokens of 4 prompts with 4012 cached at most 132 us (760 TFLOP/s), by the scaled pair conversion of
-// e4m3 codes (163 by way of fp32) and by stepping through the table without a division (4 % of 138). Heads of 64 run three workgroups per CU, two with a soft cap (three spill; level: 276
-// against 273 us in bf16, 294 against 301 in fp16).
+// bf16): the next 512 tokens of 4 prompts with 4012 cached at most 127 us (796 TFLOP/s), by the scaled pair conversion of
+// e4m3 codes (163 by way of fp32) and by stepping through the table without a division (4 % of 135). Heads of 64 run three
+// workgroups per CU, heads of 128 two. With a soft cap 205 us for 166 (heads of 64: 170 for 122).
 #include "tile_attention.hpp"
 
 namespace llmopt {

@@ -188,8 +188,13 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
     for (int r = 0; r < 8; ++r) sc[r] = acc[r / 4][r % 4] * (score_scale * t.ks[UNI ? r / 4 : r]);
     if (capped) {
+      if (QT != kDtF32 && a.softcap <= kShortCap) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) sc[r] = tanhf(sc[r]) * cap2;
+        for (int r = 0; r < 8; ++r) sc[r] = short_cap(sc[r] * (2.0f * kLog2e), cap2);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) sc[r] = tanhf(sc[r]) * cap2;
+      }
     }
     const bool masked = t.bits != ~0u || t0 + 31 > first_pos;
     uint32_t keep = 0xFFu;

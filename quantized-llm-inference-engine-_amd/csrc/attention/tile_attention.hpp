@@ -82,17 +82,6 @@ __device__ __forceinline__ float other_half_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// tanh within 2^-21 of its value: its series up to x^9 below 0.3 (the next term is 5e-8 of it), else (1 - t) / (1 + t) with
-// t = e^(-2 |x|), of which 1 - t is off by 2^-22 at 0.3 and by less above. A capped score is then off by 2^-21 of itself, which the
-// probabilities' 8 or 11 bits do not show.
-__device__ __forceinline__ float tanh_of(float x) {
-  const float x2 = x * x;
-  const float near = x * __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, 62.0f / 2835, -17.0f / 315), 2.0f / 15), -1.0f / 3), 1.0f);
-  const float t = __builtin_amdgcn_exp2f(__builtin_fabsf(x) * (-2.0f * kLog2e));
-  const float far = (1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t);
-  return __builtin_fabsf(x) < 0.3f ? near : __builtin_copysignf(far, x);
-}
-
 // Place of 16-byte chunk c within row r of a K or V tile: 16 rows of one K chunk, and the four rows of a transposing
 // read of V, fall on distinct banks.
 template <int HD>
@@ -179,7 +168,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   const float magnitude = __builtin_fabsf(a.scale) * kLog2e;
   const float c2 = CAP ? kLog2e : magnitude > 0.0f ? magnitude : 1e-30f;
   const uint32_t q_sign = !CAP && a.scale < 0.0f ? 0x80008000u : 0u;
-  const float cap_scale = CAP ? a.scale / a.softcap : 0.0f;
+  const float cap_scale = CAP ? a.scale / a.softcap : 0.0f, cap_exp = cap_scale * (2.0f * kLog2e);
   float m_run = neg_inf, mc = 0.0f, l_run = 0.0f;  // the row's running maximum, m_run c2 (0 without keys), this lane's
                                                    // share of the sum
   f32x16 o[kD];
@@ -370,10 +359,17 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
     }
     const int t0 = i * kKeys;
     if constexpr (CAP) {
+      if (a.softcap <= kShortCap) {
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
+        for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) sc.s[kb][v] = tanh_of(sc.s[kb][v] * cap_scale) * a.softcap;
+          for (int v = 0; v < 16; ++v) sc.s[kb][v] = short_cap(sc.s[kb][v] * cap_exp, a.softcap);
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sc.s[kb][v] = tanh_of(sc.s[kb][v] * cap_scale) * a.softcap;
+      }
     }
     if (mask != ~uint64_t(0) || t0 + kKeys - 1 > first_pos) {
 #pragma unroll

@@ -291,6 +291,15 @@ def test_scale_and_softcap(q_len, scale, softcap):
         _check(_each(q.to(dtype), cache, table, lens, scale, softcap), q.to(dtype), cache, table, lens, scale, softcap)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("scale,softcap", [(0.5, 64.0), (0.5, 65.0), (-0.3, 1e5), (0.5, 0.25)])
+def test_soft_caps_of_both_kinds(dtype, scale, softcap):
+    cache, table = _filled(2, 150, 16, 2, 64, torch.int8, seed=13)
+    lens = torch.tensor([150, 40], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 4, 33, 64, generator=torch.Generator(device="cuda").manual_seed(14), device="cuda").to(dtype)
+    _check(_each(q, cache, table, lens, scale, softcap), q, cache, table, lens, scale, softcap)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("q_len", [1, 48])

@@ -85,6 +85,13 @@ def test_scale_and_softcap(scale, softcap):
     _check(PackedAttention(4, 2, 128, scale=scale, softcap=softcap).forward(q, k, v, cu), q, k, v, cu, scale, softcap)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale,softcap", [(0.5, 64.0), (0.5, 65.0), (-0.3, 1e5), (0.5, 0.25)])
+def test_soft_caps_of_both_kinds(dtype, scale, softcap):
+    q, k, v, cu = _inputs([150, 31], 4, 2, 64, dtype, seed=10)
+    _check(PackedAttention(4, 2, 64, scale=scale, softcap=softcap).forward(q, k, v, cu), q, k, v, cu, scale, softcap)
+
+
 def test_rows_behind_the_last_sequence():
     q, k, v, cu = _inputs([50, 20], 8, 2, 64, torch.bfloat16, padding=90, seed=3)
     for t in (q, k, v):
