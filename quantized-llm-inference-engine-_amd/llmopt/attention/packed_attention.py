@@ -12,6 +12,8 @@ from __future__ import annotations
 
 import torch
 
+from llmopt.attention.paged_attention import AttentionBackend
+
 __all__ = ["PackedAttention"]
 
 
@@ -24,10 +26,11 @@ class PackedAttention:
         head_dim: Per-head dimension.
         scale: Softmax scale, ``head_dim ** -0.5`` by default.
         softcap: With a positive value, scores become ``tanh(score / softcap) * softcap``.
+        backend: ``"auto"``, ``"hip"`` or ``"sdpa"`` (see :class:`AttentionBackend`).
     """
 
     def __init__(self, num_heads: int, num_kv_heads: int, head_dim: int, scale: float | None = None,
-                 softcap: float = 0.0) -> None:
+                 softcap: float = 0.0, backend: str = "auto") -> None:
         if num_kv_heads < 1 or num_heads < 1 or num_heads % num_kv_heads != 0:
             raise ValueError("num_heads must be a positive multiple of num_kv_heads")
         if head_dim < 1:
@@ -38,6 +41,7 @@ class PackedAttention:
         self.group_size = num_heads // num_kv_heads
         self.scale = scale if scale is not None else head_dim**-0.5
         self.softcap = softcap
+        self.backend = AttentionBackend.detect(backend)
 
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tensor,
                 out: torch.Tensor | None = None) -> torch.Tensor:
@@ -46,7 +50,7 @@ class PackedAttention:
         ``cu_seqlens [sequences + 1]`` starts at 0 and does not fall. Returns ``[tokens, heads, head_dim]`` in the
         query's dtype; rows behind the last sequence are zeros, in a given ``out`` left as they were.
 
-        fp32, head dims other than 64 and 128, host tensors, and inputs that need a gradient (the kernel has no
+        fp32, head dims other than 64 and 128, host tensors, backends other than ``"hip"``, and inputs that need a gradient (the kernel has no
         backward pass) run the same sums in torch, one sequence at a time.
         """
         if tuple(query.shape[1:]) != (self.num_heads, self.head_dim) or query.dim() != 3 \
@@ -55,7 +59,7 @@ class PackedAttention:
                              f"{self.num_kv_heads}, {self.head_dim}], got {tuple(query.shape)}, {tuple(key.shape)}, "
                              f"{tuple(value.shape)}")
         grad = torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad)
-        if query.device.type == "cuda" and not grad:
+        if self.backend == "hip" and query.device.type == "cuda" and not grad:
             from llmopt.kernels import ops
 
             try:

@@ -134,7 +134,12 @@ class PagedAttentionLayer(nn.Module):
         self.fused_ops = True  # False: the torch rotary sequence even on HIP devices
         self.attn = PagedAttention(self.num_heads, self.num_kv_heads, self.head_dim,
                                    config=PagedAttentionConfig(block_size=16), backend=backend)
-        self.packed = PackedAttention(self.num_heads, self.num_kv_heads, self.head_dim)
+
+    @property
+    def packed(self) -> PackedAttention:
+        """The attention of packed prompts, with the scale, soft cap and backend that ``attn`` has now."""
+        return PackedAttention(self.num_heads, self.num_kv_heads, self.head_dim, scale=self.attn.scale,
+                               softcap=self.attn.config.softcap, backend=self.attn.backend)
 
     def fuse_qkv(self) -> bool:
         """Merge quantized q, k and v projections into one :class:`FusedQuantLinear`."""
