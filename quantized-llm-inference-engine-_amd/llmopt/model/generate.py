@@ -96,7 +96,6 @@ class GreedyGenerator:
         out = torch.empty(seqs, steps, dtype=torch.long, device=dev)
 
         # ---- prefill ----
-        offsets = torch.zeros(seqs, dtype=torch.int32, device=dev)
         if ragged:
             ids = torch.cat([p.to(dev) for p in prompts])
             pos = torch.cat([torch.arange(n, device=dev) for n in lengths])
@@ -108,11 +107,10 @@ class GreedyGenerator:
             ids = prompts.to(dev).reshape(-1)
             pos = torch.arange(plen, device=dev).repeat(seqs)
             lens = torch.full((seqs,), plen, dtype=torch.int32, device=dev)
-            shape = {"q_len": plen}
+            shape = {"q_len": plen, "token_offsets": torch.zeros(seqs, dtype=torch.int32, device=dev)}
         self._sync()
         t0 = time.perf_counter()
-        logits = self.model(ids, pos, cache=cache, block_ids=table, context_lens=lens, token_offsets=offsets,
-                            last_only=True, **shape).last_logits()
+        logits = self.model(ids, pos, cache=cache, block_ids=table, context_lens=lens, last_only=True, **shape).last_logits()
         out[:, 0] = _argmax(logits)
         self._sync()
         prefill_s = time.perf_counter() - t0

@@ -30,6 +30,19 @@ def _hip(x: torch.Tensor) -> bool:
     return x.device.type == "cuda" and x.dtype in (torch.bfloat16, torch.float16)
 
 
+def whole_prompt_offsets(token_offsets: torch.Tensor | None) -> torch.Tensor | None:
+    """The offsets of packed prompts, which attend over their own rows only: none may begin behind cached tokens. None
+    where all are 0."""
+    if token_offsets is None:
+        return None
+    if token_offsets.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise ValueError("packed prompts begin at position 0: leave token_offsets out where a graph is captured")
+    if bool((token_offsets > 0).any()):
+        raise ValueError("packed prompts are whole and begin at position 0: token_offsets > 0 would skip the cached "
+                         "tokens in front of them (continue such prompts with context_lens and q_len)")
+    return token_offsets if bool((token_offsets < 0).any()) else None
+
+
 class RMSNorm(nn.Module):
     """``x / sqrt(mean(x^2) + eps) * weight`` in fp32, returned in the input dtype
     (``layers.py:14-31``)."""
@@ -113,8 +126,10 @@ class PagedAttentionLayer(nn.Module):
 
     With ``cu_seqlens [seq + 1]`` the rows are whole prompts of different lengths, packed one after the other
     (:class:`PackedAttention`): each attends causally over its own keys and values as they are computed, which go
-    into the cache, if there is one, from ``token_offsets`` (default 0); the cache is a
-    :class:`llmopt.cache.QuantizedPagedKVCache`, and ``context_lens`` and ``q_len`` are not used.
+    into the cache, if there is one, from position 0; the cache is a
+    :class:`llmopt.cache.QuantizedPagedKVCache`, and ``context_lens`` and ``q_len`` are not used. What is cached already
+    is not attended over, so positive ``token_offsets`` raise ``ValueError`` (a negative one keeps its sequence out of the
+    cache); they are read for that, which waits for the device, and left out in a captured graph.
     """
 
     def __init__(self, config: object, layer_idx: int, backend: str = "auto") -> None:
@@ -261,6 +276,7 @@ class PagedAttentionLayer(nn.Module):
         if cache is not None and block_ids is not None:
             if not hasattr(cache, "write_packed"):
                 raise TypeError(f"packed prompts need a QuantizedPagedKVCache, not a {type(cache).__name__}")
+            token_offsets = whole_prompt_offsets(token_offsets)
             if token_offsets is None:
                 token_offsets = torch.zeros(int(cu_seqlens.shape[0]) - 1, dtype=torch.int32, device=q.device)
             cache.write_packed(self.layer_idx, block_ids, token_offsets, cu_seqlens, k, v)

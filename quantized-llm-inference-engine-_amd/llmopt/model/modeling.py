@@ -20,7 +20,7 @@ from torch import nn
 
 from llmopt.logits import last_token_hidden
 from llmopt.model.config import ModelConfig
-from llmopt.model.layers import DecoderLayer, RMSNorm
+from llmopt.model.layers import DecoderLayer, RMSNorm, whole_prompt_offsets
 
 __all__ = ["DecoderOnlyModel", "ModelOutput", "fuse_projections_", "random_quantized_model", "reference_twin"]
 
@@ -71,6 +71,8 @@ class DecoderOnlyModel(nn.Module):
         if token_offsets is None and context_lens is not None and block_ids is not None and cu_seqlens is None:
             # Where this step's tokens go in the cache: computed once here, not in every layer.
             token_offsets = context_lens - q_len
+        if cu_seqlens is not None and token_offsets is not None and cache is not None and block_ids is not None:
+            token_offsets = whole_prompt_offsets(token_offsets)  # read once here, not in every layer
         pending = None  # each layer's MLP output, added inside the next norm's kernel
         last = len(self.layers) - 1
         # The final norm takes the last layer's partial sums too unless it first keeps only each

@@ -33,3 +33,29 @@ def test_packed_prompts_follow_the_layers_attention(scale, softcap):
                         q_len=9).logits.reshape(18, -1)
     # the same fp32 sums in another order, through two layers
     torch.testing.assert_close(packed, uniform, atol=1e-5, rtol=1e-4)
+
+
+def test_packed_prompts_behind_cached_tokens_are_refused():
+    """Packed prompts attend over their own rows only, so a cached prefix in front of them would be lost."""
+    model = _model()
+    cache = model.allocate_cache(4, 16, torch.int8, "cpu")
+    table = torch.arange(4, dtype=torch.int32).view(2, 2)
+    ids, positions, cu = torch.arange(12), torch.arange(6).repeat(2), torch.tensor([0, 6, 12])
+    layer, hidden = model.layers[0].self_attn, torch.randn(12, model.config.hidden_size)
+    with torch.no_grad():
+        for offsets in (torch.tensor([0, 3]), torch.tensor([[4], [0]], dtype=torch.int32)):
+            with pytest.raises(ValueError, match="position 0"):
+                model(ids, positions, cache=cache, block_ids=table, token_offsets=offsets, cu_seqlens=cu)
+            with pytest.raises(ValueError, match="position 0"):
+                layer(hidden, positions, cache, table, token_offsets=offsets, cu_seqlens=cu)
+        assert not bool(cache.key_codes.any())
+        want = model(ids, positions, cache=cache, block_ids=table, cu_seqlens=cu).logits
+        codes = cache.key_codes.clone()
+        cache.reset()
+        # zeros are the default, and a negative offset keeps its sequence out of the cache
+        got = model(ids, positions, cache=cache, block_ids=table, token_offsets=torch.tensor([0, -1]), cu_seqlens=cu).logits
+        assert torch.equal(got, want) and not bool(cache.key_codes[:, 2:].any())
+        model(ids, positions, cache=cache, block_ids=table, token_offsets=torch.zeros(2, dtype=torch.int32), cu_seqlens=cu)
+        assert torch.equal(cache.key_codes, codes)
+        # without a cache there is nothing in front of them
+        assert torch.equal(model(ids, positions, token_offsets=torch.tensor([0, 3]), cu_seqlens=cu).logits, want)
