@@ -20,6 +20,8 @@ from dataclasses import dataclass
 
 import torch
 
+from llmopt.cache import QuantizedPagedKVCache
+
 __all__ = ["GenerationResult", "GreedyGenerator"]
 
 
@@ -50,7 +52,8 @@ def _argmax(logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tens
 
 class GreedyGenerator:
     """Greedy decoding of a batch of prompts with ``model``: of equal length, or over an 8-bit cache of any
-    lengths, which are prefilled packed.
+    lengths. Over an 8-bit cache prompts are prefilled packed, in either form: they attend over their own keys and
+    values as computed, and the decode steps over the quantized ones.
 
     Args:
         model: a :class:`DecoderOnlyModel` (any device).
@@ -77,8 +80,9 @@ class GreedyGenerator:
     def generate(self, prompts: torch.Tensor | Sequence[torch.Tensor], steps: int,
                  forced: torch.Tensor | None = None) -> GenerationResult:
         """Generate ``steps`` tokens per prompt (``prompts [seq, prompt_len]``, or a list of prompts ``[n]``
-        of any lengths from 1, for a ``cache_dtype`` of 8 bits). With ``forced [seq, steps]`` the step inputs are those tokens instead of the argmax (teacher forcing);
-        ``tokens`` then still holds the argmax of every step."""
+        of any lengths from 1, for a ``cache_dtype`` of 8 bits). With ``forced [seq, steps]`` the step
+        inputs are those tokens instead of the argmax (teacher forcing); ``tokens`` then still holds
+        the argmax of every step."""
         if steps < 1:
             raise ValueError("steps must be >= 1")
         dev = self.device
@@ -96,8 +100,9 @@ class GreedyGenerator:
         out = torch.empty(seqs, steps, dtype=torch.long, device=dev)
 
         # ---- prefill ----
-        if ragged:
-            ids = torch.cat([p.to(dev) for p in prompts])
+        if ragged or isinstance(cache, QuantizedPagedKVCache):
+            lengths = lengths if ragged else [plen] * seqs
+            ids = torch.cat([p.to(dev) for p in prompts]) if ragged else prompts.to(dev).reshape(-1)
             pos = torch.cat([torch.arange(n, device=dev) for n in lengths])
             lens = torch.tensor(lengths, dtype=torch.int32, device=dev)
             cu = torch.zeros(seqs + 1, dtype=torch.int32, device=dev)

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from llmopt.attention import PagedAttention, PagedAttentionConfig
-from llmopt.model import DecoderOnlyModel, ModelConfig
+from llmopt.model import DecoderOnlyModel, GreedyGenerator, ModelConfig
 
 
 def _model(seed=0):
@@ -59,3 +59,12 @@ def test_packed_prompts_behind_cached_tokens_are_refused():
         assert torch.equal(cache.key_codes, codes)
         # without a cache there is nothing in front of them
         assert torch.equal(model(ids, positions, token_offsets=torch.tensor([0, 3]), cu_seqlens=cu).logits, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+def test_prompts_of_one_length_in_either_form(dtype):
+    """A tensor of prompts and a list of the same prompts are the same prefill over an 8-bit cache."""
+    generator = GreedyGenerator(_model(2), block_size=8, cache_dtype=dtype)
+    prompts = torch.randint(0, 512, (3, 13))
+    a, b = generator.generate(prompts, 5), generator.generate(list(prompts), 5)
+    assert torch.equal(a.prefill_logits, b.prefill_logits) and torch.equal(a.tokens, b.tokens)
