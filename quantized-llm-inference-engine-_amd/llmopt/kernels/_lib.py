@@ -171,8 +171,17 @@ def library_path() -> Path:
     return Path(__file__).resolve().parent / "libllmopt_qlinear.so"
 
 
+def _missing(path: Path, name: str):  # noqa: ANN202
+    def entry(*_args):  # noqa: ANN002, ANN202
+        raise RuntimeError(f"{path} has no {name}: it was built from earlier sources. Build it again with "
+                           "`python -m llmopt.kernels.build`")
+
+    return entry
+
+
 def load_library() -> ctypes.CDLL:
-    """Load (once) and return the kernel library; raise if it has not been built."""
+    """Load (once) and return the kernel library; raise if it has not been built. A library of this ABI version from
+    before some entry point was added serves the others, and a call of that one raises."""
     global _handle
     if _handle is not None:
         return _handle
@@ -185,13 +194,17 @@ def load_library() -> ctypes.CDLL:
                     "`python -m llmopt.kernels.build` (hipcc, gfx950)"
                 )
             lib = ctypes.CDLL(str(path))
-            for name, (restype, argtypes) in _SIGNATURES.items():
-                fn = getattr(lib, name)
-                fn.restype = restype
-                fn.argtypes = argtypes
             version = lib.llmopt_q_abi_version()
             if version != ABI_VERSION:
                 raise RuntimeError(f"{path} has ABI version {version}, expected {ABI_VERSION}")
+            for name, (restype, argtypes) in _SIGNATURES.items():
+                try:
+                    fn = getattr(lib, name)
+                except AttributeError:
+                    setattr(lib, name, _missing(path, name))
+                    continue
+                fn.restype = restype
+                fn.argtypes = argtypes
             _handle = lib
     return _handle
 
@@ -207,8 +220,8 @@ def binding_path() -> Path:
 def load_binding():  # noqa: ANN201 - the extension module, or None
     """Load (once) and return the native host path of the linears, of the 8-bit KV cache and of packed
     attention (``csrc/torch_binding.cpp``), with
-    the kernel library's entry points attached. None, with one warning, where it is not built or does not
-    load into this torch: calls then take the general path, the same kernels through ctypes."""
+    the kernel library's entry points attached. None, with one warning, where it is not built, does not
+    load into this torch, or it or the library is from before an entry point that it attaches: calls then take the general path, the same kernels through ctypes."""
     global _binding, _binding_tried
     if _binding_tried:
         return _binding
@@ -231,7 +244,7 @@ def load_binding():  # noqa: ANN201 - the extension module, or None
                     "llmopt_kvq_write", "llmopt_kvq_attention_workspace", "llmopt_kvq_attention",
                     "llmopt_packed_attention")))
                 _binding = module
-            except (ImportError, OSError) as exc:
+            except (ImportError, OSError, AttributeError, ctypes.ArgumentError) as exc:
                 warnings.warn(f"the linears' native host path is not available ({exc}); calls go through ctypes, "
                               "some 10 us longer each. Build it with `python -m llmopt.kernels.build`",
                               RuntimeWarning, stacklevel=2)
