@@ -13,6 +13,7 @@ from __future__ import annotations
 import torch
 
 from llmopt.attention.paged_attention import AttentionBackend
+from llmopt.utils.autograd import is_differentiated
 
 __all__ = ["PackedAttention"]
 
@@ -50,15 +51,15 @@ class PackedAttention:
         ``cu_seqlens [sequences + 1]`` starts at 0 and does not fall. Returns ``[tokens, heads, head_dim]`` in the
         query's dtype; rows behind the last sequence are zeros, in a given ``out`` left as they were.
 
-        fp32, head dims other than 64 and 128, host tensors, backends other than ``"hip"``, and inputs that need a gradient (the kernel has no
-        backward pass) run the same sums in torch, one sequence at a time.
+        fp32, head dims other than 64 and 128, host tensors, backends other than ``"hip"``, and inputs that need a
+        gradient or carry a tangent (the kernel has no derivative) run the same sums in torch, one sequence at a time.
         """
         if tuple(query.shape[1:]) != (self.num_heads, self.head_dim) or query.dim() != 3 \
                 or tuple(key.shape) != (query.shape[0], self.num_kv_heads, self.head_dim) or key.shape != value.shape:
             raise ValueError(f"expected query [tokens, {self.num_heads}, {self.head_dim}] and key, value [tokens, "
                              f"{self.num_kv_heads}, {self.head_dim}], got {tuple(query.shape)}, {tuple(key.shape)}, "
                              f"{tuple(value.shape)}")
-        grad = torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad)
+        grad = is_differentiated(query, key, value)
         if self.backend == "hip" and query.device.type == "cuda" and not grad:
             from llmopt.kernels import ops
 
