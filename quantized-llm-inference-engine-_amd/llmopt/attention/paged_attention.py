@@ -18,6 +18,7 @@ from dataclasses import dataclass
 import torch
 
 from llmopt.cache.quantized_cache import QuantizedPagedKVCache
+from llmopt.utils.autograd import is_differentiated
 from llmopt.utils.logging import get_logger
 
 __all__ = ["AttentionBackend", "PagedAttention", "PagedAttentionConfig", "merge_states"]
@@ -120,17 +121,19 @@ class PagedAttention:
         context length after this step's K/V were written. Returns ``[seq, heads, q_len, head_dim]``
         in the query's dtype. ``cache`` is a :class:`PagedKVCache` or a :class:`QuantizedPagedKVCache`.
         Query position ``i`` of a sequence sits at ``ctx - q_len + i`` and
-        sees keys up to and including its own position.
+        sees keys up to and including its own position. A query that needs a gradient or carries a tangent
+        takes the torch sequence over a :class:`QuantizedPagedKVCache` (its kernels have no derivative).
         """
         seqs = int(query.shape[0])
         q_len = query_lens if query_lens is not None else int(query.shape[2])
         if q_len == 0:
             return torch.zeros((seqs, self.num_heads, 0, self.head_dim), dtype=query.dtype, device=query.device)
-        if self.backend == "hip" and query.device.type == "cuda":
+        quantized = isinstance(cache, QuantizedPagedKVCache)
+        if self.backend == "hip" and query.device.type == "cuda" and not (quantized and is_differentiated(query)):
             from llmopt.kernels import ops
 
             try:
-                if isinstance(cache, QuantizedPagedKVCache):
+                if quantized:
                     return ops.cache_attention(query, cache, layer_idx, block_ids, context_lens, q_len, self.scale,
                                                self.config.softcap)
                 if q_len == 1:

@@ -7,7 +7,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from llmopt.attention import PackedAttention
+from llmopt.attention import PackedAttention, PagedAttention
+from llmopt.cache import QuantizedPagedKVCache
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +36,35 @@ def test_a_tangent_through_packed_prompts(which):
     # the same fp32 sums on the host, each rounded once to bf16: one step apart at most where they round apart
     for a, b in zip(got, want):
         torch.testing.assert_close(a.cpu().float(), b.float(), atol=2.0**-8, rtol=2.0**-7)
+
+
+@pytest.mark.parametrize("q_len", [1, 5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_querys_derivatives_over_the_8_bit_cache(dtype, q_len):
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    cache = QuantizedPagedKVCache(1, 8, 16, 2, 64, device="cuda")
+    table = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    lens = torch.tensor([50, 31], dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(2, 64, 2, 64, generator=gen, device="cuda") for _ in range(2))
+    cache.write(0, table, torch.zeros_like(lens), k, v)
+    host = QuantizedPagedKVCache.from_tensors(*(t.cpu() for t in (cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales)))
+    q, weight = (torch.randn(2, 4, q_len, 64, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    attention = PagedAttention(4, 2, 64)
+    plain = attention.forward(q, cache, 0, table, lens)
+    assert not plain.requires_grad
+    grads, tangents = [], []
+    for dev, store in (("cuda", cache), ("cpu", host)):
+        leaf = q.detach().to(dev).requires_grad_()
+        out = attention.forward(leaf, store, 0, table.to(dev), lens.to(dev))
+        (out.float() * weight.to(dev).float()).sum().backward()
+        grads.append(leaf.grad.cpu().float())
+        with torch.no_grad():
+            assert not attention.forward(leaf, store, 0, table.to(dev), lens.to(dev)).requires_grad
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(q.to(dev), weight.to(dev))
+            tangents.append(forward_ad.unpack_dual(attention.forward(dual, store, 0, table.to(dev), lens.to(dev))).tangent.cpu().float())
+    # fp32 sums of 50 terms of some units, of which bf16 results are rounded once
+    atol, rtol = (2.0**-8, 2.0**-7) if dtype == torch.bfloat16 else (1e-5, 1e-4)
+    for a, b in (grads, tangents):
+        assert bool(b.any())
+        torch.testing.assert_close(a, b, atol=atol, rtol=rtol)
