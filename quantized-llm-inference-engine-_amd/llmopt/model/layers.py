@@ -22,6 +22,7 @@ from llmopt.attention.paged_attention import PagedAttention, PagedAttentionConfi
 from llmopt.model.rotary import RotaryEmbedding, apply_rotary_pos_emb
 from llmopt.quantization.fused import FusedQuantLinear, QuantSwiGLU
 from llmopt.quantization.quant_linear import QuantLinear
+from llmopt.utils.autograd import is_differentiated
 
 __all__ = ["DecoderLayer", "PagedAttentionLayer", "RMSNorm", "SwiGLUMLP"]
 
@@ -265,7 +266,7 @@ class PagedAttentionLayer(nn.Module):
         q = q.reshape(total, self.num_heads, self.head_dim)
         k = k.reshape(total, self.num_kv_heads, self.head_dim)
         v = v.reshape(total, self.num_kv_heads, self.head_dim)
-        if self.fused_ops and _hip(q):
+        if self.fused_ops and _hip(q) and not is_differentiated(q, k):  # the rotary kernel has no derivative
             from llmopt.kernels import ops
 
             self.rotary.check(positions)

@@ -9,6 +9,8 @@ from torch.autograd import forward_ad
 
 from llmopt.attention import PackedAttention, PagedAttention
 from llmopt.cache import QuantizedPagedKVCache
+from llmopt.model import ModelConfig
+from llmopt.model.layers import PagedAttentionLayer
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +70,29 @@ def test_a_querys_derivatives_over_the_8_bit_cache(dtype, q_len):
     for a, b in (grads, tangents):
         assert bool(b.any())
         torch.testing.assert_close(a, b, atol=atol, rtol=rtol)
+
+
+@pytest.mark.parametrize("cached", [False, True])
+def test_a_gradient_through_a_layers_packed_prompts(cached):
+    """Every term of it, those through the rotated queries and keys among them: against the layer without fused steps."""
+    torch.manual_seed(3)
+    config = ModelConfig.tiny()
+    layer = PagedAttentionLayer(config, 0).to("cuda", torch.bfloat16)
+    cu = torch.tensor([0, 11, 24], dtype=torch.int32, device="cuda")
+    positions = torch.cat([torch.arange(11), torch.arange(13)]).cuda()
+    hidden, weight = (torch.randn(24, config.hidden_size, device="cuda").bfloat16() for _ in range(2))
+    sides = []
+    for fused in (True, False):
+        layer.fused_ops = fused
+        layer.zero_grad()
+        cache = QuantizedPagedKVCache(1, 4, 16, config.num_key_value_heads, config.head_dim, device="cuda") if cached else None
+        table = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2) if cached else None
+        leaf = hidden.clone().requires_grad_()
+        (layer(leaf, positions, cache, table, cu_seqlens=cu) * weight).float().sum().backward()
+        sides.append([leaf.grad] + [p.weight.grad for p in (layer.q_proj, layer.k_proj, layer.v_proj, layer.o_proj)])
+    for a, b in zip(*sides):
+        assert b is not None and bool(b.any())
+        assert torch.equal(a, b)  # the same torch operations
+    with torch.no_grad():  # and without a gradient the kernels, as before
+        layer.fused_ops = True
+        assert not layer(hidden, positions, cu_seqlens=cu).requires_grad
