@@ -82,7 +82,8 @@ int llmopt_kvq_attention(const void* query, int q_dtype, int64_t q_seq_stride, i
  * Causal attention over packed prompts: sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 of query
  * [total_tokens, num_heads, head_dim] and key / value [total_tokens, kv_heads, head_dim] (token and head strides in
  * elements, all of dtype F16 or BF16); a token sees its sequence's tokens up to itself. cu_seqlens starts at 0
- * and does not fall. Rows behind the last sequence are cleared in out (zero_tail) or left as they are. Supported:
+ * and does not fall. Rows behind the last sequence are cleared in out (zero_tail) or left as they are. out shares no
+ * memory with query, key or value, nor one of its rows with another. Supported:
  * head_dim 64 or 128, any number of heads per KV head, every row 16-byte aligned (pointers and strides); otherwise
  * LLMOPT_ERR_UNSUPPORTED.
  */

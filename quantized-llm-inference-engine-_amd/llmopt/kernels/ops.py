@@ -816,12 +816,30 @@ def kvq_attention(query: torch.Tensor, key_codes: torch.Tensor, key_scales: torc
     return view
 
 
+def _may_share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two ``[rows, heads, d]`` tensors of one element size may have an element in common: their extents meet, and
+    they are not side by side within rows of one stride (as slices of a fused projection's output are)."""
+    size = a.element_size()
+
+    def extent(t: torch.Tensor, dims: range) -> int:
+        return size * (1 + sum((t.shape[d] - 1) * t.stride(d) for d in dims))
+
+    if a.numel() == 0 or b.numel() == 0 or a.data_ptr() + extent(a, range(3)) <= b.data_ptr() \
+            or b.data_ptr() + extent(b, range(3)) <= a.data_ptr():
+        return False
+    row = a.stride(0) * size
+    if row == 0 or a.stride(0) != b.stride(0):
+        return True
+    ahead = (b.data_ptr() - a.data_ptr()) % row  # where b's rows begin, counted from a's
+    return ahead < extent(a, range(1, 3)) or ahead + extent(b, range(1, 3)) > row
+
+
 def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tensor,
                      scale: float, softcap: float = 0.0, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention over packed prompts: ``query [tokens, heads, head_dim]``, ``key``/``value`` ``[tokens, kv_heads,
     head_dim]`` (fp16 or bf16, any token and head strides), sequence ``s`` the rows ``cu_seqlens[s]`` up to
-    ``cu_seqlens[s + 1]``. Rows behind the last sequence are zeros, in a given ``out`` left as they were. Raises
-    ``NotImplementedError`` for fp32 and for head dims other than 64 and 128."""
+    ``cu_seqlens[s + 1]``. Rows behind the last sequence are zeros, in a given ``out`` left as they were; an ``out`` that
+    may share memory with the inputs is computed beside it and copied. Raises ``NotImplementedError`` for fp32 and for head dims other than 64 and 128."""
     binding = load_binding() if out is None and query.is_cuda else None
     if binding is not None:  # the plain form of a call, in native code
         result = binding.packed_attention(query, key, value, cu_seqlens, scale, softcap)
@@ -860,7 +878,8 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     result = out
     if out is None:
         result = torch.empty(tokens, heads, hd, dtype=query.dtype, device=dev)
-    elif not rows16(out):
+    elif not rows16(out) or any(_may_share_memory(out, t) for t in (query, key, value)):
+        # Workgroups read query, key and value rows that others have finished.
         result = out.clone(memory_format=torch.contiguous_format)
     if tokens:
         cu = _int32(cu_seqlens, dev)
