@@ -862,11 +862,11 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if out is not None and (out.shape != query.shape or out.dtype != query.dtype):
         raise ValueError(f"packed_attention: out must be {tuple(query.shape)} {query.dtype}")
     if out is not None:  # rows that share memory would be written by several workgroups
-        extent = hd
-        for stride, size in sorted((out.stride(d), out.shape[d]) for d in (0, 1)):
-            if size > 1 and stride < extent:
+        extent = 1  # of what the smaller strides span
+        for stride, size in sorted((out.stride(d), out.shape[d]) for d in range(3) if out.shape[d] > 1):
+            if stride < extent:
                 raise ValueError(f"packed_attention: out's rows overlap (strides {out.stride()})")
-            extent = max(extent, stride * (size - 1) + extent)
+            extent += stride * (size - 1)
     if query.dtype == torch.float32 or hd not in (64, 128):
         raise NotImplementedError(f"packed_attention: {query.dtype}, head_dim {hd}")
 

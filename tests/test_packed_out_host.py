@@ -61,3 +61,22 @@ def test_what_may_share_memory():
         agree += may == share
     assert agree > 0.8 * len(views) ** 2  # it may say so of rows that only pass each other
     assert not ops._may_share_memory(flat[:0].view(0, 2, 4), views[0])
+
+
+def test_out_in_any_order_of_its_dimensions(launched):
+    """Only an out whose own elements share memory is refused, whichever of its strides is the inner one."""
+    q, k = torch.zeros(6, 4, 64).half(), torch.zeros(6, 2, 64).half()
+    flat = torch.zeros(4 * 6 * 4 * 64).half()
+    for strides in ((256, 1, 4), (1, 384, 6), (64, 384, 1), (512, 128, 2), (1, 6, 24), (256, 64, 1)):
+        out = flat.as_strided((6, 4, 64), strides)
+        assert len(_elements(out)) == out.numel()
+        assert ops.packed_attention(q, k, k, CU, 0.125, out=out) is out
+    launched.clear()
+    for strides in ((256, 64, 2), (256, 1, 1), (128, 1, 2), (0, 1, 4), (1, 1, 8)):
+        out = flat.as_strided((6, 4, 64), strides)
+        assert len(_elements(out)) < out.numel()
+        with pytest.raises(ValueError, match="overlap"):
+            ops.packed_attention(q, k, k, CU, 0.125, out=out)
+    assert not launched
+    one = flat.as_strided((1, 4, 64), (0, 64, 1))  # a stride that nothing steps along
+    ops.packed_attention(q[:1], k[:1], k[:1], CU, 0.125, out=one)
