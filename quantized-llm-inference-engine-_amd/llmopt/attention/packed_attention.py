@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import torch
 
-from llmopt.attention.paged_attention import AttentionBackend
+from llmopt.attention.paged_attention import AttentionBackend, weighted_values
 from llmopt.utils.autograd import is_differentiated
 
 __all__ = ["PackedAttention"]
@@ -86,7 +86,7 @@ class PackedAttention:
                 scores = torch.tanh(scores / self.softcap) * self.softcap
             hidden = torch.ones(hi - lo, hi - lo, dtype=torch.bool, device=query.device).triu(1)
             scores = scores.masked_fill(hidden, float("-inf"))
-            parts.append(torch.matmul(torch.softmax(scores, -1), v).transpose(0, 1).to(query.dtype))
+            parts.append(weighted_values(torch.softmax(scores, -1), ~hidden, v).transpose(0, 1).to(query.dtype))
         if out is not None:
             if len(cu) > 1:
                 out[cu[0] : cu[-1]] = torch.cat(parts[1:])

@@ -75,6 +75,24 @@ class AttentionBackend:
         raise ValueError(f"unknown attention backend: {requested!r}")
 
 
+def weighted_values(probs: torch.Tensor, visible: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+    """``probs [..., rows, keys] @ v [..., keys, d]`` in which a key that is not ``visible [..., rows, keys]`` to a row does
+    not reach it, whatever its value is: in a plain product a weight of 0 times an infinity or NaN would."""
+    out = torch.matmul(probs, v)
+    if bool(out.isfinite().all()):
+        return out
+
+    def reached(weights: torch.Tensor, what: torch.Tensor) -> torch.Tensor:
+        return torch.matmul(weights.to(v.dtype).expand(probs.shape), what.to(v.dtype)) > 0
+
+    plus, minus = v == torch.inf, v == -torch.inf
+    some, zero = visible & (probs > 0), visible & (probs == 0)
+    up, down = reached(some, plus), reached(some, minus)
+    unknown = reached(visible, v.isnan()) | reached(zero, plus | minus) | (up & down)
+    extra = torch.zeros_like(out).masked_fill(up, torch.inf).masked_fill(down, -torch.inf).masked_fill(unknown, torch.nan)
+    return torch.matmul(probs, v.masked_fill(~v.isfinite(), 0.0)) + extra
+
+
 class PagedAttention:
     """Attention that reads K/V from a paged KV cache (``paged_attention.py:113-300``).
 

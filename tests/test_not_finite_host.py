@@ -1,0 +1,38 @@
+"""Infinities and NaN in keys and values on the host: they reach the tokens that see them and no others, as in the
+kernels. CPU only."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from llmopt.attention import PackedAttention
+
+
+def _alike(a, b):
+    assert torch.equal(a.isnan(), b.isnan())
+    torch.testing.assert_close(a, b, equal_nan=True, atol=2e-6, rtol=1e-5)  # fp32 sums of 20 terms in another order
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("side", ["key", "value"])
+def test_packed_prompts(side, bad):
+    gen = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(33, h, 16, generator=gen) for h in (4, 2, 2))
+    cu = torch.tensor([0, 20, 33])
+    attention = PackedAttention(4, 2, 16)
+    want = attention.forward(q, k, v, cu)
+    {"key": k, "value": v}[side][12, 1, 3] = bad
+    if side == "value" and bad == float("inf"):
+        v[15, 1, 3] = -bad  # both infinities: no number for who sees both
+    got = attention.forward(q, k, v, cu)
+    assert torch.equal(got[20:], want[20:]) and torch.equal(got[:, :2], want[:, :2])
+    _alike(got[:12], want[:12])
+    for t in range(12, 20):  # each token alone over what it sees
+        for h in (2, 3):
+            s = (k[: t + 1, 1] @ q[t, h]) * 16**-0.5
+            p = torch.softmax(s, 0)
+            _alike(got[t, h], (p[:, None] * v[: t + 1, 1]).sum(0))
+    if side == "value":
+        assert not bool(got[12:20, 2:, 3].isfinite().any())
+        assert bool(got[12:20, 2:, torch.arange(16) != 3].isfinite().all())
