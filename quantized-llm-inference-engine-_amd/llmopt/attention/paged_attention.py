@@ -75,6 +75,10 @@ class AttentionBackend:
         raise ValueError(f"unknown attention backend: {requested!r}")
 
 
+def _product(probs: torch.Tensor, _visible: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+    return torch.matmul(probs, v)
+
+
 def weighted_values(probs: torch.Tensor, visible: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
     """``probs [..., rows, keys] @ v [..., keys, d]`` in which a key that is not ``visible [..., rows, keys]`` to a row does
     not reach it, whatever its value is: in a plain product a weight of 0 times an infinity or NaN would."""
@@ -169,9 +173,11 @@ class PagedAttention:
         keys, values, valid = cache.gather(layer_idx, block_ids, context_lens)
         k = keys.permute(0, 2, 1, 3)
         v = values.permute(0, 2, 1, 3)
+        # A block of the 8-bit cache that is marked NaN must not reach the tokens in front of it.
+        weigh = weighted_values if quantized else _product
         if self.config.split_kv and self.config.split_size < k.shape[2]:
-            return self._split(query, k, v, valid, context_lens, q_len)
-        return self._dense(query, k, v, valid, context_lens, q_len)
+            return self._split(query, k, v, valid, context_lens, q_len, weigh)
+        return self._dense(query, k, v, valid, context_lens, q_len, weigh)
 
     # ---- the torch sequence ----------------------------------------------------------------------
 
@@ -201,28 +207,34 @@ class PagedAttention:
             scores = torch.tanh(scores / self.config.softcap) * self.config.softcap
         return scores
 
-    def _dense(self, q, k, v, valid, context_lens, q_len):  # noqa: ANN001, ANN202
+    def _dense(self, q, k, v, valid, context_lens, q_len, weigh):  # noqa: ANN001, ANN202
         k, v = self._per_query_head(k, v)
-        scores = self._scores(q, k).masked_fill(~self._mask(valid, context_lens, q_len), float("-inf"))
+        mask = self._mask(valid, context_lens, q_len)
+        scores = self._scores(q, k).masked_fill(~mask, float("-inf"))
         probs = torch.nan_to_num(torch.softmax(scores, dim=-1), nan=0.0)
-        return torch.matmul(probs, v).to(q.dtype)
+        return weigh(probs, mask, v).to(q.dtype)
 
-    def _split(self, q, k, v, valid, context_lens, q_len):  # noqa: ANN001, ANN202
+    def _split(self, q, k, v, valid, context_lens, q_len, weigh):  # noqa: ANN001, ANN202
         """Context chunks of ``split_size`` keys merged by log-sum-exp (``paged_attention.py:237-290``)."""
         k, v = self._per_query_head(k, v)
         out = lse = None
         for lo in range(0, k.shape[2], self.config.split_size):
             hi = min(lo + self.config.split_size, k.shape[2])
-            scores = self._scores(q, k[:, :, lo:hi])
-            scores = scores.masked_fill(~self._mask(valid[:, lo:hi], context_lens - lo, q_len), float("-inf"))
+            mask = self._mask(valid[:, lo:hi], context_lens - lo, q_len)
+            scores = self._scores(q, k[:, :, lo:hi]).masked_fill(~mask, float("-inf"))
             part_lse = torch.logsumexp(scores, dim=-1)
             probs = torch.nan_to_num(torch.softmax(scores, dim=-1), nan=0.0)
-            part = torch.matmul(probs, v[:, :, lo:hi].contiguous())
+            part = weigh(probs, mask, v[:, :, lo:hi].contiguous())
             if out is None:
                 out, lse = part, part_lse
             else:
                 out, lse = merge_states(out, part, lse, part_lse)
-        return torch.nan_to_num(out, nan=0.0).to(q.dtype)
+                if weigh is not _product:  # two parts without keys: no weights yet
+                    out = out.masked_fill((lse == -torch.inf).unsqueeze(-1), 0.0)
+        if weigh is _product:
+            return torch.nan_to_num(out, nan=0.0).to(q.dtype)
+        # Zeros without keys and for a sum that is no number; a value that is none stays.
+        return torch.where(lse.isfinite().unsqueeze(-1), out, torch.zeros_like(out)).to(q.dtype)
 
     def __repr__(self) -> str:
         return (
