@@ -86,7 +86,9 @@ class PackedAttention:
                 scores = torch.tanh(scores / self.softcap) * self.softcap
             hidden = torch.ones(hi - lo, hi - lo, dtype=torch.bool, device=query.device).triu(1)
             scores = scores.masked_fill(hidden, float("-inf"))
-            parts.append(weighted_values(torch.softmax(scores, -1), ~hidden, v).transpose(0, 1).to(query.dtype))
+            none = (scores == float("-inf")).all(-1, keepdim=True)  # no weights: zeros, as in the kernel
+            probs = torch.softmax(scores.masked_fill(none, 0.0), -1).masked_fill(none, 0.0)
+            parts.append(weighted_values(probs, ~hidden, v).transpose(0, 1).to(query.dtype))
         if out is not None:
             if len(cu) > 1:
                 out[cu[0] : cu[-1]] = torch.cat(parts[1:])

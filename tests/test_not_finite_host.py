@@ -64,3 +64,10 @@ def test_a_block_marked_nan_in_the_8_bit_cache(dtype, split):
     assert not bool(rows[:, :, :20].any()) and bool(rows[:, :, 20:].all())
     far = attention.forward(q, cache, 0, torch.tensor([[-1, -1, -1, -1, 0]]), lens)  # keys only behind three splits
     assert not bool(far[:, :, :22].any()) and bool(far[:, :, 22:].all())
+
+
+def test_a_token_whose_scores_are_all_minus_infinity():
+    q, k, v = torch.ones(5, 2, 8), torch.ones(5, 1, 8), torch.ones(5, 1, 8)
+    k[:2, 0, 0] = -float("inf")
+    out = PackedAttention(2, 1, 8).forward(q, k, v, torch.tensor([0, 5]))
+    assert not bool(out[:2].any()) and bool((out[2:] == 1).all())
