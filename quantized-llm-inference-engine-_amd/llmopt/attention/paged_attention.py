@@ -170,6 +170,8 @@ class PagedAttention:
                 )
             except NotImplementedError:
                 pass  # a shape outside the kernels: the torch sequence below
+        if quantized:
+            query = query[:, :, :q_len]  # as the kernels take it
         keys, values, valid = cache.gather(layer_idx, block_ids, context_lens)
         k = keys.permute(0, 2, 1, 3)
         v = values.permute(0, 2, 1, 3)

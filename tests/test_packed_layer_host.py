@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from llmopt.attention import PagedAttention, PagedAttentionConfig
+from llmopt.cache import QuantizedPagedKVCache
 from llmopt.model import DecoderOnlyModel, GreedyGenerator, ModelConfig
 
 
@@ -68,3 +69,17 @@ def test_prompts_of_one_length_in_either_form(dtype):
     prompts = torch.randint(0, 512, (3, 13))
     a, b = generator.generate(prompts, 5), generator.generate(list(prompts), 5)
     assert torch.equal(a.prefill_logits, b.prefill_logits) and torch.equal(a.tokens, b.tokens)
+
+
+@pytest.mark.parametrize("q_len", [1, 4])
+def test_fewer_query_tokens_than_the_query_holds(q_len):
+    """Over the 8-bit cache the first ``query_lens`` tokens count, on the host as on the device."""
+    gen = torch.Generator().manual_seed(3)
+    cache = QuantizedPagedKVCache(1, 4, 16, 2, 32)
+    table, lens = torch.arange(4).view(2, 2), torch.tensor([20, 25])
+    k = torch.randn(2, 25, 2, 32, generator=gen)
+    cache.write(0, table, torch.zeros(2, dtype=torch.long), k, k.flip(1))
+    q = torch.randn(2, 4, 6, 32, generator=gen)
+    attention = PagedAttention(4, 2, 32)
+    out = attention.forward(q, cache, 0, table, lens, q_len)
+    assert torch.equal(out, attention.forward(q[:, :, :q_len].contiguous(), cache, 0, table, lens))
