@@ -330,6 +330,7 @@ class DecoderLayer(nn.Module):
             normed = self.input_layernorm(hidden)
         else:
             normed, hidden = self.input_layernorm.add_forward(pending, hidden)
-        attn = self.self_attn(normed, positions, cache, block_ids, context_lens, token_offsets, q_len, cu_seqlens)
+        packed = {} if cu_seqlens is None else {"cu_seqlens": cu_seqlens}  # an attention put in here need not take it
+        attn = self.self_attn(normed, positions, cache, block_ids, context_lens, token_offsets, q_len, **packed)
         normed, hidden = self.post_attention_layernorm.add_forward(attn, hidden)
         return hidden, self.mlp(normed, defer=defer_mlp)

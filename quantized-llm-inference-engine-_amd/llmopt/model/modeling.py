@@ -78,11 +78,12 @@ class DecoderOnlyModel(nn.Module):
         # The final norm takes the last layer's partial sums too unless it first keeps only each
         # sequence's last row (last_only with several tokens per sequence).
         defer_last = not last_only or (q_len == 1 and cu_seqlens is None)
+        packed = {} if cu_seqlens is None else {"cu_seqlens": cu_seqlens}
         for i, layer in enumerate(self.layers):
             # A layer may hand its down projection's partial sums to the next norm.
             hidden, pending = layer.forward_chained(hidden, pending, positions, cache=cache, block_ids=block_ids,
                                                     context_lens=context_lens, token_offsets=token_offsets,
-                                                    q_len=q_len, cu_seqlens=cu_seqlens,
+                                                    q_len=q_len, **packed,
                                                     defer_mlp=self.defer_reductions and (i < last or defer_last))
         seqs = int(hidden.shape[0]) // max(1, q_len)
         if cu_seqlens is not None:

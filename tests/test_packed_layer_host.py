@@ -83,3 +83,21 @@ def test_fewer_query_tokens_than_the_query_holds(q_len):
     attention = PagedAttention(4, 2, 32)
     out = attention.forward(q, cache, 0, table, lens, q_len)
     assert torch.equal(out, attention.forward(q[:, :, :q_len].contiguous(), cache, 0, table, lens))
+
+
+def test_an_attention_or_layer_of_the_callers_own():
+    """What is put in place of a layer's attention, or of a layer, need not know packed prompts while there are none."""
+
+    class Attention(torch.nn.Module):
+        def forward(self, hidden, positions, cache, block_ids, context_lens, token_offsets, q_len):  # noqa: ANN001, ANN201
+            return 2 * hidden
+
+    class Layer(torch.nn.Module):
+        def forward_chained(self, hidden, pending, positions, cache=None, block_ids=None, context_lens=None,  # noqa: ANN001, ANN201
+                            token_offsets=None, q_len=1, defer_mlp=False):
+            return hidden, pending
+
+    model = _model()
+    model.layers[0].self_attn, model.layers[1] = Attention(), Layer()
+    with torch.no_grad():
+        assert model(torch.arange(6), torch.arange(6), q_len=6).logits.shape == (1, 6, 512)
