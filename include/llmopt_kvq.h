@@ -6,8 +6,9 @@
  *
  * One layer's cache, for keys and for values each:
  *   codes  [num_blocks, kv_heads, block_size, head_dim], one byte each: int8 or e4m3 (OCP, no infinities)
- *   scales [num_blocks, kv_heads] fp32, powers of two: a code stands for code x scale. 0: nothing but zeros was
- *          written; NaN: something infinite or NaN was, and the block's numbers of that head read as NaN.
+ *   scales [num_blocks, kv_heads] fp32, as written powers of two: a code stands for code x scale. 0: nothing but zeros
+ *          was written; NaN: something infinite or NaN was, and the block's numbers of that head read as NaN. Other
+ *          positive scales of the caller's are read alike (LLMOPT_KVQ_ALGO_TILES rounds code x scale to bf16).
  * Token t of sequence s lives in block block_ids[s * ldb + t / block_size] at slot t % block_size. block_ids, token
  * offsets, lengths and cu_seqlens are int32. No counterpart in the reference, whose cache holds 16- and 32-bit
  * numbers (src/llmopt/cache/paged_cache.py:137-331); the tables and lengths are its own.

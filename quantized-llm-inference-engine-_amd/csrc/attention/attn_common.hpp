@@ -132,8 +132,9 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
   }
 }
 
-// Bytes 2 HI and 2 HI + 1 of a word times their scale as a bf16 pair, exactly. The e4m3 conversion takes a power of
-// two with it (by its exponent alone: NaN gives NaN, and 0, whose codes are zeros, 2^-127).
+// Bytes 2 HI and 2 HI + 1 of a word times their scale as a bf16 pair, exactly for a power of two (and a product that bf16
+// holds). The e4m3 conversion takes the scale's exponent with it and nothing else (NaN gives NaN, and 0, whose codes are
+// zeros, 2^-127): the caller multiplies by what another scale has left.
 template <int FMT, bool HI>
 __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float scale) {
   if constexpr (FMT == kFmtE4m3)

@@ -5,8 +5,8 @@
 // `group` query heads that share the KV head, token-major, 32 rows per wave. It walks the keys in tiles of 64, held as
 // 16-bit rows in a double buffer in LDS that all rows read:
 //   * packed: by direct loads, one tile ahead;
-//   * codes: loaded into registers one tile ahead, dequantized exactly to bf16 (code x power of two) behind the
-//     tile's products, and stored.
+//   * codes: loaded into registers one tile ahead, dequantized to bf16 behind the tile's products (code x power of two:
+//     exactly; code x another scale: rounded), and stored.
 // Per tile and wave, on v_mfma_f32_32x32x16:
 //   * S^T = K Q^T (A: 32 keys x 16 dims from LDS, B: 16 dims x 32 rows, in registers): lane l holds row l % 32
 //     against 16 keys of each block of 32 -- keys 8 q + 4 (l / 32) + r --, so a row's softmax takes one exchange
@@ -296,6 +296,31 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
       }
     }
   };
+  // Keys and values of tile i, just stored: e4m3 codes were scaled by their scale's exponent alone, and a scale of the caller's
+  // that is no power of two has a factor left. One test per tile: a test with each conversion cost 4 % of a chunk.
+  auto store_factors = [&](int i, const Held& hk, const Held& hv) {
+    if constexpr (FMT == kFmtE4m3) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int j = 0; j < kCLoads; ++j) bits |= (kRawKeys ? 0u : __float_as_uint(hk.scale[j])) | __float_as_uint(hv.scale[j]);
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64((bits & 0x807FFFFFu) != 0) == 0, 1)) return;
+#pragma unroll
+      for (int k = kRawKeys ? 1 : 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < kCLoads; ++j) {
+          const Held& h = k == 0 ? hk : hv;
+          const int r = wave * kTr + kCrl * j + lane / kCpr, c = 2 * (lane % kCpr);
+          const uint32_t s = __float_as_uint(h.scale[j]);
+          const float f = (s & 0x7F800000u) ? __uint_as_float((s & 0x807FFFFFu) | 0x3F800000u) : 0.0f;  // 0: below 2^-126
+#pragma unroll 1
+          for (int x = 0; x < 8; ++x) {  // word by word, this lane's own: more at once spills at heads of 64
+            const int at = k == 0 ? k_chunk<HD>(r, c + x / 4) : v_chunk<HD>(r, c + x / 4);
+            uint32_t* const p = reinterpret_cast<uint32_t*>((k == 0 ? k_buf(i) : v_buf(i)) + r * kRowBytes + 16 * at) + x % 4;
+            *p = pack_bf16(__uint_as_float(*p << 16) * f, __uint_as_float(*p & 0xFFFF0000u) * f);
+          }
+        }
+    }
+  };
 
   // Per-lane LDS addresses of V: key 4 half + (lane % 16) / 4, dims 16 ((lane / 16) % 2) + 4 (lane % 4) of a block.
   const int vkey = 4 * half + ((lane & 15) >> 2);
@@ -452,6 +477,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
       fetch_query();
       store_codes(0, first_tile, hk, place.mask);
       store_codes(1, first_tile, hv, place.mask);
+      store_factors(first_tile, hk, hv);
       wait_vmcnt<0>();
       load_query();
       for (int i = first_tile; i < n_tiles; ++i) {
@@ -469,6 +495,7 @@ __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
         if (i + 1 < n_tiles) {
           store_codes(0, i + 1, hk, place.mask);
           store_codes(1, i + 1, hv, place.mask);
+          store_factors(i + 1, hk, hv);
         }
       }
     }

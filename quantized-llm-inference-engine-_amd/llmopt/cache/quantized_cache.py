@@ -78,8 +78,9 @@ class QuantizedPagedKVCache:
     @classmethod
     def from_tensors(cls, key_codes: torch.Tensor, key_scales: torch.Tensor, value_codes: torch.Tensor,
                      value_scales: torch.Tensor) -> QuantizedPagedKVCache:
-        """A cache over tensors that exist already (shapes as the attributes; shared, not copied). The scales must
-        be powers of two, 0 or NaN, and the codes finite."""
+        """A cache over tensors that exist already (shapes as the attributes; shared, not copied). The codes must be
+        finite and the scales not negative. Scales need not be the powers of two that a write gives: a code stands for code x scale
+        under any, and a write keeps the larger scale; attention of chunks then rounds code x scale to bf16."""
         cache = cls.__new__(cls)
         if key_codes.is_cuda:  # the checks below in native code: 0.6 us instead of 4
             from llmopt.kernels import ops
