@@ -211,17 +211,18 @@ __device__ __forceinline__ Packed find_packed(const int32_t* cu_seqlens, int64_t
   }
 }
 
-// Soft cap, cap tanh(x), as cap - 2 cap / (1 + 2^y) with y = 2 x log2(e): off by up to 2^-21 of the cap. Taken up to kShortCap,
-// where that is 3e-5 in a score and so 2^-15 of a probability, which is rounded to 8 or 11 bits: 4 prompts of 2048 203 us, with
-// tanh_of 263, with the library's tanhf 300.
+// Soft cap, cap tanh(x), as cap - 2 cap / (1 + 2^y) with y = 2 x log2(e): off by up to 2^-21 of the cap. Taken for 16-bit queries
+// up to kShortCap, where that is 3e-5 in a score and so 2^-15 of a probability, a sixteenth of what an fp16 output is rounded
+// by (2^-11), also where two pieces hold 16 bits of the probability. 4 prompts of 2048 in bf16 208 us, with tanh_of 265, with
+// the library's tanhf 300; chunks of 4 x 512 tokens over int8 codes in fp16 218 and 270, tanhf spills.
 constexpr float kShortCap = 64.0f;
 __device__ __forceinline__ float short_cap(float y, float cap) {
   return __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y)), cap);
 }
 
 // tanh within 2^-21 of its value: its series up to x^9 below 0.3 (the next term is 5e-8 of it), else (1 - t) / (1 + t) with
-// t = e^(-2 |x|), of which 1 - t is off by 2^-22 at 0.3 and by less above. A capped score is then off by 2^-21 of itself, which the
-// probabilities' 8 or 11 bits do not show.
+// t = e^(-2 |x|), of which 1 - t is off by 2^-22 at 0.3 and by less above. A capped score is then off by 2^-21 of itself: 2^-15
+// of a probability at a score of 64, more at larger ones, as the product's own rounding (2^-24 per term).
 __device__ __forceinline__ float tanh_of(float x) {
   const float x2 = x * x;
   const float near = x * __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, 62.0f / 2835, -17.0f / 315), 2.0f / 15), -1.0f / 3), 1.0f);
