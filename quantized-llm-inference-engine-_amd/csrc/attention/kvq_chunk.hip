@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(H
   w.rows = rows;
   w.row0 = row0;
   w.row0_tok = int(uint32_t(row0) / uint32_t(a.group));
-  w.base = a.context_lens[s] - int(a.q_len);
+  w.base = max(a.context_lens[s], 0) - int(a.q_len);
   const int last = int(uint32_t(min(row0 + kRows, rows) - 1) / uint32_t(a.group));
   w.t_end = max(0, min(w.base + last + 1, int(a.c.ldb * a.c.block_size)));
   if (a.splits > 1) {

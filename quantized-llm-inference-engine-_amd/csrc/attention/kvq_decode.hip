@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))
     const uint32_t bi = uint32_t(tile_t0(lane / 2) + 16 * (lane & 1)) / bs;
     if (bi < ldb) first_entry = table[bi];
   }
-  const int base = a.context_lens[s] - q_len;  // position of query token 0
+  const int base = max(a.context_lens[s], 0) - q_len;  // position of query token 0
   const int q_pos = row_ok ? base + tok : -1;
   const int first_pos = base + int(uint32_t(16 * rb) / uint32_t(a.group));
   // The rows' keys: t < t_end, within the table (its width in tokens is below 2^31, checked on the host).
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(256) kvq_merge_kernel(const KvqAttnArgs a) {
     for (int d = 0; d < kD; ++d) ahead[i][d] = i < a.splits ? part[i * stride * HD + d] : 0.0f;
   float lse = lane < a.splits ? lse_at[lane * stride] : neg_inf;
   // The splits that the row's block of 16 ran.
-  const int base = a.context_lens[s] - int(a.q_len);
+  const int base = max(a.context_lens[s], 0) - int(a.q_len);
   const int last_tok = int(uint32_t(min((r & ~15) + 15, rows - 1)) / uint32_t(a.group));
   const int t_end = max(0, min(base + last_tok + 1, int(a.c.ldb * a.c.block_size)));
   const int span = int(a.tiles_per_split) * 32;
