@@ -151,6 +151,9 @@ class PagedAttention:
         if q_len == 0:
             return torch.zeros((seqs, self.num_heads, 0, self.head_dim), dtype=query.dtype, device=query.device)
         quantized = isinstance(cache, QuantizedPagedKVCache)
+        if quantized and (cache.num_kv_heads != self.num_kv_heads or query.shape[1] != self.num_heads):
+            raise ValueError(f"attention of {self.num_heads} heads over {self.num_kv_heads} KV heads does not match a query of "
+                             f"{int(query.shape[1])} and a cache of {cache.num_kv_heads}")
         if self.backend == "hip" and query.device.type == "cuda" and not (quantized and is_differentiated(query)):
             from llmopt.kernels import ops
 

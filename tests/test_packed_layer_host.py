@@ -101,3 +101,12 @@ def test_an_attention_or_layer_of_the_callers_own():
     model.layers[0].self_attn, model.layers[1] = Attention(), Layer()
     with torch.no_grad():
         assert model(torch.arange(6), torch.arange(6), q_len=6).logits.shape == (1, 6, 512)
+
+
+def test_heads_that_are_not_the_attentions():
+    """Another number of heads in the query or in the 8-bit cache is refused, before a kernel would group them its own way."""
+    cache = QuantizedPagedKVCache(1, 2, 16, 2, 64)
+    table, lens = torch.tensor([[0]]), torch.tensor([5])
+    for attention, heads in ((PagedAttention(8, 4, 64), 8), (PagedAttention(8, 1, 64), 8), (PagedAttention(8, 2, 64), 4)):
+        with pytest.raises(ValueError, match="KV heads"):
+            attention.forward(torch.zeros(1, heads, 1, 64), cache, 0, table, lens)
