@@ -14,12 +14,9 @@ namespace {
 
 using namespace tile;
 
-constexpr int kThreads = 256;
-
 template <int FMT, bool QF16, int HD, bool CAP>
-__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : 2, HD == 64 ? 3 : 2)))
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 : 2, HD == 64 ? 3 : 2)))
     kvq_chunk_kernel(const KvqAttnArgs a) {
-  constexpr int kRows = 128;
   __shared__ __align__(16) uint8_t lds[4 * kKeys * HD * 2 + (QF16 ? 2 * kKeys * 4 : 0)];
   // Workgroups in the order (KV head, row block, sequence), a sequence's last blocks (the longest walks) first.
   const uint32_t kv_heads = uint32_t(a.c.kv_heads);
@@ -62,19 +59,19 @@ __global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(H
   w.block_size = uint32_t(a.c.block_size);
   w.ldb = uint32_t(a.c.ldb);
   w.num_blocks = uint32_t(a.c.num_blocks);
-  attend<kSrcCodes, FMT, false, QF16, HD, QF16 ? 2 : 1, 4, CAP>(w, lds);
+  attend<kSrcCodes, FMT, false, QF16, HD, QF16 ? 2 : 1, CAP>(w, lds);
 }
 
 template <int FMT, bool QF16, bool CAP>
 hipError_t launch_hd(const KvqAttnArgs& a, hipStream_t stream) {
-  const int64_t blocks = (a.group * a.q_len + 127) / 128;
+  const int64_t blocks = (a.group * a.q_len + kRows - 1) / kRows;
   const int64_t grid = blocks * a.c.kv_heads * a.num_seqs;
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
   const dim3 grid3(unsigned(grid), unsigned(a.splits));
   if (a.c.head_dim == 128)
-    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 128, CAP>), grid3, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 128, CAP>), grid3, dim3(64 * kWaves), 0, stream, a);
   else
-    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 64, CAP>), grid3, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((kvq_chunk_kernel<FMT, QF16, 64, CAP>), grid3, dim3(64 * kWaves), 0, stream, a);
   if (a.splits > 1) return launch_kvq_merge(a, QF16 ? kDtF16 : kDtBf16, stream);
   return hipGetLastError();
 }

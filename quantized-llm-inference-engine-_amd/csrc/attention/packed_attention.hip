@@ -10,10 +10,9 @@ namespace {
 
 using namespace tile;
 
-template <bool F16, int HD, int W, bool CAP>
-__global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : CAP ? 3 : 4, HD == 128 ? 2 : CAP ? 3 : 4)))
+template <bool F16, int HD, bool CAP>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 2 : CAP ? 3 : 4, HD == 128 ? 2 : CAP ? 3 : 4)))
     packed_attention_kernel(const PackedAttnArgs a) {
-  constexpr int kRows = 32 * W;
   __shared__ __align__(16) uint8_t lds[4 * kKeys * HD * 2];
   const uint32_t kv_heads = uint32_t(a.kv_heads);
   const uint32_t unit = blockIdx.x / kv_heads, kvh = blockIdx.x - unit * kv_heads;
@@ -25,8 +24,8 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(HD 
     // Rows in front of the first sequence (there are none in a proper call) and behind the last one: zeros.
     const int64_t lo = a.num_seqs > 0 ? cu(0) : a.total_tokens, hi = a.num_seqs > 0 ? cu(a.num_seqs) : a.total_tokens;
     const int64_t per_row = a.group * (HD / 8);
-    for (int64_t i = (unit - a.blocks) * (64 * W) + threadIdx.x; i < (lo + a.total_tokens - hi) * per_row;
-         i += a.tail_blocks * (64 * W)) {
+    for (int64_t i = (unit - a.blocks) * (64 * kWaves) + threadIdx.x; i < (lo + a.total_tokens - hi) * per_row;
+         i += a.tail_blocks * (64 * kWaves)) {
       const int64_t r = i / per_row, x = i - r * per_row;
       const int64_t tok = r < lo ? r : hi + r - lo;
       uint16_t* dst = static_cast<uint16_t*>(a.out) + tok * a.o_tok_stride + (kvh * int64_t(a.group) + x / (HD / 8)) * a.o_head_stride;
@@ -62,21 +61,20 @@ __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(HD 
   w.k_tok_stride = a.k_tok_stride;
   w.v_tok_stride = a.v_tok_stride;
   w.len = int(len);
-  attend<kSrcPacked, 0, F16, F16, HD, 1, W, CAP>(w, lds);
+  attend<kSrcPacked, 0, F16, F16, HD, 1, CAP>(w, lds);
 }
 
-template <bool F16, int HD, int W>
+template <bool F16, int HD>
 hipError_t launch(PackedAttnArgs a, hipStream_t stream) {
-  constexpr int kRows = 32 * W;
   a.blocks = a.num_seqs > 0 ? a.total_tokens * a.group / kRows + a.num_seqs : 0;
   a.tail_blocks = a.zero_tail ? 32 : 0;
   const int64_t grid = (a.blocks + a.tail_blocks) * a.kv_heads;
   if (grid <= 0) return hipSuccess;
   if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
   if (a.softcap > 0.0f)
-    hipLaunchKernelGGL((packed_attention_kernel<F16, HD, W, true>), dim3(unsigned(grid)), dim3(64 * W), 0, stream, a);
+    hipLaunchKernelGGL((packed_attention_kernel<F16, HD, true>), dim3(unsigned(grid)), dim3(64 * kWaves), 0, stream, a);
   else
-    hipLaunchKernelGGL((packed_attention_kernel<F16, HD, W, false>), dim3(unsigned(grid)), dim3(64 * W), 0, stream, a);
+    hipLaunchKernelGGL((packed_attention_kernel<F16, HD, false>), dim3(unsigned(grid)), dim3(64 * kWaves), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -84,8 +82,8 @@ hipError_t launch(PackedAttnArgs a, hipStream_t stream) {
 
 hipError_t launch_packed_attention(const PackedAttnArgs& a, int dtype, int64_t head_dim, hipStream_t stream) {
   if (a.total_tokens == 0) return hipSuccess;
-  if (dtype == kDtBf16) return head_dim == 128 ? launch<false, 128, 4>(a, stream) : launch<false, 64, 4>(a, stream);
-  return head_dim == 128 ? launch<true, 128, 4>(a, stream) : launch<true, 64, 4>(a, stream);
+  if (dtype == kDtBf16) return head_dim == 128 ? launch<false, 128>(a, stream) : launch<false, 64>(a, stream);
+  return head_dim == 128 ? launch<true, 128>(a, stream) : launch<true, 64>(a, stream);
 }
 
 }  // namespace llmopt

@@ -38,6 +38,8 @@ namespace tile {
 enum : int { kSrcPacked = 0, kSrcCodes = 1 };
 
 constexpr int kKeys = 64;
+constexpr int kWaves = 4;             // of a workgroup
+constexpr int kRows = 32 * kWaves;    // query rows of a workgroup
 constexpr float kLog2e = 1.44269504088896340736f;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
@@ -123,14 +125,14 @@ struct Work {
 };
 
 // KP: 16-bit pieces of a probability. F16: fp16 operands (packed fp16), else bf16. QF16: the
-// query's and output's type is fp16 (else bf16). W: waves. CAP: the scores are soft-capped.
-template <int SRC, int FMT, bool F16, bool QF16, int HD, int KP, int W, bool CAP>
+// query's and output's type is fp16 (else bf16). CAP: the scores are soft-capped.
+template <int SRC, int FMT, bool F16, bool QF16, int HD, int KP, bool CAP>
 __device__ __forceinline__ void attend(const Work& a, uint8_t* lds) {
   constexpr int kCh = HD / 8;               // 16-byte chunks per 16-bit row
   constexpr int kRowBytes = HD * 2;
   constexpr int kTile = kKeys * kRowBytes;  // one K (or V) tile
   constexpr int kRpl = 64 / kCh;            // 16-bit rows per wave load (1 KB)
-  constexpr int kTr = kKeys / W;            // rows of a tile that a wave brings in
+  constexpr int kTr = kKeys / kWaves;       // rows of a tile that a wave brings in
   constexpr int kLoads = kTr / kRpl;        // packed: in wave loads of K and of V
   constexpr int kCpr = HD / 16;             // codes: 16-byte loads per row
   constexpr int kCrl = 64 / kCpr;           // codes: rows per wave load
