@@ -146,14 +146,14 @@ class PagedAttention:
         sees keys up to and including its own position. A query that needs a gradient or carries a tangent
         takes the torch sequence over a :class:`QuantizedPagedKVCache` (its kernels have no derivative).
         """
-        seqs = int(query.shape[0])
-        q_len = query_lens if query_lens is not None else int(query.shape[2])
+        shape = query.shape
+        q_len = query_lens if query_lens is not None else shape[2]
         if q_len == 0:
-            return torch.zeros((seqs, self.num_heads, 0, self.head_dim), dtype=query.dtype, device=query.device)
+            return torch.zeros((shape[0], self.num_heads, 0, self.head_dim), dtype=query.dtype, device=query.device)
         quantized = isinstance(cache, QuantizedPagedKVCache)
-        if quantized and (cache.num_kv_heads != self.num_kv_heads or query.shape[1] != self.num_heads):
+        if quantized and (cache.num_kv_heads != self.num_kv_heads or shape[1] != self.num_heads):
             raise ValueError(f"attention of {self.num_heads} heads over {self.num_kv_heads} KV heads does not match a query of "
-                             f"{int(query.shape[1])} and a cache of {cache.num_kv_heads}")
+                             f"{shape[1]} and a cache of {cache.num_kv_heads}")
         if self.backend == "hip" and query.device.type == "cuda" and not (quantized and is_differentiated(query)):
             from llmopt.kernels import ops
 
