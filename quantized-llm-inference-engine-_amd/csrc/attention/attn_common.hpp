@@ -2,13 +2,13 @@
 // their exact conversions to MFMA operands.
 //
 // Cache of one layer (llmopt_kvq.h): codes [num_blocks, kv_heads, block_size, head_dim], one byte each, and one
-// fp32 scale per (block, KV head), a power of two (0: nothing but zeros; NaN: something that was not finite was
-// written). A block of one head is one contiguous run of bytes: 2 KB at 16 tokens of 128.
+// fp32 scale per (block, KV head), as written a power of two (0: nothing but zeros; NaN: something that was not finite
+// was written). A block of one head is one contiguous run of bytes: 2 KB at 16 tokens of 128.
 //
 // int8 codes (at most 8 significant bits) and e4m3 codes (4) are exact bf16 and fp16 numbers, so the operands of
 // the products are the codes themselves; a key's scale multiplies its scores, a value's scale its probability, in
 // fp32. A power of two commutes with every rounding to bf16 (both have 8 exponent bits), so this gives what
-// dequantized operands would.
+// dequantized operands would; another scale of the caller's rounds a value's product on its own.
 #pragma once
 
 #include "../qcommon.hpp"

@@ -71,6 +71,10 @@ int describe_cache(llmopt::KvqCache& c, const void* key_codes, const float* key_
 //   * Workgroups of eight waves, one per CU, in one round: 1 sequence of 8000 in 32 splits 14.2 (4 splits 23.5), 8 of 4096
 //     in 4 splits 19.6 (1 33, 8 23.3), 32 of 640 in 1 split 12.5 (2 19.2); past 256 pairs none (64 of 8192: 147 - 165; 2
 //     splits 176). A split has a tile per wave at least, and up to 24 tiles stay whole but for a few pairs: the merge costs 3.
+//   * Short contexts, the rule's splits against one, in a graph: 1 sequence of 384 (2 splits) 8.2 against 7.1, of 512 (2) 8.4 against
+//     8.0, of 641 (3) 8.5 against 9.9, of 1024 (4) 8.5 against 11.8; 2 and 3 sequences alike; 8 of 800 (4) 9.0 against 10.7, of 1024
+//     9.2 against 12.1; 16 of 800 (2) 11.6 against 10.9, of 1024 12.2 against 13.3. Up to 256 tokens there is one. Where a pair has 12 - 16
+//     tiles, or 16 sequences 25, one split would be 0.4 - 1.1 faster.
 //   * Four waves, two workgroups per CU, from 512 pairs over tables of up to 2048 tokens: 64 of 640 18.0 (eight waves 21.4),
 //     128 of 1024 47 (57), 64 of 2048 45.7 (46.3); longer ones 162 (147).
 //   * Tables much wider than their contexts: a split is at most 1024 tokens for a few pairs, 8192 for many.

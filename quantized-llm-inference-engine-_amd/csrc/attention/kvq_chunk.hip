@@ -4,9 +4,14 @@
 //
 // Bound by issue: each of a CU's workgroups dequantizes its own tiles (a conversion per two codes, for int8 as many scalings, then
 // 16-byte LDS stores), beside the softmax and the MFMAs. Measured (MI355X, 32 query and 8 KV heads of 128, e4m3 codes,
-// bf16): the next 512 tokens of 4 prompts with 4012 cached at most 127 us (796 TFLOP/s), by the scaled pair conversion of
-// e4m3 codes (163 by way of fp32) and by stepping through the table without a division (4 % of 135). Heads of 64 run three
-// workgroups per CU, heads of 128 two. With a soft cap 205 us for 166 (heads of 64: 170 for 122).
+// bf16): the next 512 tokens of 4 prompts of up to 4012 tokens 123 - 134 us (752 - 820 TFLOP/s), by the scaled pair conversion
+// of e4m3 codes (163 by way of fp32) and by stepping through the table without a division (4 % of 135). Heads of 64 run three
+// workgroups per CU, heads of 128 two. The same chunks, contexts of 2507 - 4012, back to back in a graph (us; with a soft cap of
+// 30, of 100):
+//   bf16 e4m3, heads of 128 123 (164, 213)    heads of 64 80 (125, 180)
+//   bf16 int8              140 (179, 238)                90 (138, 195)
+//   fp16 e4m3              169 (200, 254)               113 (159, 217)
+//   fp16 int8              184 (218, 270)               122 (170, 223)
 #include "tile_attention.hpp"
 
 namespace llmopt {

@@ -22,7 +22,7 @@
 //
 // Bound by HBM at large batches (64 sequences of up to 8192, int8: 811 MB in 153 us, 5.3 TB/s, what a large copy
 // reaches), by the chain of loads (length, table, codes, next codes) at small ones: 32 sequences of up to 640 in e4m3 10.8 us (32 MB;
-// 24 with up to 4000 tokens and heads of 64 in fp16 17.9, one of 641 9.2 with its merge, in a graph). Sixteen waves
+// 24 with up to 4000 tokens and heads of 64 in fp16 17.9, one of 641 8.5 with its merge, in a graph). Sixteen waves
 // per workgroup spill; one tile in flight, non-temporal loads and non-temporal queries measured level or slower.
 //
 // Roundings: bf16 queries: probabilities in bf16 (the sum adds them as rounded). fp16 queries: keys as fp16 operands,

@@ -4,8 +4,8 @@
 // them in registers (blocks of more than 8 x 64 chunks of 8 numbers are read twice), takes their largest magnitude, fixes
 // the scale and writes the codes. Bound by HBM (3 bytes per 16-bit number) and, one wave's work being 4 KB, by its chain of
 // loads: lengths and offsets, then the rows and the table entry together. Measured (MI355X, bf16, 8 heads of 128, blocks of
-// 16): 32 prompts of 1 - 1024 tokens 22.5 us (104 MB, 4.6 TB/s; 36 with the table before the rows and numbers held as fp32),
-// one token of 256 sequences 5.9, of one sequence 4.4.
+// 16): 32 prompts of 1 - 1024 tokens 20.8 us (104 MB, 5.0 TB/s; 36 with the table before the rows and numbers held as fp32),
+// one token of 256 sequences 5.5, of one sequence 4.2.
 //   need  = 2^e, the smallest e >= -126 with amax <= top 2^e (top = 127 or 448), 0 for amax = 0, NaN for a row
 //           that holds an infinity or a NaN
 //   scale = need where the write holds the block's slot 0 (the block starts anew), else max(old, need)

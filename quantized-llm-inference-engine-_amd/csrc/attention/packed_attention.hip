@@ -1,7 +1,7 @@
 // Causal attention over packed prompts (PackedAttention.forward): sequence s is rows cu_seqlens[s] .. cu_seqlens[s + 1]
 // - 1 of query [total, heads, d] and key / value [total, kv_heads, d]; a token sees its sequence's tokens up to itself.
-// The tile kernel of tile_attention.hpp over 16-bit rows (its times are there). Four workgroups per CU at heads of 64, two of
-// 128 (registers and LDS alike); the grid is sized by the rows, one block more per sequence, without reading cu_seqlens
+// The tile kernel of tile_attention.hpp over 16-bit rows (its times are there). Four workgroups per CU at heads of 64 (three with
+// a soft cap), two of 128 (registers and LDS alike); the grid is sized by the rows, one block more per sequence, without reading cu_seqlens
 // on the host, so a workgroup first finds its sequence by a search with one ballot per 64 of them.
 #include "tile_attention.hpp"
 

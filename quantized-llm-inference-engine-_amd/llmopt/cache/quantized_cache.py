@@ -7,8 +7,8 @@ scale``. Block tables, offsets and lengths are those of :class:`llmopt.cache.Pag
 
 The scales are powers of two: with ``top`` the format's largest number (127 or 448), a block and head whose largest
 magnitude is ``amax`` takes ``2^e`` for the smallest ``e >= -126`` with ``amax <= top 2^e`` (0 if all is zero), and a number
-``x`` the code ``x / 2^e``, rounded to nearest, ties to even. So a code times its scale is exact in bf16 and fp32, and the
-same numbers give the same codes everywhere; int8 loses at most one bit of its range to it, e4m3 no precision.
+``x`` the code ``x / 2^e``, rounded to nearest, ties to even. So a code times its scale is exact in bf16 and fp32 (down to bf16's
+smallest number, 2^-133: an e4m3 code may be 2^-9 and a scale 2^-126), and the same numbers give the same codes everywhere; int8 loses at most one bit of its range to it, e4m3 no precision.
 
 A write that holds a block's slot 0 starts the block anew: its scale is that of the new tokens, and what other slots held
 is void (a block that another request gave back needs no clearing). Any other write keeps the larger of the old and the
