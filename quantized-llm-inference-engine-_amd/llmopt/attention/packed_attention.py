@@ -77,6 +77,7 @@ class PackedAttention:
         tokens = int(query.shape[0])
         cu = [min(max(int(c), 0), tokens) for c in cu_seqlens.tolist()]
         parts = [torch.zeros_like(query[: cu[0] if len(cu) > 1 else tokens])]
+        finite = bool(value.isfinite().all())  # read once, not in every sequence
         for lo, hi in zip(cu, cu[1:]):
             q = query[lo:hi].transpose(0, 1).float()
             k = key[lo:hi].transpose(0, 1).float().repeat_interleave(self.group_size, 0)
@@ -88,7 +89,8 @@ class PackedAttention:
             scores = scores.masked_fill(hidden, float("-inf"))
             none = (scores == float("-inf")).all(-1, keepdim=True)  # no weights: zeros, as in the kernel
             probs = torch.softmax(scores.masked_fill(none, 0.0), -1).masked_fill(none, 0.0)
-            parts.append(weighted_values(probs, ~hidden, v).transpose(0, 1).to(query.dtype))
+            out_rows = torch.matmul(probs, v) if finite else weighted_values(probs, ~hidden, v)
+            parts.append(out_rows.transpose(0, 1).to(query.dtype))
         if out is not None:
             if len(cu) > 1:
                 out[cu[0] : cu[-1]] = torch.cat(parts[1:])
