@@ -8,7 +8,8 @@ scale``. Block tables, offsets and lengths are those of :class:`llmopt.cache.Pag
 The scales are powers of two: with ``top`` the format's largest number (127 or 448), a block and head whose largest
 magnitude is ``amax`` takes ``2^e`` for the smallest ``e >= -126`` with ``amax <= top 2^e`` (0 if all is zero), and a number
 ``x`` the code ``x / 2^e``, rounded to nearest, ties to even. So a code times its scale is exact in bf16 and fp32 (down to bf16's
-smallest number, 2^-133: an e4m3 code may be 2^-9 and a scale 2^-126), and the same numbers give the same codes everywhere; int8 loses at most one bit of its range to it, e4m3 no precision.
+smallest number, 2^-133: an e4m3 code may be 2^-9 and a scale 2^-126), and the same numbers give the same codes everywhere;
+int8 loses at most one bit of its range to it, e4m3 no precision.
 
 A write that holds a block's slot 0 starts the block anew: its scale is that of the new tokens, and what other slots held
 is void (a block that another request gave back needs no clearing). Any other write keeps the larger of the old and the
@@ -79,8 +80,8 @@ class QuantizedPagedKVCache:
     def from_tensors(cls, key_codes: torch.Tensor, key_scales: torch.Tensor, value_codes: torch.Tensor,
                      value_scales: torch.Tensor) -> QuantizedPagedKVCache:
         """A cache over tensors that exist already (shapes as the attributes; shared, not copied). The codes must be
-        finite and the scales not negative. Scales need not be the powers of two that a write gives: a code stands for code x scale
-        under any, and a write keeps the larger scale; attention of chunks then rounds code x scale to bf16."""
+        finite and the scales not negative. Scales need not be the powers of two that a write gives: a code stands for
+        ``code * scale`` under any, and a write keeps the larger scale; attention of chunks then rounds that to bf16."""
         cache = cls.__new__(cls)
         if key_codes.is_cuda:  # the checks below in native code: 0.6 us instead of 4
             from llmopt.kernels import ops

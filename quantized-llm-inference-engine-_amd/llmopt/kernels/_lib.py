@@ -221,7 +221,8 @@ def load_binding():  # noqa: ANN201 - the extension module, or None
     """Load (once) and return the native host path of the linears, of the 8-bit KV cache and of packed
     attention (``csrc/torch_binding.cpp``), with
     the kernel library's entry points attached. None, with one warning, where it is not built, does not
-    load into this torch, or it or the library is from before an entry point that it attaches: calls then take the general path, the same kernels through ctypes."""
+    load into this torch, or it or the library is from before an entry point that it attaches: calls then take
+    the general path, the same kernels through ctypes."""
     global _binding, _binding_tried
     if _binding_tried:
         return _binding

@@ -820,18 +820,17 @@ def _may_share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two ``[rows, heads, d]`` tensors of one element size may have an element in common: their extents meet, and
     they are not side by side within rows of one stride (as slices of a fused projection's output are)."""
     size = a.element_size()
-
-    def extent(t: torch.Tensor, dims: range) -> int:
-        return size * (1 + sum((t.shape[d] - 1) * t.stride(d) for d in dims))
-
-    if a.numel() == 0 or b.numel() == 0 or a.data_ptr() + extent(a, range(3)) <= b.data_ptr() \
-            or b.data_ptr() + extent(b, range(3)) <= a.data_ptr():
+    (rows, heads, d), (sa, sh, sd) = a.shape, a.stride()
+    a_row, a_rows = 1 + (heads - 1) * sh + (d - 1) * sd, (rows - 1) * sa
+    (rows, heads, d), (sb, sh, sd) = b.shape, b.stride()
+    b_row, b_rows = 1 + (heads - 1) * sh + (d - 1) * sd, (rows - 1) * sb
+    ahead = (b.data_ptr() - a.data_ptr()) // size  # where b begins, counted from a
+    if ahead >= a_rows + a_row or -ahead >= b_rows + b_row or a.numel() == 0 or b.numel() == 0:
         return False
-    row = a.stride(0) * size
-    if row == 0 or a.stride(0) != b.stride(0):
+    if sa == 0 or sa != sb:
         return True
-    ahead = (b.data_ptr() - a.data_ptr()) % row  # where b's rows begin, counted from a's
-    return ahead < extent(a, range(1, 3)) or ahead + extent(b, range(1, 3)) > row
+    ahead %= sa  # where b's rows begin, counted from a's
+    return ahead < a_row or ahead + b_row > sa
 
 
 def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -839,7 +838,8 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     """Causal attention over packed prompts: ``query [tokens, heads, head_dim]``, ``key``/``value`` ``[tokens, kv_heads,
     head_dim]`` (fp16 or bf16, any token and head strides), sequence ``s`` the rows ``cu_seqlens[s]`` up to
     ``cu_seqlens[s + 1]``. Rows behind the last sequence are zeros, in a given ``out`` left as they were; an ``out`` that
-    may share memory with the inputs is computed beside it and copied. Raises ``NotImplementedError`` for fp32 and for head dims other than 64 and 128."""
+    may share memory with the inputs is computed beside it and copied. Raises ``NotImplementedError`` for fp32 and for
+    head dims other than 64 and 128."""
     binding = load_binding() if out is None and query.is_cuda else None
     if binding is not None:  # the plain form of a call, in native code
         result = binding.packed_attention(query, key, value, cu_seqlens, scale, softcap)
