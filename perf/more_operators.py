@@ -1,9 +1,9 @@
 """The operators of a decoder in 8-bit floating point: what is measured of them, and their plain forms.
 
-Weights and activations are float8_e4m3fn codes with fp32 scales, a number being its code times its scale: activations
-``[tokens, K]`` have one scale for each token and 128 columns, weights ``[N, K]`` one for each block of 128 x 128. With
-``amax`` a group's largest magnitude, its scale is ``max(amax, 2^-100) / 448`` and a number ``x`` has the code ``x * (448 /
-max(amax, 2^-100))`` rounded to the nearest, ties to even.
+Weights and activations are float8_e4m3fn codes with float8_e8m0fnu scales (powers of two), a number being its code times its
+scale: activations ``[tokens, K]`` have one scale for each token and 128 columns, weights ``[N, K]`` one for each block of
+128 x 128. A group whose largest magnitude is ``amax`` has the scale ``2^e`` for the smallest ``e >= -127`` with ``amax <= 448
+2^e``, and a number ``x`` the code ``x / 2^e`` rounded to the nearest, ties to even.
 
 * ``quantize``: :func:`quantize_float8`, of a layer's activations (``rows`` 1) or of a weight (``rows`` 128). Outputs: codes, scales;
 * ``norm``: :func:`rmsnorm_float8`, a layer's norm with the residual's addition in front of it, its output in codes for the projection
@@ -29,7 +29,7 @@ own = False
 
 DEV = "cuda"
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
-F8 = torch.float8_e4m3fn
+F8, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 EPS = 1e-5
 
 # (hidden, intermediate, rows of the fused q, k and v projections): the 8B decoder and the default configuration
@@ -76,11 +76,12 @@ def draw(rng):
     if rng.random() < 0.4:  # a width of no configuration: its last block of 128 is a part of one
         hidden, wide, qkv = 16 * rng.randint(8, 256), 16 * rng.randint(8, 640), rng.randint(100, 6144)
     tokens = _log_int(rng, 1, 8192)
-    dtype = rng.choice(["bf16", "bf16", "fp16", "fp32"])
+    dtype = rng.choice(["bf16", "bf16", "fp16"])
     if kind == "quantize":
+        dtype = rng.choice([dtype, "fp32"])
         return {"kind": kind, "tokens": tokens, "k": rng.choice([hidden, wide]), "rows": rng.choice([1, 1, 128]), "dtype": dtype}
     if kind == "norm":
-        return {"kind": kind, "tokens": tokens, "k": hidden, "residual": rng.random() < 0.7, "dtype": rng.choice(["bf16", "bf16", "fp16"])}
+        return {"kind": kind, "tokens": tokens, "k": hidden, "residual": rng.random() < 0.7, "dtype": dtype}
     if kind == "linear":
         n, k = rng.choice([(qkv, hidden), (hidden, wide)])
         return {"kind": kind, "tokens": tokens, "n": n, "k": k, "bias": rng.random() < 0.3, "dtype": dtype}
@@ -103,13 +104,14 @@ def _spread(groups, rows, shape):
 
 
 def _plain_codes(x, rows):
-    amax = _groups(x.abs(), rows).clamp(min=2.0**-100)
-    codes = (x * _spread(448.0 / amax, rows, x.shape)).clamp(-448.0, 448.0).to(F8)
-    return codes, amax / 448.0
+    m, p = torch.frexp(_groups(x.abs(), rows))  # amax = m 2^p with m in [0.5, 1), and 448 = 0.875 2^9
+    e = (p - 9 + (m > 0.875).to(p.dtype)).clamp(min=-127)
+    codes = torch.ldexp(x, -_spread(e, rows, x.shape)).to(F8)
+    return codes, (e + 127).to(torch.uint8).view(E8)
 
 
-def _numbers(codes, scales, rows, dtype=torch.float32):
-    return codes.to(dtype) * _spread(scales.to(dtype), rows, codes.shape)
+def _numbers(codes, scales, rows):
+    return codes.float() * _spread(scales.float(), rows, codes.shape)
 
 
 def _plain(s):
@@ -208,16 +210,16 @@ def work(case):
     tokens, k = case["tokens"], case["k"]
     blocks = -(-k // 128)
     if case["kind"] == "quantize":
-        return {"bytes": tokens * k * (_size(case) + 1) + 4 * blocks * -(-tokens // case["rows"]), "flops": 3 * tokens * k}
+        return {"bytes": tokens * k * (_size(case) + 1) + blocks * -(-tokens // case["rows"]), "flops": 2 * tokens * k}
     if case["kind"] == "norm":
         moved = _size(case) * (3 if case["residual"] else 1) + 1
-        return {"bytes": tokens * (k * moved + 4 * blocks) + k * _size(case), "flops": 7 * tokens * k}
+        return {"bytes": tokens * (k * moved + blocks) + k * _size(case), "flops": 7 * tokens * k}
     n = case["n"]
-    x = tokens * (k + 4 * blocks)
-    weight = n * k + 4 * blocks * -(-n // 128)
+    x = tokens * (k + blocks)
+    weight = n * k + blocks * -(-n // 128)
     if case["kind"] == "linear":
         return {"bytes": x + weight + (tokens + int(case["bias"])) * n * _size(case), "flops": 2 * tokens * n * k}
-    return {"bytes": x + 2 * weight + tokens * (n + 4 * -(-n // 128)), "flops": 4 * tokens * n * k}
+    return {"bytes": x + 2 * weight + tokens * (n + -(-n // 128)), "flops": 4 * tokens * n * k}
 
 
 # ---- the definition in 64 bits --------------------------------------------------------------------
@@ -234,10 +236,12 @@ def _exact_codes(x, rows):
         amax = part.abs().amax(1)
         if rows > 1:
             amax = torch.stack([piece.amax() for piece in amax.split(rows)])
-        scales[:, b] = amax.clamp(min=2.0**-100) / 448.0
+        e = torch.ceil(torch.log2(amax / 448.0).clamp(min=-127.0))
+        e = torch.where(amax > 448.0 * torch.exp2(e), e + 1, torch.where((e > -127) & (amax <= 448.0 * torch.exp2(e - 1)), e - 1, e))
+        scales[:, b] = torch.exp2(e)
         v = part / scales[:, b].repeat_interleave(rows)[:tokens, None]
         step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0**-6))) - 3)  # e4m3: three fraction bits
-        codes[:, 128 * b : 128 * b + 128] = (torch.round(v / step) * step).clamp(-448.0, 448.0)
+        codes[:, 128 * b : 128 * b + 128] = torch.round(v / step) * step
     return codes, scales
 
 
