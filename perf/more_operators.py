@@ -225,8 +225,9 @@ def work(case):
 # ---- the definition in 64 bits --------------------------------------------------------------------
 
 
-def _exact_codes(x, rows):
-    """The nearest code of each number (float64), ties to even, and the scales."""
+def _exact_codes(x, rows, rounded=False):
+    """What each number (float64) is in units of its scale, and the scales. A computed output of any type is compared with
+    the number that it rounds; where the rounding is all there is to compute, with the nearest code, ties to even."""
     tokens, k = x.shape
     up, across = -(-tokens // rows), -(-k // 128)
     scales = torch.empty(up, across, dtype=torch.float64, device=DEV)
@@ -240,8 +241,10 @@ def _exact_codes(x, rows):
         e = torch.where(amax > 448.0 * torch.exp2(e), e + 1, torch.where((e > -127) & (amax <= 448.0 * torch.exp2(e - 1)), e - 1, e))
         scales[:, b] = torch.exp2(e)
         v = part / scales[:, b].repeat_interleave(rows)[:tokens, None]
-        step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0**-6))) - 3)  # e4m3: three fraction bits
-        codes[:, 128 * b : 128 * b + 128] = torch.round(v / step) * step
+        if rounded:
+            step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0**-6))) - 3)  # e4m3: three fraction bits
+            v = torch.round(v / step) * step
+        codes[:, 128 * b : 128 * b + 128] = v
     return codes, scales
 
 
@@ -259,7 +262,7 @@ def _exact_product(x, w):
 def exact(case, seed):
     s = prepare(case, seed)
     if case["kind"] == "quantize":
-        codes, scales = _exact_codes(s["x"].double(), case["rows"])
+        codes, scales = _exact_codes(s["x"].double(), case["rows"], rounded=True)
         return {"codes": codes, "scales": scales}
     if case["kind"] == "norm":
         h, hidden = s["x"].double(), {}
