@@ -105,7 +105,7 @@ def _spread(groups, rows, shape):
 
 def _plain_codes(x, rows):
     m, p = torch.frexp(_groups(x.abs(), rows))  # amax = m 2^p with m in [0.5, 1), and 448 = 0.875 2^9
-    e = (p - 9 + (m > 0.875).to(p.dtype)).clamp(min=-127)
+    e = torch.where(m > 0, p - 9 + (m > 0.875).to(p.dtype), -127).clamp(min=-127)
     codes = torch.ldexp(x, -_spread(e, rows, x.shape)).to(F8)
     return codes, (e + 127).to(torch.uint8).view(E8)
 
