@@ -156,6 +156,23 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _int, _p, _i64, _i64, _i64, _i64, _i64, ctypes.c_float,
          ctypes.c_float, _p, _i64, _i64, _int, _p],
     ),
+    "llmopt_f8_last_error": (ctypes.c_char_p, []),
+    "llmopt_f8_quantize": (_int, [_p, _i64, _int, _i64, _i64, _i64, _p, _i64, _p, _i64, _p]),
+    "llmopt_f8_rmsnorm": (
+        _int,
+        [_p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, ctypes.c_float, _int, _p],
+    ),
+    "llmopt_f8_linear_workspace": (_size, [_i64, _i64, _i64]),
+    "llmopt_f8_linear": (
+        _int,
+        [_p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _int, _p, _size, _p],
+    ),
+    "llmopt_f8_swiglu_workspace": (_size, [_i64, _i64, _i64]),
+    "llmopt_f8_swiglu": (
+        _int,
+        [_p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _size,
+         _p],
+    ),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 ABI_VERSION = 1
@@ -258,8 +275,13 @@ def call(rc: int, what: str) -> None:
     if rc == 0:
         return
     lib = load_library()
-    kvq = what.startswith(("llmopt_kvq", "llmopt_packed"))  # include/llmopt_kvq.h keeps its own message
-    message = (lib.llmopt_kvq_last_error() if kvq else lib.llmopt_q_last_error()).decode(errors="replace")
+    if what.startswith(("llmopt_kvq", "llmopt_packed")):  # include/llmopt_kvq.h keeps its own message
+        message = lib.llmopt_kvq_last_error()
+    elif what.startswith("llmopt_f8"):  # and so does include/llmopt_float8.h
+        message = lib.llmopt_f8_last_error()
+    else:
+        message = lib.llmopt_q_last_error()
+    message = message.decode(errors="replace")
     if rc == ERR_INVALID_ARG:
         raise ValueError(f"{what}: {message}")
     if rc == ERR_UNSUPPORTED:

@@ -1,8 +1,8 @@
 """Weight quantization: RTN, GPTQ, packed storage and ``QuantLinear``.
 
 Exports the same names as the reference's ``src/llmopt/quantization/__init__.py:30-49``, plus
-the fused projections of :mod:`llmopt.quantization.fused` and the packed checkpoint of
-:mod:`llmopt.quantization.checkpoint` (which have no counterpart there).
+the fused projections of :mod:`llmopt.quantization.fused`, the packed checkpoint of
+:mod:`llmopt.quantization.checkpoint` and 8-bit floating point (:mod:`llmopt.quantization.float8`) (which have no counterpart there).
 """
 
 from __future__ import annotations
@@ -14,6 +14,16 @@ from llmopt.quantization.calibration import (
     apply_quantization,
 )
 from llmopt.quantization.checkpoint import is_quantized_checkpoint, load_quantized_, save_quantized
+from llmopt.quantization.float8 import (
+    Float8Linear,
+    Float8SwiGLU,
+    Float8Tensor,
+    float8_linear,
+    float8_swiglu,
+    quantize_float8,
+    quantize_model_float8_,
+    rmsnorm_float8,
+)
 from llmopt.quantization.fused import FusedQuantLinear, QuantSwiGLU, concat_rows, interleave_gate_up
 from llmopt.quantization.quant_linear import (
     QuantLinear,
@@ -37,6 +47,9 @@ from llmopt.quantization.quantizers import (
 __all__ = [
     "CalibrationHarness",
     "CalibrationResult",
+    "Float8Linear",
+    "Float8SwiGLU",
+    "Float8Tensor",
     "FusedQuantLinear",
     "GPTQQuantizer",
     "HessianCollector",
@@ -51,13 +64,18 @@ __all__ = [
     "choose_qparams",
     "concat_rows",
     "dequantize",
+    "float8_linear",
+    "float8_swiglu",
     "interleave_gate_up",
     "is_quantized_checkpoint",
     "load_quantized_",
     "pack_int4",
+    "quantize_float8",
     "quantize_model_",
+    "quantize_model_float8_",
     "quantize_to_codes",
     "replace_linear_modules",
+    "rmsnorm_float8",
     "save_quantized",
     "unpack_int4",
 ]
