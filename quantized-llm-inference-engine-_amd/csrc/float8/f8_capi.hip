@@ -49,6 +49,11 @@ int check_rows(const char* what, const void* p, int64_t rows, int64_t cols, int6
     if (rc_ != LLMOPT_OK) return rc_;        \
   } while (0)
 
+// Whether rows of codes are what the tiled kernels read: whole 16-byte pieces, and offsets within a tile in 32 bits.
+bool tiled_rows(const void* p, int64_t ld, int64_t cols) {
+  return aligned(p, 16) && ld % 16 == 0 && cols % 16 == 0 && ld <= (int64_t(1) << 21) && cols > 0;
+}
+
 // Workgroups of a grid of `a` x `b`.
 int check_grid(int64_t a, int64_t b) {
   if (a > 0 && b > kMaxInt / a) return fail(LLMOPT_ERR_UNSUPPORTED, "%lld x %lld workgroups are too many", (long long)a, (long long)b);
@@ -113,6 +118,20 @@ int llmopt_f8_linear(const void* x, int64_t ldx, const void* x_scales, int64_t l
   CHECK(check_rows("w_scales", w_scales, groups(N), groups(K), ldws));
   CHECK(check_rows("y", y, M, N, ldy));
   CHECK(check_grid((M + 15) / 16, (N + 63) / 64));
+  if (M > 64 && tiled_rows(x, ldx, K) && tiled_rows(w, ldw, K)) {
+    F8TilesArgs t{};
+    t.x = static_cast<const uint8_t*>(x);
+    t.ldx = ldx;
+    t.x_scales = static_cast<const uint8_t*>(x_scales);
+    t.ldxs = ldxs;
+    t.w[0] = {static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws};
+    t.bias = bias;
+    t.y = y;
+    t.ldy = ldy;
+    t.M = M, t.N = N, t.K = K;
+    t.vec = aligned(y, 16) && ldy % 8 == 0;
+    return hip_status(launch_f8_tiles(t, out_dtype, static_cast<hipStream_t>(stream)), "llmopt_f8_linear");
+  }
   const F8LinearArgs a{static_cast<const uint8_t*>(x), ldx, static_cast<const uint8_t*>(x_scales), ldxs, {static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws},
                        bias, y, ldy, M, N, K};
   return hip_status(launch_f8_linear_any(a, out_dtype, static_cast<hipStream_t>(stream)), "llmopt_f8_linear");
@@ -138,6 +157,22 @@ int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t l
   CHECK(check_grid((M + 15) / 16, (N + 63) / 64));
   CHECK(check_grid(M, groups(N)));
   if (M == 0 || N == 0) return LLMOPT_OK;
+  if (M > 64 && tiled_rows(x, ldx, K) && tiled_rows(gate, ldg, K) && tiled_rows(up, ldu, K)) {
+    F8TilesArgs t{};
+    t.x = static_cast<const uint8_t*>(x);
+    t.ldx = ldx;
+    t.x_scales = static_cast<const uint8_t*>(x_scales);
+    t.ldxs = ldxs;
+    t.w[0] = {static_cast<const uint8_t*>(gate), ldg, static_cast<const uint8_t*>(gate_scales), ldgs};
+    t.w[1] = {static_cast<const uint8_t*>(up), ldu, static_cast<const uint8_t*>(up_scales), ldus};
+    t.codes = static_cast<uint8_t*>(codes);
+    t.ldc = ldc;
+    t.scales = static_cast<uint8_t*>(scales);
+    t.lds = lds;
+    t.M = M, t.N = N, t.K = K;
+    t.vec = aligned(codes, 16) && ldc % 16 == 0;
+    return hip_status(launch_f8_tiles(t, 0, static_cast<hipStream_t>(stream)), "llmopt_f8_swiglu");
+  }
   const size_t need = llmopt_f8_swiglu_workspace(M, N, K);
   if (workspace_bytes < need || (need && !workspace) || !aligned(workspace, 16))
     return fail(LLMOPT_ERR_WORKSPACE, "llmopt_f8_swiglu needs %zu bytes of workspace, aligned to 16", need);

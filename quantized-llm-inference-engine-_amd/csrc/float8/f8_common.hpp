@@ -2,6 +2,8 @@
 // quantizing of a group of 128 numbers.
 #pragma once
 
+#include <type_traits>
+
 #include "../qcommon.hpp"
 
 namespace llmopt {
@@ -68,9 +70,31 @@ struct F8ActArgs {
   int64_t rows, cols;
 };
 
+// The tiled kernels: y = x w[0]^T + bias, or silu(x w[0]^T) * (x w[1]^T) quantized where w[1] has codes. All rows of codes are
+// 16-byte aligned, K a multiple of 16, and the strides at most 2^21.
+struct F8TilesArgs {
+  const uint8_t* x;
+  int64_t ldx;
+  const uint8_t* x_scales;
+  int64_t ldxs;
+  F8Weight w[2];
+  const void* bias;
+  void* y;
+  int64_t ldy;
+  uint8_t* codes;
+  int64_t ldc;
+  uint8_t* scales;
+  int64_t lds;
+  int64_t M, N, K;
+  int vec;  // the output's rows are 16-byte aligned
+  int steps;
+  uint32_t tiles_n, tiles_m;
+};
+
 hipError_t launch_f8_quantize(const F8QuantArgs& a, int dtype, int64_t block_rows, hipStream_t stream);
 hipError_t launch_f8_rmsnorm(const F8NormArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_f8_act(const F8ActArgs& a, hipStream_t stream);
+hipError_t launch_f8_tiles(const F8TilesArgs& a, int out_dtype, hipStream_t stream);
 hipError_t launch_f8_linear_any(const F8LinearArgs& a, int out_dtype, hipStream_t stream);
 
 // ---- groups -----------------------------------------------------------------------------------------
