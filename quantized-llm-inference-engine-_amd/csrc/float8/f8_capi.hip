@@ -129,8 +129,9 @@ int llmopt_f8_linear(const void* x, int64_t ldx, const void* x_scales, int64_t l
     t.y = y;
     t.ldy = ldy;
     t.M = M, t.N = N, t.K = K;
+    t.splits = 1;
     t.vec = aligned(y, 16) && ldy % 8 == 0;
-    return hip_status(launch_f8_tiles(t, out_dtype, static_cast<hipStream_t>(stream)), "llmopt_f8_linear");
+    return hip_status(launch_f8_tiles(t, F8Shape::k256x256, out_dtype, static_cast<hipStream_t>(stream)), "llmopt_f8_linear");
   }
   const F8LinearArgs a{static_cast<const uint8_t*>(x), ldx, static_cast<const uint8_t*>(x_scales), ldxs, {static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws},
                        bias, y, ldy, M, N, K};
@@ -170,8 +171,9 @@ int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t l
     t.scales = static_cast<uint8_t*>(scales);
     t.lds = lds;
     t.M = M, t.N = N, t.K = K;
+    t.splits = 1;
     t.vec = aligned(codes, 16) && ldc % 16 == 0;
-    return hip_status(launch_f8_tiles(t, 0, static_cast<hipStream_t>(stream)), "llmopt_f8_swiglu");
+    return hip_status(launch_f8_tiles(t, F8Shape::k256x256, 0, static_cast<hipStream_t>(stream)), "llmopt_f8_swiglu");
   }
   const size_t need = llmopt_f8_swiglu_workspace(M, N, K);
   if (workspace_bytes < need || (need && !workspace) || !aligned(workspace, 16))

@@ -88,13 +88,54 @@ struct F8TilesArgs {
   int64_t M, N, K;
   int vec;  // the output's rows are 16-byte aligned
   int steps;
-  uint32_t tiles_n, tiles_m;
+  uint32_t tiles_n, tiles_m;         // (set by the launch)
+  uint32_t splits, steps_per_split;  // of K over workgroups
+  float* parts;                      // splits > 1: [splits][M][ld_parts]
+  int64_t ld_parts;
+};
+
+// A workgroup's tile: weight rows x tokens.
+enum class F8Shape { k256x256, k256x128, k256x64, k128x128, k128x64 };
+
+// The kernels of few tokens (at most 64); operands as in F8TilesArgs.
+struct F8DecodeArgs {
+  const uint8_t* x;
+  int64_t ldx;
+  const uint8_t* x_scales;
+  int64_t ldxs;
+  F8Weight w[2];
+  const void* bias;
+  void* y;
+  int64_t ldy;
+  uint8_t* codes;  // the gated product's
+  int64_t ldc;
+  uint8_t* scales;
+  int64_t lds;
+  int64_t M, N, K;
+  int vec;  // the codes' rows are 4-byte aligned
+  uint32_t steps, tiles_n;
+  uint32_t splits, steps_per_split;  // of K over workgroups
+  float* parts;                      // splits > 1: [splits][M][ld_parts]
+  int64_t ld_parts;
 };
 
 hipError_t launch_f8_quantize(const F8QuantArgs& a, int dtype, int64_t block_rows, hipStream_t stream);
 hipError_t launch_f8_rmsnorm(const F8NormArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_f8_act(const F8ActArgs& a, hipStream_t stream);
-hipError_t launch_f8_tiles(const F8TilesArgs& a, int out_dtype, hipStream_t stream);
+hipError_t launch_f8_tiles(const F8TilesArgs& a, F8Shape shape, int out_dtype, hipStream_t stream);
+// The sum of `splits` parts [M, ld_parts] in their order, plus the bias, rounded into y.
+struct F8JoinArgs {
+  const float* parts;
+  uint32_t splits;
+  int64_t M, N, ld_parts;  // (a multiple of 16)
+  const void* bias;
+  void* y;
+  int64_t ldy;
+};
+hipError_t launch_f8_join(const F8JoinArgs& a, int out_dtype, hipStream_t stream);
+// rt: tiles of 16 features a workgroup (1 or 2).
+hipError_t launch_f8_decode(const F8DecodeArgs& a, int rt, int out_dtype, hipStream_t stream);
+hipError_t launch_f8_decode_gated(const F8DecodeArgs& a, hipStream_t stream);
 hipError_t launch_f8_linear_any(const F8LinearArgs& a, int out_dtype, hipStream_t stream);
 
 // ---- groups -----------------------------------------------------------------------------------------

@@ -10,14 +10,39 @@ constexpr int kStep = kF8Group;  // columns of a step: one scale
 // Byte offsets that a buffer load finds behind its buffer's end: zeros.
 constexpr uint32_t kOutside = 0x7FFFFFF0u;
 
-template <int WN, int WM, int TM, bool GATED, class Out>
+constexpr int kChunk = 32;        // steps whose scales are in LDS at a time
+constexpr int kScaleRow = kChunk + 4;  // bytes of a row of them (16 rows in 16 banks)
+
+// Of an operand's scales, what one thread brings to LDS: a row's bytes of the steps first .. first + 31.
+struct ScaleRow {
+  uint32_t v[kChunk / 4];
+  __device__ __forceinline__ void load(const uint8_t* row, int first, int steps) {
+    const int count = steps - first < kChunk ? steps - first : kChunk;
+#pragma unroll
+    for (int i = 0; i < kChunk / 4; ++i) {
+      v[i] = 0;
+      if (4 * i + 4 <= count) {
+        __builtin_memcpy(&v[i], row + first + 4 * i, 4);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (4 * i + e < count) v[i] |= uint32_t(row[first + 4 * i + e]) << (8 * e);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* to) const {
+#pragma unroll
+    for (int i = 0; i < kChunk / 4; ++i) reinterpret_cast<uint32_t*>(to)[i] = v[i];
+  }
+};
+
+template <int WN, int WM, int TM, int STAGES, bool GATED, bool PARTS, class Out>
 __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2, 2)))
     tiles_kernel(const F8TilesArgs a) {
   constexpr int kWaves = WN * WM;
   constexpr int kRowsN = 128 * WN, kRowsM = 16 * TM * WM;
   constexpr int kStage = (kRowsN + kRowsM) * kStep;
-  constexpr uint32_t kBuffer = kStage <= 32768 ? 32768 : 65536;  // from one stage's buffer to the other's
-  static_assert(kStage <= 65536, "two stages in LDS");
+  static_assert(64 * kWaves >= kRowsM + 2, "a thread for every row of scales");
   constexpr int kLoadsN = kRowsN / 8 / kWaves, kLoadsM = kRowsM / 8 / kWaves;
   static_assert(kLoadsN * 8 * kWaves == kRowsN && kLoadsM * 8 * kWaves == kRowsM, "whole loads for every wave");
   extern __shared__ __align__(1024) uint8_t lds[];
@@ -31,11 +56,18 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
   // `kSweep` token tiles per sweep over the features, whose operands then meet in its L2.
   constexpr uint32_t kSweep = 4;
   uint32_t id = blockIdx.x;
-  const uint32_t count = gridDim.x;
   {
-    const uint32_t per = count / 8, rest = count % 8, xcd = id % 8, at = id / 8;
+    const uint32_t per = gridDim.x / 8, rest = gridDim.x % 8, xcd = id % 8, at = id / 8;
     id = xcd * per + min(xcd, rest) + at;
   }
+  uint32_t split = 0;
+  if (PARTS) {  // the parts of a sum one after the other
+    const uint32_t tiles = a.tiles_n * a.tiles_m;
+    split = __builtin_amdgcn_readfirstlane(id / tiles);
+    id -= split * tiles;
+  }
+  const int s_begin = PARTS ? int(split * a.steps_per_split) : 0;
+  const int s_end = PARTS ? min(s_begin + int(a.steps_per_split), a.steps) : a.steps;
   const uint32_t in_sweep = kSweep * a.tiles_n;
   const uint32_t first_m = id / in_sweep * kSweep;
   const uint32_t rows_m = min(a.tiles_m - first_m, kSweep);
@@ -49,7 +81,7 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
   // ---- loads: lane l of load j brings 16 bytes of row 8 (..) + l / 8, its chunk l % 8 swizzled ----
   constexpr int kWide = GATED ? kRowsN / 2 : kRowsN;  // features of a tile
   const int rows_n = a.N - n0 < kWide ? int(a.N - n0) : kWide, rows_mm = a.M - m0 < kRowsM ? int(a.M - m0) : kRowsM;
-  const uint32_t K = uint32_t(a.K);
+  const uint32_t K = uint32_t(a.K), k_end = PARTS ? min(K, uint32_t(s_end) * kStep) : K;
   const auto wq0 = make_rsrc(a.w[0].codes + n0 * a.w[0].ld, uint32_t(rows_n - 1) * uint32_t(a.w[0].ld) + K);
   const auto wq1 = make_rsrc(a.w[GATED].codes + n0 * a.w[GATED].ld, uint32_t(rows_n - 1) * uint32_t(a.w[GATED].ld) + K);
   const auto xq = make_rsrc(a.x + m0 * a.ldx, uint32_t(rows_mm - 1) * uint32_t(a.ldx) + K);
@@ -67,57 +99,66 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
   off_n[0] = uint32_t(base_n(0) + lane / 8) * uint32_t(a.w[0].ld);
   off_n[1] = uint32_t(base_n(0) + lane / 8) * uint32_t(a.w[GATED].ld);
   const uint32_t off_m = uint32_t(base_m(0) + lane / 8) * uint32_t(a.ldx) + col_m;
-  auto load_stage = [&](int step, uint8_t* buf) {
+  // Loads first .. last - 1 of a stage.
+  constexpr int kLoads = kLoadsN + kLoadsM;
+  auto load_stage = [&](int step, uint8_t* buf, int first, int last) {
     const uint32_t k = uint32_t(step) * kStep;
-    const bool whole = k + kStep <= K;  // else columns behind the end are zeros
+    const bool whole = k + kStep <= k_end;  // else columns behind the end are zeros
     // The strides are opaque here, so that offsets are computed where they are used and hold no registers.
     uint32_t ld[3] = {uint32_t(a.w[0].ld), uint32_t(a.w[GATED].ld), uint32_t(a.ldx)};
     asm volatile("" : "+s"(ld[0]), "+s"(ld[1]), "+s"(ld[2]));
 #pragma unroll
-    for (int j = 0; j < kLoadsN; ++j) {
-      const bool second = GATED && j >= kHalf;
-      uint32_t o = off_n[second] + uint32_t(8 * (second ? j - kHalf : j)) * ld[second] + col_n(j);
-      if (!whole) o = k + col_n(j) < K ? o : kOutside;
-      load_lds16_cached(second ? wq1 : wq0, buf + base_n(j) * kStep, o, k);
-    }
-#pragma unroll
-    for (int j = 0; j < kLoadsM; ++j) {
-      uint32_t o = off_m + uint32_t(8 * j) * ld[2];
-      if (!whole) o = k + col_m < K ? o : kOutside;
-      load_lds16_cached(xq, buf + (kRowsN + base_m(j)) * kStep, o, k);
+    for (int j = first; j < last; ++j) {
+      if (j < kLoadsN) {
+        const bool second = GATED && j >= kHalf;
+        uint32_t o = off_n[second] + uint32_t(8 * (second ? j - kHalf : j)) * ld[second] + col_n(j);
+        if (!whole) o = k + col_n(j) < k_end ? o : kOutside;
+        load_lds16_cached(second ? wq1 : wq0, buf + base_n(j) * kStep, o, k);
+      } else {
+        uint32_t o = off_m + uint32_t(8 * (j - kLoadsN)) * ld[2];
+        if (!whole) o = k + col_m < k_end ? o : kOutside;
+        load_lds16_cached(xq, buf + (kRowsN + base_m(j - kLoadsN)) * kStep, o, k);
+      }
     }
   };
 
-  // ---- scales ----
-  const auto xs = make_rsrc(a.x_scales + m0 * a.ldxs, uint32_t(rows_mm - 1) * uint32_t(a.ldxs) + uint32_t(a.steps));
-  const uint32_t xs_off = uint32_t(wm * TM * 16 + r) * uint32_t(a.ldxs);
-  const uint32_t ws_row = GATED ? tn : min(tn * WN + wn, uint32_t((a.N - 1) / kF8Group));
-  const auto ws0 = make_rsrc(a.w[0].scales + ws_row * a.w[0].lds, uint32_t(a.steps));
-  const auto ws1 = make_rsrc(a.w[GATED].scales + ws_row * a.w[GATED].lds, uint32_t(a.steps));
+  // ---- scales: a chunk of steps at a time in LDS, a row of tokens or of the weight's blocks a thread ----
+  uint8_t* const scales = lds + STAGES * kStage;
+  const uint8_t* scale_row = nullptr;
+  {
+    const int t = threadIdx.x;
+    if (t < kRowsM) {
+      scale_row = a.x_scales + (m0 + min(t, rows_mm - 1)) * a.ldxs;
+    } else if (t < kRowsM + (GATED ? 2 : WN)) {
+      const int second = t - kRowsM;
+      if (GATED)
+        scale_row = a.w[second].scales + tn * a.w[second].lds;
+      else
+        scale_row = a.w[0].scales + min(tn * WN + second, uint32_t((a.N - 1) / kF8Group)) * a.w[0].lds;
+    }
+  }
+  const uint8_t* const sx_at = scales + (wm * TM * 16 + r) * kScaleRow;
+  const uint8_t* const sw_at = scales + (kRowsM + (GATED ? 0 : wn)) * kScaleRow;
   uint32_t sx[TM], sw[2], sx_next[TM], sw_next[2];
-  auto load_scales = [&](int step, uint32_t* x, uint32_t* w) {
-    uint32_t ld = uint32_t(a.ldxs);
-    asm volatile("" : "+s"(ld));
+  auto read_scales = [&](int step, uint32_t* x, uint32_t* w) {
 #pragma unroll
-    for (int t = 0; t < TM; ++t) x[t] = __builtin_amdgcn_raw_buffer_load_b8(xs, int(xs_off + uint32_t(16 * t) * ld), step, 0);
-    w[0] = __builtin_amdgcn_raw_buffer_load_b8(ws0, 0, step, 0);
-    if (GATED) w[1] = __builtin_amdgcn_raw_buffer_load_b8(ws1, 0, step, 0);
+    for (int u = 0; u < TM; ++u) x[u] = sx_at[u * 16 * kScaleRow + step];
+    w[0] = sw_at[step];
+    if (GATED) w[1] = sw_at[kScaleRow + step];
   };
 
   // ---- fragments ----
   // The weight's rows are dealt to the matrix core so that a lane's sums of its 8 tiles are neighbours: lane (r, g) gets rows
   // 32 g + 4 t + i of the wave's 128 in tile t, element i (gated: 16 g + 4 t + i of the gate's 64, then of up's).
   const int row_n = GATED ? wn * 64 + (r >> 2) * 16 + (r & 3) : wn * 128 + (r >> 2) * 32 + (r & 3);
-  const int at_n = row_n * kStep + 16 * (g ^ (r & 7)), at_m = (kRowsN + wm * TM * 16 + r) * kStep + 16 * (g ^ (r & 7));
-  // Four addresses, of either half of the columns, that turn to the other buffer at each step (a power of two apart).
-  uint32_t frag_at[4] = {uint32_t(at_n), uint32_t(at_n ^ 64), uint32_t(at_m), uint32_t(at_m ^ 64)};
-  auto frag = [&](int which, int offset) {
-    const u32x4 lo = *reinterpret_cast<const u32x4*>(lds + frag_at[which] + offset);
-    const u32x4 hi = *reinterpret_cast<const u32x4*>(lds + frag_at[which + 1] + offset);
+  uint32_t at_n = row_n * kStep + 16 * (g ^ (r & 7)), at_m = (kRowsN + wm * TM * 16 + r) * kStep + 16 * (g ^ (r & 7));
+  auto frag = [&](uint32_t at, int offset) {
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(lds + at + offset);
+    const u32x4 hi = *reinterpret_cast<const u32x4*>(lds + (at ^ 64) + offset);
     return __builtin_bit_cast(i32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  auto frag_n = [&](int t) { return frag(0, (GATED ? (t >> 2) * kWide + (t & 3) * 4 : t * 4) * kStep); };
-  auto frag_m = [&](int u) { return frag(2, u * 16 * kStep); };
+  auto frag_n = [&](int t) { return frag(at_n, (GATED ? (t >> 2) * kWide + (t & 3) * 4 : t * 4) * kStep); };
+  auto frag_m = [&](int u) { return frag(at_m, u * 16 * kStep); };
 
   f32x4 acc[8][TM];
 #pragma unroll
@@ -125,65 +166,94 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
 #pragma unroll
     for (int u = 0; u < TM; ++u) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // A step's 32 (8 TM) products are dealt to four phases of two weight tiles. In each, the weight tiles of the next phase come
-  // from LDS. In front of the last phase everything of this step is in registers and the next stage in LDS (a barrier), so
-  // that phase brings in the next step's first fragments, each token tile's when its registers have served, and starts the
-  // loads of the stage after the next into this step's buffer.
+  // A step's 8 TM products are dealt to four phases of two weight tiles. In each, the weight tiles of the next phase come from
+  // LDS. In front of the last phase everything of this step is in registers and the next stage in LDS (a barrier), so that
+  // phase brings in the next step's first fragments, each token tile's when its registers have served, and starts the loads
+  // of STAGES stages on into this step's buffer. The loop's body has no branch: the compiler would move products behind it.
+  // A load that finds the queue full holds up its wave, products behind it included; so they are dealt to two phases, the
+  // last and the next step's first, between the products.
+  constexpr int kSlots = 2 * TM;
+  auto load_slot = [&](int step, uint8_t* to, int slot) { load_stage(step, to, kLoads * slot / kSlots, kLoads * (slot + 1) / kSlots); };
   i32x8 b[TM], w[4];
   auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
-  load_stage(0, lds);
-  load_scales(0, sx, sw);
-  load_stage(1, lds + kBuffer);
-  wait_vmcnt<0>();
-  __builtin_amdgcn_s_barrier();
-  fence();
-#pragma unroll
-  for (int u = 0; u < TM; ++u) b[u] = frag_m(u);
-  w[0] = frag_n(0);
-  w[1] = frag_n(1);
   auto mul = [&](int t, int u) { acc[t][u] = mfma_f8(w[t & 3], b[u], acc[t][u], sw[GATED ? t >> 2 : 0], sx[u]); };
-#pragma unroll 1
-  for (int s = 0; s < a.steps; ++s) {
-    load_scales(s + 1, sx_next, sw_next);  // (zeros behind the end)
-    fence();
 #pragma unroll
-    for (int phase = 0; phase < 3; ++phase) {
-      const int t = 2 * phase;
-#pragma unroll
-      for (int u = 0; u < TM; ++u) {
-        if (u == 0) w[(t + 2) & 3] = frag_n(t + 2);
-        if (u == TM / 2) w[(t + 3) & 3] = frag_n(t + 3);
-        mul(t, u);
-        mul(t + 1, u);
-        fence();
-      }
+  for (int i = 0; i < STAGES; ++i) load_stage(s_begin + i, lds + i * kStage, 0, i < STAGES - 1 ? kLoads : kLoads * TM / kSlots);
+  uint32_t buf = 0, freed = (STAGES - 1) * kStage;  // the step's stage, and the one before it
+  for (int c = s_begin; c < s_end; c += kChunk) {
+    __builtin_amdgcn_s_barrier();  // the chunk before this one has been read
+    if (scale_row) {
+      ScaleRow row;
+      row.load(scale_row, c, s_end);
+      row.store(scales + threadIdx.x * kScaleRow);
     }
     wait_lgkmcnt0();
     wait_vmcnt<0>();
     __builtin_amdgcn_s_barrier();
     fence();
+    read_scales(0, sx, sw);
+    if (c == s_begin) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) frag_at[i] ^= kBuffer;
-    load_stage(s + 2, lds + (s & 1) * kBuffer);  // (zeros behind the end)
-    fence();
-#pragma unroll
-    for (int u = 0; u < TM; ++u) {
-      if (u == 0) w[0] = frag_n(0);
-      if (u == TM / 2) w[1] = frag_n(1);
-      mul(6, u);
-      mul(7, u);
-      fence();
-      b[u] = frag_m(u);
+      for (int u = 0; u < TM; ++u) b[u] = frag_m(u);
+      w[0] = frag_n(0);
+      w[1] = frag_n(1);
     }
+    const int last = min(s_end - c, kChunk);
+#pragma unroll 1
+    for (int s = 0; s < last; ++s) {
 #pragma unroll
-    for (int u = 0; u < TM; ++u) sx[u] = sx_next[u];
-    sw[0] = sw_next[0];
-    if (GATED) sw[1] = sw_next[1];
-    fence();
+      for (int phase = 0; phase < 3; ++phase) {
+        const int t = 2 * phase;
+#pragma unroll
+        for (int u = 0; u < TM; ++u) {
+          if (u == 0) w[(t + 2) & 3] = frag_n(t + 2);
+          if (u == TM / 2) w[(t + 3) & 3] = frag_n(t + 3);
+          mul(t, u);
+          if (phase == 0) load_slot(c + s + STAGES - 1, lds + freed, TM + u);  // (zeros behind the end)
+          mul(t + 1, u);
+          fence();
+        }
+      }
+      read_scales(s + 1, sx_next, sw_next);  // (of the next chunk: read again)
+      wait_lgkmcnt0();
+      wait_vmcnt<(STAGES - 2) * kLoads>();
+      __builtin_amdgcn_s_barrier();
+      fence();
+      const uint32_t next = buf == (STAGES - 1) * kStage ? 0u : buf + kStage;
+      at_n += next - buf, at_m += next - buf, freed = buf, buf = next;
+      fence();
+#pragma unroll
+      for (int u = 0; u < TM; ++u) {
+        if (u == 0) w[0] = frag_n(0);
+        if (u == TM / 2) w[1] = frag_n(1);
+        mul(6, u);
+        load_slot(c + s + STAGES, lds + freed, u);
+        mul(7, u);
+        fence();
+        b[u] = frag_m(u);
+      }
+#pragma unroll
+      for (int u = 0; u < TM; ++u) sx[u] = sx_next[u];
+      sw[0] = sw_next[0];
+      if (GATED) sw[1] = sw_next[1];
+      fence();
+    }
   }
+  wait_vmcnt<0>();  // zeros on their way into LDS
 
   // ---- results ----
-  if constexpr (!GATED) {
+  if constexpr (PARTS) {  // rows of a multiple of 16 features
+    const int64_t n = n0 + wn * 128 + 32 * g;
+#pragma unroll
+    for (int u = 0; u < TM; ++u) {
+      const int64_t m = m0 + (wm * TM + u) * 16 + r;
+      if (m >= a.M) continue;
+      float* out = a.parts + (int64_t(split) * a.M + m) * a.ld_parts + n;
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        if (n + 4 * t < a.N) *reinterpret_cast<f32x4*>(out + 4 * t) = acc[t][u];
+    }
+  } else if constexpr (!GATED) {
     using Raw = typename Out::raw;
     const int64_t n = n0 + wn * 128 + 32 * g;
     const Raw* bias = static_cast<const Raw*>(a.bias);
@@ -258,28 +328,48 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
   }
 }
 
-template <int WN, int WM, int TM, bool GATED, class Out>
-hipError_t launch(F8TilesArgs a, hipStream_t stream) {
+template <int WN, int WM, int TM, int STAGES, bool GATED, bool PARTS, class Out>
+hipError_t launch(const F8TilesArgs& a, hipStream_t stream) {
   constexpr int kRowsN = 128 * WN, kRowsM = 16 * TM * WM;
-  a.tiles_n = uint32_t((a.N + (GATED ? kRowsN / 2 : kRowsN) - 1) / (GATED ? kRowsN / 2 : kRowsN));
-  a.tiles_m = uint32_t((a.M + kRowsM - 1) / kRowsM);
-  a.steps = int((a.K + kStep - 1) / kStep);
-  constexpr int kStage = (kRowsN + kRowsM) * kStep;
-  constexpr int kBytes = (kStage <= 32768 ? 32768 : 65536) + kStage;
-  auto* kernel = tiles_kernel<WN, WM, TM, GATED, Out>;
+  constexpr int kBytes = STAGES * (kRowsN + kRowsM) * kStep + (kRowsM + 2) * kScaleRow;
+  static_assert(kBytes <= 160 * 1024, "stages and scales fit LDS");
+  auto* kernel = tiles_kernel<WN, WM, TM, STAGES, GATED, PARTS, Out>;
   static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (ready != hipSuccess) return ready;
-  hipLaunchKernelGGL(kernel, dim3(a.tiles_n * a.tiles_m), dim3(64 * WN * WM), kBytes, stream, a);
+  hipLaunchKernelGGL(kernel, dim3(a.tiles_n * a.tiles_m * a.splits), dim3(64 * WN * WM), kBytes, stream, a);
   return hipGetLastError();
+}
+
+template <int WN, int WM, int TM, int STAGES>
+hipError_t launch_shape(F8TilesArgs a, int out_dtype, hipStream_t stream) {
+  constexpr int kRowsN = 128 * WN, kRowsM = 16 * TM * WM;
+  const bool gated = a.w[1].codes != nullptr;
+  const int64_t wide = gated ? kRowsN / 2 : kRowsN;
+  a.tiles_n = uint32_t((a.N + wide - 1) / wide);
+  a.tiles_m = uint32_t((a.M + kRowsM - 1) / kRowsM);
+  a.steps = int((a.K + kStep - 1) / kStep);
+  if (a.splits > 1) {
+    const hipError_t err = launch<WN, WM, TM, STAGES, false, true, ActBf16>(a, stream);
+    if (err != hipSuccess) return err;
+    return launch_f8_join({a.parts, a.splits, a.M, a.N, a.ld_parts, a.bias, a.y, a.ldy}, out_dtype, stream);
+  }
+  if constexpr (WN == 2) {
+    if (gated) return launch<WN, WM, TM, STAGES, true, false, ActBf16>(a, stream);
+  }
+  if (out_dtype == kDtF16) return launch<WN, WM, TM, STAGES, false, false, ActF16>(a, stream);
+  return launch<WN, WM, TM, STAGES, false, false, ActBf16>(a, stream);
 }
 
 }  // namespace
 
-hipError_t launch_f8_tiles(const F8TilesArgs& a, int out_dtype, hipStream_t stream) {
-  if (a.M == 0 || a.N == 0) return hipSuccess;
-  if (a.w[1].codes) return launch<2, 4, 4, true, ActBf16>(a, stream);
-  if (out_dtype == kDtF16) return launch<2, 4, 4, false, ActF16>(a, stream);
-  return launch<2, 4, 4, false, ActBf16>(a, stream);
+hipError_t launch_f8_tiles(const F8TilesArgs& a, F8Shape shape, int out_dtype, hipStream_t stream) {
+  switch (shape) {
+    case F8Shape::k256x256: return launch_shape<2, 4, 4, 2>(a, out_dtype, stream);
+    case F8Shape::k256x128: return launch_shape<2, 4, 2, 3>(a, out_dtype, stream);
+    case F8Shape::k256x64: return launch_shape<2, 4, 1, 3>(a, out_dtype, stream);
+    case F8Shape::k128x128: return launch_shape<1, 4, 2, 2>(a, out_dtype, stream);
+    default: return launch_shape<1, 4, 1, 3>(a, out_dtype, stream);
+  }
 }
 
 }  // namespace llmopt
