@@ -57,13 +57,13 @@ int llmopt_f8_linear(const void* x, int64_t ldx, const void* x_scales, int64_t l
                      const void* w, int64_t ldw, const void* w_scales, int64_t ldws, const void* bias, void* y,
                      int64_t ldy, int64_t N, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Bytes of workspace that llmopt_f8_swiglu needs. */
+/* Bytes of workspace with which llmopt_f8_swiglu is fastest (0: it uses none). */
 size_t llmopt_f8_swiglu_workspace(int64_t M, int64_t N, int64_t K);
 
 /*
  * silu(x gate^T) * (x up^T), with silu(g) = g / (1 + exp(-g)) in fp32 on the fp32 sums, quantized by rows into codes [M, N]
- * and scales. x as in llmopt_f8_linear, gate and up weights [N, K]. Needs llmopt_f8_swiglu_workspace bytes, else
- * LLMOPT_ERR_WORKSPACE.
+ * and scales. x as in llmopt_f8_linear, gate and up weights [N, K]. With less workspace than llmopt_f8_swiglu_workspace
+ * asks for, another kernel runs (correct, slower).
  */
 int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t ldxs, int64_t M, int64_t K,
                      const void* gate, int64_t ldg, const void* gate_scales, int64_t ldgs, const void* up, int64_t ldu,

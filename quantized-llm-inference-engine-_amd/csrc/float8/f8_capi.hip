@@ -2,6 +2,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <algorithm>
+
 #include "../../../include/llmopt_float8.h"
 #include "../../../include/llmopt_qlinear.h"
 #include "f8_common.hpp"
@@ -49,15 +51,72 @@ int check_rows(const char* what, const void* p, int64_t rows, int64_t cols, int6
     if (rc_ != LLMOPT_OK) return rc_;        \
   } while (0)
 
-// Whether rows of codes are what the tiled kernels read: whole 16-byte pieces, and offsets within a tile in 32 bits.
-bool tiled_rows(const void* p, int64_t ld, int64_t cols) {
-  return aligned(p, 16) && ld % 16 == 0 && cols % 16 == 0 && ld <= (int64_t(1) << 21) && cols > 0;
+// Whether rows of codes are what the decode and tiled kernels read: whole 16-byte pieces, and offsets within a tile in 32 bits
+// (those of a row's scales, too).
+bool tiled_rows(const void* p, int64_t ld, int64_t cols, int64_t ld_scales = 0) {
+  constexpr int64_t kMost = int64_t(1) << 21;
+  return aligned(p, 16) && ld % 16 == 0 && cols % 16 == 0 && ld <= kMost && cols > 0 && cols <= kMost && ld_scales <= kMost;
 }
 
 // Workgroups of a grid of `a` x `b`.
 int check_grid(int64_t a, int64_t b) {
   if (a > 0 && b > kMaxInt / a) return fail(LLMOPT_ERR_UNSUPPORTED, "%lld x %lld workgroups are too many", (long long)a, (long long)b);
   return LLMOPT_OK;
+}
+
+// ---- the choice of kernels --------------------------------------------------------------------------
+
+constexpr int64_t kFewTokens = 16;  // what the decode kernel takes
+
+// A tile's shape and the parts of K: the least of an estimate of the time. A workgroup's step of 128 columns takes `alone`
+// us where few workgroups run and `full` where every CU has its share; a round of workgroups (256 of them, or 512 where two
+// fit a CU) adds `round`, the first loads and the results; parts are written and read again at some 2.7 TB/s.
+// Measured (MI355X, in a graph, us; the estimate's choice first): 4096 x 14336, 8192 tokens, 256 x 256 383, 256 x 128 472, 256 x
+// 64 637; 1024 tokens, 256 x 128 in two parts 78, 256 x 64 88, 256 x 256 161; 256 tokens, 256 x 64 in four parts 37, whole 85;
+// 32 tokens, 128 x 64 in eight parts 19, whole 59; 6144 x 4096, 200 tokens, 128 x 64 19, 256 x 64 26, 256 x 256 57; 1536 x
+// 1040, 777 tokens, 128 x 64 9.8, 128 x 128 13, 256 x 256 24.
+struct Tile {
+  F8Shape shape;
+  int64_t n, m, per_cu;
+  double alone, full, round;
+};
+constexpr Tile kTiles[] = {
+    {F8Shape::k256x256, 256, 256, 1, 1.38, 1.70, 5.0}, {F8Shape::k256x128, 256, 128, 1, 0.83, 1.05, 4.0},
+    {F8Shape::k256x64, 256, 64, 1, 0.75, 0.71, 3.0},   {F8Shape::k128x128, 128, 128, 2, 0.94, 1.10, 3.5},
+    {F8Shape::k128x64, 128, 64, 2, 0.53, 0.71, 3.0},
+};
+
+struct Plan {
+  F8Shape shape;
+  int64_t splits, steps_per_split;
+};
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int64_t padded(int64_t n) { return up(n, 16) * 16; }
+
+size_t parts_bytes(int64_t M, int64_t N, int64_t splits) {
+  return splits > 1 ? size_t(splits) * size_t(M) * size_t(padded(N)) * sizeof(float) : 0;
+}
+
+Plan plan_tiles(int64_t M, int64_t N, int64_t K, bool gated, size_t workspace) {
+  Plan best{F8Shape::k256x256, 1, 1};
+  double least = 1e30;
+  const int64_t steps = std::max<int64_t>(1, groups(K));
+  for (const Tile& t : kTiles) {
+    if (gated && t.n != 256) continue;  // a group of 128 features of both weights
+    const int64_t tiles = up(N, gated ? t.n / 2 : t.n) * up(M, t.m);
+    for (int64_t splits = 1; splits <= (gated ? 1 : 8); splits *= 2) {
+      const int64_t per = up(steps, splits);
+      if (splits > 1 && (per < 4 || up(steps, per) != splits || parts_bytes(M, N, splits) > workspace)) break;
+      const int64_t count = tiles * splits, rounds = up(count, 256 * t.per_cu);
+      const double load = std::min(1.0, double(count) / (256.0 * double(t.per_cu)));
+      double us = double(rounds) * (double(per) * (t.alone + (t.full - t.alone) * load) + t.round) + 2.0;
+      if (splits > 1) us += 3.0 + double(M) * double(N) * 8.0 * double(splits) / 2.7e6;
+      if (us < least) least = us, best = Plan{t.shape, splits, per};
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -102,14 +161,14 @@ int llmopt_f8_rmsnorm(const void* x, int64_t ldx, const void* residual, int64_t 
 }
 
 size_t llmopt_f8_linear_workspace(int64_t M, int64_t N, int64_t K) {
-  (void)M, (void)N, (void)K;
-  return 0;
+  if (M <= kFewTokens || N < 1 || K < 1 || M > kMaxInt || N > kMaxInt || K > kMaxInt) return 0;
+  const Plan plan = plan_tiles(M, N, K, false, SIZE_MAX);
+  return parts_bytes(M, N, plan.splits);
 }
 
 int llmopt_f8_linear(const void* x, int64_t ldx, const void* x_scales, int64_t ldxs, int64_t M, int64_t K,
                      const void* w, int64_t ldw, const void* w_scales, int64_t ldws, const void* bias, void* y,
                      int64_t ldy, int64_t N, int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
-  (void)workspace, (void)workspace_bytes;
   if (!valid_dtype(out_dtype)) return fail(LLMOPT_ERR_INVALID_ARG, "bad dtype code %d", out_dtype);
   if (out_dtype == LLMOPT_DTYPE_F32) return fail(LLMOPT_ERR_UNSUPPORTED, "the product is fp16 or bf16");
   CHECK(check_rows("x", x, M, K, ldx));
@@ -117,78 +176,80 @@ int llmopt_f8_linear(const void* x, int64_t ldx, const void* x_scales, int64_t l
   CHECK(check_rows("w", w, N, K, ldw));
   CHECK(check_rows("w_scales", w_scales, groups(N), groups(K), ldws));
   CHECK(check_rows("y", y, M, N, ldy));
-  CHECK(check_grid((M + 15) / 16, (N + 63) / 64));
-  if (M > 64 && tiled_rows(x, ldx, K) && tiled_rows(w, ldw, K)) {
-    F8TilesArgs t{};
-    t.x = static_cast<const uint8_t*>(x);
-    t.ldx = ldx;
-    t.x_scales = static_cast<const uint8_t*>(x_scales);
-    t.ldxs = ldxs;
-    t.w[0] = {static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws};
-    t.bias = bias;
-    t.y = y;
-    t.ldy = ldy;
-    t.M = M, t.N = N, t.K = K;
-    t.splits = 1;
-    t.vec = aligned(y, 16) && ldy % 8 == 0;
-    return hip_status(launch_f8_tiles(t, F8Shape::k256x256, out_dtype, static_cast<hipStream_t>(stream)), "llmopt_f8_linear");
+  CHECK(check_grid(8 * up(M, 16), up(N, 64)));
+  if (M == 0 || N == 0) return LLMOPT_OK;
+  F8TilesArgs t{};
+  t.x = static_cast<const uint8_t*>(x);
+  t.ldx = ldx;
+  t.x_scales = static_cast<const uint8_t*>(x_scales);
+  t.ldxs = ldxs;
+  t.w[0] = {static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws};
+  t.bias = bias;
+  t.y = y;
+  t.ldy = ldy;
+  t.M = M, t.N = N, t.K = K;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (!tiled_rows(x, ldx, K, ldxs) || !tiled_rows(w, ldw, K)) return hip_status(launch_f8_any(t, out_dtype, st), "llmopt_f8_linear");
+  if (M <= kFewTokens) {
+    const F8DecodeArgs d{t.x, ldx, t.x_scales, ldxs, {t.w[0], {}}, bias, y, ldy, M, N, K, 0, 0};
+    return hip_status(launch_f8_decode(d, out_dtype, st), "llmopt_f8_linear");
   }
-  const F8LinearArgs a{static_cast<const uint8_t*>(x), ldx, static_cast<const uint8_t*>(x_scales), ldxs, {static_cast<const uint8_t*>(w), ldw, static_cast<const uint8_t*>(w_scales), ldws},
-                       bias, y, ldy, M, N, K};
-  return hip_status(launch_f8_linear_any(a, out_dtype, static_cast<hipStream_t>(stream)), "llmopt_f8_linear");
+  const Plan plan = plan_tiles(M, N, K, false, workspace && aligned(workspace, 16) ? workspace_bytes : 0);
+  t.vec = aligned(y, 16) && ldy % 8 == 0;
+  t.splits = uint32_t(plan.splits);
+  t.steps_per_split = uint32_t(plan.steps_per_split);
+  t.parts = static_cast<float*>(workspace);
+  t.ld_parts = padded(N);
+  return hip_status(launch_f8_tiles(t, plan.shape, out_dtype, st), "llmopt_f8_linear");
 }
 
 size_t llmopt_f8_swiglu_workspace(int64_t M, int64_t N, int64_t K) {
-  (void)K;
-  return M > 0 && N > 0 ? size_t(M) * size_t((N + 7) / 8 * 8) * 2 * sizeof(float) : 0;
+  return M > 0 && M <= kFewTokens && N > 0 && K > 0 ? size_t(2) * size_t(M) * size_t(padded(N)) * sizeof(float) : 0;
 }
 
 int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t ldxs, int64_t M, int64_t K,
-                     const void* gate, int64_t ldg, const void* gate_scales, int64_t ldgs, const void* up, int64_t ldu,
+                     const void* gate, int64_t ldg, const void* gate_scales, int64_t ldgs, const void* up_, int64_t ldu,
                      const void* up_scales, int64_t ldus, int64_t N, void* codes, int64_t ldc, void* scales,
                      int64_t lds, void* workspace, size_t workspace_bytes, void* stream) {
   CHECK(check_rows("x", x, M, K, ldx));
   CHECK(check_rows("x_scales", x_scales, M, groups(K), ldxs));
   CHECK(check_rows("gate", gate, N, K, ldg));
   CHECK(check_rows("gate_scales", gate_scales, groups(N), groups(K), ldgs));
-  CHECK(check_rows("up", up, N, K, ldu));
+  CHECK(check_rows("up", up_, N, K, ldu));
   CHECK(check_rows("up_scales", up_scales, groups(N), groups(K), ldus));
   CHECK(check_rows("codes", codes, M, N, ldc));
   CHECK(check_rows("scales", scales, M, groups(N), lds));
-  CHECK(check_grid((M + 15) / 16, (N + 63) / 64));
-  CHECK(check_grid(M, groups(N)));
+  CHECK(check_grid(up(M, 16), up(N, 64)));
   if (M == 0 || N == 0) return LLMOPT_OK;
-  if (M > 64 && tiled_rows(x, ldx, K) && tiled_rows(gate, ldg, K) && tiled_rows(up, ldu, K)) {
-    F8TilesArgs t{};
-    t.x = static_cast<const uint8_t*>(x);
-    t.ldx = ldx;
-    t.x_scales = static_cast<const uint8_t*>(x_scales);
-    t.ldxs = ldxs;
-    t.w[0] = {static_cast<const uint8_t*>(gate), ldg, static_cast<const uint8_t*>(gate_scales), ldgs};
-    t.w[1] = {static_cast<const uint8_t*>(up), ldu, static_cast<const uint8_t*>(up_scales), ldus};
-    t.codes = static_cast<uint8_t*>(codes);
-    t.ldc = ldc;
-    t.scales = static_cast<uint8_t*>(scales);
-    t.lds = lds;
-    t.M = M, t.N = N, t.K = K;
-    t.splits = 1;
-    t.vec = aligned(codes, 16) && ldc % 16 == 0;
-    return hip_status(launch_f8_tiles(t, F8Shape::k256x256, 0, static_cast<hipStream_t>(stream)), "llmopt_f8_swiglu");
-  }
-  const size_t need = llmopt_f8_swiglu_workspace(M, N, K);
-  if (workspace_bytes < need || (need && !workspace) || !aligned(workspace, 16))
-    return fail(LLMOPT_ERR_WORKSPACE, "llmopt_f8_swiglu needs %zu bytes of workspace, aligned to 16", need);
-  const int64_t ld = (N + 7) / 8 * 8;
-  float* sums = static_cast<float*>(workspace);
-  F8LinearArgs a{static_cast<const uint8_t*>(x), ldx, static_cast<const uint8_t*>(x_scales), ldxs, {static_cast<const uint8_t*>(gate), ldg, static_cast<const uint8_t*>(gate_scales), ldgs},
-                 nullptr, sums, ld, M, N, K};
+  F8TilesArgs t{};
+  t.x = static_cast<const uint8_t*>(x);
+  t.ldx = ldx;
+  t.x_scales = static_cast<const uint8_t*>(x_scales);
+  t.ldxs = ldxs;
+  t.w[0] = {static_cast<const uint8_t*>(gate), ldg, static_cast<const uint8_t*>(gate_scales), ldgs};
+  t.w[1] = {static_cast<const uint8_t*>(up_), ldu, static_cast<const uint8_t*>(up_scales), ldus};
+  t.codes = static_cast<uint8_t*>(codes);
+  t.ldc = ldc;
+  t.scales = static_cast<uint8_t*>(scales);
+  t.lds = lds;
+  t.M = M, t.N = N, t.K = K;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  CHECK(hip_status(launch_f8_linear_any(a, LLMOPT_DTYPE_F32, st), "llmopt_f8_swiglu"));
-  a.w = {static_cast<const uint8_t*>(up), ldu, static_cast<const uint8_t*>(up_scales), ldus};
-  a.y = sums + M * ld;
-  CHECK(hip_status(launch_f8_linear_any(a, LLMOPT_DTYPE_F32, st), "llmopt_f8_swiglu"));
-  const F8ActArgs act{sums, sums + M * ld, ld, static_cast<uint8_t*>(codes), ldc, static_cast<uint8_t*>(scales), lds, M, N};
-  return hip_status(launch_f8_act(act, st), "llmopt_f8_swiglu");
+  // Without columns a weight has no codes to point to.
+  if (K == 0) t.w[0].codes = t.w[1].codes = static_cast<const uint8_t*>(codes);
+  if (!tiled_rows(x, ldx, K, ldxs) || !tiled_rows(gate, ldg, K) || !tiled_rows(up_, ldu, K))
+    return hip_status(launch_f8_any(t, 0, st), "llmopt_f8_swiglu");
+  if (workspace && aligned(workspace, 16) && M <= kFewTokens && workspace_bytes >= llmopt_f8_swiglu_workspace(M, N, K)) {
+    float* sums = static_cast<float*>(workspace);
+    const int64_t ld = padded(N);
+    const F8DecodeArgs d{t.x, ldx, t.x_scales, ldxs, {t.w[0], t.w[1]}, nullptr, sums, ld, M, N, K, 0, 0};
+    CHECK(hip_status(launch_f8_decode(d, kDtF32, st), "llmopt_f8_swiglu"));
+    const F8ActArgs act{sums, sums + M * ld, ld, t.codes, ldc, t.scales, lds, M, N};
+    return hip_status(launch_f8_act(act, st), "llmopt_f8_swiglu");
+  }
+  const Plan plan = plan_tiles(M, N, K, true, 0);
+  t.vec = aligned(codes, 16) && ldc % 16 == 0;
+  t.splits = 1;
+  return hip_status(launch_f8_tiles(t, plan.shape, 0, st), "llmopt_f8_swiglu");
 }
 
 }  // extern "C"

@@ -46,18 +46,6 @@ struct F8Weight {
   int64_t lds;
 };
 
-struct F8LinearArgs {
-  const uint8_t* x;  // [M, K]
-  int64_t ldx;
-  const uint8_t* x_scales;  // [M, ceil(K / 128)]
-  int64_t ldxs;
-  F8Weight w;
-  const void* bias;  // [N] of the output's type; null: none
-  void* y;
-  int64_t ldy;
-  int64_t M, N, K;
-};
-
 // silu(gate) * up of fp32 sums, quantized by rows.
 struct F8ActArgs {
   const float* gate;  // [rows, cols], rows of `ld` elements; up likewise
@@ -70,8 +58,8 @@ struct F8ActArgs {
   int64_t rows, cols;
 };
 
-// The tiled kernels: y = x w[0]^T + bias, or silu(x w[0]^T) * (x w[1]^T) quantized where w[1] has codes. All rows of codes are
-// 16-byte aligned, K a multiple of 16, and the strides at most 2^21.
+// Products of x [M, K] with weights [N, K]: y = x w[0]^T + bias, or silu(x w[0]^T) * (x w[1]^T) quantized where w[1] has codes.
+// For the tiled kernels all rows of codes are 16-byte aligned, K is a multiple of 16, and the strides are at most 2^21.
 struct F8TilesArgs {
   const uint8_t* x;
   int64_t ldx;
@@ -97,7 +85,8 @@ struct F8TilesArgs {
 // A workgroup's tile: weight rows x tokens.
 enum class F8Shape { k256x256, k256x128, k256x64, k128x128, k128x64 };
 
-// The kernels of few tokens (at most 64); operands as in F8TilesArgs.
+// The kernel of at most 16 tokens; operands as in F8TilesArgs. With a second weight its product's rows come in y behind the
+// first one's (and there is no bias).
 struct F8DecodeArgs {
   const uint8_t* x;
   int64_t ldx;
@@ -107,16 +96,8 @@ struct F8DecodeArgs {
   const void* bias;
   void* y;
   int64_t ldy;
-  uint8_t* codes;  // the gated product's
-  int64_t ldc;
-  uint8_t* scales;
-  int64_t lds;
   int64_t M, N, K;
-  int vec;  // the codes' rows are 4-byte aligned
-  uint32_t steps, tiles_n;
-  uint32_t splits, steps_per_split;  // of K over workgroups
-  float* parts;                      // splits > 1: [splits][M][ld_parts]
-  int64_t ld_parts;
+  uint32_t steps, tiles;  // (set by the launch)
 };
 
 hipError_t launch_f8_quantize(const F8QuantArgs& a, int dtype, int64_t block_rows, hipStream_t stream);
@@ -133,10 +114,9 @@ struct F8JoinArgs {
   int64_t ldy;
 };
 hipError_t launch_f8_join(const F8JoinArgs& a, int out_dtype, hipStream_t stream);
-// rt: tiles of 16 features a workgroup (1 or 2).
-hipError_t launch_f8_decode(const F8DecodeArgs& a, int rt, int out_dtype, hipStream_t stream);
-hipError_t launch_f8_decode_gated(const F8DecodeArgs& a, hipStream_t stream);
-hipError_t launch_f8_linear_any(const F8LinearArgs& a, int out_dtype, hipStream_t stream);
+hipError_t launch_f8_decode(F8DecodeArgs a, int out_dtype, hipStream_t stream);
+// Rows of any alignment; the gated product where w[1] has codes. (The other kernels' sizes are not set.)
+hipError_t launch_f8_any(const F8TilesArgs& a, int out_dtype, hipStream_t stream);
 
 // ---- groups -----------------------------------------------------------------------------------------
 
@@ -173,6 +153,9 @@ __device__ __forceinline__ uint32_t f8_codes4(float a, float b, float c, float d
   const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
   return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true));
 }
+
+// silu(gate) * up in fp32; the exponential is the hardware's (a few steps of fp32).
+__device__ __forceinline__ float f8_swiglu(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
 
 // Eight neighbouring numbers of a row, from column c on; zeros behind `cols`.
 template <class Act>

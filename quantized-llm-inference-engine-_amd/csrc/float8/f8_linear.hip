@@ -1,7 +1,5 @@
-// y = x w^T + bias of codes with block scales, for rows of any length, stride and alignment: the kernel of shapes that the
-// tiled ones do not take.
-//
-// A wave multiplies 16 rows of the weight with 16 tokens, a group of 128 columns at a time (mfma_f8).
+// Products of rows of any length, stride and alignment: the kernels of shapes that the others do not take. A wave multiplies 16
+// rows of the weight with 16 tokens, a group of 128 columns at a time, straight from memory.
 #include "f8_common.hpp"
 #include "f8_mfma.hpp"
 
@@ -23,42 +21,87 @@ __device__ __forceinline__ i32x8 load32(const uint8_t* row, int64_t k, int64_t K
   return v;
 }
 
+// acc[t] += 16 rows of weight t from n0 on times 16 tokens from m0 on; rows and tokens behind the last repeat it.
+template <int W>
+__device__ __forceinline__ void sums_any(const F8TilesArgs& a, int64_t n0, int64_t m0, f32x4 (&acc)[W]) {
+  const int r = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+  const int64_t m = m0 + r < a.M ? m0 + r : a.M - 1, n = n0 + r < a.N ? n0 + r : a.N - 1;
+  const uint8_t* xr = a.x + m * a.ldx;
+  const uint8_t* xs = a.x_scales + m * a.ldxs;
+#pragma unroll
+  for (int t = 0; t < W; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int64_t k = 0; k < a.K; k += kF8Group) {
+    const i32x8 xv = load32(xr, k + 32 * g, a.K);
+    const uint32_t sx = xs[k / kF8Group];
+#pragma unroll
+    for (int t = 0; t < W; ++t)
+      acc[t] = mfma_f8(load32(a.w[t].codes + n * a.w[t].ld, k + 32 * g, a.K), xv, acc[t],
+                       a.w[t].scales[(n0 / kF8Group) * a.w[t].lds + k / kF8Group], sx);
+  }
+}
+
 template <class Out>
-__global__ void __launch_bounds__(256) linear_any_kernel(const F8LinearArgs a, uint32_t token_tiles) {
+__global__ void __launch_bounds__(256) linear_any_kernel(const F8TilesArgs a, uint32_t token_tiles) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t nb = blockIdx.x / token_tiles;
   const int64_t n0 = (int64_t(nb) * 4 + wave) * 16, m0 = int64_t(blockIdx.x - nb * token_tiles) * 16;
   if (n0 >= a.N) return;
-  const int r = lane & 15, g = lane >> 4;
-  const int64_t m = m0 + r, mr = m < a.M ? m : a.M - 1, nr = n0 + r < a.N ? n0 + r : a.N - 1;
-  const uint8_t* xr = a.x + mr * a.ldx;
-  const uint8_t* wr = a.w.codes + nr * a.w.ld;
-  const uint8_t* xs = a.x_scales + mr * a.ldxs;
-  const uint8_t* ws = a.w.scales + (n0 / kF8Group) * a.w.lds;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t k = 0; k < a.K; k += kF8Group) {
-    const i32x8 wv = load32(wr, k + 32 * g, a.K), xv = load32(xr, k + 32 * g, a.K);
-    acc = mfma_f8(wv, xv, acc, ws[k / kF8Group], xs[k / kF8Group]);
-  }
+  f32x4 acc[1];
+  sums_any<1>(a, n0, m0, acc);
+  const int64_t m = m0 + (lane & 15);
   if (m >= a.M) return;
   auto* y = static_cast<typename Out::raw*>(a.y) + m * a.ldy;
   const auto* bias = static_cast<const typename Out::raw*>(a.bias);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t n = n0 + 4 * g + i;
-    if (n < a.N) y[n] = Out::store(bias ? acc[i] + Out::load(bias[n]) : acc[i]);
+    const int64_t n = n0 + 4 * (lane >> 4) + i;
+    if (n < a.N) y[n] = Out::store(bias ? acc[0][i] + Out::load(bias[n]) : acc[0][i]);
   }
+}
+
+// A workgroup takes a group of 128 features, a wave 16 of them.
+__global__ void __launch_bounds__(512) gated_any_kernel(const F8TilesArgs a, uint32_t token_tiles) {
+  __shared__ uint32_t tops[8][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const uint32_t nb = blockIdx.x / token_tiles;
+  const int64_t n0 = int64_t(nb) * kF8Group + 16 * wave, m0 = int64_t(blockIdx.x - nb * token_tiles) * 16;
+  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  uint32_t top = 0;
+  if (n0 < a.N) {
+    f32x4 acc[2];
+    sums_any<2>(a, n0, m0, acc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n0 + 4 * g + i < a.N) v[i] = f8_swiglu(acc[0][i], acc[1][i]);
+      top = max(top, magnitude(v[i]));
+    }
+    top = max(top, uint32_t(__shfl_xor(int(top), 16, 64)));
+    top = max(top, uint32_t(__shfl_xor(int(top), 32, 64)));
+  }
+  if (g == 0) tops[wave][r] = top;
+  __syncthreads();
+  const int64_t m = m0 + r;
+  if (m >= a.M) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, tops[i][r]);
+  const uint32_t scale = f8_scale(top), codes = f8_codes4(v[0], v[1], v[2], v[3], f8_inverse(scale));
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n0 + 4 * g + i < a.N) a.codes[m * a.ldc + n0 + 4 * g + i] = uint8_t(codes >> (8 * i));
+  if (wave == 0 && g == 0) a.scales[m * a.lds + nb] = uint8_t(scale);
 }
 
 }  // namespace
 
-hipError_t launch_f8_linear_any(const F8LinearArgs& a, int out_dtype, hipStream_t stream) {
-  if (a.M == 0 || a.N == 0) return hipSuccess;
+hipError_t launch_f8_any(const F8TilesArgs& a, int out_dtype, hipStream_t stream) {
   const int64_t tiles = (a.M + 15) / 16;
+  if (a.w[1].codes) {
+    const dim3 grid(unsigned(tiles * ((a.N + kF8Group - 1) / kF8Group)));
+    hipLaunchKernelGGL(gated_any_kernel, grid, dim3(512), 0, stream, a, uint32_t(tiles));
+    return hipGetLastError();
+  }
   const dim3 grid(unsigned(tiles * ((a.N + 63) / 64)));
-  if (out_dtype == kDtF32)
-    hipLaunchKernelGGL(linear_any_kernel<ActF32>, grid, dim3(256), 0, stream, a, uint32_t(tiles));
-  else if (out_dtype == kDtF16)
+  if (out_dtype == kDtF16)
     hipLaunchKernelGGL(linear_any_kernel<ActF16>, grid, dim3(256), 0, stream, a, uint32_t(tiles));
   else
     hipLaunchKernelGGL(linear_any_kernel<ActBf16>, grid, dim3(256), 0, stream, a, uint32_t(tiles));

@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kThreads) act_kernel(const F8ActArgs a, uint32
   load8<ActF32>(a.gate + row * a.ld, c, a.cols, vec, g);
   load8<ActF32>(a.up + row * a.ld, c, a.cols, vec, u);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) g[i] = g[i] / (1.0f + __expf(-g[i])) * u[i];
+  for (int i = 0; i < 8; ++i) g[i] = f8_swiglu(g[i], u[i]);
   quantize8(g, a.codes + row * a.ldc, a.scales + row * a.lds, c, a.cols, vec);
 }
 

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float gate = acc[i >> 2][u][i & 3], up = acc[4 + (i >> 2)][u][i & 3];
-        v[u][i] = f0 + i < rows_n ? gate / (1.0f + __expf(-gate)) * up : 0.0f;
+        v[u][i] = f0 + i < rows_n ? f8_swiglu(gate, up) : 0.0f;
         top[u] = max(top[u], magnitude(v[u][i]));
       }
       top[u] = max(top[u], uint32_t(__shfl_xor(int(top[u]), 16, 64)));

@@ -302,15 +302,27 @@ def test_the_c_abi_refuses_before_anything_reaches_a_device():
         assert linear(**bad) == -1, bad
     assert linear(m=0) == 0 and linear(n=0) == 0
 
-    def swiglu(ldg=256, lds=1, need=None, ws=p, n=8):
-        size = lib.llmopt_f8_swiglu_workspace(4, n, 256) if need is None else need
-        return lib.llmopt_f8_swiglu(p, 256, p, 2, 4, 256, p, ldg, p, 2, p, 256, p, 2, n, p, 8, p, lds, ws, size, None)
+    def swiglu(ldg=256, lds=1, n=8, up=p):
+        return lib.llmopt_f8_swiglu(p, 256, p, 2, 4, 256, p, ldg, p, 2, up, 256, p, 2, n, p, 8, p, lds, None, 0, None)
 
     assert swiglu(ldg=255) == -1 and b"gate" in lib.llmopt_f8_last_error()
-    assert swiglu(n=0) == 0
-    if lib.llmopt_f8_swiglu_workspace(4, 8, 256):
-        assert swiglu(need=0) == -4 and b"workspace" in lib.llmopt_f8_last_error()
-        assert swiglu(ws=None) == -4
+    assert swiglu(up=None) == -1 and b"up is null" in lib.llmopt_f8_last_error()
+    assert swiglu(lds=0) == -1 and swiglu(n=0) == 0
+
+
+def test_workspaces():
+    """None for sizes that are not split or refused, and never more than the parts of eight."""
+    lib = _lib.load_library()
+    for m, n, k in ((0, 10, 10), (-1, 10, 10), (10, 0, 10), (10, 10, 0), (1, 4096, 4096), (8192, 4096, 14336), (1 << 40, 5, 5)):
+        assert lib.llmopt_f8_linear_workspace(m, n, k) == 0, (m, n, k)
+    assert lib.llmopt_f8_linear_workspace(32, 4096, 14336) > 0
+    for m in (17, 32, 100, 256, 1000):
+        for n in (1, 100, 4096, 28672):
+            for k in (16, 1040, 14336):
+                ws = lib.llmopt_f8_linear_workspace(m, n, k)
+                assert 0 <= ws <= 8 * m * (n + 15) * 4 and ws % (m * 64) == 0
+    assert lib.llmopt_f8_swiglu_workspace(17, 4096, 4096) == 0 and lib.llmopt_f8_swiglu_workspace(0, 8, 8) == 0
+    assert lib.llmopt_f8_swiglu_workspace(3, 50, 77) == 2 * 3 * 64 * 4
 
 
 @pytest.mark.parametrize("rc,kind", [(-1, ValueError), (-2, NotImplementedError), (-4, RuntimeError)])
