@@ -1,4 +1,5 @@
-// The per-call host path of a packed linear, of the 8-bit KV cache's calls and of packed attention, in native code: checks the plain form of a call (contiguous
+// The per-call host path of a packed linear, of the 8-bit KV cache's calls, of packed attention and of the steps in 8-bit
+// floating point, in native code: checks the plain form of a call (contiguous
 // tensors of the expected dtypes and shapes on one device), allocates the output and the workspace from
 // torch's caching allocator and calls the C ABI on the current stream. The checks run on every call and
 // nothing is kept between calls. A call in any other form returns None, and the caller takes the general
@@ -374,7 +375,268 @@ PyObject* packed_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- 8-bit floating point (include/llmopt_float8.h) ----
+
+using F8QuantizeFn = int (*)(const void*, int64_t, int, int64_t, int64_t, int64_t, void*, int64_t, void*, int64_t, void*);
+using F8NormFn = int (*)(const void*, int64_t, const void*, int64_t, void*, int64_t, const void*, void*, int64_t, void*,
+                         int64_t, int64_t, int64_t, float, int, void*);
+using F8WorkspaceFn = size_t (*)(int64_t, int64_t, int64_t);
+using F8LinearFn = int (*)(const void*, int64_t, const void*, int64_t, int64_t, int64_t, const void*, int64_t, const void*,
+                           int64_t, const void*, void*, int64_t, int64_t, int, void*, size_t, void*);
+using F8SwigluFn = int (*)(const void*, int64_t, const void*, int64_t, int64_t, int64_t, const void*, int64_t, const void*,
+                           int64_t, const void*, int64_t, const void*, int64_t, int64_t, void*, int64_t, void*, int64_t,
+                           void*, size_t, void*);
+
+struct F8Api {
+  F8QuantizeFn quantize = nullptr;
+  F8NormFn norm = nullptr;
+  F8WorkspaceFn linear_ws = nullptr;
+  F8LinearFn linear = nullptr;
+  F8WorkspaceFn swiglu_ws = nullptr;
+  F8SwigluFn swiglu = nullptr;
+} g_f8;
+
+// attach_f8(quantize, rmsnorm, linear_workspace, linear, swiglu_workspace, swiglu): the C ABI's addresses.
+PyObject* attach_f8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "attach_f8 takes six addresses");
+    return nullptr;
+  }
+  void* p[6];
+  for (int i = 0; i < 6; ++i) {
+    p[i] = PyLong_AsVoidPtr(args[i]);
+    if (!p[i] && PyErr_Occurred()) return nullptr;
+  }
+  g_f8 = {reinterpret_cast<F8QuantizeFn>(p[0]), reinterpret_cast<F8NormFn>(p[1]), reinterpret_cast<F8WorkspaceFn>(p[2]),
+          reinterpret_cast<F8LinearFn>(p[3]), reinterpret_cast<F8WorkspaceFn>(p[4]), reinterpret_cast<F8SwigluFn>(p[5])};
+  Py_RETURN_NONE;
+}
+
+int64_t f8_groups(int64_t n) { return (n + 127) / 128; }
+
+// A tensor of at least one dimension as rows: its last dimension's, `ld` elements apart.
+struct Rows {
+  int64_t rows = 0, cols = 0, ld = 0;
+
+  bool of(const at::Tensor& t) {
+    const int64_t dim = t.dim();
+    if (dim < 1 || t.layout() != at::kStrided || t.numel() == 0) return false;
+    cols = t.size(dim - 1);
+    rows = t.numel() / cols;
+    ld = cols;
+    if (t.is_contiguous()) return true;
+    if (dim != 2 || t.stride(1) != 1 || t.stride(0) < cols) return false;
+    ld = t.stride(0);
+    return true;
+  }
+};
+
+// Codes with scales (block_rows 1: activations [..., K], 128: a weight [N, K]) on one HIP device.
+struct F8Tensor {
+  Rows codes, scales;
+  const at::Tensor *c = nullptr, *s = nullptr;
+
+  bool of(PyObject* codes_, PyObject* scales_, int64_t block_rows) {
+    c = tensor_of(codes_), s = tensor_of(scales_);
+    if (!c || !s || !c->device().is_cuda() || c->scalar_type() != at::kFloat8_e4m3fn ||
+        s->scalar_type() != at::kFloat8_e8m0fnu || s->device() != c->device() || !codes.of(*c) || !scales.of(*s))
+      return false;
+    if (scales.cols != f8_groups(codes.cols) || s->dim() != c->dim()) return false;
+    if (block_rows == 128) return c->dim() == 2 && scales.rows == f8_groups(codes.rows);
+    for (int64_t d = 0; d + 1 < c->dim(); ++d)
+      if (c->size(d) != s->size(d)) return false;
+    return block_rows == 1;
+  }
+};
+
+at::Tensor empty_like_rows(const at::Tensor& t, int64_t cols, at::ScalarType type) {
+  c10::SmallVector<int64_t, 6> shape(t.sizes().begin(), t.sizes().end());
+  shape.back() = cols;
+  return at::empty(shape, at::TensorOptions().device(t.device()).dtype(type));
+}
+
+PyObject* wrap2(at::Tensor a, at::Tensor b) {
+  PyObject *x = THPVariable_Wrap(std::move(a)), *y = THPVariable_Wrap(std::move(b));
+  PyObject* r = x && y ? PyTuple_Pack(2, x, y) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  return r;
+}
+
+// f8_check(codes, scales, block_rows) -> True where they belong together, or None where the general checks have to look.
+PyObject* f8_check(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 3) {
+    PyErr_SetString(PyExc_TypeError, "f8_check takes three arguments");
+    return nullptr;
+  }
+  HANDLE_TH_ERRORS
+  const int64_t block_rows = PyLong_AsLongLong(args[2]);
+  if (block_rows == -1 && PyErr_Occurred()) PyErr_Clear();
+  F8Tensor t;
+  if (!t.of(args[0], args[1], block_rows)) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// f8_quantize(x, block_rows) -> (codes, scales), or None.
+PyObject* f8_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 2 || !g_f8.quantize) {
+    PyErr_SetString(PyExc_TypeError, "f8_quantize takes two arguments, after attach_f8");
+    return nullptr;
+  }
+  HANDLE_TH_ERRORS
+  if (!THPVariable_CheckExact(args[0])) Py_RETURN_NONE;
+  const at::Tensor* x = tensor_of(args[0]);
+  const int64_t block_rows = PyLong_AsLongLong(args[1]);
+  if (block_rows == -1 && PyErr_Occurred()) PyErr_Clear();
+  Rows r;
+  const int dtype = x ? dtype_code(*x) : -1;
+  if (dtype < 0 || !x->device().is_cuda() || !on_current_device(x->device()) || !r.of(*x) ||
+      !(block_rows == 1 || (block_rows == 128 && x->dim() == 2)))
+    Py_RETURN_NONE;
+  const int64_t across = f8_groups(r.cols);
+  at::Tensor codes = empty_like_rows(*x, r.cols, at::kFloat8_e4m3fn);
+  at::Tensor scales = block_rows == 1
+                          ? empty_like_rows(*x, across, at::kFloat8_e8m0fnu)
+                          : at::empty({f8_groups(r.rows), across}, codes.options().dtype(at::kFloat8_e8m0fnu));
+  void* stream = c10::hip::getCurrentHIPStream(x->device().index()).stream();
+  const void* xp = x->const_data_ptr();
+  void *cp = codes.mutable_data_ptr(), *sp = scales.mutable_data_ptr();
+  int rc;
+  {
+    pybind11::gil_scoped_release released;
+    rc = g_f8.quantize(xp, r.ld, dtype, r.rows, r.cols, block_rows, cp, r.cols, sp, across, stream);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  return wrap2(std::move(codes), std::move(scales));
+  END_HANDLE_TH_ERRORS
+}
+
+// f8_rmsnorm(x, weight, eps, residual or None) -> (codes, scales, h or None), or None.
+PyObject* f8_rmsnorm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 4 || !g_f8.norm) {
+    PyErr_SetString(PyExc_TypeError, "f8_rmsnorm takes four arguments, after attach_f8");
+    return nullptr;
+  }
+  HANDLE_TH_ERRORS
+  if (!THPVariable_CheckExact(args[0])) Py_RETURN_NONE;
+  const at::Tensor *x = tensor_of(args[0]), *w = tensor_of(args[1]), *res = tensor_of(args[3]);
+  const double eps = PyFloat_AsDouble(args[2]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  Rows r, rr;
+  const int dtype = x ? dtype_code(*x) : -1;
+  if (dtype < 1 || !w || (!res && args[3] != Py_None) || !x->device().is_cuda() || !on_current_device(x->device()) ||
+      !r.of(*x) || w->device() != x->device() || w->scalar_type() != x->scalar_type() || w->dim() != 1 ||
+      w->size(0) != r.cols || !w->is_contiguous())
+    Py_RETURN_NONE;
+  if (res && (res->device() != x->device() || res->scalar_type() != x->scalar_type() || res->sizes() != x->sizes() || !rr.of(*res)))
+    Py_RETURN_NONE;
+  const int64_t across = f8_groups(r.cols);
+  at::Tensor codes = empty_like_rows(*x, r.cols, at::kFloat8_e4m3fn), scales = empty_like_rows(*x, across, at::kFloat8_e8m0fnu), h;
+  if (res) h = empty_like_rows(*x, r.cols, x->scalar_type());
+  void* stream = c10::hip::getCurrentHIPStream(x->device().index()).stream();
+  const void *xp = x->const_data_ptr(), *wp = w->const_data_ptr(), *rp = res ? res->const_data_ptr() : nullptr;
+  void *cp = codes.mutable_data_ptr(), *sp = scales.mutable_data_ptr(), *hp = res ? h.mutable_data_ptr() : nullptr;
+  int rc;
+  {
+    pybind11::gil_scoped_release released;
+    rc = g_f8.norm(xp, r.ld, rp, rr.ld, hp, r.cols, wp, cp, r.cols, sp, across, r.rows, r.cols, float(eps), dtype, stream);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  PyObject *a = THPVariable_Wrap(std::move(codes)), *b = THPVariable_Wrap(std::move(scales)), *c = Py_None;
+  if (res)
+    c = THPVariable_Wrap(std::move(h));
+  else
+    Py_INCREF(c);
+  PyObject* out = a && b && c ? PyTuple_Pack(3, a, b, c) : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  Py_XDECREF(c);
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// f8_linear(x codes, x scales, w codes, w scales, bias or None, dtype) -> [..., N], or None. dtype: 1 fp16, 2 bf16.
+PyObject* f8_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6 || !g_f8.linear) {
+    PyErr_SetString(PyExc_TypeError, "f8_linear takes six arguments, after attach_f8");
+    return nullptr;
+  }
+  HANDLE_TH_ERRORS
+  if (!THPVariable_CheckExact(args[0])) Py_RETURN_NONE;
+  F8Tensor x, w;
+  const at::Tensor* bias = tensor_of(args[4]);
+  const int64_t dtype = PyLong_AsLongLong(args[5]);
+  if (dtype == -1 && PyErr_Occurred()) PyErr_Clear();
+  if ((!bias && args[4] != Py_None) || (dtype != 1 && dtype != 2) || !x.of(args[0], args[1], 1) ||
+      !w.of(args[2], args[3], 128) || w.codes.cols != x.codes.cols || w.c->device() != x.c->device() ||
+      !on_current_device(x.c->device()))
+    Py_RETURN_NONE;
+  const at::ScalarType type = dtype == 1 ? at::kHalf : at::kBFloat16;
+  const int64_t M = x.codes.rows, K = x.codes.cols, N = w.codes.rows;
+  if (bias && (bias->device() != x.c->device() || bias->scalar_type() != type || bias->dim() != 1 || bias->size(0) != N ||
+               !bias->is_contiguous()))
+    Py_RETURN_NONE;
+  const size_t ws_bytes = g_f8.linear_ws(M, N, K);
+  at::Tensor y = empty_like_rows(*x.c, N, type), ws;
+  if (ws_bytes) ws = at::empty({int64_t(ws_bytes)}, y.options().dtype(at::kByte));
+  void* stream = c10::hip::getCurrentHIPStream(x.c->device().index()).stream();
+  const void *xc = x.c->const_data_ptr(), *xs = x.s->const_data_ptr(), *wc = w.c->const_data_ptr(), *wsc = w.s->const_data_ptr();
+  const void* bp = bias ? bias->const_data_ptr() : nullptr;
+  void *yp = y.mutable_data_ptr(), *wp = ws_bytes ? ws.mutable_data_ptr() : nullptr;
+  int rc;
+  {
+    pybind11::gil_scoped_release released;
+    rc = g_f8.linear(xc, x.codes.ld, xs, x.scales.ld, M, K, wc, w.codes.ld, wsc, w.scales.ld, bp, yp, N, N, int(dtype), wp,
+                     ws_bytes, stream);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// f8_swiglu(x codes, x scales, gate codes, gate scales, up codes, up scales) -> (codes, scales), or None.
+PyObject* f8_swiglu(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6 || !g_f8.swiglu) {
+    PyErr_SetString(PyExc_TypeError, "f8_swiglu takes six arguments, after attach_f8");
+    return nullptr;
+  }
+  HANDLE_TH_ERRORS
+  if (!THPVariable_CheckExact(args[0])) Py_RETURN_NONE;
+  F8Tensor x, g, u;
+  if (!x.of(args[0], args[1], 1) || !g.of(args[2], args[3], 128) || !u.of(args[4], args[5], 128) ||
+      g.codes.cols != x.codes.cols || g.c->sizes() != u.c->sizes() || g.c->device() != x.c->device() ||
+      u.c->device() != x.c->device() || !on_current_device(x.c->device()))
+    Py_RETURN_NONE;
+  const int64_t M = x.codes.rows, K = x.codes.cols, N = g.codes.rows;
+  const size_t ws_bytes = g_f8.swiglu_ws(M, N, K);
+  at::Tensor codes = empty_like_rows(*x.c, N, at::kFloat8_e4m3fn), scales = empty_like_rows(*x.c, f8_groups(N), at::kFloat8_e8m0fnu), ws;
+  if (ws_bytes) ws = at::empty({int64_t(ws_bytes)}, codes.options().dtype(at::kByte));
+  void* stream = c10::hip::getCurrentHIPStream(x.c->device().index()).stream();
+  const void *p[6] = {x.c->const_data_ptr(), x.s->const_data_ptr(), g.c->const_data_ptr(),
+                      g.s->const_data_ptr(), u.c->const_data_ptr(), u.s->const_data_ptr()};
+  void *cp = codes.mutable_data_ptr(), *sp = scales.mutable_data_ptr(), *wp = ws_bytes ? ws.mutable_data_ptr() : nullptr;
+  int rc;
+  {
+    pybind11::gil_scoped_release released;
+    rc = g_f8.swiglu(p[0], x.codes.ld, p[1], x.scales.ld, M, K, p[2], g.codes.ld, p[3], g.scales.ld, p[4], u.codes.ld, p[5],
+                     u.scales.ld, N, cp, N, sp, f8_groups(N), wp, ws_bytes, stream);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  return wrap2(std::move(codes), std::move(scales));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"attach_f8", reinterpret_cast<PyCFunction>(attach_f8), METH_FASTCALL, nullptr},
+    {"f8_check", reinterpret_cast<PyCFunction>(f8_check), METH_FASTCALL, nullptr},
+    {"f8_quantize", reinterpret_cast<PyCFunction>(f8_quantize), METH_FASTCALL, nullptr},
+    {"f8_rmsnorm", reinterpret_cast<PyCFunction>(f8_rmsnorm), METH_FASTCALL, nullptr},
+    {"f8_linear", reinterpret_cast<PyCFunction>(f8_linear), METH_FASTCALL, nullptr},
+    {"f8_swiglu", reinterpret_cast<PyCFunction>(f8_swiglu), METH_FASTCALL, nullptr},
     {"attach", reinterpret_cast<PyCFunction>(attach), METH_FASTCALL, nullptr},
     {"attach_kvq", reinterpret_cast<PyCFunction>(attach_kvq), METH_FASTCALL, nullptr},
     {"linear", reinterpret_cast<PyCFunction>(linear), METH_FASTCALL, nullptr},

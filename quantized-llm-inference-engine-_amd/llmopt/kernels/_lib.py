@@ -235,8 +235,8 @@ def binding_path() -> Path:
 
 
 def load_binding():  # noqa: ANN201 - the extension module, or None
-    """Load (once) and return the native host path of the linears, of the 8-bit KV cache and of packed
-    attention (``csrc/torch_binding.cpp``), with
+    """Load (once) and return the native host path of the linears, of the 8-bit KV cache, of packed
+    attention and of the steps in 8-bit floating point (``csrc/torch_binding.cpp``), with
     the kernel library's entry points attached. None, with one warning, where it is not built, does not
     load into this torch, or it or the library is from before an entry point that it attaches: calls then take
     the general path, the same kernels through ctypes."""
@@ -261,6 +261,9 @@ def load_binding():  # noqa: ANN201 - the extension module, or None
                 module.attach_kvq(*(ctypes.cast(getattr(lib, name), _p).value for name in (
                     "llmopt_kvq_write", "llmopt_kvq_attention_workspace", "llmopt_kvq_attention",
                     "llmopt_packed_attention")))
+                module.attach_f8(*(ctypes.cast(getattr(lib, name), _p).value for name in (
+                    "llmopt_f8_quantize", "llmopt_f8_rmsnorm", "llmopt_f8_linear_workspace", "llmopt_f8_linear",
+                    "llmopt_f8_swiglu_workspace", "llmopt_f8_swiglu")))
                 _binding = module
             except (ImportError, OSError, AttributeError, ctypes.ArgumentError) as exc:
                 warnings.warn(f"the linears' native host path is not available ({exc}); calls go through ctypes, "

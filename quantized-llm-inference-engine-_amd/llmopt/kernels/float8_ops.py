@@ -1,15 +1,16 @@
 """Torch-facing wrappers over the entry points of ``include/llmopt_float8.h``: quantizing, RMSNorm with a quantized output,
 the projection and the gated MLP product in 8-bit floating point. The checks, errors and streams are those of
-:mod:`llmopt.kernels.ops`; :mod:`llmopt.quantization.float8` is what a user calls."""
+:mod:`llmopt.kernels.ops`; :mod:`llmopt.quantization.float8` is what a user calls. The plain form of a call (contiguous or
+row-strided tensors on the current device) has its checks, allocations and launch in native code."""
 
 from __future__ import annotations
 
 import torch
 
-from llmopt.kernels._lib import DTYPE_CODES, call, load_library
+from llmopt.kernels._lib import DTYPE_CODES, call, load_binding, load_library
 from llmopt.kernels.ops import _launching_on, _same_device, _stream_handle
 
-__all__ = ["linear", "quantize", "rmsnorm", "rmsnorm_supported", "swiglu"]
+__all__ = ["belong_together", "linear", "quantize", "rmsnorm", "rmsnorm_supported", "swiglu"]
 
 GROUP = 128
 
@@ -31,8 +32,20 @@ def _ld(x: torch.Tensor) -> int:
     return max(x.stride(0), x.shape[1]) if x.shape[0] > 1 else x.shape[1]
 
 
+def belong_together(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) -> bool:
+    """Whether these are codes and their scales on a HIP device, checked in native code; False also where that cannot say."""
+    binding = load_binding()
+    return binding is not None and binding.f8_check(codes, scales, block_rows) is True
+
+
 def quantize(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
-    """Codes ``[rows, cols]`` and scales of a matrix ``x`` (``llmopt_f8_quantize``)."""
+    """Codes of ``x [..., cols]`` and their scales (``llmopt_f8_quantize``)."""
+    binding = load_binding()
+    if binding is not None:
+        out = binding.f8_quantize(x, block_rows)
+        if out is not None:
+            return out
+    lead = x.shape[:-1]
     if x.dtype not in DTYPE_CODES:
         x = x.to(torch.float32)
     x = _rows(x)
@@ -48,7 +61,7 @@ def quantize(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tens
                 ),
                 "llmopt_f8_quantize",
             )
-    return codes, scales
+    return (codes.view(*lead, cols), scales.view(*lead, _groups(cols))) if block_rows == 1 else (codes, scales)
 
 
 def rmsnorm_supported(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None) -> bool:
@@ -61,7 +74,12 @@ def rmsnorm_supported(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
 
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None
             ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
-    """Codes ``[rows, hidden]``, scales, and ``residual + x`` of the residual's shape (``llmopt_f8_rmsnorm``)."""
+    """Codes of ``x``'s shape, their scales, and ``residual + x`` (``llmopt_f8_rmsnorm``)."""
+    binding = load_binding()
+    if binding is not None:
+        out = binding.f8_rmsnorm(x, weight, eps, residual)
+        if out is not None:
+            return out
     shape = x.shape
     x = _rows(x)
     rows, hidden = (int(d) for d in x.shape)
@@ -83,14 +101,20 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.T
                 ),
                 "llmopt_f8_rmsnorm",
             )
-    return codes, scales, None if h is None else h.view(shape)
+    return codes.view(shape), scales.view(*shape[:-1], _groups(hidden)), None if h is None else h.view(shape)
 
 
 def linear(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
            bias: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor:
-    """``[M, N]`` of ``dtype``: codes ``x [M, K]`` with scales ``[M, ceil(K / 128)]`` times codes ``w [N, K]`` with scales
+    """``[..., N]`` of ``dtype``: codes ``x [..., K]`` with scales ``[..., ceil(K / 128)]`` times codes ``w [N, K]`` with scales
     ``[ceil(N / 128), ceil(K / 128)]``, plus ``bias [N]`` of ``dtype`` (``llmopt_f8_linear``)."""
+    binding = load_binding()
+    if binding is not None:
+        y = binding.f8_linear(x, x_scales, w, w_scales, bias, DTYPE_CODES[dtype])
+        if y is not None:
+            return y
     _same_device(x, x_scales, w, w_scales, bias)
+    lead = x.shape[:-1]
     x, w, x_scales, w_scales = _rows(x), _rows(w), _rows(x_scales), _rows(w_scales)
     (m, k), n = x.shape, int(w.shape[0])
     y = torch.empty(m, n, dtype=dtype, device=x.device)
@@ -108,12 +132,18 @@ def linear(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: t
                 ),
                 "llmopt_f8_linear",
             )
-    return y
+    return y.view(*lead, n)
 
 
 def swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor,
            up_scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """Codes ``[M, N]`` and scales of ``silu(x gate^T) * (x up^T)`` (``llmopt_f8_swiglu``)."""
+    """Codes ``[..., N]`` and scales of ``silu(x gate^T) * (x up^T)`` (``llmopt_f8_swiglu``)."""
+    binding = load_binding()
+    if binding is not None:
+        out = binding.f8_swiglu(x, x_scales, gate, gate_scales, up, up_scales)
+        if out is not None:
+            return out
+    lead = x.shape[:-1]
     _same_device(x, x_scales, gate, gate_scales, up, up_scales)
     x, gate, up = _rows(x), _rows(gate), _rows(up)
     x_scales, gate_scales, up_scales = _rows(x_scales), _rows(gate_scales), _rows(up_scales)
@@ -134,4 +164,4 @@ def swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, gate_sca
                 ),
                 "llmopt_f8_swiglu",
             )
-    return codes, scales
+    return codes.view(*lead, n), scales.view(*lead, _groups(n))

@@ -68,6 +68,11 @@ class Float8Tensor:
 
     def __post_init__(self) -> None:
         codes, scales = self.codes, self.scales
+        if codes.is_cuda:
+            from llmopt.kernels import float8_ops
+
+            if float8_ops.belong_together(codes, scales, self.block_rows):  # what is checked here, in native code
+                return
         if codes.dtype != F8 or scales.dtype != E8:
             raise TypeError(f"expected float8_e4m3fn codes and float8_e8m0fnu scales, got {codes.dtype} and {scales.dtype}")
         if self.block_rows == 1 and codes.dim() > 0:
@@ -133,11 +138,11 @@ def _quantize_torch(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, tor
     return codes.contiguous(), torch.where(finite, e + 127, 255).to(torch.uint8).view(E8)
 
 
-def _rows_tensor(codes: torch.Tensor, scales: torch.Tensor, lead: torch.Size) -> Float8Tensor:
-    """Codes and scales of rows, in the leading shape of what was quantized."""
-    if len(lead) == 1:
-        return Float8Tensor(codes, scales)
-    return Float8Tensor(codes.view(*lead, codes.shape[-1]), scales.view(*lead, scales.shape[-1]))
+def _made(codes: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> Float8Tensor:
+    """Codes and scales that a kernel made: nothing to check."""
+    out = Float8Tensor.__new__(Float8Tensor)
+    out.codes, out.scales, out.block_rows = codes, scales, block_rows
+    return out
 
 
 def quantize_float8(x: torch.Tensor, block_rows: int = 1) -> Float8Tensor:
@@ -150,10 +155,11 @@ def quantize_float8(x: torch.Tensor, block_rows: int = 1) -> Float8Tensor:
     if x.is_cuda:
         from llmopt.kernels import float8_ops
 
-        codes, scales = float8_ops.quantize(x.detach(), block_rows)
-    else:
-        codes, scales = _quantize_torch(x.reshape(-1, x.shape[-1]), block_rows)
-    return Float8Tensor(codes, scales, block_rows) if block_rows != 1 else _rows_tensor(codes, scales, x.shape[:-1])
+        return _made(*float8_ops.quantize(x, block_rows), block_rows)
+    codes, scales = _quantize_torch(x.reshape(-1, x.shape[-1]), block_rows)
+    if block_rows == 1:
+        codes, scales = codes.view(x.shape), scales.view(*x.shape[:-1], scales.shape[1])
+    return _made(codes, scales, block_rows)
 
 
 def rmsnorm_float8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None
@@ -169,8 +175,8 @@ def rmsnorm_float8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: 
         from llmopt.kernels import float8_ops
 
         if float8_ops.rmsnorm_supported(x, weight, residual):
-            codes, scales, h = float8_ops.rmsnorm(x, weight.detach(), eps, residual)
-            return _rows_tensor(codes, scales, x.shape[:-1]), x if h is None else h
+            codes, scales, h = float8_ops.rmsnorm(x, weight, eps, residual)
+            return _made(codes, scales), x if h is None else h
     h = x if residual is None else residual + x
     h32 = h.detach().float()
     y = h32 * torch.rsqrt(h32.pow(2).mean(-1, keepdim=True) + eps) * weight.detach().float()
@@ -209,11 +215,9 @@ def float8_linear(x: Float8Tensor, w: Float8Tensor, bias: torch.Tensor | None = 
     if x.is_cuda:
         from llmopt.kernels import float8_ops
 
-        y = float8_ops.linear(x.codes, x.scales, w.codes, w.scales, None if bias is None else bias.detach(), dtype)
-    else:
-        y = _product_torch(x, w)
-        y = (y if bias is None else y + bias.float()).to(dtype)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
+        return float8_ops.linear(x.codes, x.scales, w.codes, w.scales, bias, dtype)
+    y = _product_torch(x, w)
+    return (y if bias is None else y + bias.float()).to(dtype).view(*x.shape[:-1], n)
 
 
 def float8_swiglu(x: Float8Tensor, gate: Float8Tensor, up: Float8Tensor) -> Float8Tensor:
@@ -226,11 +230,10 @@ def float8_swiglu(x: Float8Tensor, gate: Float8Tensor, up: Float8Tensor) -> Floa
     if x.is_cuda:
         from llmopt.kernels import float8_ops
 
-        codes, scales = float8_ops.swiglu(x.codes, x.scales, gate.codes, gate.scales, up.codes, up.scales)
-    else:
-        g = _product_torch(x, gate)
-        codes, scales = _quantize_torch(g / (1.0 + torch.exp(-g)) * _product_torch(x, up), 1)
-    return _rows_tensor(codes, scales, x.shape[:-1])
+        return _made(*float8_ops.swiglu(x.codes, x.scales, gate.codes, gate.scales, up.codes, up.scales))
+    g = _product_torch(x, gate)
+    y = g / (1.0 + torch.exp(-g)) * _product_torch(x, up)
+    return quantize_float8(y.view(*x.shape[:-1], gate.shape[0]))
 
 
 # ---- layers -----------------------------------------------------------------------------------------
