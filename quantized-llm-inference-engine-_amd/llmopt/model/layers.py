@@ -10,6 +10,10 @@ devices the attention step writes K/V with the cache-write kernels and, for one 
 per sequence, runs the paged decode-attention kernel; RMSNorm (with the residual add in front
 of it) and the rotary embedding run as one kernel each (``llmopt_rmsnorm``, ``llmopt_rope``)
 with the reference's roundings. Elsewhere every step is the reference's torch sequence.
+
+Where the projections behind a norm hold their weights in 8-bit floating point (:class:`Float8Linear`,
+``quantize_model_float8_``), the norm hands them its output quantized (:meth:`RMSNorm.forward_float8`), and gate and up
+theirs to the down projection (:class:`Float8SwiGLU`), unless a derivative is needed.
 """
 
 from __future__ import annotations
@@ -20,6 +24,7 @@ from torch import nn
 from llmopt.attention.packed_attention import PackedAttention
 from llmopt.attention.paged_attention import PagedAttention, PagedAttentionConfig
 from llmopt.model.rotary import RotaryEmbedding, apply_rotary_pos_emb
+from llmopt.quantization.float8 import Float8Linear, Float8SwiGLU, Float8Tensor, FusedFloat8Linear, rmsnorm_float8
 from llmopt.quantization.fused import FusedQuantLinear, QuantSwiGLU
 from llmopt.quantization.quant_linear import QuantLinear
 from llmopt.utils.autograd import is_differentiated
@@ -82,6 +87,17 @@ class RMSNorm(nn.Module):
         h = residual + x
         return self._reference(h), h
 
+    def forward_float8(self, x: torch.Tensor) -> Float8Tensor:
+        """:meth:`forward` quantized by rows for a projection in 8-bit floating point, without a rounding to 16 bits
+        between (:func:`rmsnorm_float8`)."""
+        return rmsnorm_float8(x, self.weight, self.eps)[0]
+
+    def add_forward_float8(self, x, residual: torch.Tensor) -> tuple[Float8Tensor, torch.Tensor]:  # noqa: ANN001
+        """:meth:`add_forward` with its first result as :meth:`forward_float8` gives it."""
+        if not isinstance(x, torch.Tensor):
+            x = x.materialize()
+        return rmsnorm_float8(x, self.weight, self.eps, residual=residual)
+
 
 class SwiGLUMLP(nn.Module):
     """``down(silu(gate(x)) * up(x))`` (``layers.py:34-44``)."""
@@ -91,12 +107,21 @@ class SwiGLUMLP(nn.Module):
         self.gate_proj = nn.Linear(hidden_size, intermediate_size, bias=False)
         self.up_proj = nn.Linear(hidden_size, intermediate_size, bias=False)
         self.down_proj = nn.Linear(intermediate_size, hidden_size, bias=False)
-        self.gate_up: QuantSwiGLU | None = None
+        self.gate_up: QuantSwiGLU | Float8SwiGLU | None = None
+
+    def takes_float8(self) -> bool:
+        """Whether :meth:`forward` takes its input quantized (:class:`Float8Tensor`)."""
+        return isinstance(self.gate_up, Float8SwiGLU)
 
     def fuse_gate_up(self) -> bool:
         """Merge quantized gate and up projections into one :class:`QuantSwiGLU`; returns
-        whether it did (both must be :class:`QuantLinear` with the same settings)."""
+        whether it did (both must be :class:`QuantLinear` with the same settings). Where they and the down projection
+        are :class:`Float8Linear`, gate and up become a :class:`Float8SwiGLU`."""
         if self.gate_up is not None:
+            return True
+        if all(isinstance(p, Float8Linear) for p in (self.gate_proj, self.up_proj, self.down_proj)):
+            self.gate_up = Float8SwiGLU(self.gate_proj, self.up_proj)
+            del self.gate_proj, self.up_proj
             return True
         if not (isinstance(self.gate_proj, QuantLinear) and isinstance(self.up_proj, QuantLinear)):
             return False
@@ -145,7 +170,7 @@ class PagedAttentionLayer(nn.Module):
         self.k_proj = nn.Linear(hidden, self.num_kv_heads * self.head_dim, bias=False)
         self.v_proj = nn.Linear(hidden, self.num_kv_heads * self.head_dim, bias=False)
         self.o_proj = nn.Linear(self.num_heads * self.head_dim, hidden, bias=False)
-        self.qkv_proj: FusedQuantLinear | None = None
+        self.qkv_proj: FusedQuantLinear | FusedFloat8Linear | None = None
         self.rotary = RotaryEmbedding(self.head_dim, config.max_position_embeddings, config.rope_theta)
         self.fused_ops = True  # False: the torch rotary sequence even on HIP devices
         self.attn = PagedAttention(self.num_heads, self.num_kv_heads, self.head_dim,
@@ -157,11 +182,24 @@ class PagedAttentionLayer(nn.Module):
         return PackedAttention(self.num_heads, self.num_kv_heads, self.head_dim, scale=self.attn.scale,
                                softcap=self.attn.config.softcap, backend=self.attn.backend)
 
+    def takes_float8(self) -> bool:
+        """Whether :meth:`forward` takes its input quantized (:class:`Float8Tensor`)."""
+        if self.qkv_proj is not None:
+            return isinstance(self.qkv_proj, FusedFloat8Linear)
+        return all(isinstance(p, Float8Linear) for p in (self.q_proj, self.k_proj, self.v_proj))
+
     def fuse_qkv(self) -> bool:
-        """Merge quantized q, k and v projections into one :class:`FusedQuantLinear`."""
+        """Merge quantized q, k and v projections into one :class:`FusedQuantLinear`, or :class:`Float8Linear` ones into one
+        :class:`FusedFloat8Linear` (False where q or k has no multiple of 128 rows)."""
         if self.qkv_proj is not None:
             return True
         parts = (self.q_proj, self.k_proj, self.v_proj)
+        if all(isinstance(p, Float8Linear) for p in parts):
+            if any(p.out_features % 128 for p in parts[:2]):
+                return False
+            self.qkv_proj = FusedFloat8Linear(parts)
+            del self.q_proj, self.k_proj, self.v_proj
+            return True
         if not all(isinstance(p, QuantLinear) for p in parts):
             return False
         self.qkv_proj = FusedQuantLinear(parts)
@@ -326,11 +364,17 @@ class DecoderLayer(nn.Module):
         kernel, so a stack of layers runs one fused add + norm per residual add. With
         ``defer_mlp`` the MLP output may be its down projection's partial sums, which the next
         layer's first norm adds up (one launch fewer, the same bits)."""
-        if pending is None:
-            normed = self.input_layernorm(hidden)
-        else:
-            normed, hidden = self.input_layernorm.add_forward(pending, hidden)
+        normed, hidden = self._normed(self.input_layernorm, self.self_attn, hidden, pending)
         packed = {} if cu_seqlens is None else {"cu_seqlens": cu_seqlens}  # an attention put in here need not take it
         attn = self.self_attn(normed, positions, cache, block_ids, context_lens, token_offsets, q_len, **packed)
-        normed, hidden = self.post_attention_layernorm.add_forward(attn, hidden)
+        normed, hidden = self._normed(self.post_attention_layernorm, self.mlp, hidden, attn)
         return hidden, self.mlp(normed, defer=defer_mlp)
+
+    @staticmethod
+    def _normed(norm: nn.Module, consumer: nn.Module, hidden: torch.Tensor, added) -> tuple[object, torch.Tensor]:  # noqa: ANN001
+        """``(norm(h), h)`` with ``h = hidden + added``, or ``hidden`` where nothing is to be added; the first quantized
+        where ``consumer`` takes it so and no derivative is needed."""
+        if getattr(norm, "fused_ops", False) and getattr(consumer, "takes_float8", bool)() \
+                and not is_differentiated(hidden, norm.weight, *([added] if isinstance(added, torch.Tensor) else [])):
+            return (norm.forward_float8(hidden), hidden) if added is None else norm.add_forward_float8(added, hidden)
+        return (norm(hidden), hidden) if added is None else norm.add_forward(added, hidden)

@@ -18,6 +18,7 @@ from llmopt.quantization.float8 import (
     Float8Linear,
     Float8SwiGLU,
     Float8Tensor,
+    FusedFloat8Linear,
     float8_linear,
     float8_swiglu,
     quantize_float8,
@@ -50,6 +51,7 @@ __all__ = [
     "Float8Linear",
     "Float8SwiGLU",
     "Float8Tensor",
+    "FusedFloat8Linear",
     "FusedQuantLinear",
     "GPTQQuantizer",
     "HessianCollector",

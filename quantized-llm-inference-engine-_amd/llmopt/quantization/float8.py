@@ -11,7 +11,8 @@ checkpoint with other scales is quantized anew from its numbers.
 * :func:`rmsnorm_float8`: RMSNorm, with the residual's addition in front of it, its output quantized;
 * :func:`float8_linear`: a projection of quantized activations by a quantized weight;
 * :func:`float8_swiglu`: ``silu(x gate^T) * (x up^T)``, quantized for the projection behind it;
-* :class:`Float8Linear`, :class:`Float8SwiGLU` and :func:`quantize_model_float8_`: the layers made of them.
+* :class:`Float8Linear`, :class:`FusedFloat8Linear`, :class:`Float8SwiGLU` and :func:`quantize_model_float8_`: the layers made
+  of them.
 
 On HIP devices each is hand-written kernels (``include/llmopt_float8.h``); on the host the same definitions run in torch.
 Products of the matrix cores are sums in fp32 but for what lies below 2^-13 of the largest of eight neighbouring products,
@@ -35,6 +36,7 @@ __all__ = [
     "Float8Linear",
     "Float8SwiGLU",
     "Float8Tensor",
+    "FusedFloat8Linear",
     "float8_linear",
     "float8_swiglu",
     "quantize_float8",
@@ -274,26 +276,6 @@ class Float8Linear(nn.Module):
         return cls(quantize_float8(linear.weight.detach(), block_rows=GROUP), linear.bias,
                    compute_dtype or linear.weight.dtype)
 
-    @classmethod
-    def concat(cls, parts: Sequence[Float8Linear]) -> Float8Linear:
-        """One layer with the rows of several over one input (q, k and v). All but the last need a multiple of 128 rows, so
-        that no scale covers two of them."""
-        if not parts:
-            raise ValueError("nothing to fuse")
-        first = parts[0]
-        for p in parts:
-            if p.in_features != first.in_features or p.compute_dtype != first.compute_dtype:
-                raise ValueError("fused layers need the same in_features and compute dtype")
-        if any(p.out_features % GROUP for p in parts[:-1]):
-            raise ValueError(f"all but the last of the fused layers need a multiple of {GROUP} rows")
-        bias = None
-        if any(p.bias is not None for p in parts):
-            bias = torch.cat([torch.zeros(p.out_features, dtype=p.compute_dtype, device=p.weight_codes.device)
-                              if p.bias is None else p.bias for p in parts])
-        codes = torch.cat([p.weight_codes.view(torch.uint8) for p in parts]).view(F8)
-        scales = torch.cat([p.weight_scales.view(torch.uint8) for p in parts]).view(E8)
-        return cls(Float8Tensor(codes, scales, GROUP), bias, first.compute_dtype)
-
     def _apply(self, fn, recurse: bool = True):  # noqa: ANN001, ANN202 - nn.Module signature
         # module.to(dtype) converts floating-point buffers: the codes and their scales keep their types.
         kept = {name: self._buffers[name] for name in ("weight_codes", "weight_scales")}
@@ -320,6 +302,37 @@ class Float8Linear(nn.Module):
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+class FusedFloat8Linear(nn.Module):
+    """Several :class:`Float8Linear` over one input as one weight (q, k and v): ``forward(x)`` returns ``tuple(part(x) for part
+    in parts)``, column slices of one tensor, from one product. All but the last part need a multiple of 128 rows, so that no
+    scale covers two of them."""
+
+    def __init__(self, parts: Sequence[Float8Linear]) -> None:
+        super().__init__()
+        if not parts:
+            raise ValueError("nothing to fuse")
+        first = parts[0]
+        for p in parts:
+            if p.in_features != first.in_features or p.compute_dtype != first.compute_dtype:
+                raise ValueError("fused layers need the same in_features and compute dtype")
+        if any(p.out_features % GROUP for p in parts[:-1]):
+            raise ValueError(f"all but the last of the fused layers need a multiple of {GROUP} rows")
+        bias = None
+        if any(p.bias is not None for p in parts):
+            bias = torch.cat([torch.zeros(p.out_features, dtype=p.compute_dtype, device=p.weight_codes.device)
+                              if p.bias is None else p.bias for p in parts])
+        codes = torch.cat([p.weight_codes.view(torch.uint8) for p in parts]).view(F8)
+        scales = torch.cat([p.weight_scales.view(torch.uint8) for p in parts]).view(E8)
+        self.linear = Float8Linear(Float8Tensor(codes, scales, GROUP), bias, first.compute_dtype)
+        self.out_features = [p.out_features for p in parts]
+
+    def forward(self, x: torch.Tensor | Float8Tensor) -> tuple[torch.Tensor, ...]:
+        return tuple(torch.split(self.linear(x), self.out_features, dim=-1))
+
+    def extra_repr(self) -> str:
+        return f"out_features={self.out_features}"
 
 
 def _straight_through(x: torch.Tensor) -> torch.Tensor:

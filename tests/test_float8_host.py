@@ -8,7 +8,8 @@ import torch
 from torch import nn
 
 from llmopt.kernels import _lib
-from llmopt.quantization import (Float8Linear, Float8SwiGLU, Float8Tensor, float8_linear, float8_swiglu, quantize_float8,
+from llmopt.model import DecoderOnlyModel, GreedyGenerator, ModelConfig, fuse_projections_
+from llmopt.quantization import (Float8Linear, Float8SwiGLU, Float8Tensor, FusedFloat8Linear, float8_linear, float8_swiglu, quantize_float8,
                                  quantize_model_float8_, rmsnorm_float8)
 from oracle import float8_oracle as oracle
 
@@ -118,15 +119,17 @@ def test_float8_linear_layer(bias):
 
 def test_parts_of_one_layer():
     parts = [Float8Linear.from_float(_linear(200, n, b, i)) for i, (n, b) in enumerate([(256, False), (128, True), (70, False)])]
-    one, x = Float8Linear.concat(parts), _x(3, 200, 1, torch.bfloat16)
-    # a bias of zeros changes -0 to 0 at most
-    torch.testing.assert_close(one(x), torch.cat([p(x) for p in parts], -1), atol=0, rtol=0)
+    one, x = FusedFloat8Linear(parts), _x(3, 200, 1, torch.bfloat16)
+    got = one(x)
+    assert [g.shape[1] for g in got] == one.out_features == [256, 128, 70]
+    for g, p in zip(got, parts):  # a bias of zeros changes -0 to 0 at most
+        torch.testing.assert_close(g, p(x), atol=0, rtol=0)
     with pytest.raises(ValueError, match="multiple of 128"):
-        Float8Linear.concat(parts[::-1])
+        FusedFloat8Linear(parts[::-1])
     with pytest.raises(ValueError, match="same in_features"):
-        Float8Linear.concat([parts[0], Float8Linear.from_float(_linear(100, 10))])
+        FusedFloat8Linear([parts[0], Float8Linear.from_float(_linear(100, 10))])
     with pytest.raises(ValueError, match="nothing"):
-        Float8Linear.concat([])
+        FusedFloat8Linear([])
 
 
 def test_swiglu_layer():
@@ -162,6 +165,65 @@ def test_quantizing_a_model():
     assert model(_x(2, 100, 0, torch.bfloat16)).shape == (2, 10)
     with pytest.raises(TypeError, match="float16 or bfloat16"):
         quantize_model_float8_(nn.Sequential(nn.Linear(8, 8)))
+
+
+# ---- the decoder -----------------------------------------------------------------------------------
+
+
+def _model(fuse=True, **sizes):
+    torch.manual_seed(0)
+    config = ModelConfig.tiny(vocab_size=64)
+    for name, value in sizes.items():
+        setattr(config, name, value)
+    model = quantize_model_float8_(DecoderOnlyModel(config, dtype=torch.bfloat16).eval())
+    return (model, fuse_projections_(model)) if fuse else model
+
+
+@pytest.mark.parametrize("sizes,fused", [({}, 4), ({"num_key_value_heads": 1}, 2)])
+def test_a_model_in_8_bit_floating_point(sizes, fused):
+    """Fused projections take the norms' quantized outputs; unfused ones, the same numbers."""
+    model, count = _model(**sizes)
+    assert count == fused  # a key projection of 64 rows is not fused
+    plain = _model(fuse=False, **sizes)
+    ids, pos = torch.arange(10) % 64, torch.arange(10)
+    with torch.no_grad():
+        got = model(ids, pos, q_len=10).logits
+        want = plain(ids, pos, q_len=10).logits
+    assert got.shape == (1, 10, 64)
+    # unfused, the gated product is rounded to bf16 on its way to the down projection: 2^-9 of it, where both round to e4m3
+    assert float((got - want).float().norm() / want.float().norm()) < 0.05
+    dense = DecoderOnlyModel(model.config, dtype=torch.bfloat16)
+    torch.manual_seed(0)
+    assert all(m.takes_float8() for layer in model.layers for m in (layer.self_attn, layer.mlp))
+    assert not any(m.takes_float8() for layer in dense.layers for m in (layer.self_attn, layer.mlp))
+
+
+def test_the_norms_hand_on_quantized_outputs_unless_a_derivative_is_needed():
+    model, _ = _model()
+    seen = []
+    for layer in model.layers:
+        for m in (layer.self_attn, layer.mlp):
+            m.register_forward_pre_hook(lambda mod, args: seen.append(type(args[0])))
+    ids, pos = torch.arange(6), torch.arange(6)
+    with torch.no_grad():
+        model(ids, pos, q_len=6)
+    assert seen == [Float8Tensor] * 4
+    seen.clear()
+    out = model(ids, pos, q_len=6).logits
+    assert seen == [torch.Tensor] * 4
+    out.float().sum().backward()
+    grads = [model.embed_tokens.weight.grad] + [n.weight.grad for layer in model.layers
+                                                for n in (layer.input_layernorm, layer.post_attention_layernorm)]
+    assert all(g is not None and bool(g.any()) for g in grads)
+
+
+def test_generation_with_a_model_in_8_bit_floating_point():
+    model, _ = _model()
+    prompts = torch.arange(12).view(2, 6)
+    tokens = GreedyGenerator(model).generate(prompts, 4).tokens
+    assert tokens.shape == (2, 4)
+    ragged = GreedyGenerator(model, cache_dtype=torch.int8).generate([prompts[0], prompts[1, :3]], 3).tokens
+    assert ragged.shape == (2, 3)
 
 
 # ---- derivatives -----------------------------------------------------------------------------------
