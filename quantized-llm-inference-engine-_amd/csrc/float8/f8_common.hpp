@@ -154,8 +154,23 @@ __device__ __forceinline__ uint32_t f8_codes4(float a, float b, float c, float d
   return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true));
 }
 
-// silu(gate) * up in fp32; the exponential is the hardware's (a few steps of fp32).
-__device__ __forceinline__ float f8_swiglu(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
+// silu(gate) * up in fp32, with the hardware's exponential and reciprocal (a step of fp32 each; 2^-22 |gate| of the
+// exponential's argument). Far below zero the exponential is infinite and the product 0.
+__device__ __forceinline__ float f8_swiglu(float gate, float up) {
+  return gate * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(gate * -1.44269504f)) * up;
+}
+
+// Two numbers as 16-bit ones, to nearest, ties to even.
+template <class Out>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (Out::id == kDtBf16) {
+    const f32x2 v = {lo, hi};
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, pair));
+  } else {
+    return uint32_t(Out::store(lo)) | (uint32_t(Out::store(hi)) << 16);
+  }
+}
 
 // Eight neighbouring numbers of a row, from column c on; zeros behind `cols`.
 template <class Act>
@@ -181,7 +196,7 @@ __device__ __forceinline__ void load8(const typename Act::raw* row, int64_t c, i
 
 __device__ __forceinline__ void store_codes8(uint8_t* row, int64_t c, int64_t cols, bool vec, u32x2 w) {
   if (vec) {
-    if (c < cols) *reinterpret_cast<u32x2*>(row + c) = w;
+    if (c < cols) __builtin_nontemporal_store(w, reinterpret_cast<u32x2*>(row + c));
     return;
   }
 #pragma unroll

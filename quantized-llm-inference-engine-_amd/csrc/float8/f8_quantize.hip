@@ -117,6 +117,40 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_rows_kernel(const F8NormArgs
   }
 }
 
+// Rows of up to kThreads * 8 * NIT: the stream stays in registers between the two passes, and everything that is read is on
+// its way at once.
+template <class Act, int NIT>
+__global__ void __launch_bounds__(kThreads) rmsnorm_held_kernel(const F8NormArgs a) {
+  using Raw = typename Act::raw;
+  __shared__ float part[kThreads / 64];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  float h[NIT][8], w[NIT][8];
+#pragma unroll
+  for (int i = 0; i < NIT; ++i) stream8<Act>(a, row, 8 * tid + i * kChunk, h[i]);
+#pragma unroll
+  for (int i = 0; i < NIT; ++i) load8<Act>(static_cast<const Raw*>(a.weight), 8 * tid + i * kChunk, a.hidden, a.vec, w[i]);
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NIT; ++i) {
+    if (a.residual) store_stream8<Act>(a, row, 8 * tid + i * kChunk, h[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(h[i][e], h[i][e], ss);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) ss += __shfl_xor(ss, off, 64);
+  if ((tid & 63) == 0) part[tid >> 6] = ss;
+  __syncthreads();
+  const float total = (part[0] + part[1]) + (part[2] + part[3]);
+  const float inv = __frsqrt_rn(total / float(a.hidden) + a.eps);
+#pragma unroll
+  for (int i = 0; i < NIT; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[i][e] = h[i][e] * inv * w[i][e];
+    quantize8(h[i], a.codes + row * a.ldc, a.scales + row * a.lds, 8 * tid + i * kChunk, a.hidden, a.vec);
+  }
+}
+
 // silu(gate) * up, a workgroup per `kChunk` columns of a row.
 __global__ void __launch_bounds__(kThreads) act_kernel(const F8ActArgs a, uint32_t chunks, int vec) {
   const int64_t row = blockIdx.x / chunks;
@@ -155,14 +189,23 @@ hipError_t launch_f8_quantize(const F8QuantArgs& a, int dtype, int64_t block_row
   return hipGetLastError();
 }
 
+template <class Act>
+static hipError_t launch_norm(const F8NormArgs& a, hipStream_t stream) {
+  const dim3 grid(unsigned(a.rows)), block(kThreads);
+  if (a.hidden <= kChunk)
+    hipLaunchKernelGGL((rmsnorm_held_kernel<Act, 1>), grid, block, 0, stream, a);
+  else if (a.hidden <= 2 * kChunk)
+    hipLaunchKernelGGL((rmsnorm_held_kernel<Act, 2>), grid, block, 0, stream, a);
+  else if (a.hidden <= 4 * kChunk)
+    hipLaunchKernelGGL((rmsnorm_held_kernel<Act, 4>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL(rmsnorm_rows_kernel<Act>, grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
 hipError_t launch_f8_rmsnorm(const F8NormArgs& a, int dtype, hipStream_t stream) {
   if (a.rows == 0 || a.hidden == 0) return hipSuccess;
-  const dim3 grid = dim3(unsigned(a.rows));
-  if (dtype == kDtF16)
-    hipLaunchKernelGGL(rmsnorm_rows_kernel<ActF16>, grid, dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL(rmsnorm_rows_kernel<ActBf16>, grid, dim3(kThreads), 0, stream, a);
-  return hipGetLastError();
+  return dtype == kDtF16 ? launch_norm<ActF16>(a, stream) : launch_norm<ActBf16>(a, stream);
 }
 
 hipError_t launch_f8_act(const F8ActArgs& a, hipStream_t stream) {

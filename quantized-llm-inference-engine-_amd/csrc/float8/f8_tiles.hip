@@ -41,50 +41,72 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
     tiles_kernel(const F8TilesArgs a) {
   constexpr int kWaves = WN * WM;
   constexpr int kRowsN = 128 * WN, kRowsM = 16 * TM * WM;
+  constexpr int kWide = GATED ? kRowsN / 2 : kRowsN;  // features of a tile
   constexpr int kStage = (kRowsN + kRowsM) * kStep;
-  static_assert(64 * kWaves >= kRowsM + 2, "a thread for every row of scales");
-  constexpr int kLoadsN = kRowsN / 8 / kWaves, kLoadsM = kRowsM / 8 / kWaves;
+  constexpr int kLoadsN = kRowsN / 8 / kWaves, kLoadsM = kRowsM / 8 / kWaves, kLoads = kLoadsN + kLoadsM;
   static_assert(kLoadsN * 8 * kWaves == kRowsN && kLoadsM * 8 * kWaves == kRowsM, "whole loads for every wave");
+  static_assert(64 * kWaves >= kRowsM + 2, "a thread for every row of scales");
+  // What a wave stores of a whole tile, at least.
+  constexpr int kStores = PARTS ? 8 * TM : GATED ? TM : 4 * TM;
   extern __shared__ __align__(1024) uint8_t lds[];
+  uint8_t* const scales = lds + STAGES * kStage;
+  uint32_t* const tops = reinterpret_cast<uint32_t*>(scales + (kRowsM + 2) * kScaleRow);  // [2][kRowsM] (gated)
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wn = wave % WN, wm = wave / WN;
   const int r = lane & 15, g = lane >> 4;
+  auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
 
-  // Tile order: neighbouring workgroups go to different XCDs, so each XCD takes a run of tiles of its own; within it
-  // `kSweep` token tiles per sweep over the features, whose operands then meet in its L2.
-  constexpr uint32_t kSweep = 4;
-  uint32_t id = blockIdx.x;
-  {
-    const uint32_t per = gridDim.x / 8, rest = gridDim.x % 8, xcd = id % 8, at = id / 8;
-    id = xcd * per + min(xcd, rest) + at;
-  }
-  uint32_t split = 0;
-  if (PARTS) {  // the parts of a sum one after the other
-    const uint32_t tiles = a.tiles_n * a.tiles_m;
-    split = __builtin_amdgcn_readfirstlane(id / tiles);
-    id -= split * tiles;
-  }
-  const int s_begin = PARTS ? int(split * a.steps_per_split) : 0;
-  const int s_end = PARTS ? min(s_begin + int(a.steps_per_split), a.steps) : a.steps;
-  const uint32_t in_sweep = kSweep * a.tiles_n;
-  const uint32_t first_m = id / in_sweep * kSweep;
-  const uint32_t rows_m = min(a.tiles_m - first_m, kSweep);
-  const uint32_t left = id % in_sweep;
-  // (quotients are computed in vector registers; buffers and scalar offsets want scalar ones)
-  const uint32_t tn = __builtin_amdgcn_readfirstlane(left / rows_m);
-  const uint32_t tm = __builtin_amdgcn_readfirstlane(first_m + left - left / rows_m * rows_m);
-  const int64_t m0 = int64_t(tm) * kRowsM;
-  const int64_t n0 = int64_t(tn) * (GATED ? kRowsN / 2 : kRowsN);
+  // ---- tiles: workgroup i takes i, i + grid, ... ----
+  // Neighbouring workgroups go to different XCDs, so each XCD takes a run of tiles of its own; within it `kSweep` token
+  // tiles per sweep over the features, whose operands then meet in its L2.
+  const uint32_t tiles = a.tiles_n * a.tiles_m, count = tiles * (PARTS ? a.splits : 1);
+  struct Tile {
+    uint32_t tn, tm, split;
+    int begin, steps;  // its steps of 128 columns
+  };
+  auto tile_of = [&](uint32_t id) {
+    constexpr uint32_t kSweep = 4;
+    const uint32_t per = count / 8, rest = count % 8, xcd = id % 8;
+    id = xcd * per + min(xcd, rest) + id / 8;
+    Tile t;
+    t.split = PARTS ? __builtin_amdgcn_readfirstlane(id / tiles) : 0;
+    if (PARTS) id -= t.split * tiles;
+    const uint32_t in_sweep = kSweep * a.tiles_n, first_m = id / in_sweep * kSweep;
+    const uint32_t rows_m = min(a.tiles_m - first_m, kSweep), left = id % in_sweep;
+    // (quotients are computed in vector registers; buffers and scalar offsets want scalar ones)
+    t.tn = __builtin_amdgcn_readfirstlane(left / rows_m);
+    t.tm = __builtin_amdgcn_readfirstlane(first_m + left - left / rows_m * rows_m);
+    t.begin = PARTS ? int(t.split * a.steps_per_split) : 0;
+    t.steps = PARTS ? min(int(a.steps_per_split), a.steps - t.begin) : a.steps;
+    return t;
+  };
+  auto rows_n_of = [&](const Tile& t) {
+    const int64_t left = a.N - int64_t(t.tn) * kWide;
+    return left < kWide ? int(left) : kWide;
+  };
+  auto rows_m_of = [&](const Tile& t) {
+    const int64_t left = a.M - int64_t(t.tm) * kRowsM;
+    return left < kRowsM ? int(left) : kRowsM;
+  };
 
   // ---- loads: lane l of load j brings 16 bytes of row 8 (..) + l / 8, its chunk l % 8 swizzled ----
-  constexpr int kWide = GATED ? kRowsN / 2 : kRowsN;  // features of a tile
-  const int rows_n = a.N - n0 < kWide ? int(a.N - n0) : kWide, rows_mm = a.M - m0 < kRowsM ? int(a.M - m0) : kRowsM;
-  const uint32_t K = uint32_t(a.K), k_end = PARTS ? min(K, uint32_t(s_end) * kStep) : K;
-  const auto wq0 = make_rsrc(a.w[0].codes + n0 * a.w[0].ld, uint32_t(rows_n - 1) * uint32_t(a.w[0].ld) + K);
-  const auto wq1 = make_rsrc(a.w[GATED].codes + n0 * a.w[GATED].ld, uint32_t(rows_n - 1) * uint32_t(a.w[GATED].ld) + K);
-  const auto xq = make_rsrc(a.x + m0 * a.ldx, uint32_t(rows_mm - 1) * uint32_t(a.ldx) + K);
+  const uint32_t K = uint32_t(a.K);
+  struct Source {  // of a tile's stages
+    __amdgpu_buffer_rsrc_t w[2], x;
+    uint32_t k_end;
+  };
+  auto source_of = [&](const Tile& t) {
+    const int64_t n0 = int64_t(t.tn) * kWide, m0 = int64_t(t.tm) * kRowsM;
+    const uint32_t rows_n = uint32_t(rows_n_of(t)), rows_m = uint32_t(rows_m_of(t));
+    Source s;
+    s.w[0] = make_rsrc(a.w[0].codes + n0 * a.w[0].ld, (rows_n - 1) * uint32_t(a.w[0].ld) + K);
+    s.w[1] = make_rsrc(a.w[GATED].codes + n0 * a.w[GATED].ld, (rows_n - 1) * uint32_t(a.w[GATED].ld) + K);
+    s.x = make_rsrc(a.x + m0 * a.ldx, (rows_m - 1) * uint32_t(a.ldx) + K);
+    s.k_end = PARTS ? min(K, uint32_t(t.begin + t.steps) * kStep) : K;
+    return s;
+  };
   // LDS row of load j's first lane; the chunk that a lane brings: its own position swizzled by its row.
   constexpr int kShift = GATED ? 4 : 5, kHalf = kLoadsN / 2;
   auto base_n = [&](int j) {
@@ -100,10 +122,9 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
   off_n[1] = uint32_t(base_n(0) + lane / 8) * uint32_t(a.w[GATED].ld);
   const uint32_t off_m = uint32_t(base_m(0) + lane / 8) * uint32_t(a.ldx) + col_m;
   // Loads first .. last - 1 of a stage.
-  constexpr int kLoads = kLoadsN + kLoadsM;
-  auto load_stage = [&](int step, uint8_t* buf, int first, int last) {
+  auto load_stage = [&](const Source& src, int step, uint8_t* buf, int first, int last) {
     const uint32_t k = uint32_t(step) * kStep;
-    const bool whole = k + kStep <= k_end;  // else columns behind the end are zeros
+    const bool whole = k + kStep <= src.k_end;  // else columns behind the end are zeros
     // The strides are opaque here, so that offsets are computed where they are used and hold no registers.
     uint32_t ld[3] = {uint32_t(a.w[0].ld), uint32_t(a.w[GATED].ld), uint32_t(a.ldx)};
     asm volatile("" : "+s"(ld[0]), "+s"(ld[1]), "+s"(ld[2]));
@@ -112,35 +133,51 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
       if (j < kLoadsN) {
         const bool second = GATED && j >= kHalf;
         uint32_t o = off_n[second] + uint32_t(8 * (second ? j - kHalf : j)) * ld[second] + col_n(j);
-        if (!whole) o = k + col_n(j) < k_end ? o : kOutside;
-        load_lds16_cached(second ? wq1 : wq0, buf + base_n(j) * kStep, o, k);
+        if (!whole) o = k + col_n(j) < src.k_end ? o : kOutside;
+        load_lds16_cached(src.w[second], buf + base_n(j) * kStep, o, k);
       } else {
         uint32_t o = off_m + uint32_t(8 * (j - kLoadsN)) * ld[2];
-        if (!whole) o = k + col_m < k_end ? o : kOutside;
-        load_lds16_cached(xq, buf + (kRowsN + base_m(j - kLoadsN)) * kStep, o, k);
+        if (!whole) o = k + col_m < src.k_end ? o : kOutside;
+        load_lds16_cached(src.x, buf + (kRowsN + base_m(j - kLoadsN)) * kStep, o, k);
       }
     }
   };
+  // A load that finds the queue full holds up its wave, products behind it included; so they are dealt to two phases, between
+  // the products.
+  constexpr int kSlots = 2 * TM;
+  auto load_slot = [&](const Source& src, int step, uint8_t* to, int slot) {
+    load_stage(src, step, to, kLoads * slot / kSlots, kLoads * (slot + 1) / kSlots);
+  };
 
   // ---- scales: a chunk of steps at a time in LDS, a row of tokens or of the weight's blocks a thread ----
-  uint8_t* const scales = lds + STAGES * kStage;
-  const uint8_t* scale_row = nullptr;
-  {
-    const int t = threadIdx.x;
-    if (t < kRowsM) {
-      scale_row = a.x_scales + (m0 + min(t, rows_mm - 1)) * a.ldxs;
-    } else if (t < kRowsM + (GATED ? 2 : WN)) {
-      const int second = t - kRowsM;
+  ScaleRow row;  // of the chunk after the one in LDS
+  auto load_scales = [&](const Tile& t, int first) {
+    const int i = threadIdx.x;
+    const uint8_t* at = nullptr;
+    if (i < kRowsM) {
+      at = a.x_scales + (int64_t(t.tm) * kRowsM + min(i, rows_m_of(t) - 1)) * a.ldxs;
+    } else if (i < kRowsM + (GATED ? 2 : WN)) {
+      const int second = i - kRowsM;
       if (GATED)
-        scale_row = a.w[second].scales + tn * a.w[second].lds;
+        at = a.w[second].scales + t.tn * a.w[second].lds;
       else
-        scale_row = a.w[0].scales + min(tn * WN + second, uint32_t((a.N - 1) / kF8Group)) * a.w[0].lds;
+        at = a.w[0].scales + min(t.tn * WN + second, uint32_t((a.N - 1) / kF8Group)) * a.w[0].lds;
     }
-  }
+    if (at) row.load(at, t.begin + first, t.begin + t.steps);
+  };
+  auto store_scales = [&] {
+    wait_lgkmcnt0();
+    __builtin_amdgcn_s_barrier();  // the chunk before this one has been read
+    if (threadIdx.x < kRowsM + 2) row.store(scales + threadIdx.x * kScaleRow);
+    wait_lgkmcnt0();
+    __builtin_amdgcn_s_barrier();
+    fence();
+  };
   const uint8_t* const sx_at = scales + (wm * TM * 16 + r) * kScaleRow;
   const uint8_t* const sw_at = scales + (kRowsM + (GATED ? 0 : wn)) * kScaleRow;
   uint32_t sx[TM], sw[2], sx_next[TM], sw_next[2];
   auto read_scales = [&](int step, uint32_t* x, uint32_t* w) {
+    step %= kChunk;
 #pragma unroll
     for (int u = 0; u < TM; ++u) x[u] = sx_at[u * 16 * kScaleRow + step];
     w[0] = sw_at[step];
@@ -160,183 +197,241 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
   auto frag_n = [&](int t) { return frag(at_n, (GATED ? (t >> 2) * kWide + (t & 3) * 4 : t * 4) * kStep); };
   auto frag_m = [&](int u) { return frag(at_m, u * 16 * kStep); };
 
-  f32x4 acc[8][TM];
-#pragma unroll
-  for (int t = 0; t < 8; ++t)
-#pragma unroll
-    for (int u = 0; u < TM; ++u) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
+  // ---- products ----
   // A step's 8 TM products are dealt to four phases of two weight tiles. In each, the weight tiles of the next phase come from
   // LDS. In front of the last phase everything of this step is in registers and the next stage in LDS (a barrier), so that
   // phase brings in the next step's first fragments, each token tile's when its registers have served, and starts the loads
-  // of STAGES stages on into this step's buffer. The loop's body has no branch: the compiler would move products behind it.
-  // A load that finds the queue full holds up its wave, products behind it included; so they are dealt to two phases, the
-  // last and the next step's first, between the products.
-  constexpr int kSlots = 2 * TM;
-  auto load_slot = [&](int step, uint8_t* to, int slot) { load_stage(step, to, kLoads * slot / kSlots, kLoads * (slot + 1) / kSlots); };
+  // of STAGES stages on into this step's buffer. A turn of the loop is a step's last phase and the next one's first three; it
+  // has no branch: the compiler would move products behind it.
+  f32x4 acc[8][TM];
   i32x8 b[TM], w[4];
-  auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+  uint32_t buf = 0;  // of the step
   auto mul = [&](int t, int u) { acc[t][u] = mfma_f8(w[t & 3], b[u], acc[t][u], sw[GATED ? t >> 2 : 0], sx[u]); };
+  auto advance = [&] {
+    const uint32_t next = buf == (STAGES - 1) * kStage ? 0u : buf + kStage;
+    at_n += next - buf, at_m += next - buf, buf = next;
+  };
+  auto phases = [&](auto&& between) {  // the first three of a step
 #pragma unroll
-  for (int i = 0; i < STAGES; ++i) load_stage(s_begin + i, lds + i * kStage, 0, i < STAGES - 1 ? kLoads : kLoads * TM / kSlots);
-  uint32_t buf = 0, freed = (STAGES - 1) * kStage;  // the step's stage, and the one before it
-  for (int c = s_begin; c < s_end; c += kChunk) {
-    __builtin_amdgcn_s_barrier();  // the chunk before this one has been read
-    if (scale_row) {
-      ScaleRow row;
-      row.load(scale_row, c, s_end);
-      row.store(scales + threadIdx.x * kScaleRow);
-    }
-    wait_lgkmcnt0();
-    wait_vmcnt<0>();
-    __builtin_amdgcn_s_barrier();
-    fence();
-    read_scales(0, sx, sw);
-    if (c == s_begin) {
-#pragma unroll
-      for (int u = 0; u < TM; ++u) b[u] = frag_m(u);
-      w[0] = frag_n(0);
-      w[1] = frag_n(1);
-    }
-    const int last = min(s_end - c, kChunk);
-#pragma unroll 1
-    for (int s = 0; s < last; ++s) {
-#pragma unroll
-      for (int phase = 0; phase < 3; ++phase) {
-        const int t = 2 * phase;
-#pragma unroll
-        for (int u = 0; u < TM; ++u) {
-          if (u == 0) w[(t + 2) & 3] = frag_n(t + 2);
-          if (u == TM / 2) w[(t + 3) & 3] = frag_n(t + 3);
-          mul(t, u);
-          if (phase == 0) load_slot(c + s + STAGES - 1, lds + freed, TM + u);  // (zeros behind the end)
-          mul(t + 1, u);
-          fence();
-        }
-      }
-      read_scales(s + 1, sx_next, sw_next);  // (of the next chunk: read again)
-      wait_lgkmcnt0();
-      wait_vmcnt<(STAGES - 2) * kLoads>();
-      __builtin_amdgcn_s_barrier();
-      fence();
-      const uint32_t next = buf == (STAGES - 1) * kStage ? 0u : buf + kStage;
-      at_n += next - buf, at_m += next - buf, freed = buf, buf = next;
-      fence();
+    for (int phase = 0; phase < 3; ++phase) {
+      const int t = 2 * phase;
 #pragma unroll
       for (int u = 0; u < TM; ++u) {
-        if (u == 0) w[0] = frag_n(0);
-        if (u == TM / 2) w[1] = frag_n(1);
-        mul(6, u);
-        load_slot(c + s + STAGES, lds + freed, u);
-        mul(7, u);
+        if (u == 0) w[(t + 2) & 3] = frag_n(t + 2);
+        if (u == TM / 2) w[(t + 3) & 3] = frag_n(t + 3);
+        mul(t, u);
+        if (phase == 0) between(u);
+        mul(t + 1, u);
         fence();
-        b[u] = frag_m(u);
       }
+    }
+  };
+  // Step s's last phase and step s + 1's others; at most OPEN of the loads and stores issued so far may be under way in front of
+  // it. The stage `load` of `src` is loaded (zeros behind its end).
+  auto turn = [&](int s, const Source& src, int load, auto open) {
+    read_scales(s + 1, sx_next, sw_next);
+    wait_lgkmcnt0();
+    wait_vmcnt<decltype(open)::value>();
+    __builtin_amdgcn_s_barrier();
+    fence();
+    uint8_t* const freed = lds + buf;
+    advance();
+    fence();
 #pragma unroll
-      for (int u = 0; u < TM; ++u) sx[u] = sx_next[u];
-      sw[0] = sw_next[0];
-      if (GATED) sw[1] = sw_next[1];
+    for (int u = 0; u < TM; ++u) {
+      if (u == 0) w[0] = frag_n(0);
+      if (u == TM / 2) w[1] = frag_n(1);
+      mul(6, u);
+      load_slot(src, load, freed, u);
+      mul(7, u);
       fence();
+      b[u] = frag_m(u);
     }
-  }
-  wait_vmcnt<0>();  // zeros on their way into LDS
+#pragma unroll
+    for (int u = 0; u < TM; ++u) sx[u] = sx_next[u];
+    sw[0] = sw_next[0];
+    if (GATED) sw[1] = sw_next[1];
+    fence();
+    phases([&](int u) { load_slot(src, load, freed, TM + u); });
+  };
 
-  // ---- results ----
-  if constexpr (PARTS) {  // rows of a multiple of 16 features
-    const int64_t n = n0 + wn * 128 + 32 * g;
+  uint32_t id = blockIdx.x;
+  Tile tile = tile_of(id);
+  Source source = source_of(tile);  // of the stages that are loaded
 #pragma unroll
-    for (int u = 0; u < TM; ++u) {
-      const int64_t m = m0 + (wm * TM + u) * 16 + r;
-      if (m >= a.M) continue;
-      float* out = a.parts + (int64_t(split) * a.M + m) * a.ld_parts + n;
+  for (int i = 0; i < STAGES; ++i) load_stage(source, tile.begin + i, lds + i * kStage, 0, kLoads);
+  load_scales(tile, 0);
+  wait_vmcnt<0>();
+  bool stored = false;  // a whole tile's results after the loads of this one's stages
+  for (;;) {
+    // The tile after this one, whose first stages follow this one's last (there are more than STAGES steps then).
+    const bool more = id + gridDim.x < count;
+    const Tile next = more ? tile_of(id + gridDim.x) : tile;
+
+    store_scales();  // (and a barrier)
+    if (tile.steps > kChunk)
+      load_scales(tile, kChunk);
+    else if (more)
+      load_scales(next, 0);
+    read_scales(0, sx, sw);
 #pragma unroll
-      for (int t = 0; t < 8; ++t)
-        if (n + 4 * t < a.N) *reinterpret_cast<f32x4*>(out + 4 * t) = acc[t][u];
+    for (int u = 0; u < TM; ++u) b[u] = frag_m(u);
+    w[0] = frag_n(0);
+    w[1] = frag_n(1);
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int u = 0; u < TM; ++u) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    fence();
+    phases([](int) {});
+
+    const int last = tile.steps - 1, own = max(0, tile.steps - STAGES);  // from turn `own` on the next tile's stages are loaded
+    int load = tile.begin + STAGES;
+    // The stages that a turn waits for were loaded in front of the results' stores.
+    if (own > 0 && stored) turn(0, source, load++, std::integral_constant<int, (STAGES - 2) * kLoads + kStores>{});
+    for (int s = load - tile.begin - STAGES; s < last;) {
+      if ((s + 1) % kChunk == 0) {
+        store_scales();
+        if (s + 1 + kChunk < tile.steps)
+          load_scales(tile, s + 1 + kChunk);
+        else if (more)
+          load_scales(next, 0);
+      }
+      if (s == own) {
+        source = source_of(next), load = next.begin;
+        if (!more) source.k_end = 0;
+      }
+      const int end = min(s < own ? own : last, (s + 1) / kChunk * kChunk + kChunk - 1);
+#pragma unroll 1
+      for (; s < end; ++s) turn(s, source, load++, std::integral_constant<int, (STAGES - 2) * kLoads>{});
     }
-  } else if constexpr (!GATED) {
-    using Raw = typename Out::raw;
-    const int64_t n = n0 + wn * 128 + 32 * g;
-    const Raw* bias = static_cast<const Raw*>(a.bias);
+    wait_lgkmcnt0();
+    __builtin_amdgcn_s_barrier();  // the last stage is in registers
+    fence();
 #pragma unroll
     for (int u = 0; u < TM; ++u) {
-      const int64_t m = m0 + (wm * TM + u) * 16 + r;
-      if (m >= a.M) continue;
-      Raw* y = static_cast<Raw*>(a.y) + m * a.ldy;
+      mul(6, u);
+      mul(7, u);
+    }
+    // All that was loaded so far has to be here before the next tile begins: the scales and its stages but the last. It is
+    // waited for now, while no stores are under way.
+    wait_vmcnt<0>();
 #pragma unroll
-      for (int t = 0; t < 8; t += 2) {
-        float v[8];
+    for (uint32_t& v : row.v) asm volatile("" : "+v"(v));
+    fence();
+    if (last <= own) {  // a walk of one step, or none that the next tile's stages begin in
+      source = source_of(next), load = next.begin;
+      if (!more) source.k_end = 0;
+    }
+    load_stage(source, load, lds + buf, 0, kLoads);
+    advance();
+    fence();
+
+    // ---- results ----
+    const int64_t n0 = int64_t(tile.tn) * kWide, m0 = int64_t(tile.tm) * kRowsM;
+    const int rows_n = rows_n_of(tile);
+    if constexpr (PARTS) {  // rows of a multiple of 16 features
+      const int64_t n = n0 + wn * 128 + 32 * g;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] = acc[t + i / 4][u][i & 3];
-          const int64_t at = n + 4 * t + i;
-          if (bias && at < a.N) v[i] += Out::load(bias[at]);
+      for (int u = 0; u < TM; ++u) {
+        const int64_t m = m0 + (wm * TM + u) * 16 + r;
+        if (m >= a.M) continue;
+        float* out = a.parts + (int64_t(tile.split) * a.M + m) * a.ld_parts + n;
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          if (n + 4 * t < a.N) *reinterpret_cast<f32x4*>(out + 4 * t) = acc[t][u];
+      }
+    } else if constexpr (!GATED) {
+      using Raw = typename Out::raw;
+      const int64_t n = n0 + wn * 128 + 32 * g;
+      const Raw* bias = static_cast<const Raw*>(a.bias);
+#pragma unroll
+      for (int u = 0; u < TM; ++u) {
+        const int64_t m = m0 + (wm * TM + u) * 16 + r;
+        if (m >= a.M) continue;
+        Raw* y = static_cast<Raw*>(a.y) + m * a.ldy;
+#pragma unroll
+        for (int t = 0; t < 8; t += 2) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[i] = acc[t + i / 4][u][i & 3];
+            const int64_t at = n + 4 * t + i;
+            if (bias && at < a.N) v[i] += Out::load(bias[at]);
+          }
+          u32x4 out;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) out[i] = pack16<Out>(v[2 * i], v[2 * i + 1]);
+          if (a.vec && n + 4 * t + 8 <= a.N) {
+            *reinterpret_cast<u32x4*>(y + n + 4 * t) = out;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (n + 4 * t + i < a.N) y[n + 4 * t + i] = Raw(out[i >> 1] >> (16 * (i & 1)));
+          }
         }
-        u32x4 w;
+      }
+    } else {
+      // A group's 128 features lie in two waves, 16 in a lane: the largest magnitude goes across lanes and through LDS.
+      float v[TM][16];
+      const int f0 = wn * 64 + 16 * g;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = uint32_t(Out::store(v[2 * i])) | (uint32_t(Out::store(v[2 * i + 1])) << 16);
-        if (a.vec && n + 4 * t + 8 <= a.N) {
-          *reinterpret_cast<u32x4*>(y + n + 4 * t) = w;
+      for (int u = 0; u < TM; ++u) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float gate = acc[i >> 2][u][i & 3], up = acc[4 + (i >> 2)][u][i & 3];
+          v[u][i] = f0 + i < rows_n ? f8_swiglu(gate, up) : 0.0f;
+          top = max(top, magnitude(v[u][i]));
+        }
+        top = max(top, uint32_t(__shfl_xor(int(top), 16, 64)));
+        top = max(top, uint32_t(__shfl_xor(int(top), 32, 64)));
+        if (g == 0) tops[wn * kRowsM + (wm * TM + u) * 16 + r] = top;
+      }
+      wait_lgkmcnt0();
+      __builtin_amdgcn_s_barrier();
+#pragma unroll
+      for (int u = 0; u < TM; ++u) {
+        const int at = (wm * TM + u) * 16 + r;
+        const int64_t m = m0 + at;
+        if (m >= a.M) continue;
+        const uint32_t scale = f8_scale(max(tops[at], tops[kRowsM + at]));
+        const float inv = f8_inverse(scale);
+        if (wn == 0 && g == 0) a.scales[m * a.lds + tile.tn] = uint8_t(scale);
+        u32x4 out;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = f8_codes4(v[u][4 * i], v[u][4 * i + 1], v[u][4 * i + 2], v[u][4 * i + 3], inv);
+        uint8_t* to = a.codes + m * a.ldc + n0 + f0;
+        if (a.vec && f0 + 16 <= rows_n) {
+          *reinterpret_cast<u32x4*>(to) = out;
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (n + 4 * t + i < a.N) y[n + 4 * t + i] = Raw(w[i >> 1] >> (16 * (i & 1)));
+          for (int i = 0; i < 16; ++i)
+            if (f0 + i < rows_n) to[i] = uint8_t(out[i >> 2] >> (8 * (i & 3)));
         }
       }
     }
-  } else {
-    // A group's 128 features lie in two waves, 16 in a lane: the largest magnitude goes across lanes and through LDS.
-    wait_lgkmcnt0();
-    __syncthreads();
-    uint32_t* tops = reinterpret_cast<uint32_t*>(lds);  // [2][kRowsM]
-    float v[TM][16];
-    uint32_t top[TM];
-    const int f0 = wn * 64 + 16 * g;
-#pragma unroll
-    for (int u = 0; u < TM; ++u) {
-      top[u] = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float gate = acc[i >> 2][u][i & 3], up = acc[4 + (i >> 2)][u][i & 3];
-        v[u][i] = f0 + i < rows_n ? f8_swiglu(gate, up) : 0.0f;
-        top[u] = max(top[u], magnitude(v[u][i]));
-      }
-      top[u] = max(top[u], uint32_t(__shfl_xor(int(top[u]), 16, 64)));
-      top[u] = max(top[u], uint32_t(__shfl_xor(int(top[u]), 32, 64)));
-      if (g == 0) tops[wn * kRowsM + (wm * TM + u) * 16 + r] = top[u];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < TM; ++u) {
-      const int row = (wm * TM + u) * 16 + r;
-      const int64_t m = m0 + row;
-      if (m >= a.M) continue;
-      const uint32_t scale = f8_scale(max(tops[row], tops[kRowsM + row]));
-      const float inv = f8_inverse(scale);
-      if (wn == 0 && g == 0) a.scales[m * a.lds + n0 / kF8Group] = uint8_t(scale);
-      u32x4 w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = f8_codes4(v[u][4 * i], v[u][4 * i + 1], v[u][4 * i + 2], v[u][4 * i + 3], inv);
-      uint8_t* out = a.codes + m * a.ldc + n0 + f0;
-      if (a.vec && f0 + 16 <= rows_n) {
-        *reinterpret_cast<u32x4*>(out) = w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (f0 + i < rows_n) out[i] = uint8_t(w[i >> 2] >> (8 * (i & 3)));
-      }
-    }
+    if (!more) break;
+    stored = a.vec && rows_n == kWide && m0 + kRowsM <= a.M;
+    tile = next, id += gridDim.x;
   }
+  wait_vmcnt<0>();  // zeros on their way into LDS
 }
 
 template <int WN, int WM, int TM, int STAGES, bool GATED, bool PARTS, class Out>
 hipError_t launch(const F8TilesArgs& a, hipStream_t stream) {
   constexpr int kRowsN = 128 * WN, kRowsM = 16 * TM * WM;
-  constexpr int kBytes = STAGES * (kRowsN + kRowsM) * kStep + (kRowsM + 2) * kScaleRow;
+  constexpr int kBytes = STAGES * (kRowsN + kRowsM) * kStep + (kRowsM + 2) * kScaleRow + (GATED ? 8 * kRowsM : 0);
   static_assert(kBytes <= 160 * 1024, "stages and scales fit LDS");
   auto* kernel = tiles_kernel<WN, WM, TM, STAGES, GATED, PARTS, Out>;
   static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (ready != hipSuccess) return ready;
-  hipLaunchKernelGGL(kernel, dim3(a.tiles_n * a.tiles_m * a.splits), dim3(64 * WN * WM), kBytes, stream, a);
+  // As many workgroups as the chip holds, each with its tiles one after the other: the next one's first stages are loaded, and
+  // this one's results stored, beside the products. Walks too short for that: a workgroup for each tile.
+  const uint32_t count = a.tiles_n * a.tiles_m * a.splits, held = 256 * (kBytes <= 80 * 1024 ? 2 : 1);
+  const int shortest = a.splits > 1 ? a.steps - int((a.splits - 1) * a.steps_per_split) : a.steps;
+  const uint32_t grid = shortest > STAGES && count > held ? held : count;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * WN * WM), kBytes, stream, a);
   return hipGetLastError();
 }
 

@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Exceptions.h>
@@ -412,6 +413,11 @@ PyObject* attach_f8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// Whether a result computed from `t` now has to carry a derivative.
+bool differentiated(const at::Tensor& t) {
+  return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined();
+}
+
 int64_t f8_groups(int64_t n) { return (n + 127) / 128; }
 
 // A tensor of at least one dimension as rows: its last dimension's, `ld` elements apart.
@@ -529,7 +535,7 @@ PyObject* f8_rmsnorm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Rows r, rr;
   const int dtype = x ? dtype_code(*x) : -1;
   if (dtype < 1 || !w || (!res && args[3] != Py_None) || !x->device().is_cuda() || !on_current_device(x->device()) ||
-      !r.of(*x) || w->device() != x->device() || w->scalar_type() != x->scalar_type() || w->dim() != 1 ||
+      !r.of(*x) || differentiated(*x) || (res && differentiated(*res)) || w->device() != x->device() || w->scalar_type() != x->scalar_type() || w->dim() != 1 ||
       w->size(0) != r.cols || !w->is_contiguous())
     Py_RETURN_NONE;
   if (res && (res->device() != x->device() || res->scalar_type() != x->scalar_type() || res->sizes() != x->sizes() || !rr.of(*res)))

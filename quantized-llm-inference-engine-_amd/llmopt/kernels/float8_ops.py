@@ -1,7 +1,7 @@
 """Torch-facing wrappers over the entry points of ``include/llmopt_float8.h``: quantizing, RMSNorm with a quantized output,
 the projection and the gated MLP product in 8-bit floating point. The checks, errors and streams are those of
-:mod:`llmopt.kernels.ops`; :mod:`llmopt.quantization.float8` is what a user calls. The plain form of a call (contiguous or
-row-strided tensors on the current device) has its checks, allocations and launch in native code."""
+:mod:`llmopt.kernels.ops`; :mod:`llmopt.quantization.float8` is what a user calls. The plain form of a call has its checks,
+allocations and launch in native code (:func:`native`)."""
 
 from __future__ import annotations
 
@@ -10,7 +10,7 @@ import torch
 from llmopt.kernels._lib import DTYPE_CODES, call, load_binding, load_library
 from llmopt.kernels.ops import _launching_on, _same_device, _stream_handle
 
-__all__ = ["belong_together", "linear", "quantize", "rmsnorm", "rmsnorm_supported", "swiglu"]
+__all__ = ["linear", "native", "quantize", "rmsnorm", "rmsnorm_supported", "swiglu"]
 
 GROUP = 128
 
@@ -32,19 +32,29 @@ def _ld(x: torch.Tensor) -> int:
     return max(x.stride(0), x.shape[1]) if x.shape[0] > 1 else x.shape[1]
 
 
-def belong_together(codes: torch.Tensor, scales: torch.Tensor, block_rows: int) -> bool:
-    """Whether these are codes and their scales on a HIP device, checked in native code; False also where that cannot say."""
-    binding = load_binding()
-    return binding is not None and binding.f8_check(codes, scales, block_rows) is True
+class _NoBinding:
+    """Where the native path is not built: every call takes the general one."""
+
+    @staticmethod
+    def _none(*_args: object) -> None:
+        return None
+
+    f8_check = f8_quantize = f8_rmsnorm = f8_linear = f8_swiglu = _none
+
+
+_NO_BINDING = _NoBinding()
+
+
+def native():  # noqa: ANN201 - the extension module
+    """The native path: ``f8_check(codes, scales, block_rows)``, ``f8_quantize(x, block_rows)``, ``f8_rmsnorm(x, weight, eps,
+    residual)``, ``f8_linear(codes, scales, codes, scales, bias, dtype)`` and ``f8_swiglu``, of which each gives what the function
+    of its name here does for the plain form of a call -- contiguous or row-strided tensors that belong together, on the current
+    device, without derivatives -- and None for any other form, which those functions take."""
+    return load_binding() or _NO_BINDING
 
 
 def quantize(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes of ``x [..., cols]`` and their scales (``llmopt_f8_quantize``)."""
-    binding = load_binding()
-    if binding is not None:
-        out = binding.f8_quantize(x, block_rows)
-        if out is not None:
-            return out
     lead = x.shape[:-1]
     if x.dtype not in DTYPE_CODES:
         x = x.to(torch.float32)
@@ -75,11 +85,6 @@ def rmsnorm_supported(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None
             ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
     """Codes of ``x``'s shape, their scales, and ``residual + x`` (``llmopt_f8_rmsnorm``)."""
-    binding = load_binding()
-    if binding is not None:
-        out = binding.f8_rmsnorm(x, weight, eps, residual)
-        if out is not None:
-            return out
     shape = x.shape
     x = _rows(x)
     rows, hidden = (int(d) for d in x.shape)
@@ -108,11 +113,6 @@ def linear(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: t
            bias: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor:
     """``[..., N]`` of ``dtype``: codes ``x [..., K]`` with scales ``[..., ceil(K / 128)]`` times codes ``w [N, K]`` with scales
     ``[ceil(N / 128), ceil(K / 128)]``, plus ``bias [N]`` of ``dtype`` (``llmopt_f8_linear``)."""
-    binding = load_binding()
-    if binding is not None:
-        y = binding.f8_linear(x, x_scales, w, w_scales, bias, DTYPE_CODES[dtype])
-        if y is not None:
-            return y
     _same_device(x, x_scales, w, w_scales, bias)
     lead = x.shape[:-1]
     x, w, x_scales, w_scales = _rows(x), _rows(w), _rows(x_scales), _rows(w_scales)
@@ -138,11 +138,6 @@ def linear(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: t
 def swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor,
            up_scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes ``[..., N]`` and scales of ``silu(x gate^T) * (x up^T)`` (``llmopt_f8_swiglu``)."""
-    binding = load_binding()
-    if binding is not None:
-        out = binding.f8_swiglu(x, x_scales, gate, gate_scales, up, up_scales)
-        if out is not None:
-            return out
     lead = x.shape[:-1]
     _same_device(x, x_scales, gate, gate_scales, up, up_scales)
     x, gate, up = _rows(x), _rows(gate), _rows(up)

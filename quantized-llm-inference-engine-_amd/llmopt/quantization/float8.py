@@ -29,6 +29,7 @@ from dataclasses import dataclass
 import torch
 from torch import nn
 
+from llmopt.kernels import float8_ops
 from llmopt.quantization.quant_linear import replace_linear_modules
 from llmopt.utils.autograd import is_differentiated
 
@@ -47,6 +48,7 @@ __all__ = [
 GROUP = 128
 F8, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 OUT_DTYPES = (torch.float16, torch.bfloat16)
+_DTYPE_CODES = {torch.float16: 1, torch.bfloat16: 2}
 
 
 def _groups(n: int) -> int:
@@ -70,11 +72,8 @@ class Float8Tensor:
 
     def __post_init__(self) -> None:
         codes, scales = self.codes, self.scales
-        if codes.is_cuda:
-            from llmopt.kernels import float8_ops
-
-            if float8_ops.belong_together(codes, scales, self.block_rows):  # what is checked here, in native code
-                return
+        if codes.is_cuda and float8_ops.native().f8_check(codes, scales, self.block_rows):
+            return  # what is checked here, in native code
         if codes.dtype != F8 or scales.dtype != E8:
             raise TypeError(f"expected float8_e4m3fn codes and float8_e8m0fnu scales, got {codes.dtype} and {scales.dtype}")
         if self.block_rows == 1 and codes.dim() > 0:
@@ -149,14 +148,15 @@ def _made(codes: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> Flo
 
 def quantize_float8(x: torch.Tensor, block_rows: int = 1) -> Float8Tensor:
     """Quantize activations ``x [..., K]``, or with ``block_rows=128`` a weight ``[N, K]`` (see the module)."""
+    made = float8_ops.native().f8_quantize(x, block_rows) if x.is_cuda else None
+    if made is not None:
+        return _made(*made, block_rows)
     _float(x, "x")
     if block_rows not in (1, GROUP):
         raise ValueError(f"a scale covers 1 or {GROUP} rows, not {block_rows}")
     if block_rows == GROUP and x.dim() != 2:
         raise ValueError(f"expected a 2D weight, got shape {tuple(x.shape)}")
     if x.is_cuda:
-        from llmopt.kernels import float8_ops
-
         return _made(*float8_ops.quantize(x, block_rows), block_rows)
     codes, scales = _quantize_torch(x.reshape(-1, x.shape[-1]), block_rows)
     if block_rows == 1:
@@ -168,17 +168,17 @@ def rmsnorm_float8(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: 
                    ) -> tuple[Float8Tensor, torch.Tensor]:
     """``(norm(h), h)`` with ``h = residual + x`` rounded to their type (``x`` without a residual): ``norm(h) = h /
     sqrt(mean(h^2) + eps) * weight`` in fp32, quantized by rows without another rounding."""
+    made = float8_ops.native().f8_rmsnorm(x, weight, eps, residual) if x.is_cuda else None
+    if made is not None:
+        return _made(made[0], made[1]), x if residual is None else made[2]
     _float(x, "x")
     if weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
         raise ValueError(f"a norm of {tuple(x.shape)} needs a weight of [{x.shape[-1]}], got {tuple(weight.shape)}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"the residual must be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
-    if x.is_cuda and not is_differentiated(x, *(() if residual is None else (residual,))):
-        from llmopt.kernels import float8_ops
-
-        if float8_ops.rmsnorm_supported(x, weight, residual):
-            codes, scales, h = float8_ops.rmsnorm(x, weight, eps, residual)
-            return _made(codes, scales), x if h is None else h
+    if not is_differentiated(x, *(() if residual is None else (residual,))) and float8_ops.rmsnorm_supported(x, weight, residual):
+        codes, scales, h = float8_ops.rmsnorm(x, weight, eps, residual)
+        return _made(codes, scales), x if h is None else h
     h = x if residual is None else residual + x
     h32 = h.detach().float()
     y = h32 * torch.rsqrt(h32.pow(2).mean(-1, keepdim=True) + eps) * weight.detach().float()
@@ -205,6 +205,10 @@ def float8_linear(x: Float8Tensor, w: Float8Tensor, bias: torch.Tensor | None = 
                   dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x w^T + bias`` of activations ``[..., K]`` and a weight ``[N, K]``: ``[..., N]`` of ``dtype`` (fp16 or bf16, also the
     bias's)."""
+    if x.codes.is_cuda and x.block_rows == 1 and w.block_rows == GROUP:
+        y = float8_ops.native().f8_linear(x.codes, x.scales, w.codes, w.scales, bias, _DTYPE_CODES.get(dtype, 0))
+        if y is not None:
+            return y
     _check_product(x, w)
     n = int(w.shape[0])
     if dtype not in OUT_DTYPES:
@@ -215,8 +219,6 @@ def float8_linear(x: Float8Tensor, w: Float8Tensor, bias: torch.Tensor | None = 
         if tuple(bias.shape) != (n,):
             raise ValueError(f"a bias of [{n}] expected, got {tuple(bias.shape)}")
     if x.is_cuda:
-        from llmopt.kernels import float8_ops
-
         return float8_ops.linear(x.codes, x.scales, w.codes, w.scales, bias, dtype)
     y = _product_torch(x, w)
     return (y if bias is None else y + bias.float()).to(dtype).view(*x.shape[:-1], n)
@@ -225,13 +227,15 @@ def float8_linear(x: Float8Tensor, w: Float8Tensor, bias: torch.Tensor | None = 
 def float8_swiglu(x: Float8Tensor, gate: Float8Tensor, up: Float8Tensor) -> Float8Tensor:
     """``silu(x gate^T) * (x up^T)`` of activations ``[..., K]`` and two weights ``[N, K]``, in fp32 up to its quantizing by
     rows: ``[..., N]``."""
+    if x.codes.is_cuda and x.block_rows == 1 and gate.block_rows == up.block_rows == GROUP:
+        made = float8_ops.native().f8_swiglu(x.codes, x.scales, gate.codes, gate.scales, up.codes, up.scales)
+        if made is not None:
+            return _made(*made)
     _check_product(x, gate, "gate")
     _check_product(x, up, "up")
     if gate.shape != up.shape:
         raise ValueError(f"gate and up have different shapes: {tuple(gate.shape)}, {tuple(up.shape)}")
     if x.is_cuda:
-        from llmopt.kernels import float8_ops
-
         return _made(*float8_ops.swiglu(x.codes, x.scales, gate.codes, gate.scales, up.codes, up.scales))
     g = _product_torch(x, gate)
     y = g / (1.0 + torch.exp(-g)) * _product_torch(x, up)
