@@ -1,15 +1,20 @@
-// The products of up to 16 tokens: bound by the weight's bytes, which go from memory straight into the matrix core's operands.
+// The products of up to 16 tokens: bound by the weight's bytes.
 //
 // A workgroup takes 16 features, and its waves the steps of 128 columns in turn, four at a time; their sums are added in LDS
 // in a fixed order. What bounds it next to the memory is the rate of a CU's load instructions, 20 ns or so for each that brings a
-// kilobyte (25 bytes a cycle; measured): so the tokens' codes come as whole lines (a load of their rows as the matrix core
-// wants them would bring each line of one token 16 times) and scales four at a time.
+// kilobyte (25 bytes a cycle; measured): so codes come as whole lines straight into LDS of the wave's own (loaded into the matrix
+// core's operands, a line of one token would be asked for 16 times), and scales four at a time.
 //
 // Measured (MI355X, in a graph, weights from memory, us; 1 / 4 / 8 / 16 tokens):
-//   6144 x 4096 8.4 / 8.5 / 9.0 / 10.8, 4096 x 14336 13.8 / 13.3 / 14.3 / 16.3 (4.3 TB/s), 28672 x 4096 24.2 / 23.7 / 25.3 / 29.1
-//   (4.9 TB/s). With codes and scales loaded by each lane for itself 10.2, 17.5 and 34.3 at one token, 14.7, 19.6 and 43.1 at 16.
-//   Four waves a workgroup are up to 12 % faster than eight from 512 workgroups on (28672 x 4096, 16 tokens: 33.0), and as much
-//   slower below (4096 x 4096: 7.5 against 7.1); 32 features a workgroup are slower but for 16 tokens at 6144 x 4096 (9.1).
+//   6144 x 4096 7.2 / 7.4 / 9.1 / 10.0, 4096 x 14336 11.6 / 11.9 / 12.0 / 13.0 (5.0 TB/s), 28672 x 4096 22.3 / 22.7 / 26.1 / 28.9
+//   (5.3 TB/s), 1536 x 1024 2.9 / 3.0 / 3.1 / 3.1.
+// Codes and scales loaded by each lane for itself: 10.2, 17.5 and 34.3 at one token, 14.7, 19.6 and 43.1 at 16.
+// The weight's codes into registers (HELD) instead of LDS: 8.4, 13.7, 24.2 and 3.3 at one token, but at more than four tokens, whose
+// LDS leaves room for fewer waves, faster from some 640 workgroups on (28672 x 4096 8 / 16 tokens 28.5 / 31.2 in LDS, 14336 x
+// 4096 16.9 / 18.4 against 15.7 / 17.4; 6144 x 4096 the same).
+// Eight waves where each has one group of steps (17 to 32 steps; no second buffer), else four: 4096 x 4096 5.6 against 5.7 (16
+// tokens 6.6 against 6.8), 4096 x 14336 11.7 against 11.6 (4 tokens 12.2 against 11.9), 1024 x 2816 4.1 against 3.9, 8192 x 2048 at 16
+// tokens 7.3 against 5.6.
 #include "f8_common.hpp"
 #include "f8_mfma.hpp"
 
@@ -20,23 +25,43 @@ constexpr uint32_t kOutside = 0x7FFFFFF0u;
 
 constexpr uint32_t kGroup = 4;  // steps that a wave takes at a time: four scales are one word
 
-// Sums of 16 weight rows with at most XR tokens over the steps of one wave. The tokens' codes go to LDS of the wave's own,
-// the weight's into registers; two groups of steps are on their way.
-template <int XR>
+// Sums of 16 weight rows with at most XR tokens over the steps of one wave. The tokens' codes go to LDS of the wave's own, the
+// weight's too (whole lines, past the caches) or into registers (HELD); up to two groups of steps are on their way.
+template <int XR, bool HELD>
 struct Walk {
   static constexpr int kXLines = kGroup * XR, kXLoads = (kXLines + 7) / 8;
-  static constexpr int kXBytes = kXLoads * 1024;  // of a group
-  static constexpr int kLoads = kXLoads + 2 + 2 * int(kGroup);  // (two more for each scale where they are read one by one)
+  static constexpr int kWLoads = 2 * int(kGroup);
+  static constexpr int kWBytes = HELD ? 0 : kWLoads * 1024, kBytes = kWBytes + kXLoads * 1024;  // of a group, in LDS
+  static constexpr int kLoads = kXLoads + 2 + kWLoads;  // (two more for each scale where they are read one by one)
 
   __amdgpu_buffer_rsrc_t wq, ws, xq, xs;
-  uint32_t w_off;  // this lane's row
+  uint32_t w_off[2];  // HELD: this lane's row; else the two that it brings
   uint32_t ldx, xs_off, M, K, steps;
-  uint8_t* lds;  // two groups' codes
+  uint8_t* lds;
 
   struct Slot {
-    u32x4 w[kGroup][2];
+    u32x4 w[HELD ? kGroup : 1][2];
     uint32_t sw, sx;
   };
+
+  __device__ __forceinline__ Walk(const F8DecodeArgs& a, const F8Weight& w, uint32_t n0, uint8_t* lds_) {
+    const uint32_t lane = threadIdx.x & 63, r = lane & 15, rows = min(uint32_t(a.N) - n0, 16u);
+    K = uint32_t(a.K);
+    M = uint32_t(a.M);
+    steps = a.steps;
+    ldx = uint32_t(a.ldx);
+    lds = lds_;
+    xq = make_rsrc(a.x, (M - 1) * ldx + K);
+    xs = make_rsrc(a.x_scales, (M - 1) * uint32_t(a.ldxs) + steps);
+    xs_off = min(r, M - 1) * uint32_t(a.ldxs);
+    wq = make_rsrc(w.codes + int64_t(n0) * w.ld, (rows - 1) * uint32_t(w.ld) + K);
+    ws = make_rsrc(w.scales + n0 / kF8Group * w.lds, steps);
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t row = HELD ? r : 8 * h + (lane >> 3);
+      w_off[h] = row < rows ? row * uint32_t(w.ld) : kOutside / 2;  // rows behind the last read as zeros
+    }
+  }
 
   // Four scales from step on, as a word; those behind the end are zeros (a NaN there would reach the sums).
   __device__ __forceinline__ uint32_t scales(__amdgpu_buffer_rsrc_t q, uint32_t off, uint32_t step) const {
@@ -49,33 +74,44 @@ struct Walk {
   }
 
   __device__ __forceinline__ void load(Slot& s, uint32_t group, int parity) const {
-    const int lane = threadIdx.x & 63, g = lane >> 4;
-    const uint32_t step = group * kGroup;
+    const uint32_t lane = threadIdx.x & 63, step = group * kGroup;
+    uint8_t* const to = lds + parity * kBytes;
 #pragma unroll
     for (int i = 0; i < kXLoads; ++i) {
       const uint32_t line = 8 * i + (lane >> 3), m = line % XR;
       const uint32_t k = (step + line / XR) * kF8Group + 16 * ((lane & 7) ^ (m & 7));
-      load_lds16_cached(xq, lds + parity * kXBytes + 1024 * i, line < kXLines && m < M && k < K ? m * ldx + k : kOutside, 0);
+      load_lds16_cached(xq, to + kWBytes + 1024 * i, line < kXLines && m < M && k < K ? m * ldx + k : kOutside, 0);
     }
     s.sx = scales(xs, xs_off, step);
     s.sw = scales(ws, 0, step);
 #pragma unroll
-    for (uint32_t j = 0; j < kGroup; ++j) {
-      const uint32_t k = (step + j) * kF8Group + 16 * g;
-      s.w[j][0] = buf_load16(wq, k < K ? w_off + k : kOutside, 0);
-      s.w[j][1] = buf_load16(wq, k + 64 < K ? w_off + k + 64 : kOutside, 0);
+    for (int i = 0; i < kWLoads; ++i) {
+      if constexpr (HELD) {  // half the columns of a step for each row
+        const uint32_t k = (step + i / 2) * kF8Group + 64 * (i & 1) + 16 * (lane >> 4);
+        s.w[i / 2][i & 1] = buf_load16(wq, k < K ? w_off[0] + k : kOutside, 0);
+      } else {  // a step for eight rows
+        const uint32_t k = (step + i / 2) * kF8Group + 16 * ((lane & 7) ^ (lane >> 3));
+        load_lds16(wq, to + 1024 * i, k < K ? w_off[i & 1] + k : kOutside, 0);
+      }
     }
   }
 
   __device__ __forceinline__ void multiply(const Slot& s, int parity, f32x4& acc) const {
-    const int lane = threadIdx.x & 63, g = lane >> 4, m = (lane & 15) % XR;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, m = r % XR;
+    const uint8_t* const from = lds + parity * kBytes;
+    auto operand = [&](const uint8_t* line, int swizzle) {
+      const u32x4 lo = *reinterpret_cast<const u32x4*>(line + 16 * (g ^ swizzle));
+      const u32x4 hi = *reinterpret_cast<const u32x4*>(line + 16 * ((g + 4) ^ swizzle));
+      return __builtin_bit_cast(i32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
     auto one = [&](auto step) {
       constexpr int J = decltype(step)::value;
-      const uint8_t* at = lds + parity * kXBytes + (J * XR + m) * kF8Group;
-      const u32x4 lo = *reinterpret_cast<const u32x4*>(at + 16 * (g ^ (m & 7)));
-      const u32x4 hi = *reinterpret_cast<const u32x4*>(at + 16 * ((g + 4) ^ (m & 7)));
-      const i32x8 x = __builtin_bit_cast(i32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      const i32x8 w = __builtin_bit_cast(i32x8, __builtin_shufflevector(s.w[J][0], s.w[J][1], 0, 1, 2, 3, 4, 5, 6, 7));
+      const i32x8 x = operand(from + kWBytes + (J * XR + m) * kF8Group, m & 7);
+      i32x8 w;
+      if constexpr (HELD)
+        w = __builtin_bit_cast(i32x8, __builtin_shufflevector(s.w[J][0], s.w[J][1], 0, 1, 2, 3, 4, 5, 6, 7));
+      else
+        w = operand(from + (J * 16 + r) * kF8Group, r & 7);
       acc = mfma_f8<J, J>(w, x, acc, s.sw, s.sx);
     };
     one(std::integral_constant<int, 0>{});
@@ -95,7 +131,7 @@ struct Walk {
       if (group + stride < end) {
         load(slot[1 - P], group + stride, 1 - P);
         __builtin_amdgcn_sched_barrier(0);
-        wait_vmcnt<kLoads>();  // all but those of the next group
+        wait_vmcnt<kLoads>();  // all but those of the next group, which are as many at least
       } else {
         wait_vmcnt<0>();
       }
@@ -111,41 +147,29 @@ struct Walk {
 };
 
 // y of 16 features and M <= XR tokens. With a second weight the workgroups behind `tiles` take that one, and their rows of y come
-// behind the first one's.
-template <int XR, int WAVES, class Out>
-__global__ void __launch_bounds__(64 * WAVES) decode_kernel(const F8DecodeArgs a) {
-  using W = Walk<XR>;
-  __shared__ __align__(1024) uint8_t codes[WAVES][2 * W::kXBytes];
-  __shared__ __align__(16) float sums[WAVES][64][4];
+// behind the first one's. LDS: `buffers` groups of each wave (two where a wave has more than one).
+template <int XR, bool HELD, int WAVES, class Out>
+__global__ void __launch_bounds__(64 * WAVES) decode_kernel(const F8DecodeArgs a, int buffers) {
+  using W = Walk<XR, HELD>;
+  static_assert(W::kBytes >= 1024, "room for a wave's sums");
+  extern __shared__ __align__(1024) uint8_t lds[];
   const int lane = threadIdx.x & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t r = lane & 15, g = lane >> 4;
+  const uint32_t r = lane & 15, g = lane >> 4, M = uint32_t(a.M);
   const bool second = blockIdx.x >= a.tiles;
-  const F8Weight w = second ? a.w[1] : a.w[0];
   const uint32_t n0 = (second ? blockIdx.x - a.tiles : blockIdx.x) * 16;
-  const uint32_t rows_n = min(uint32_t(a.N) - n0, 16u), M = uint32_t(a.M);
+  uint8_t* const own = lds + wave * uint32_t(buffers * W::kBytes);
 
-  W walk;
-  walk.K = uint32_t(a.K);
-  walk.M = M;
-  walk.steps = a.steps;
-  walk.ldx = uint32_t(a.ldx);
-  walk.xq = make_rsrc(a.x, (M - 1) * walk.ldx + walk.K);
-  walk.xs = make_rsrc(a.x_scales, (M - 1) * uint32_t(a.ldxs) + a.steps);
-  walk.xs_off = min(r, M - 1) * uint32_t(a.ldxs);
-  walk.lds = codes[wave];
-  walk.wq = make_rsrc(w.codes + int64_t(n0) * w.ld, (rows_n - 1) * uint32_t(w.ld) + walk.K);
-  walk.ws = make_rsrc(w.scales + n0 / kF8Group * w.lds, a.steps);
-  walk.w_off = r < rows_n ? r * uint32_t(w.ld) : kOutside / 2;  // rows behind the last read as zeros
+  const W walk(a, second ? a.w[1] : a.w[0], n0, own);
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   walk.run(wave, WAVES, (a.steps + kGroup - 1) / kGroup, acc);
 
-  *reinterpret_cast<f32x4*>(sums[wave][lane]) = acc;
+  *reinterpret_cast<f32x4*>(own + 16 * lane) = acc;  // nothing is on its way there any more
   __syncthreads();
   if (wave != 0 || r >= M) return;
 #pragma unroll
   for (int i = 1; i < WAVES; ++i) {
-    const f32x4 p = *reinterpret_cast<const f32x4*>(sums[i][lane]);
+    const f32x4 p = *reinterpret_cast<const f32x4*>(lds + i * buffers * W::kBytes + 16 * lane);
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] += p[e];
   }
@@ -181,24 +205,29 @@ __global__ void __launch_bounds__(256) join_kernel(const F8JoinArgs a) {
     if (n + e < a.N) y[n + e] = Out::store(bias ? v[e] + Out::load(bias[n + e]) : v[e]);
 }
 
-template <int XR, int WAVES>
-hipError_t launch(const F8DecodeArgs& a, int out_dtype, hipStream_t stream) {
-  const dim3 grid(a.tiles * (a.w[1].codes ? 2 : 1)), block(64 * WAVES);
-  if (out_dtype == kDtF32)
-    hipLaunchKernelGGL((decode_kernel<XR, WAVES, ActF32>), grid, block, 0, stream, a);
-  else if (out_dtype == kDtF16)
-    hipLaunchKernelGGL((decode_kernel<XR, WAVES, ActF16>), grid, block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((decode_kernel<XR, WAVES, ActBf16>), grid, block, 0, stream, a);
+template <int XR, bool HELD, int WAVES, class Out>
+hipError_t launch_out(const F8DecodeArgs& a, hipStream_t stream) {
+  auto* kernel = decode_kernel<XR, HELD, WAVES, Out>;
+  const int buffers = a.steps > kGroup * WAVES ? 2 : 1, bytes = WAVES * buffers * Walk<XR, HELD>::kBytes;
+  static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  if (ready != hipSuccess) return ready;
+  hipLaunchKernelGGL(kernel, dim3(a.tiles * (a.w[1].codes ? 2 : 1)), dim3(64 * WAVES), bytes, stream, a, buffers);
   return hipGetLastError();
 }
 
-template <int WAVES>
+template <int XR, bool HELD, int WAVES>
+hipError_t launch(const F8DecodeArgs& a, int out_dtype, hipStream_t stream) {
+  if (out_dtype == kDtF32) return launch_out<XR, HELD, WAVES, ActF32>(a, stream);
+  if (out_dtype == kDtF16) return launch_out<XR, HELD, WAVES, ActF16>(a, stream);
+  return launch_out<XR, HELD, WAVES, ActBf16>(a, stream);
+}
+
+template <int XR>
 hipError_t launch_rows(const F8DecodeArgs& a, int out_dtype, hipStream_t stream) {
-  if (a.M == 1) return launch<1, WAVES>(a, out_dtype, stream);
-  if (a.M <= 4) return launch<4, WAVES>(a, out_dtype, stream);
-  if (a.M <= 8) return launch<8, WAVES>(a, out_dtype, stream);
-  return launch<16, WAVES>(a, out_dtype, stream);
+  if constexpr (XR > 4) {
+    if (a.tiles * (a.w[1].codes ? 2 : 1) >= 640) return launch<XR, true, 8>(a, out_dtype, stream);
+  }
+  return a.steps > 16 && a.steps <= 32 ? launch<XR, false, 8>(a, out_dtype, stream) : launch<XR, false, 4>(a, out_dtype, stream);
 }
 
 }  // namespace
@@ -215,8 +244,10 @@ hipError_t launch_f8_join(const F8JoinArgs& a, int out_dtype, hipStream_t stream
 hipError_t launch_f8_decode(F8DecodeArgs a, int out_dtype, hipStream_t stream) {
   a.steps = uint32_t((a.K + kF8Group - 1) / kF8Group);
   a.tiles = uint32_t((a.N + 15) / 16);
-  const uint32_t count = a.tiles * (a.w[1].codes ? 2 : 1);
-  return count >= 512 ? launch_rows<4>(a, out_dtype, stream) : launch_rows<8>(a, out_dtype, stream);
+  if (a.M == 1) return launch_rows<1>(a, out_dtype, stream);
+  if (a.M <= 4) return launch_rows<4>(a, out_dtype, stream);
+  if (a.M <= 8) return launch_rows<8>(a, out_dtype, stream);
+  return launch_rows<16>(a, out_dtype, stream);
 }
 
 }  // namespace llmopt
