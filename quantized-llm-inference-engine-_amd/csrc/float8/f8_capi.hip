@@ -81,9 +81,9 @@ struct Tile {
   double alone, full, round;
 };
 constexpr Tile kTiles[] = {
-    {F8Shape::k256x256, 256, 256, 1, 1.38, 1.70, 5.0}, {F8Shape::k256x128, 256, 128, 1, 0.83, 1.05, 4.0},
-    {F8Shape::k256x64, 256, 64, 1, 0.75, 0.71, 3.0},   {F8Shape::k128x128, 128, 128, 2, 0.94, 1.10, 3.5},
-    {F8Shape::k128x64, 128, 64, 2, 0.53, 0.71, 3.0},
+    {F8Shape::k256x256, 256, 256, 1, 1.38, 1.62, 5.0}, {F8Shape::k256x128, 256, 128, 1, 0.83, 0.98, 4.0},
+    {F8Shape::k256x64, 256, 64, 1, 0.75, 0.64, 3.0},   {F8Shape::k128x128, 128, 128, 2, 0.94, 1.07, 3.5},
+    {F8Shape::k128x64, 128, 64, 2, 0.53, 0.69, 3.0},
 };
 
 struct Plan {

@@ -104,7 +104,7 @@ hipError_t launch_f8_quantize(const F8QuantArgs& a, int dtype, int64_t block_row
 hipError_t launch_f8_rmsnorm(const F8NormArgs& a, int dtype, hipStream_t stream);
 hipError_t launch_f8_act(const F8ActArgs& a, hipStream_t stream);
 hipError_t launch_f8_tiles(const F8TilesArgs& a, F8Shape shape, int out_dtype, hipStream_t stream);
-// The sum of `splits` parts [M, ld_parts] in their order, plus the bias, rounded into y.
+// The sum of `splits` (2, 4 or 8) parts [M, ld_parts] in their order, plus the bias, rounded into y.
 struct F8JoinArgs {
   const float* parts;
   uint32_t splits;

@@ -1,9 +1,9 @@
 // The products of up to 16 tokens: bound by the weight's bytes.
 //
 // A workgroup takes 16 features, and its waves the steps of 128 columns in turn, four at a time; their sums are added in LDS
-// in a fixed order. What bounds it next to the memory is the rate of a CU's load instructions, 20 ns or so for each that brings a
-// kilobyte (25 bytes a cycle; measured): so codes come as whole lines straight into LDS of the wave's own (loaded into the matrix
-// core's operands, a line of one token would be asked for 16 times), and scales four at a time.
+// in a fixed order. What bounds it next to the memory is a CU's load instructions: one of eight whole lines takes it 8 ns, one
+// of 16 half lines 15 (measured on cached data). So codes come as whole lines straight into LDS of the wave's own (loaded into the
+// matrix core's operands, a line of one token would be asked for 16 times), and scales four at a time.
 //
 // Measured (MI355X, in a graph, weights from memory, us; 1 / 4 / 8 / 16 tokens):
 //   6144 x 4096 7.2 / 7.4 / 9.1 / 10.0, 4096 x 14336 11.6 / 11.9 / 12.0 / 13.0 (5.0 TB/s), 28672 x 4096 22.3 / 22.7 / 26.1 / 28.9
@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(64 * WAVES) decode_kernel(const F8DecodeArgs a
     if (n + e < a.N) y[n + e] = Out::store(bias ? acc[e] + Out::load(bias[n + e]) : acc[e]);
 }
 
-// The splits' parts, added in their order, plus the bias. Four features a thread.
-template <class Out>
+// The splits' parts, added in their order, plus the bias. Four features a thread, all their parts on their way at once.
+template <int SPLITS, class Out>
 __global__ void __launch_bounds__(256) join_kernel(const F8JoinArgs a) {
   using Raw = typename Out::raw;
   const uint32_t per_row = uint32_t(a.ld_parts / 4);
@@ -192,17 +192,31 @@ __global__ void __launch_bounds__(256) join_kernel(const F8JoinArgs a) {
   if (m >= a.M) return;
   const float* p = a.parts + int64_t(m) * a.ld_parts + n;
   const int64_t plane = a.M * a.ld_parts;
-  f32x4 v = *reinterpret_cast<const f32x4*>(p);
-  for (uint32_t s = 1; s < a.splits; ++s) {
-    const f32x4 q = *reinterpret_cast<const f32x4*>(p + s * plane);
+  f32x4 part[SPLITS];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += q[e];
-  }
+  for (int s = 0; s < SPLITS; ++s) part[s] = *reinterpret_cast<const f32x4*>(p + s * plane);
+  f32x4 v = part[0];
+#pragma unroll
+  for (int s = 1; s < SPLITS; ++s)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += part[s][e];
   Raw* y = static_cast<Raw*>(a.y) + m * a.ldy;
   const Raw* bias = static_cast<const Raw*>(a.bias);
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (n + e < a.N) y[n + e] = Out::store(bias ? v[e] + Out::load(bias[n + e]) : v[e]);
+}
+
+template <class Out>
+hipError_t launch_join(const F8JoinArgs& a, hipStream_t stream) {
+  const dim3 grid(uint32_t((a.M * (a.ld_parts / 4) + 255) / 256));
+  switch (a.splits) {
+    case 2: hipLaunchKernelGGL((join_kernel<2, Out>), grid, dim3(256), 0, stream, a); break;
+    case 4: hipLaunchKernelGGL((join_kernel<4, Out>), grid, dim3(256), 0, stream, a); break;
+    case 8: hipLaunchKernelGGL((join_kernel<8, Out>), grid, dim3(256), 0, stream, a); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
 }
 
 template <int XR, bool HELD, int WAVES, class Out>
@@ -233,12 +247,7 @@ hipError_t launch_rows(const F8DecodeArgs& a, int out_dtype, hipStream_t stream)
 }  // namespace
 
 hipError_t launch_f8_join(const F8JoinArgs& a, int out_dtype, hipStream_t stream) {
-  const dim3 grid(uint32_t((a.M * (a.ld_parts / 4) + 255) / 256));
-  if (out_dtype == kDtF16)
-    hipLaunchKernelGGL(join_kernel<ActF16>, grid, dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL(join_kernel<ActBf16>, grid, dim3(256), 0, stream, a);
-  return hipGetLastError();
+  return out_dtype == kDtF16 ? launch_join<ActF16>(a, stream) : launch_join<ActBf16>(a, stream);
 }
 
 hipError_t launch_f8_decode(F8DecodeArgs a, int out_dtype, hipStream_t stream) {
