@@ -29,6 +29,5 @@ def test_no_spills_in_loops(tmp_path, source):
         products = [i for i, line in enumerate(lines) if "v_mfma" in line]
         inside = lines[products[0] : products[-1]] if products else []
         assert not any("scratch_" in line for line in inside), f"scratch accesses between the products of {name}"
-    if source != "f8_tiles.hip":  # (whose outer loop, over tiles, may hold a row of scales there)
-        bad = {k: n for k, v in kernels.items() if (n := _scratch_in_loops(v))}
-        assert not bad, f"scratch accesses inside loops: {bad}"
+    bad = {k: n for k, v in kernels.items() if (n := _scratch_in_loops(v))}
+    assert not bad, f"scratch accesses inside loops: {bad}"
