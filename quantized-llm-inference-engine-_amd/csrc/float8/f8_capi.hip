@@ -59,14 +59,18 @@ bool tiled_rows(const void* p, int64_t ld, int64_t cols, int64_t ld_scales = 0) 
 }
 
 // Workgroups of a grid of `a` x `b`.
-int check_grid(int64_t a, int64_t b) {
-  if (a > 0 && b > kMaxInt / a) return fail(LLMOPT_ERR_UNSUPPORTED, "%lld x %lld workgroups are too many", (long long)a, (long long)b);
+int check_grid(int64_t a, int64_t b, int64_t most = kMaxInt) {
+  if (a > 0 && b > most / a) return fail(LLMOPT_ERR_UNSUPPORTED, "%lld x %lld workgroups are too many", (long long)a, (long long)b);
   return LLMOPT_OK;
 }
 
+// Workgroups of 256 threads of the kernels for any rows: work-items are counted in 32 bits. (Outputs of 2^34.)
+constexpr int64_t kMostAny = (int64_t(1) << 24) - 1;
+
 // ---- the choice of kernels --------------------------------------------------------------------------
 
-constexpr int64_t kFewTokens = 16;  // what the decode kernel takes
+constexpr int64_t kFewTokens = 16;  // that the decode kernel takes of any weight
+constexpr int64_t kSomeTokens = 1024;  // that it takes at most, 32 at a time
 
 // A tile's shape and the parts of K: the least of an estimate of the time. A workgroup's step of 128 columns takes `alone`
 // us where few workgroups run and `full` where every CU has its share; a round of workgroups (256 of them, or 512 where two
@@ -81,39 +85,55 @@ struct Tile {
   double alone, full, round;
 };
 constexpr Tile kTiles[] = {
-    {F8Shape::k256x256, 256, 256, 1, 1.38, 1.62, 5.0}, {F8Shape::k256x128, 256, 128, 1, 0.83, 0.98, 4.0},
-    {F8Shape::k256x64, 256, 64, 1, 0.75, 0.64, 3.0},   {F8Shape::k128x128, 128, 128, 2, 0.94, 1.07, 3.5},
-    {F8Shape::k128x64, 128, 64, 2, 0.53, 0.69, 3.0},
+    {F8Shape::k256x256, 256, 256, 1, 1.38, 1.62, 5.0}, {F8Shape::k256x128, 256, 128, 1, 0.78, 0.93, 4.0},
+    {F8Shape::k256x64, 256, 64, 1, 0.75, 0.72, 3.0},   {F8Shape::k128x128, 128, 128, 2, 0.94, 1.07, 3.5},
+    {F8Shape::k128x64, 128, 64, 2, 0.50, 0.76, 3.0},
 };
 
 struct Plan {
   F8Shape shape;
   int64_t splits, steps_per_split;
+  bool few;  // the decode kernel instead (gated: with the sums in the workspace)
 };
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int64_t padded(int64_t n) { return up(n, 16) * 16; }
 
+size_t sums_bytes(int64_t M, int64_t N) { return size_t(2) * size_t(M) * size_t(padded(N)) * sizeof(float); }
+
+// The decode kernel's time over tiles of 32 tokens, and the gated product's second launch. One workgroup fits a CU, two where a
+// row has at most 16 steps.
+double decode_us(int64_t M, int64_t N, int64_t steps, bool gated) {
+  const int64_t count = up(N, 16) * (gated ? 2 : 1) * up(M, 32), held = steps > 16 ? 256 : 512;
+  const double load = std::min(1.0, double(count) / double(held));
+  const double step = 0.04 + (steps > 16 ? 0.06 : 0.13) * load + 0.05 * double(std::min<int64_t>(M, 32)) / 32.0;
+  return 2.0 + double(up(count, held)) * (1.0 + double(steps) * step) + (gated ? 2.0 + double(M) * double(N) * 9.0 / 4e6 : 0.0);
+}
+
 size_t parts_bytes(int64_t M, int64_t N, int64_t splits) {
   return splits > 1 ? size_t(splits) * size_t(M) * size_t(padded(N)) * sizeof(float) : 0;
 }
 
 Plan plan_tiles(int64_t M, int64_t N, int64_t K, bool gated, size_t workspace) {
-  Plan best{F8Shape::k256x256, 1, 1};
+  Plan best{F8Shape::k256x256, 1, 1, false};
   double least = 1e30;
   const int64_t steps = std::max<int64_t>(1, groups(K));
+  const bool room = !gated || workspace >= sums_bytes(M, N);
+  if (room && M <= kFewTokens) return Plan{F8Shape::k256x256, 1, steps, true};
+  if (room && M <= kSomeTokens) least = decode_us(M, N, steps, gated), best.few = true;
   for (const Tile& t : kTiles) {
     if (gated && t.n != 256) continue;  // a group of 128 features of both weights
     const int64_t tiles = up(N, gated ? t.n / 2 : t.n) * up(M, t.m);
-    for (int64_t splits = 1; splits <= (gated ? 1 : 8); splits *= 2) {
+    const int64_t most = gated || t.m == 256 ? 1 : 8;  // (with tiles this large there are smaller ones in fewer parts)
+    for (int64_t splits = 1; splits <= most; splits *= 2) {
       const int64_t per = up(steps, splits);
       if (splits > 1 && (per < 4 || up(steps, per) != splits || parts_bytes(M, N, splits) > workspace)) break;
       const int64_t count = tiles * splits, rounds = up(count, 256 * t.per_cu);
-      const double load = std::min(1.0, double(count) / (256.0 * double(t.per_cu)));
+      const double load = std::clamp(double(count) / 256.0 - double(t.per_cu - 1), 0.0, 1.0);
       double us = double(rounds) * (double(per) * (t.alone + (t.full - t.alone) * load) + t.round) + 2.0;
-      if (splits > 1) us += 3.0 + double(M) * double(N) * 8.0 * double(splits) / 2.7e6;
-      if (us < least) least = us, best = Plan{t.shape, splits, per};
+      if (splits > 1) us += 3.0 + double(M) * double(N) * 8.0 * double(splits) / 3e6;
+      if (us < least) least = us, best = Plan{t.shape, splits, per, false};
     }
   }
   return best;
@@ -161,9 +181,9 @@ int llmopt_f8_rmsnorm(const void* x, int64_t ldx, const void* residual, int64_t 
 }
 
 size_t llmopt_f8_linear_workspace(int64_t M, int64_t N, int64_t K) {
-  if (M <= kFewTokens || N < 1 || K < 1 || M > kMaxInt || N > kMaxInt || K > kMaxInt) return 0;
+  if (M < 1 || N < 1 || K < 1 || M > kMaxInt || N > kMaxInt || K > kMaxInt) return 0;
   const Plan plan = plan_tiles(M, N, K, false, SIZE_MAX);
-  return parts_bytes(M, N, plan.splits);
+  return plan.few ? 0 : parts_bytes(M, N, plan.splits);
 }
 
 int llmopt_f8_linear(const void* x, int64_t ldx, const void* x_scales, int64_t ldxs, int64_t M, int64_t K,
@@ -189,12 +209,15 @@ int llmopt_f8_linear(const void* x, int64_t ldx, const void* x_scales, int64_t l
   t.ldy = ldy;
   t.M = M, t.N = N, t.K = K;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (!tiled_rows(x, ldx, K, ldxs) || !tiled_rows(w, ldw, K)) return hip_status(launch_f8_any(t, out_dtype, st), "llmopt_f8_linear");
-  if (M <= kFewTokens) {
+  if (!tiled_rows(x, ldx, K, ldxs) || !tiled_rows(w, ldw, K)) {
+    CHECK(check_grid(up(M, 16), up(N, 64), kMostAny));
+    return hip_status(launch_f8_any(t, out_dtype, st), "llmopt_f8_linear");
+  }
+  const Plan plan = plan_tiles(M, N, K, false, workspace && aligned(workspace, 16) ? workspace_bytes : 0);
+  if (plan.few) {
     const F8DecodeArgs d{t.x, ldx, t.x_scales, ldxs, {t.w[0], {}}, bias, y, ldy, M, N, K, 0, 0};
     return hip_status(launch_f8_decode(d, out_dtype, st), "llmopt_f8_linear");
   }
-  const Plan plan = plan_tiles(M, N, K, false, workspace && aligned(workspace, 16) ? workspace_bytes : 0);
   t.vec = aligned(y, 16) && ldy % 8 == 0;
   t.splits = uint32_t(plan.splits);
   t.steps_per_split = uint32_t(plan.steps_per_split);
@@ -204,7 +227,8 @@ int llmopt_f8_linear(const void* x, int64_t ldx, const void* x_scales, int64_t l
 }
 
 size_t llmopt_f8_swiglu_workspace(int64_t M, int64_t N, int64_t K) {
-  return M > 0 && M <= kFewTokens && N > 0 && K > 0 ? size_t(2) * size_t(M) * size_t(padded(N)) * sizeof(float) : 0;
+  if (M < 1 || N < 1 || K < 1 || M > kMaxInt || N > kMaxInt || K > kMaxInt) return 0;
+  return plan_tiles(M, N, K, true, SIZE_MAX).few ? sums_bytes(M, N) : 0;
 }
 
 int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t ldxs, int64_t M, int64_t K,
@@ -236,9 +260,12 @@ int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t l
   const hipStream_t st = static_cast<hipStream_t>(stream);
   // Without columns a weight has no codes to point to.
   if (K == 0) t.w[0].codes = t.w[1].codes = static_cast<const uint8_t*>(codes);
-  if (!tiled_rows(x, ldx, K, ldxs) || !tiled_rows(gate, ldg, K) || !tiled_rows(up_, ldu, K))
+  if (!tiled_rows(x, ldx, K, ldxs) || !tiled_rows(gate, ldg, K) || !tiled_rows(up_, ldu, K)) {
+    CHECK(check_grid(up(M, 16), up(N, 64), kMostAny));
     return hip_status(launch_f8_any(t, 0, st), "llmopt_f8_swiglu");
-  if (workspace && aligned(workspace, 16) && M <= kFewTokens && workspace_bytes >= llmopt_f8_swiglu_workspace(M, N, K)) {
+  }
+  const Plan plan = plan_tiles(M, N, K, true, workspace && aligned(workspace, 16) ? workspace_bytes : 0);
+  if (plan.few) {
     float* sums = static_cast<float*>(workspace);
     const int64_t ld = padded(N);
     const F8DecodeArgs d{t.x, ldx, t.x_scales, ldxs, {t.w[0], t.w[1]}, nullptr, sums, ld, M, N, K, 0, 0};
@@ -246,7 +273,6 @@ int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t l
     const F8ActArgs act{sums, sums + M * ld, ld, t.codes, ldc, t.scales, lds, M, N};
     return hip_status(launch_f8_act(act, st), "llmopt_f8_swiglu");
   }
-  const Plan plan = plan_tiles(M, N, K, true, 0);
   t.vec = aligned(codes, 16) && ldc % 16 == 0;
   t.splits = 1;
   return hip_status(launch_f8_tiles(t, plan.shape, 0, st), "llmopt_f8_swiglu");

@@ -31,29 +31,32 @@ template <int XR, bool HELD>
 struct Walk {
   static constexpr int kXLines = kGroup * XR, kXLoads = (kXLines + 7) / 8;
   static constexpr int kWLoads = 2 * int(kGroup);
+  static constexpr int kTiles = XR > 16 ? XR / 16 : 1;  // of 16 tokens
   static constexpr int kWBytes = HELD ? 0 : kWLoads * 1024, kBytes = kWBytes + kXLoads * 1024;  // of a group, in LDS
-  static constexpr int kLoads = kXLoads + 2 + kWLoads;  // (two more for each scale where they are read one by one)
+  static constexpr int kLoads = kXLoads + kTiles + 1 + kWLoads;  // (two more for each scale where they are read one by one)
 
   __amdgpu_buffer_rsrc_t wq, ws, xq, xs;
   uint32_t w_off[2];  // HELD: this lane's row; else the two that it brings
-  uint32_t ldx, xs_off, M, K, steps;
+  uint32_t xs_off[kTiles], ldx, M, K, steps;
   uint8_t* lds;
 
   struct Slot {
     u32x4 w[HELD ? kGroup : 1][2];
-    uint32_t sw, sx;
+    uint32_t sw, sx[kTiles];
   };
 
-  __device__ __forceinline__ Walk(const F8DecodeArgs& a, const F8Weight& w, uint32_t n0, uint8_t* lds_) {
+  // Of weight rows from n0 on and the M <= XR tokens from m0 on.
+  __device__ __forceinline__ Walk(const F8DecodeArgs& a, const F8Weight& w, uint32_t n0, uint32_t m0, uint8_t* lds_) {
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, rows = min(uint32_t(a.N) - n0, 16u);
     K = uint32_t(a.K);
-    M = uint32_t(a.M);
+    M = min(uint32_t(a.M) - m0, uint32_t(XR));
     steps = a.steps;
     ldx = uint32_t(a.ldx);
     lds = lds_;
-    xq = make_rsrc(a.x, (M - 1) * ldx + K);
-    xs = make_rsrc(a.x_scales, (M - 1) * uint32_t(a.ldxs) + steps);
-    xs_off = min(r, M - 1) * uint32_t(a.ldxs);
+    xq = make_rsrc(a.x + int64_t(m0) * a.ldx, (M - 1) * ldx + K);
+    xs = make_rsrc(a.x_scales + int64_t(m0) * a.ldxs, (M - 1) * uint32_t(a.ldxs) + steps);
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) xs_off[t] = min(16 * t + r, M - 1) * uint32_t(a.ldxs);
     wq = make_rsrc(w.codes + int64_t(n0) * w.ld, (rows - 1) * uint32_t(w.ld) + K);
     ws = make_rsrc(w.scales + n0 / kF8Group * w.lds, steps);
 #pragma unroll
@@ -82,7 +85,8 @@ struct Walk {
       const uint32_t k = (step + line / XR) * kF8Group + 16 * ((lane & 7) ^ (m & 7));
       load_lds16_cached(xq, to + kWBytes + 1024 * i, line < kXLines && m < M && k < K ? m * ldx + k : kOutside, 0);
     }
-    s.sx = scales(xs, xs_off, step);
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) s.sx[t] = scales(xs, xs_off[t], step);
     s.sw = scales(ws, 0, step);
 #pragma unroll
     for (int i = 0; i < kWLoads; ++i) {
@@ -96,8 +100,8 @@ struct Walk {
     }
   }
 
-  __device__ __forceinline__ void multiply(const Slot& s, int parity, f32x4& acc) const {
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, m = r % XR;
+  __device__ __forceinline__ void multiply(const Slot& s, int parity, f32x4 (&acc)[kTiles]) const {
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const uint8_t* const from = lds + parity * kBytes;
     auto operand = [&](const uint8_t* line, int swizzle) {
       const u32x4 lo = *reinterpret_cast<const u32x4*>(line + 16 * (g ^ swizzle));
@@ -106,13 +110,16 @@ struct Walk {
     };
     auto one = [&](auto step) {
       constexpr int J = decltype(step)::value;
-      const i32x8 x = operand(from + kWBytes + (J * XR + m) * kF8Group, m & 7);
       i32x8 w;
       if constexpr (HELD)
         w = __builtin_bit_cast(i32x8, __builtin_shufflevector(s.w[J][0], s.w[J][1], 0, 1, 2, 3, 4, 5, 6, 7));
       else
         w = operand(from + (J * 16 + r) * kF8Group, r & 7);
-      acc = mfma_f8<J, J>(w, x, acc, s.sw, s.sx);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        const int m = 16 * t + r % XR;
+        acc[t] = mfma_f8<J, J>(w, operand(from + kWBytes + (J * XR + m) * kF8Group, m & 7), acc[t], s.sw, s.sx[t]);
+      }
     };
     one(std::integral_constant<int, 0>{});
     one(std::integral_constant<int, 1>{});
@@ -121,7 +128,7 @@ struct Walk {
   }
 
   // Groups first, first + stride, ... below end.
-  __device__ __forceinline__ void run(uint32_t first, uint32_t stride, uint32_t end, f32x4& acc) const {
+  __device__ __forceinline__ void run(uint32_t first, uint32_t stride, uint32_t end, f32x4 (&acc)[kTiles]) const {
     if (first >= end) return;
     Slot slot[2];
     load(slot[0], first, 0);
@@ -146,40 +153,45 @@ struct Walk {
   }
 };
 
-// y of 16 features and M <= XR tokens. With a second weight the workgroups behind `tiles` take that one, and their rows of y come
+// y of 16 features and at most XR tokens (blockIdx.y counts them). With a second weight the workgroups behind `tiles` take that one, and their rows of y come
 // behind the first one's. LDS: `buffers` groups of each wave (two where a wave has more than one).
 template <int XR, bool HELD, int WAVES, class Out>
 __global__ void __launch_bounds__(64 * WAVES) decode_kernel(const F8DecodeArgs a, int buffers) {
   using W = Walk<XR, HELD>;
-  static_assert(W::kBytes >= 1024, "room for a wave's sums");
+  static_assert(W::kBytes >= 1024 * W::kTiles, "room for a wave's sums");
   extern __shared__ __align__(1024) uint8_t lds[];
   const int lane = threadIdx.x & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t r = lane & 15, g = lane >> 4, M = uint32_t(a.M);
+  const uint32_t r = lane & 15, g = lane >> 4, m0 = blockIdx.y * XR;
   const bool second = blockIdx.x >= a.tiles;
   const uint32_t n0 = (second ? blockIdx.x - a.tiles : blockIdx.x) * 16;
   uint8_t* const own = lds + wave * uint32_t(buffers * W::kBytes);
 
-  const W walk(a, second ? a.w[1] : a.w[0], n0, own);
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  const W walk(a, second ? a.w[1] : a.w[0], n0, m0, own);
+  f32x4 acc[W::kTiles];
+#pragma unroll
+  for (int t = 0; t < W::kTiles; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   walk.run(wave, WAVES, (a.steps + kGroup - 1) / kGroup, acc);
 
-  *reinterpret_cast<f32x4*>(own + 16 * lane) = acc;  // nothing is on its way there any more
+#pragma unroll
+  for (int t = 0; t < W::kTiles; ++t) *reinterpret_cast<f32x4*>(own + 1024 * t + 16 * lane) = acc[t];  // nothing is on its way there any more
   __syncthreads();
-  if (wave != 0 || r >= M) return;
+  const int64_t m = m0 + 16 * wave + r;  // a wave for each 16 tokens
+  if (wave >= W::kTiles || (XR < 16 && r >= XR) || m >= a.M) return;
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int i = 1; i < WAVES; ++i) {
-    const f32x4 p = *reinterpret_cast<const f32x4*>(lds + i * buffers * W::kBytes + 16 * lane);
+  for (int i = 0; i < WAVES; ++i) {
+    const f32x4 p = *reinterpret_cast<const f32x4*>(lds + i * buffers * W::kBytes + 1024 * wave + 16 * lane);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += p[e];
+    for (int e = 0; e < 4; ++e) sum[e] += p[e];
   }
   const uint32_t n = n0 + 4 * g;
   using Raw = typename Out::raw;
-  Raw* y = static_cast<Raw*>(a.y) + (second ? M + r : r) * a.ldy;
+  Raw* y = static_cast<Raw*>(a.y) + (second ? a.M + m : m) * a.ldy;
   const Raw* bias = static_cast<const Raw*>(a.bias);
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (n + e < a.N) y[n + e] = Out::store(bias ? acc[e] + Out::load(bias[n + e]) : acc[e]);
+    if (n + e < a.N) y[n + e] = Out::store(bias ? sum[e] + Out::load(bias[n + e]) : sum[e]);
 }
 
 // The splits' parts, added in their order, plus the bias. Four features a thread, all their parts on their way at once.
@@ -225,7 +237,7 @@ hipError_t launch_out(const F8DecodeArgs& a, hipStream_t stream) {
   const int buffers = a.steps > kGroup * WAVES ? 2 : 1, bytes = WAVES * buffers * Walk<XR, HELD>::kBytes;
   static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
   if (ready != hipSuccess) return ready;
-  hipLaunchKernelGGL(kernel, dim3(a.tiles * (a.w[1].codes ? 2 : 1)), dim3(64 * WAVES), bytes, stream, a, buffers);
+  hipLaunchKernelGGL(kernel, dim3(a.tiles * (a.w[1].codes ? 2 : 1), uint32_t((a.M + XR - 1) / XR)), dim3(64 * WAVES), bytes, stream, a, buffers);
   return hipGetLastError();
 }
 
@@ -238,10 +250,15 @@ hipError_t launch(const F8DecodeArgs& a, int out_dtype, hipStream_t stream) {
 
 template <int XR>
 hipError_t launch_rows(const F8DecodeArgs& a, int out_dtype, hipStream_t stream) {
-  if constexpr (XR > 4) {
-    if (a.tiles * (a.w[1].codes ? 2 : 1) >= 640) return launch<XR, true, 8>(a, out_dtype, stream);
+  const bool one_group = a.steps > 16 && a.steps <= 32;  // of each of eight waves
+  if constexpr (XR > 16) {
+    return one_group ? launch<XR, true, 8>(a, out_dtype, stream) : launch<XR, true, 4>(a, out_dtype, stream);
+  } else {
+    if constexpr (XR > 4) {
+      if (a.tiles * (a.w[1].codes ? 2 : 1) >= 640) return launch<XR, true, 8>(a, out_dtype, stream);
+    }
+    return one_group ? launch<XR, false, 8>(a, out_dtype, stream) : launch<XR, false, 4>(a, out_dtype, stream);
   }
-  return a.steps > 16 && a.steps <= 32 ? launch<XR, false, 8>(a, out_dtype, stream) : launch<XR, false, 4>(a, out_dtype, stream);
 }
 
 }  // namespace
@@ -256,7 +273,8 @@ hipError_t launch_f8_decode(F8DecodeArgs a, int out_dtype, hipStream_t stream) {
   if (a.M == 1) return launch_rows<1>(a, out_dtype, stream);
   if (a.M <= 4) return launch_rows<4>(a, out_dtype, stream);
   if (a.M <= 8) return launch_rows<8>(a, out_dtype, stream);
-  return launch_rows<16>(a, out_dtype, stream);
+  if (a.M <= 16) return launch_rows<16>(a, out_dtype, stream);
+  return launch_rows<32>(a, out_dtype, stream);
 }
 
 }  // namespace llmopt

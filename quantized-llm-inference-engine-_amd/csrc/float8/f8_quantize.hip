@@ -165,10 +165,24 @@ __global__ void __launch_bounds__(kThreads) act_kernel(const F8ActArgs a, uint32
 
 }  // namespace
 
+// Work-items of a launch are counted in 32 bits.
+constexpr int64_t kMostGroups = (int64_t(1) << 32) / kThreads - 1;
+
 hipError_t launch_f8_quantize(const F8QuantArgs& a, int dtype, int64_t block_rows, hipStream_t stream) {
   if (a.rows == 0 || a.cols == 0) return hipSuccess;
   if (block_rows == 1) {
-    const int64_t chunks = (a.cols + kChunk - 1) / kChunk;
+    const int64_t chunks = (a.cols + kChunk - 1) / kChunk, most = kMostGroups / chunks;
+    if (a.rows > most) {  // in two calls
+      F8QuantArgs part = a;
+      part.rows = most;
+      const hipError_t err = launch_f8_quantize(part, dtype, 1, stream);
+      if (err != hipSuccess) return err;
+      part.x = static_cast<const uint8_t*>(a.x) + most * a.ldx * (dtype == kDtF32 ? 4 : 2);
+      part.codes += most * a.ldc;
+      part.scales += most * a.lds;
+      part.rows = a.rows - most;
+      return launch_f8_quantize(part, dtype, 1, stream);
+    }
     const dim3 grid(unsigned(a.rows * chunks));
     if (dtype == kDtF32)
       hipLaunchKernelGGL(quantize_rows_kernel<ActF32>, grid, dim3(kThreads), 0, stream, a, uint32_t(chunks));
@@ -205,6 +219,21 @@ static hipError_t launch_norm(const F8NormArgs& a, hipStream_t stream) {
 
 hipError_t launch_f8_rmsnorm(const F8NormArgs& a, int dtype, hipStream_t stream) {
   if (a.rows == 0 || a.hidden == 0) return hipSuccess;
+  if (a.rows > kMostGroups) {  // in two calls
+    F8NormArgs part = a;
+    part.rows = kMostGroups;
+    const hipError_t err = launch_f8_rmsnorm(part, dtype, stream);
+    if (err != hipSuccess) return err;
+    part.x = static_cast<const uint16_t*>(a.x) + kMostGroups * a.ldx;
+    if (a.residual) {
+      part.residual = static_cast<const uint16_t*>(a.residual) + kMostGroups * a.ldr;
+      part.h_out = static_cast<uint16_t*>(a.h_out) + kMostGroups * a.ldh;
+    }
+    part.codes += kMostGroups * a.ldc;
+    part.scales += kMostGroups * a.lds;
+    part.rows = a.rows - kMostGroups;
+    return launch_f8_rmsnorm(part, dtype, stream);
+  }
   return dtype == kDtF16 ? launch_norm<ActF16>(a, stream) : launch_norm<ActBf16>(a, stream);
 }
 

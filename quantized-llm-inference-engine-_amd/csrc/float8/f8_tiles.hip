@@ -443,10 +443,12 @@ hipError_t launch_shape(F8TilesArgs a, int out_dtype, hipStream_t stream) {
   a.tiles_n = uint32_t((a.N + wide - 1) / wide);
   a.tiles_m = uint32_t((a.M + kRowsM - 1) / kRowsM);
   a.steps = int((a.K + kStep - 1) / kStep);
-  if (a.splits > 1) {
-    const hipError_t err = launch<WN, WM, TM, STAGES, false, true, ActBf16>(a, stream);
-    if (err != hipSuccess) return err;
-    return launch_f8_join({a.parts, a.splits, a.M, a.N, a.ld_parts, a.bias, a.y, a.ldy}, out_dtype, stream);
+  if constexpr (kRowsM < 256) {
+    if (a.splits > 1) {
+      const hipError_t err = launch<WN, WM, TM, STAGES, false, true, ActBf16>(a, stream);
+      if (err != hipSuccess) return err;
+      return launch_f8_join({a.parts, a.splits, a.M, a.N, a.ld_parts, a.bias, a.y, a.ldy}, out_dtype, stream);
+    }
   }
   if constexpr (WN == 2) {
     if (gated) return launch<WN, WM, TM, STAGES, true, false, ActBf16>(a, stream);

@@ -383,7 +383,10 @@ def test_workspaces():
             for k in (16, 1040, 14336):
                 ws = lib.llmopt_f8_linear_workspace(m, n, k)
                 assert 0 <= ws <= 8 * m * (n + 15) * 4 and ws % (m * 64) == 0
-    assert lib.llmopt_f8_swiglu_workspace(17, 4096, 4096) == 0 and lib.llmopt_f8_swiglu_workspace(0, 8, 8) == 0
+    # the gated product's two sums where few tokens or features make that faster, and else none
+    assert lib.llmopt_f8_swiglu_workspace(17, 4096, 4096) == 2 * 17 * 4096 * 4
+    assert lib.llmopt_f8_swiglu_workspace(500, 4096, 4096) == 0 and lib.llmopt_f8_swiglu_workspace(0, 8, 8) == 0
+    assert lib.llmopt_f8_swiglu_workspace(1 << 40, 8, 8) == 0
     assert lib.llmopt_f8_swiglu_workspace(3, 50, 77) == 2 * 3 * 64 * 4
 
 

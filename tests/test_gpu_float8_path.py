@@ -225,18 +225,20 @@ def _call_linear(x, w, dtype, workspace):
     return y
 
 
-@pytest.mark.parametrize("m,n,k", [(17, 512, 4096), (100, 1024, 4096), (32, 300, 14336)])
+@pytest.mark.parametrize("m,n,k", [(17, 512, 4096), (100, 1024, 4096), (32, 300, 14336), (32, 4096, 14336), (100, 4100, 4112),
+                                   (200, 3584, 4096), (6337, 134, 6944)])
 def test_a_linear_with_less_workspace_than_asked_for(m, n, k):
+    """The last four split K and ask for some; the narrow weights in front of them go without."""
     gen = _gen(9)
     x, w = quantize_float8(_randn(gen, m, k)), _weight(gen, n, k)
     need = _lib.load_library().llmopt_f8_linear_workspace(m, n, k)
-    assert need > 0
+    assert (need > 0) == (m * n > 120000)
     want, off = oracle.product(_numbers(x), _numbers(w))
-    for workspace in (0, need // 2, need - 1, need):
+    for workspace in (0, need // 2, max(0, need - 1), need):
         _check_16(_call_linear(x, w, torch.bfloat16, workspace), want, off)
 
 
-@pytest.mark.parametrize("m", [1, 7, 16])
+@pytest.mark.parametrize("m", [1, 7, 16, 17, 80])
 def test_the_gated_product_without_its_workspace(m):
     gen = _gen(10)
     x, gate, up = quantize_float8(_randn(gen, m, 1024)), _weight(gen, 300, 1024), _weight(gen, 300, 1024)
@@ -246,6 +248,97 @@ def test_the_gated_product_without_its_workspace(m):
         up.codes.data_ptr(), 1024, up.scales.data_ptr(), 8, 300, codes.data_ptr(), 300, scales.data_ptr(), 3, None, 0,
         torch.cuda.current_stream().cuda_stream), "llmopt_f8_swiglu")
     oracle.check_quantized(codes, scales, *oracle.swiglu(_numbers(x), _numbers(gate), _numbers(up)))
+
+
+# ---- every kernel that a size can lead to ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("m,n,k", [
+    # up to 16 tokens' kernel, 32 at a time: one group of steps a wave, eight waves, and several groups
+    (17, 40, 16), (31, 300, 2064), (32, 1000, 4096), (33, 130, 4112), (50, 260, 208), (150, 100, 2048), (1000, 64, 640),
+    # a tile for every workgroup: 128 x 64 in 1, 2, 4 and 8 parts, then 128 x 128, 256 x 64 and 256 x 128 likewise, 256 x 256
+    (1036, 16, 16), (8249, 16, 1968), (1036, 16, 1664), (1045, 16, 3680),
+    (130, 22445, 16), (8886, 261, 13728), (8809, 16, 7456), (7202, 16, 5056),
+    (130, 20409, 16), (130, 10691, 10160), (17, 15263, 2320), (17, 7820, 5968),
+    (133, 28530, 400), (66, 27201, 7936), (6337, 134, 6944), (65, 6387, 13952),
+    (258, 22201, 16),
+    # several tiles one after the other
+    (526, 21875, 272), (513, 14350, 6528), (261, 25258, 912), (536, 23619, 400), (534, 26166, 272)])
+def test_linear_of_every_tile_and_number_of_parts(m, n, k):
+    gen = _gen(21)
+    x, w, bias = quantize_float8(_randn(gen, m, k)), _weight(gen, n, k), _randn(gen, n)
+    want, off = oracle.product(_numbers(x), _numbers(w))
+    want = want + bias.double()
+    off = off + want.abs() * 2.0**-24
+    y = float8_linear(x, w, bias)
+    _check_16(y, want, off)
+    assert torch.equal(float8_linear(x, w, bias), y)
+
+
+@pytest.mark.parametrize("m,n,k", [(17, 40, 16), (31, 300, 2064), (32, 1000, 4096), (50, 260, 4112), (700, 130, 272),
+                                   (1035, 17, 16), (8262, 129, 16), (130, 16428, 16),
+                                   (262, 12981, 928), (260, 16758, 400), (264, 22740, 272)])
+def test_the_gated_product_of_every_tile(m, n, k):
+    gen = _gen(22)
+    x, gate, up = quantize_float8(_randn(gen, m, k)), _weight(gen, n, k), _weight(gen, n, k)
+    out = float8_swiglu(x, gate, up)
+    oracle.check_quantized(out.codes, out.scales, *oracle.swiglu(_numbers(x), _numbers(gate), _numbers(up)))
+    assert _equal(float8_swiglu(x, gate, up), out)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 40, 1040), (40, 300, 1040), (70, 4100, 4112), (300, 4100, 1040), (600, 20000, 272)])
+def test_what_lies_between_and_behind_the_output_rows_is_left_as_it_was(m, n, k):
+    gen = _gen(23)
+    x, w = quantize_float8(_randn(gen, m, k)), _weight(gen, n, k)
+    for ld in (n + 5, n + 12 + -n % 8):
+        y = torch.full((m + 3, ld), 7.0, dtype=torch.bfloat16, device="cuda")
+        lib = _lib.load_library()
+        need = lib.llmopt_f8_linear_workspace(m, n, k)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+        _lib.call(lib.llmopt_f8_linear(x.codes.data_ptr(), k, x.scales.data_ptr(), x.scales.shape[1], m, k, w.codes.data_ptr(), k,
+                                       w.scales.data_ptr(), w.scales.shape[1], None, y.data_ptr(), ld, n, 2,
+                                       ws.data_ptr() if need else None, need, torch.cuda.current_stream().cuda_stream),
+                  "llmopt_f8_linear")
+        assert bool((y[:, n:] == 7.0).all() and (y[m:] == 7.0).all())
+        assert torch.equal(y[:m, :n], float8_linear(x, w))
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 40, 1040), (40, 300, 1040), (70, 14336, 272), (300, 4100, 1040), (300, 20000, 272)])
+def test_what_lies_between_and_behind_the_gated_rows_is_left_as_it_was(m, n, k):
+    gen = _gen(24)
+    x, gate, up = quantize_float8(_randn(gen, m, k)), _weight(gen, n, k), _weight(gen, n, k)
+    want, across = float8_swiglu(x, gate, up), -(-n // 128)
+    for ld in (n + 5, n + 16 + -n % 16):
+        codes = torch.full((m + 3, ld), 77, dtype=torch.uint8, device="cuda")
+        scales = torch.full((m + 3, across + 3), 78, dtype=torch.uint8, device="cuda")
+        lib = _lib.load_library()
+        need = lib.llmopt_f8_swiglu_workspace(m, n, k)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+        sx = x.scales.shape[1]
+        _lib.call(lib.llmopt_f8_swiglu(
+            x.codes.data_ptr(), k, x.scales.data_ptr(), sx, m, k, gate.codes.data_ptr(), k, gate.scales.data_ptr(), sx,
+            up.codes.data_ptr(), k, up.scales.data_ptr(), sx, n, codes.data_ptr(), ld, scales.data_ptr(), across + 3,
+            ws.data_ptr() if need else None, need, torch.cuda.current_stream().cuda_stream), "llmopt_f8_swiglu")
+        assert bool((codes[:, n:] == 77).all() and (codes[m:] == 77).all())
+        assert bool((scales[:, across:] == 78).all() and (scales[m:] == 78).all())
+        assert torch.equal(codes[:m, :n], _bits(want.codes)) and torch.equal(scales[:m, :across], _bits(want.scales))
+
+
+# ---- more rows than a launch counts ------------------------------------------------------------------
+
+
+def test_more_rows_than_one_launch_takes():
+    """Each row has a workgroup of 256, and a launch counts its work-items in 32 bits."""
+    rows, cols = (1 << 24) + 5, 24
+    x = torch.randn(1 << 16, cols, generator=_gen(25), device="cuda").bfloat16().repeat(257, 1)[:rows]
+    out, part = quantize_float8(x), quantize_float8(x[: 1 << 16])
+    assert torch.equal(_bits(out.codes)[: 256 << 16].view(256, 1 << 16, cols), _bits(part.codes).expand(256, -1, -1))
+    assert torch.equal(_bits(out.codes)[256 << 16 :], _bits(part.codes)[:5]) and torch.equal(_bits(out.scales)[-5:], _bits(part.scales)[:5])
+    weight = torch.linspace(0.5, 2.0, cols, device="cuda").bfloat16()
+    (out, h), (part, h_part) = rmsnorm_float8(x, weight, 1e-5, residual=x), rmsnorm_float8(x[: 1 << 16], weight, 1e-5, residual=x[: 1 << 16])
+    assert torch.equal(_bits(out.codes)[: 256 << 16].view(256, 1 << 16, cols), _bits(part.codes).expand(256, -1, -1))
+    assert torch.equal(_bits(out.codes)[256 << 16 :], _bits(part.codes)[:5]) and torch.equal(_bits(out.scales)[-5:], _bits(part.scales)[:5])
+    assert torch.equal(h[-5:], h_part[:5])
 
 
 # ---- offsets that pass 32 bits -----------------------------------------------------------------------
