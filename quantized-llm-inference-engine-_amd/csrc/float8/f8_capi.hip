@@ -270,7 +270,7 @@ int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t l
     const int64_t ld = padded(N);
     const F8DecodeArgs d{t.x, ldx, t.x_scales, ldxs, {t.w[0], t.w[1]}, nullptr, sums, ld, M, N, K, 0, 0};
     CHECK(hip_status(launch_f8_decode(d, kDtF32, st), "llmopt_f8_swiglu"));
-    const F8ActArgs act{sums, sums + M * ld, ld, t.codes, ldc, t.scales, lds, M, N};
+    const F8ActArgs act{{t.x, ldx, t.x_scales, ldxs, {t.w[0], t.w[1]}, K}, sums, sums + M * ld, ld, t.codes, ldc, t.scales, lds, M, N};
     return hip_status(launch_f8_act(act, st), "llmopt_f8_swiglu");
   }
   t.vec = aligned(codes, 16) && ldc % 16 == 0;

@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(64 * WAVES) decode_kernel(const F8DecodeArgs a
   extern __shared__ __align__(1024) uint8_t lds[];
   const int lane = threadIdx.x & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t r = lane & 15, g = lane >> 4, m0 = blockIdx.y * XR;
+  const uint32_t r = lane & 15, g = lane >> 4, m0 = XR > 16 ? blockIdx.y * XR : 0;
   const bool second = blockIdx.x >= a.tiles;
   const uint32_t n0 = (second ? blockIdx.x - a.tiles : blockIdx.x) * 16;
   uint8_t* const own = lds + wave * uint32_t(buffers * W::kBytes);
@@ -173,14 +173,16 @@ __global__ void __launch_bounds__(64 * WAVES) decode_kernel(const F8DecodeArgs a
   for (int t = 0; t < W::kTiles; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   walk.run(wave, WAVES, (a.steps + kGroup - 1) / kGroup, acc);
 
+  // (nothing is on its way there any more)
 #pragma unroll
-  for (int t = 0; t < W::kTiles; ++t) *reinterpret_cast<f32x4*>(own + 1024 * t + 16 * lane) = acc[t];  // nothing is on its way there any more
+  for (int t = 0; t < W::kTiles; ++t) *reinterpret_cast<f32x4*>(own + 1024 * t + 16 * lane) = acc[t];
   __syncthreads();
   const int64_t m = m0 + 16 * wave + r;  // a wave for each 16 tokens
   if (wave >= W::kTiles || (XR < 16 && r >= XR) || m >= a.M) return;
-  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4 sum = acc[0];  // of one tile wave 0 has the first summand
+  if constexpr (W::kTiles > 1) sum = *reinterpret_cast<const f32x4*>(lds + 1024 * wave + 16 * lane);
 #pragma unroll
-  for (int i = 0; i < WAVES; ++i) {
+  for (int i = 1; i < WAVES; ++i) {
     const f32x4 p = *reinterpret_cast<const f32x4*>(lds + i * buffers * W::kBytes + 1024 * wave + 16 * lane);
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] += p[e];

@@ -65,18 +65,21 @@ __global__ void __launch_bounds__(512) gated_any_kernel(const F8TilesArgs a, uin
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
   const uint32_t nb = blockIdx.x / token_tiles;
   const int64_t n0 = int64_t(nb) * kF8Group + 16 * wave, m0 = int64_t(blockIdx.x - nb * token_tiles) * 16;
-  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float v[1][4] = {{0.0f, 0.0f, 0.0f, 0.0f}};
   uint32_t top = 0;
   if (n0 < a.N) {
     f32x4 acc[2];
     sums_any<2>(a, n0, m0, acc);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (n0 + 4 * g + i < a.N) v[i] = f8_swiglu(acc[0][i], acc[1][i]);
-      top = max(top, magnitude(v[i]));
-    }
-    top = max(top, uint32_t(__shfl_xor(int(top), 16, 64)));
-    top = max(top, uint32_t(__shfl_xor(int(top), 32, 64)));
+    for (int i = 0; i < 4; ++i)
+      if (n0 + 4 * g + i < a.N && m0 + r < a.M) v[0][i] = f8_swiglu(acc[0][i], acc[1][i]);
+    uint32_t most[1] = {0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most[0] = max(most[0], magnitude(v[0][i]));
+    most[0] = max(most[0], uint32_t(__shfl_xor(int(most[0]), 16, 64)));
+    most[0] = max(most[0], uint32_t(__shfl_xor(int(most[0]), 32, 64)));
+    f8_settle<true, 15>([&] { return F8Gated{a.x, a.ldx, a.x_scales, a.ldxs, {a.w[0], a.w[1]}, a.K}; }, v, most, m0 + r, n0 + 4 * g);
+    top = most[0];
   }
   if (g == 0) tops[wave][r] = top;
   __syncthreads();
@@ -84,7 +87,7 @@ __global__ void __launch_bounds__(512) gated_any_kernel(const F8TilesArgs a, uin
   if (m >= a.M) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, tops[i][r]);
-  const uint32_t scale = f8_scale(top), codes = f8_codes4(v[0], v[1], v[2], v[3], f8_inverse(scale));
+  const uint32_t scale = f8_scale(top), codes = f8_codes4(v[0][0], v[0][1], v[0][2], v[0][3], f8_inverse(scale));
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (n0 + 4 * g + i < a.N) a.codes[m * a.ldc + n0 + 4 * g + i] = uint8_t(codes >> (8 * i));

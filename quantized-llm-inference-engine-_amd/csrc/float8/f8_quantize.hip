@@ -155,12 +155,14 @@ __global__ void __launch_bounds__(kThreads) rmsnorm_held_kernel(const F8NormArgs
 __global__ void __launch_bounds__(kThreads) act_kernel(const F8ActArgs a, uint32_t chunks, int vec) {
   const int64_t row = blockIdx.x / chunks;
   const int64_t c = int64_t(blockIdx.x - uint32_t(row) * chunks) * kChunk + 8 * threadIdx.x;
-  float g[8], u[8];
-  load8<ActF32>(a.gate + row * a.ld, c, a.cols, vec, g);
+  float g[1][8], u[8];
+  load8<ActF32>(a.gate + row * a.ld, c, a.cols, vec, g[0]);
   load8<ActF32>(a.up + row * a.ld, c, a.cols, vec, u);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) g[i] = f8_swiglu(g[i], u[i]);
-  quantize8(g, a.codes + row * a.ldc, a.scales + row * a.lds, c, a.cols, vec);
+  for (int i = 0; i < 8; ++i) g[0][i] = f8_swiglu(g[0][i], u[i]);
+  uint32_t top[1] = {largest8(g[0])};
+  f8_settle<false, 48>([&] { return a.in; }, g, top, row, c);
+  quantize8(g[0], top[0], a.codes + row * a.ldc, a.scales + row * a.lds, c, a.cols, vec);
 }
 
 }  // namespace

@@ -374,20 +374,30 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
     } else {
       // A group's 128 features lie in two waves, 16 in a lane: the largest magnitude goes across lanes and through LDS.
       float v[TM][16];
+      uint32_t top[TM];
       const int f0 = wn * 64 + 16 * g;
+      const int64_t m = m0 + wm * TM * 16 + r;
 #pragma unroll
       for (int u = 0; u < TM; ++u) {
-        uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float gate = acc[i >> 2][u][i & 3], up = acc[4 + (i >> 2)][u][i & 3];
           v[u][i] = f0 + i < rows_n ? f8_swiglu(gate, up) : 0.0f;
-          top = max(top, magnitude(v[u][i]));
         }
-        top = max(top, uint32_t(__shfl_xor(int(top), 16, 64)));
-        top = max(top, uint32_t(__shfl_xor(int(top), 32, 64)));
-        if (g == 0) tops[wn * kRowsM + (wm * TM + u) * 16 + r] = top;
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = max(most, magnitude(v[u][i]));
+        most = max(most, uint32_t(__shfl_xor(int(most), 16, 64)));
+        most = max(most, uint32_t(__shfl_xor(int(most), 32, 64)));
+        top[u] = m + 16 * u < a.M ? most : 0u;
       }
+      // (The arguments are read anew, where they are needed at all: no registers hold them beside the products.)
+      auto* args = (const F8TilesArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+      asm volatile("" : "+s"(args));
+      f8_settle<false, 15>([&] { return F8Gated{args->x, args->ldx, args->x_scales, args->ldxs, {args->w[0], args->w[1]}, args->K}; }, v, top, m, n0 + f0);
+#pragma unroll
+      for (int u = 0; u < TM; ++u)
+        if (g == 0) tops[wn * kRowsM + (wm * TM + u) * 16 + r] = top[u];
       wait_lgkmcnt0();
       __builtin_amdgcn_s_barrier();
 #pragma unroll
