@@ -49,7 +49,7 @@ struct Walk {
   __device__ __forceinline__ Walk(const F8DecodeArgs& a, const F8Weight& w, uint32_t n0, uint32_t m0, uint8_t* lds_) {
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, rows = min(uint32_t(a.N) - n0, 16u);
     K = uint32_t(a.K);
-    M = min(uint32_t(a.M) - m0, uint32_t(XR));
+    M = XR == 1 ? 1 : XR > 16 ? min(uint32_t(a.M) - m0, uint32_t(XR)) : uint32_t(a.M);
     steps = a.steps;
     ldx = uint32_t(a.ldx);
     lds = lds_;
