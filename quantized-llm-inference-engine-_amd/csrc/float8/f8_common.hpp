@@ -176,8 +176,8 @@ __device__ __forceinline__ float f8_swiglu(float gate, float up) {
 // A group's scale doubles where its largest magnitude passes 1.75 2^i, and the matrix cores' sums, some 2.5e-5 of their typical
 // size off, would put one group in 30,000 on the wrong side. So a maximum within 1e-4 of a border, one in some 3000, is taken once
 // more, from fp32 sums of exact products of the numbers that it may be. (A number that stays a little above 448 2^e rounds to that.)
-// Measured (MI355X, silu(gate) * up of 14336 x 4096, us, with and without): 4 tokens 25.9 / 25.8, 200 tokens 42 / 39 (a walk of some
-// 3 us lies in the way of the whole), 8192 tokens 2 - 3 % more.
+// Measured (MI355X, silu(gate) * up of 14336 x 4096, us, with and without): 4 tokens 25.7 / 25.8, 200 tokens 41.1 / 39.3, 8192 tokens
+// 782 / 758: half of that for the walks, of some 3 us each, half for the registers that they take.
 constexpr uint32_t kF8Near = 1536;  // in steps of the fraction's 23 bits
 __device__ __forceinline__ bool f8_near(uint32_t bits) {
   return bits < 0x7F800000u && ((bits - 0x600000u + kF8Near) & 0x7FFFFFu) < 2 * kF8Near;

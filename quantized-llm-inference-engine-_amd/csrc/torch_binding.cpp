@@ -584,7 +584,7 @@ PyObject* f8_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::ScalarType type = dtype == 1 ? at::kHalf : at::kBFloat16;
   const int64_t M = x.codes.rows, K = x.codes.cols, N = w.codes.rows;
   if (bias && (bias->device() != x.c->device() || bias->scalar_type() != type || bias->dim() != 1 || bias->size(0) != N ||
-               !bias->is_contiguous()))
+               !bias->is_contiguous() || differentiated(*bias)))
     Py_RETURN_NONE;
   const size_t ws_bytes = g_f8.linear_ws(M, N, K);
   at::Tensor y = empty_like_rows(*x.c, N, type), ws;

@@ -204,7 +204,7 @@ def _product_torch(x: Float8Tensor, w: Float8Tensor) -> torch.Tensor:
 def float8_linear(x: Float8Tensor, w: Float8Tensor, bias: torch.Tensor | None = None,
                   dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x w^T + bias`` of activations ``[..., K]`` and a weight ``[N, K]``: ``[..., N]`` of ``dtype`` (fp16 or bf16, also the
-    bias's)."""
+    bias's). With a bias that has to carry a derivative the product runs in torch."""
     if x.codes.is_cuda and x.block_rows == 1 and w.block_rows == GROUP:
         y = float8_ops.native().f8_linear(x.codes, x.scales, w.codes, w.scales, bias, _DTYPE_CODES.get(dtype, 0))
         if y is not None:
@@ -218,7 +218,7 @@ def float8_linear(x: Float8Tensor, w: Float8Tensor, bias: torch.Tensor | None = 
             raise RuntimeError(f"self and mat2 must have the same dtype, but got {bias.dtype} and {dtype}")
         if tuple(bias.shape) != (n,):
             raise ValueError(f"a bias of [{n}] expected, got {tuple(bias.shape)}")
-    if x.is_cuda:
+    if x.is_cuda and (bias is None or not is_differentiated(bias)):
         return float8_ops.linear(x.codes, x.scales, w.codes, w.scales, bias, dtype)
     y = _product_torch(x, w)
     return (y if bias is None else y + bias.float()).to(dtype).view(*x.shape[:-1], n)

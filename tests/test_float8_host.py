@@ -255,6 +255,13 @@ def test_a_tangent_goes_straight_through_the_rounding():
     assert float((y.tangent.double() - want).norm() / want.norm()) < 2.0**-8
 
 
+def test_a_bias_has_its_derivative():
+    x, w = quantize_float8(_x(6, 64, 1, torch.float32)), quantize_float8(_x(40, 64, 2, torch.float32), block_rows=128)
+    bias = torch.zeros(40, dtype=torch.bfloat16, requires_grad=True)
+    float8_linear(x, w, bias).sum().backward()
+    assert torch.equal(bias.grad, torch.full((40,), 6.0, dtype=torch.bfloat16))
+
+
 def test_a_gradient_through_the_gated_product():
     gate, up = (Float8Linear.from_float(_linear(64, 50, seed=i)) for i in (1, 2))
     x = _x(4, 64, 1, torch.bfloat16).requires_grad_()

@@ -210,6 +210,20 @@ def test_other_types_of_a_norm_run_in_torch():
     oracle.check_quantized(out.codes, out.scales, x / torch.sqrt((x * x).mean(1, keepdim=True) + 1e-6), x.abs() * 2.0**-17)
 
 
+@pytest.mark.parametrize("m", [1, 40])
+def test_a_bias_has_its_derivative(m):
+    gen = _gen(27)
+    x, w = quantize_float8(_randn(gen, m, 256)), _weight(gen, 40, 256)
+    bias = _randn(gen, 40).requires_grad_()
+    y = float8_linear(x, w, bias)
+    y.sum().backward()
+    assert torch.equal(bias.grad, torch.full_like(bias, m))
+    with torch.no_grad():
+        assert not float8_linear(x, w, bias).requires_grad
+    want, off = oracle.product(_numbers(x), _numbers(w))
+    _check_16(y.detach(), want + bias.detach().double(), off + (want + bias.detach().double()).abs() * 2.0**-24)
+
+
 # ---- without the workspace --------------------------------------------------------------------------
 
 
