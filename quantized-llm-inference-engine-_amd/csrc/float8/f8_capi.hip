@@ -221,7 +221,6 @@ int llmopt_f8_linear(const void* x, int64_t ldx, const void* x_scales, int64_t l
     const F8DecodeArgs d{t.x, ldx, t.x_scales, ldxs, {t.w[0], {}}, bias, y, ldy, M, N, K, 0, 0};
     return hip_status(launch_f8_decode(d, out_dtype, st), "llmopt_f8_linear");
   }
-  t.vec = aligned(y, 16) && ldy % 8 == 0;
   t.splits = uint32_t(plan.splits);
   t.steps_per_split = uint32_t(plan.steps_per_split);
   t.parts = static_cast<float*>(workspace);
@@ -276,7 +275,6 @@ int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t l
     const F8ActArgs act{{t.x, ldx, t.x_scales, ldxs, {t.w[0], t.w[1]}, K}, sums, sums + M * ld, ld, t.codes, ldc, t.scales, lds, M, N};
     return hip_status(launch_f8_act(act, st), "llmopt_f8_swiglu");
   }
-  t.vec = aligned(codes, 16) && ldc % 16 == 0;
   t.splits = 1;
   return hip_status(launch_f8_tiles(t, plan.shape, 0, st), "llmopt_f8_swiglu");
 }

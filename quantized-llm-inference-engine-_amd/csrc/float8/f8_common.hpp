@@ -85,7 +85,6 @@ struct F8TilesArgs {
   uint8_t* scales;
   int64_t lds;
   int64_t M, N, K;
-  int vec;  // the output's rows are 16-byte aligned
   int steps;
   uint32_t tiles_n, tiles_m;         // (set by the launch)
   uint32_t splits, steps_per_split;  // of K over workgroups

@@ -33,6 +33,10 @@ constexpr uint32_t kOutside = 0x7FFFFFF0u;
 constexpr int kChunk = 32;        // steps whose scales are in LDS at a time
 constexpr int kScaleRow = kChunk + 4;  // bytes of a row of them (16 rows in 16 banks)
 
+// Stores of 16 bytes take any address that fits their elements.
+typedef uint32_t Wide2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t Wide1 __attribute__((ext_vector_type(4), aligned(1)));
+
 // Of an operand's scales, what one thread brings to LDS: a row's bytes of the steps first .. first + 31.
 struct ScaleRow {
   uint32_t v[kChunk / 4];
@@ -71,6 +75,8 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
   extern __shared__ __align__(1024) uint8_t lds[];
   uint8_t* const scales = lds + STAGES * kStage;
   uint32_t* const tops = reinterpret_cast<uint32_t*>(scales + (kRowsM + 2) * kScaleRow);  // [2][kRowsM] (gated)
+  float* const biases = reinterpret_cast<float*>(tops);  // [kRowsN] (a whole product)
+  constexpr bool kBias = !GATED && !PARTS;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -169,8 +175,9 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
     load_stage(src, step, to, kLoads * slot / kSlots, kLoads * (slot + 1) / kSlots);
   };
 
-  // ---- scales: a chunk of steps at a time in LDS, a row of tokens or of the weight's blocks a thread ----
+  // ---- scales: a chunk of steps at a time in LDS, a row of tokens or of the weight's blocks a thread; the bias with the first ----
   ScaleRow row;  // of the chunk after the one in LDS
+  float bias_of = 0.0f;
   auto load_scales = [&](const Tile& t, int first) {
     const int i = threadIdx.x;
     const uint8_t* at = nullptr;
@@ -184,11 +191,16 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
         at = a.w[0].scales + min(t.tn * WN + second, uint32_t((a.N - 1) / kF8Group)) * a.w[0].lds;
     }
     if (at) row.load(at, t.begin + first, t.begin + t.steps);
+    if constexpr (kBias) {
+      const int64_t n = int64_t(t.tn) * kWide + i;
+      if (a.bias && first == 0 && i < kRowsN) bias_of = n < a.N ? Out::load(static_cast<const typename Out::raw*>(a.bias)[n]) : 0.0f;
+    }
   };
   auto store_scales = [&] {
     wait_lgkmcnt0();
     __builtin_amdgcn_s_barrier();  // the chunk before this one has been read
     if (threadIdx.x < kRowsM + 2) row.store(scales + threadIdx.x * kScaleRow);
+    if (kBias && threadIdx.x < kRowsN) biases[threadIdx.x] = bias_of;
     wait_lgkmcnt0();
     __builtin_amdgcn_s_barrier();
     fence();
@@ -338,6 +350,7 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
     wait_vmcnt<0>();
 #pragma unroll
     for (uint32_t& v : row.v) asm volatile("" : "+v"(v));
+    if constexpr (kBias) asm volatile("" : "+v"(bias_of));
     fence();
     if (last <= own) {  // a walk of one step, or none that the next tile's stages begin in
       source = source_of(next), load = next.begin;
@@ -364,7 +377,7 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
     } else if constexpr (!GATED) {
       using Raw = typename Out::raw;
       const int64_t n = n0 + wn * 128 + 32 * g;
-      const Raw* bias = static_cast<const Raw*>(a.bias);
+      const bool bias = a.bias != nullptr;
 #pragma unroll
       for (int u = 0; u < TM; ++u) {
         const int64_t m = m0 + (wm * TM + u) * 16 + r;
@@ -374,16 +387,16 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
         for (int t = 0; t < 8; t += 2) {
           float v[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[i] = acc[t + i / 4][u][i & 3];
-            const int64_t at = n + 4 * t + i;
-            if (bias && at < a.N) v[i] += Out::load(bias[at]);
+          for (int i = 0; i < 8; ++i) v[i] = acc[t + i / 4][u][i & 3];
+          if (bias) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += biases[wn * 128 + 32 * g + 4 * t + i];
           }
           u32x4 out;
 #pragma unroll
           for (int i = 0; i < 4; ++i) out[i] = pack16<Out>(v[2 * i], v[2 * i + 1]);
-          if (a.vec && n + 4 * t + 8 <= a.N) {
-            *reinterpret_cast<u32x4*>(y + n + 4 * t) = out;
+          if (n + 4 * t + 8 <= a.N) {
+            *reinterpret_cast<Wide2*>(y + n + 4 * t) = out;
           } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -432,8 +445,8 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
 #pragma unroll
         for (int i = 0; i < 4; ++i) out[i] = f8_codes4(v[u][4 * i], v[u][4 * i + 1], v[u][4 * i + 2], v[u][4 * i + 3], inv);
         uint8_t* to = a.codes + m * a.ldc + n0 + f0;
-        if (a.vec && f0 + 16 <= rows_n) {
-          *reinterpret_cast<u32x4*>(to) = out;
+        if (f0 + 16 <= rows_n) {
+          *reinterpret_cast<Wide1*>(to) = out;
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -442,7 +455,7 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
       }
     }
     if (!more) break;
-    stored = a.vec && rows_n == kWide && m0 + kRowsM <= a.M;
+    stored = rows_n == kWide && m0 + kRowsM <= a.M;
     tile = next, id += gridDim.x;
   }
   wait_vmcnt<0>();  // zeros on their way into LDS
@@ -451,7 +464,7 @@ __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_
 template <int WN, int WM, int TM, int STAGES, bool GATED, bool PARTS, class Out>
 hipError_t launch(const F8TilesArgs& a, hipStream_t stream) {
   constexpr int kRowsN = 128 * WN, kRowsM = 16 * TM * WM;
-  constexpr int kBytes = STAGES * (kRowsN + kRowsM) * kStep + (kRowsM + 2) * kScaleRow + (GATED ? 8 * kRowsM : 0);
+  constexpr int kBytes = STAGES * (kRowsN + kRowsM) * kStep + (kRowsM + 2) * kScaleRow + (GATED ? 8 * kRowsM : PARTS ? 0 : 4 * kRowsN);
   static_assert(kBytes <= 160 * 1024, "stages and scales fit LDS");
   auto* kernel = tiles_kernel<WN, WM, TM, STAGES, GATED, PARTS, Out>;
   static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
