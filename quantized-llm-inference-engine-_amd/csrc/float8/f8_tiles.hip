@@ -471,8 +471,8 @@ hipError_t launch(const F8TilesArgs& a, hipStream_t stream) {
   if (ready != hipSuccess) return ready;
   // As many workgroups as the chip holds, each with its tiles one after the other: the next one's first stages are loaded, and
   // this one's results stored, beside the products. Walks too short for that: a workgroup for each tile.
-  const uint32_t count = a.tiles_n * a.tiles_m * a.splits, held = 256 * (kBytes <= 80 * 1024 ? 2 : 1);
-  const int shortest = a.splits > 1 ? a.steps - int((a.splits - 1) * a.steps_per_split) : a.steps;
+  const uint32_t count = a.tiles_n * a.tiles_m * (PARTS ? a.splits : 1), held = 256 * (kBytes <= 80 * 1024 ? 2 : 1);
+  const int shortest = PARTS ? a.steps - int((a.splits - 1) * a.steps_per_split) : a.steps;
   const uint32_t grid = shortest > STAGES && count > held ? held : count;
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * WN * WM), kBytes, stream, a);
   return hipGetLastError();
@@ -486,6 +486,9 @@ hipError_t launch_shape(F8TilesArgs a, int out_dtype, hipStream_t stream) {
   a.tiles_n = uint32_t((a.N + wide - 1) / wide);
   a.tiles_m = uint32_t((a.M + kRowsM - 1) / kRowsM);
   a.steps = int((a.K + kStep - 1) / kStep);
+  // What no kernel here is for: a grid of such would be of tiles or steps that are not there.
+  if (gated ? WN != 2 || a.splits > 1 : a.splits > 1 && (kRowsM == 256 || (a.splits - 1) * a.steps_per_split >= uint32_t(a.steps)))
+    return hipErrorInvalidValue;
   if constexpr (kRowsM < 256) {
     if (a.splits > 1) {
       const hipError_t err = launch<WN, WM, TM, STAGES, false, true, ActBf16>(a, stream);
