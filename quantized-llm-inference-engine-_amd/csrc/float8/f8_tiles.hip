@@ -14,7 +14,9 @@
 //   256 x 256 in eight waves, one barrier a step: 445, 1067
 //   loads dealt among the products of two phases, scales of 32 steps at a time in LDS: 383, 765
 //   tiles one after the other, the next one's first stages beside the last products and the results' stores: 374, 737
-//   maxima next to a border of the scales summed again (f8_common.hpp): -, 760 - 780
+//   maxima next to a border of the scales summed again (f8_common.hpp): 374, 760
+//   the bias in LDS with the scales, stores of 16 bytes at any alignment: the same here; 1536 x 1024 with a bias 38 -> 26, 1536 x 1040 of
+//   777 tokens with one 11.3 -> 8.9, 5225 x 2592 of 188 tokens 18.4 -> 13.4
 // Level or worse: products of 32 x 32 (387, 799 - 823), waves of 64 rows x 32 or 64 tokens in the smaller tiles (a fifth to a third
 // fewer LDS reads, all sizes within 2 %), a prefetch into L2 (443 for 421), waves of higher priority, 1 to 32 token tiles a sweep
 // instead of 4 (within 3 %). Without the loads down takes 331, without the LDS reads 357, without either and the barrier 292: that is
