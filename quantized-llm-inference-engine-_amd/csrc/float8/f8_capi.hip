@@ -58,6 +58,10 @@ bool tiled_rows(const void* p, int64_t ld, int64_t cols, int64_t ld_scales = 0) 
   return aligned(p, 16) && ld % 16 == 0 && cols % 16 == 0 && ld <= kMost && cols > 0 && cols <= kMost && ld_scales <= kMost;
 }
 
+// The stride of `rows` rows of codes. A single row has any: its length, then, so that the rows behind it, whose positions the tiles take
+// from the stride, lie behind the operand's end.
+int64_t stride_of(int64_t rows, int64_t cols, int64_t ld) { return rows == 1 ? cols : ld; }
+
 // Workgroups of a grid of `a` x `b`.
 int check_grid(int64_t a, int64_t b, int64_t most = kMaxInt) {
   if (a > 0 && b > most / a) return fail(LLMOPT_ERR_UNSUPPORTED, "%lld x %lld workgroups are too many", (long long)a, (long long)b);
@@ -201,6 +205,7 @@ int llmopt_f8_linear(const void* x, int64_t ldx, const void* x_scales, int64_t l
   CHECK(check_rows("y", y, M, N, ldy));
   CHECK(check_grid(8 * up(M, 16), up(N, 64)));
   if (M == 0 || N == 0) return LLMOPT_OK;
+  ldx = stride_of(M, K, ldx), ldw = stride_of(N, K, ldw);
   F8TilesArgs t{};
   t.x = static_cast<const uint8_t*>(x);
   t.ldx = ldx;
@@ -247,6 +252,7 @@ int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t l
   CHECK(check_rows("scales", scales, M, groups(N), lds));
   CHECK(check_grid(up(M, 16), up(N, 64)));
   if (M == 0 || N == 0) return LLMOPT_OK;
+  ldx = stride_of(M, K, ldx), ldg = stride_of(N, K, ldg), ldu = stride_of(N, K, ldu);
   F8TilesArgs t{};
   t.x = static_cast<const uint8_t*>(x);
   t.ldx = ldx;
