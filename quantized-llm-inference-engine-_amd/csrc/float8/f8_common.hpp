@@ -172,12 +172,18 @@ __device__ __forceinline__ float f8_swiglu(float gate, float up) {
 
 // ---- maxima next to a border of the scales -------------------------------------------------------------
 
-// A group's scale doubles where its largest magnitude passes 1.75 2^i, and the matrix cores' sums, some 2.5e-5 of their typical
-// size off, would put one group in 30,000 on the wrong side. So a maximum within 1e-4 of a border, one in some 3000, is taken once
-// more, from fp32 sums of exact products of the numbers that it may be. (A number that stays a little above 448 2^e rounds to that.)
-// Measured (MI355X, silu(gate) * up of 14336 x 4096, us, with and without): 4 tokens 25.7 / 25.8, 200 tokens 41.1 / 39.3, 8192 tokens
-// 782 / 758: half of that for the walks, of some 3 us each, half for the registers that they take.
-constexpr uint32_t kF8Near = 1536;  // in steps of the fraction's 23 bits
+// A group's scale doubles where its largest magnitude passes 1.75 2^i, and the matrix cores' sums (f8_mfma.hpp) would put some groups
+// on the wrong side. So a maximum within 2^-10 of a border, one in some 350, is taken once more, from fp32 sums of exact products of
+// the numbers that it may be. (A number that stays a little above 448 2^e rounds to that.)
+// 2^-10 is more than a sum of which one product is nearly all can be off by, seven times 2^-13 of it; other sums are off by less,
+// as the bits dropped from many products go either way. How far maxima of silu(gate) * up are off, measured (MI355X, K of 512, 1024
+// and 4096, 50,000 to 100,000 groups each): channels of like strength 1.3e-5 rms, 1 % of them 8 times as strong 2.5e-5, 0.2 % 100
+// times 8e-5, one or two 1000 times and more 1.2e-4; the largest of a million 8.6e-4. Without this 3 to 13 groups in 100,000
+// would be on the wrong side, with a window of 1e-4 none of the first, but up to 8 of the last.
+// Measured (MI355X, in a graph, us, without / with 1e-4 / with 2^-10; gate and up of 14336 x 4096): 4 tokens 24.1 / 24.3 / 25.1, 200
+// tokens 35 / 38 / 38, 8192 tokens 753 / 772 / 788; 2816 x 1024, 8192 tokens 58 / 65 / 70: half of that for the walks, of some 3 us
+// each, half for the registers that they take.
+constexpr uint32_t kF8Near = 14336;  // in steps of the fraction's 23 bits
 __device__ __forceinline__ bool f8_near(uint32_t bits) {
   return bits < 0x7F800000u && ((bits - 0x600000u + kF8Near) & 0x7FFFFFu) < 2 * kF8Near;
 }

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from llmopt.kernels import _lib
-from llmopt.quantization import float8_linear, quantize_float8
+from llmopt.quantization import Float8Tensor, float8_linear, float8_swiglu, quantize_float8
 from oracle import float8_oracle as oracle
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +51,35 @@ def test_a_single_row_comes_with_any_stride(ld):
     _lib.call(lib.llmopt_f8_linear(tokens.codes.data_ptr(), 1024, tokens.scales.data_ptr(), 8, 2000, 1024, one.codes.data_ptr(), ld,
                                    one.scales.data_ptr(), 8, None, y.data_ptr(), 1, 1, 2, None, 0, _stream()), "llmopt_f8_linear")
     assert torch.equal(y, float8_linear(tokens, one))
+
+
+# ---- maxima next to a border of the scales -----------------------------------------------------------
+
+
+def _strong(gen, m, k, share, gain):
+    """Rows in which a share of the channels is `gain` times as strong as the rest."""
+    return torch.randn(m, k, generator=gen, device="cuda") * torch.where(torch.rand(k, generator=gen, device="cuda") < share, gain, 1.0)
+
+
+def _exact_scales(x, gate, up, n):
+    """The least and the greatest exponent of each group's scale for sums that are off by 1e-5: fp32 sums of a few thousand products of
+    either sign are off by a few 2^-24 of their terms' typical size, and the largest of 128 of them is no sum that its terms cancel in."""
+    want, _ = oracle.swiglu(_numbers(x), _numbers(gate), _numbers(up))
+    amax = want.abs().view(-1, n // 128, 128).amax(2)
+    return [torch.ceil(torch.log2(amax * (1 + off) / 448.0)) for off in (-1e-5, 1e-5)]
+
+
+@pytest.mark.parametrize("share,gain", [(0.01, 8.0), (0.005, 30.0), (0.002, 100.0), (0.001, 1000.0)])
+@pytest.mark.parametrize("at_once,k", [(16, 1024), (512, 1024), (1024, 2048)])
+def test_scales_are_those_of_exact_sums_where_a_few_channels_are_strong(at_once, k, share, gain):
+    """A strong channel's product takes bits of the seven beside it: sums are off by 1e-4 of the largest and more, many times what they
+    are for channels of like strength."""
+    gen, m, n = _gen(31), 4096, 14336
+    gate, up = _weight(gen, n, k), _weight(gen, n, k)
+    x = quantize_float8(_strong(gen, m, k, share, gain))
+    for first in range(0, m, at_once if at_once > 16 else 1024):
+        rows = slice(first, first + at_once)
+        part = Float8Tensor(x.codes[rows], x.scales[rows])
+        low, high = _exact_scales(part, gate, up, n)
+        e = _bits(float8_swiglu(part, gate, up).scales).double() - 127.0
+        assert bool(((e == low) | (e == high)).all())
