@@ -83,3 +83,67 @@ def test_scales_are_those_of_exact_sums_where_a_few_channels_are_strong(at_once,
         low, high = _exact_scales(part, gate, up, n)
         e = _bits(float8_swiglu(part, gate, up).scales).double() - 127.0
         assert bool(((e == low) | (e == high)).all())
+
+
+def _at_a_border(gen, gate, up, k):
+    """Of many tokens, one whose largest magnitude of the block's 128 features lies within 1e-4 of a border, but not within 2e-5, and
+    one that is far from it. Of the larger half of all: their sums do not cancel."""
+    x = quantize_float8(torch.randn(65536, k, generator=gen, device="cuda"))
+    amax = oracle.swiglu(_numbers(x), _numbers(gate), _numbers(up))[0].abs().amax(1)
+    off = torch.log2(amax / 448.0)
+    off = torch.where(amax > amax.median(), (off - off.round()).abs(), 0.0)
+    near = torch.where(off > 3e-5, off, 1.0).argmin()
+    assert float(off[near]) < 1.4e-4
+    return [Float8Tensor(x.codes[t : t + 1], x.scales[t : t + 1]) for t in (near, off.argmax())]
+
+
+def _repeated(t, rows):
+    """The rows of activations, or the block of 128 rows of a weight, over and over."""
+    times = rows // t.codes.shape[0]
+    codes, scales = (part.view(torch.uint8).repeat(times, 1).view(part.dtype) for part in (t.codes, t.scales))
+    return Float8Tensor(codes, scales, t.block_rows)
+
+
+def _us(call, calls=5):
+    best = float("inf")
+    for _ in range(4):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        for _ in range(calls):
+            call()
+        end.record()
+        end.synchronize()
+        best = min(best, start.elapsed_time(end) * 1e3 / calls)
+    return best
+
+
+@pytest.mark.parametrize("tokens", [16, 200, 1024, 4096])
+def test_equal_tokens_next_to_a_border(tokens):
+    """A batch of one token, and a weight of one block, over and over: all groups are next to the border together. They have the scale
+    of the exact sums, all the same codes, and take about as long as other tokens."""
+    gen, k, n = _gen(32), 1024, 128 * 64
+    gate, up = _weight(gen, 128, k), _weight(gen, 128, k)
+    near, far = _at_a_border(gen, gate, up, k)
+    low, high = _exact_scales(near, gate, up, 128)
+    assert torch.equal(low, high)
+    near, far, gate, up = _repeated(near, tokens), _repeated(far, tokens), _repeated(gate, n), _repeated(up, n)
+    out = float8_swiglu(near, gate, up)
+    assert bool((_bits(out.scales).double() - 127.0 == low).all())
+    assert torch.equal(_bits(out.codes), _bits(out.codes)[:1].expand(tokens, n))
+    us = [_us(lambda x=x: float8_swiglu(x, gate, up)) for x in (near, far)]
+    assert us[0] < 2 * us[1] + 10, us
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 256, 2048])
+def test_equal_features_next_to_a_border(tokens):
+    """Every feature of a weight the same: all of a group's numbers are next to the border. Not all of them are summed again, and the
+    time stays bounded: a wave takes at most 16 sums for a tile."""
+    gen, k, n = _gen(33), 1024, 1024
+    gate, up = (_repeated(quantize_float8(torch.randn(1, k, generator=gen, device="cuda") * 0.05), n) for _ in range(2))
+    gate, up = (quantize_float8(t.dequantize(), block_rows=128) for t in (gate, up))
+    near, far = _at_a_border(gen, Float8Tensor(gate.codes[:128], gate.scales[:1], 128), Float8Tensor(up.codes[:128], up.scales[:1], 128), k)
+    near, far = _repeated(near, tokens), _repeated(far, tokens)
+    out = float8_swiglu(near, gate, up)
+    oracle.check_quantized(out.codes, out.scales, *oracle.swiglu(_numbers(near), _numbers(gate), _numbers(up)))
+    us = [_us(lambda x=x: float8_swiglu(x, gate, up)) for x in (near, far)]
+    assert us[0] < 10 * us[1] + 50, us
