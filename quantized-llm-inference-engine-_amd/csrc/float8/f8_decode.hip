@@ -240,8 +240,10 @@ template <int XR, bool HELD, int WAVES, class Out>
 hipError_t launch_out(const F8DecodeArgs& a, hipStream_t stream) {
   auto* kernel = decode_kernel<XR, HELD, WAVES, Out>;
   const int buffers = a.steps > kGroup * WAVES ? 2 : 1, bytes = WAVES * buffers * Walk<XR, HELD>::kBytes;
-  static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-  if (ready != hipSuccess) return ready;
+  if (bytes > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return e;
+  }
   hipLaunchKernelGGL(kernel, dim3(a.tiles * (a.w[1].codes ? 2 : 1), uint32_t((a.M + XR - 1) / XR)), dim3(64 * WAVES), bytes, stream, a, buffers);
   return hipGetLastError();
 }

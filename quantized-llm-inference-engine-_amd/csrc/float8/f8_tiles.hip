@@ -469,8 +469,10 @@ hipError_t launch(const F8TilesArgs& a, hipStream_t stream) {
   constexpr int kBytes = STAGES * (kRowsN + kRowsM) * kStep + (kRowsM + 2) * kScaleRow + (GATED ? 8 * kRowsM : PARTS ? 0 : 4 * kRowsN);
   static_assert(kBytes <= 160 * 1024, "stages and scales fit LDS");
   auto* kernel = tiles_kernel<WN, WM, TM, STAGES, GATED, PARTS, Out>;
-  static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-  if (ready != hipSuccess) return ready;
+  if constexpr (kBytes > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != hipSuccess) return e;
+  }
   // As many workgroups as the chip holds, each with its tiles one after the other: the next one's first stages are loaded, and
   // this one's results stored, beside the products. Walks too short for that: a workgroup for each tile.
   const uint32_t count = a.tiles_n * a.tiles_m * (PARTS ? a.splits : 1), held = 256 * (kBytes <= 80 * 1024 ? 2 : 1);

@@ -68,3 +68,17 @@ def test_a_single_rows_stride_is_no_shorter_than_the_row(stub, call, ld):
     assert got[0] == 0 and got[1] == 1
     one = {"x"} if "(1, 256" in call else {"x", "w"} if "linear(1" in call else {"w", "second"} if "swiglu" in call else {"w"}
     assert all(got[2][name] == 1024 for name in one), got
+
+
+@pytest.mark.parametrize("call", ["linear(8192, 4096, 4096)", "linear(1, 4096, 14336)", "swiglu(300, 1280, 2048)"])
+def test_the_shared_memory_is_asked_for_with_each_launch(stub, call):
+    """The runtime keeps a kernel's shared memory for the device that is current, so a launch on another one asks again, and a failure
+    is that call's alone."""
+    got = _child(stub, f"""
+refuse.value = 1
+first = {call}
+refuse.value = 0
+later = [({call}, attributes.value) for _ in range(3)]
+print(json.dumps([first, launches.value, later]))""")
+    assert got[0] != 0 and got[1] == 3
+    assert got[2] == [[0, 2], [0, 3], [0, 4]]
