@@ -116,10 +116,12 @@ class SwiGLUMLP(nn.Module):
     def fuse_gate_up(self) -> bool:
         """Merge quantized gate and up projections into one :class:`QuantSwiGLU`; returns
         whether it did (both must be :class:`QuantLinear` with the same settings). Where they and the down projection
-        are :class:`Float8Linear`, gate and up become a :class:`Float8SwiGLU`."""
+        are :class:`Float8Linear`, gate and up become a :class:`Float8SwiGLU` (False where it does not take them)."""
         if self.gate_up is not None:
             return True
         if all(isinstance(p, Float8Linear) for p in (self.gate_proj, self.up_proj, self.down_proj)):
+            if Float8SwiGLU.refusal(self.gate_proj, self.up_proj) is not None:
+                return False
             self.gate_up = Float8SwiGLU(self.gate_proj, self.up_proj)
             del self.gate_proj, self.up_proj
             return True
@@ -186,16 +188,17 @@ class PagedAttentionLayer(nn.Module):
         """Whether :meth:`forward` takes its input quantized (:class:`Float8Tensor`)."""
         if self.qkv_proj is not None:
             return isinstance(self.qkv_proj, FusedFloat8Linear)
-        return all(isinstance(p, Float8Linear) for p in (self.q_proj, self.k_proj, self.v_proj))
+        parts = (self.q_proj, self.k_proj, self.v_proj)
+        return all(isinstance(p, Float8Linear) and p.compute_dtype == parts[0].compute_dtype for p in parts)
 
     def fuse_qkv(self) -> bool:
         """Merge quantized q, k and v projections into one :class:`FusedQuantLinear`, or :class:`Float8Linear` ones into one
-        :class:`FusedFloat8Linear` (False where q or k has no multiple of 128 rows)."""
+        :class:`FusedFloat8Linear` (False where it does not take them, as where q or k has no multiple of 128 rows)."""
         if self.qkv_proj is not None:
             return True
         parts = (self.q_proj, self.k_proj, self.v_proj)
         if all(isinstance(p, Float8Linear) for p in parts):
-            if any(p.out_features % 128 for p in parts[:2]):
+            if FusedFloat8Linear.refusal(parts) is not None:
                 return False
             self.qkv_proj = FusedFloat8Linear(parts)
             del self.q_proj, self.k_proj, self.v_proj

@@ -315,14 +315,10 @@ class FusedFloat8Linear(nn.Module):
 
     def __init__(self, parts: Sequence[Float8Linear]) -> None:
         super().__init__()
-        if not parts:
-            raise ValueError("nothing to fuse")
+        reason = self.refusal(parts)
+        if reason is not None:
+            raise ValueError(reason)
         first = parts[0]
-        for p in parts:
-            if p.in_features != first.in_features or p.compute_dtype != first.compute_dtype:
-                raise ValueError("fused layers need the same in_features and compute dtype")
-        if any(p.out_features % GROUP for p in parts[:-1]):
-            raise ValueError(f"all but the last of the fused layers need a multiple of {GROUP} rows")
         bias = None
         if any(p.bias is not None for p in parts):
             bias = torch.cat([torch.zeros(p.out_features, dtype=p.compute_dtype, device=p.weight_codes.device)
@@ -331,6 +327,17 @@ class FusedFloat8Linear(nn.Module):
         scales = torch.cat([p.weight_scales.view(torch.uint8) for p in parts]).view(E8)
         self.linear = Float8Linear(Float8Tensor(codes, scales, GROUP), bias, first.compute_dtype)
         self.out_features = [p.out_features for p in parts]
+
+    @staticmethod
+    def refusal(parts: Sequence[Float8Linear]) -> str | None:
+        """Why ``parts`` cannot be fused; None where they can."""
+        if not parts:
+            return "nothing to fuse"
+        if any(p.in_features != parts[0].in_features or p.compute_dtype != parts[0].compute_dtype for p in parts):
+            return "fused layers need the same in_features and compute dtype"
+        if any(p.out_features % GROUP for p in parts[:-1]):
+            return f"all but the last of the fused layers need a multiple of {GROUP} rows"
+        return None
 
     def forward(self, x: torch.Tensor | Float8Tensor) -> tuple[torch.Tensor, ...]:
         return tuple(torch.split(self.linear(x), self.out_features, dim=-1))
@@ -351,11 +358,19 @@ class Float8SwiGLU(nn.Module):
 
     def __init__(self, gate: Float8Linear, up: Float8Linear) -> None:
         super().__init__()
-        if gate.weight_codes.shape != up.weight_codes.shape or gate.compute_dtype != up.compute_dtype:
-            raise ValueError("gate and up need the same shape and compute dtype")
-        if gate.bias is not None or up.bias is not None:
-            raise ValueError("gate and up must have no bias")
+        reason = self.refusal(gate, up)
+        if reason is not None:
+            raise ValueError(reason)
         self.gate_proj, self.up_proj = gate, up
+
+    @staticmethod
+    def refusal(gate: Float8Linear, up: Float8Linear) -> str | None:
+        """Why ``gate`` and ``up`` cannot be one product; None where they can."""
+        if gate.weight_codes.shape != up.weight_codes.shape or gate.compute_dtype != up.compute_dtype:
+            return "gate and up need the same shape and compute dtype"
+        if gate.bias is not None or up.bias is not None:
+            return "gate and up must have no bias"
+        return None
 
     def forward(self, x: torch.Tensor | Float8Tensor) -> torch.Tensor | Float8Tensor:
         if isinstance(x, torch.Tensor):
