@@ -5,12 +5,14 @@ allocations and launch in native code (:func:`native`)."""
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from llmopt.kernels._lib import DTYPE_CODES, call, load_binding, load_library
 from llmopt.kernels.ops import _launching_on, _same_device, _stream_handle
 
-__all__ = ["linear", "native", "quantize", "rmsnorm", "rmsnorm_supported", "swiglu"]
+__all__ = ["as_rows", "linear", "native", "quantize", "rmsnorm", "rmsnorm_supported", "swiglu"]
 
 GROUP = 128
 
@@ -19,9 +21,14 @@ def _groups(n: int) -> int:
     return -(-n // GROUP)
 
 
+def as_rows(x: torch.Tensor) -> torch.Tensor:
+    """``[..., K]`` as a matrix, also where ``K`` is 0 (the number of rows is not left to be found)."""
+    return x.reshape(math.prod(x.shape[:-1]), x.shape[-1]) if x.dim() != 2 else x
+
+
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``[..., K]`` as a matrix with a unit inner stride and rows that do not overlap; a view where that is possible."""
-    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    x = as_rows(x)
     rows, cols = x.shape
     if (cols > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < cols):
         x = x.contiguous()

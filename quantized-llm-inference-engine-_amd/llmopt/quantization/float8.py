@@ -135,7 +135,7 @@ def _quantize_torch(x: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, tor
     m, p = torch.frexp(torch.where(finite, amax, 0.0))  # amax = m 2^p with m in [0.5, 1), and 448 = 0.875 2^9
     e = torch.where(m > 0, p - 9 + (m > 0.875).to(p.dtype), -127).clamp(min=-127)
     codes = torch.where(finite[:, None, :, None], torch.ldexp(groups, -e[:, None, :, None]), 0.0)
-    codes = codes.reshape(-1, _groups(k) * GROUP)[:rows, :k].to(F8)
+    codes = codes.reshape(groups.shape[0] * block_rows, _groups(k) * GROUP)[:rows, :k].to(F8)
     return codes.contiguous(), torch.where(finite, e + 127, 255).to(torch.uint8).view(E8)
 
 
@@ -158,7 +158,7 @@ def quantize_float8(x: torch.Tensor, block_rows: int = 1) -> Float8Tensor:
         raise ValueError(f"expected a 2D weight, got shape {tuple(x.shape)}")
     if x.is_cuda:
         return _made(*float8_ops.quantize(x, block_rows), block_rows)
-    codes, scales = _quantize_torch(x.reshape(-1, x.shape[-1]), block_rows)
+    codes, scales = _quantize_torch(float8_ops.as_rows(x), block_rows)
     if block_rows == 1:
         codes, scales = codes.view(x.shape), scales.view(*x.shape[:-1], scales.shape[1])
     return _made(codes, scales, block_rows)
@@ -198,7 +198,7 @@ def _product_torch(x: Float8Tensor, w: Float8Tensor) -> torch.Tensor:
     if x.device != w.device:
         raise RuntimeError("Expected all tensors to be on the same device, but found at least two devices, "
                            f"{x.device} and {w.device}!")
-    return torch.matmul(x.dequantize().reshape(-1, x.shape[-1]), w.dequantize().t())
+    return torch.matmul(float8_ops.as_rows(x.dequantize()), w.dequantize().t())
 
 
 def float8_linear(x: Float8Tensor, w: Float8Tensor, bias: torch.Tensor | None = None,

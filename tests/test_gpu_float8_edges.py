@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from llmopt.kernels import _lib
-from llmopt.quantization import Float8Tensor, float8_linear, float8_swiglu, quantize_float8
+from llmopt.quantization import Float8Tensor, float8_linear, float8_swiglu, quantize_float8, rmsnorm_float8
 from oracle import float8_oracle as oracle
 
 pytestmark = pytest.mark.gpu
@@ -147,3 +147,21 @@ def test_equal_features_next_to_a_border(tokens):
     oracle.check_quantized(out.codes, out.scales, *oracle.swiglu(_numbers(near), _numbers(gate), _numbers(up)))
     us = [_us(lambda x=x: float8_swiglu(x, gate, up)) for x in (near, far)]
     assert us[0] < 10 * us[1] + 50, us
+
+
+# ---- no columns, tokens or features ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lead", [(), (3,), (0,), (2, 3), (2, 0)])
+def test_no_columns_no_tokens_no_features(lead):
+    x, w = quantize_float8(torch.zeros(*lead, 0, device="cuda")), quantize_float8(torch.zeros(5, 0, device="cuda"), block_rows=128)
+    assert x.codes.shape == x.scales.shape == (*lead, 0) and w.scales.shape == (1, 0)
+    bias = torch.arange(5, dtype=torch.bfloat16, device="cuda")
+    assert torch.equal(float8_linear(x, w, bias), bias.expand(*lead, 5))
+    act = float8_swiglu(x, w, w)
+    assert act.codes.shape == (*lead, 5) and act.scales.shape == (*lead, 1) and not bool(act.dequantize().any())
+    zeros = torch.zeros(*lead, 0, dtype=torch.bfloat16, device="cuda")
+    out, h = rmsnorm_float8(zeros, zeros.new_zeros(0), 1e-5, residual=zeros)
+    assert out.codes.shape == h.shape == (*lead, 0)
+    x, none = quantize_float8(torch.ones(*lead, 200, device="cuda")), quantize_float8(torch.zeros(0, 200, device="cuda"), block_rows=128)
+    assert float8_linear(x, none).shape == (*lead, 0) and float8_swiglu(x, none, none).scales.shape == (*lead, 0)
