@@ -82,3 +82,31 @@ later = [({call}, attributes.value) for _ in range(3)]
 print(json.dumps([first, launches.value, later]))""")
     assert got[0] != 0 and got[1] == 3
     assert got[2] == [[0, 2], [0, 3], [0, 4]]
+
+
+# The tiles' launch itself, as no entry point calls it. F8TilesArgs: four words of x, four for each weight, then bias, y, ldy, codes, ldc,
+# scales, lds, M, N and K, five 32-bit numbers, of which the last two are the parts of K and the steps in each, parts and their stride.
+TILES = r"""
+launch = lib._ZN6llmopt15launch_f8_tilesERKNS_11F8TilesArgsENS_7F8ShapeEiP12ihipStream_t
+def tiles(shape, m, n, k, splits, per, gated=False):
+    p = 1 << 20
+    weight = [p, k, p, -(-k // 128)]
+    block = struct.pack("<22q5i4x2q", p, k, p, -(-k // 128), *weight, *(weight if gated else [0] * 4), 0, p, n, p, n, p, -(-n // 128),
+                        m, n, k, 0, 0, 0, splits, per, p, n)
+    before = launches.value
+    return launch(ctypes.c_char_p(block), shape, 2, None), launches.value - before
+"""
+
+
+def test_the_tiles_refuse_parts_of_k_that_they_have_no_kernel_for(stub):
+    """Tiles of 256 tokens and the gated product are whole; a grid of parts would be of tiles that are not there. Neither may a part
+    begin behind the last step."""
+    code = TILES + "print(json.dumps([tiles(*c) for c in json.loads('''%s''')]))"
+    whole = [[shape, 300, 512, 1024, 1, 8] for shape in range(5)]
+    parts = [[shape, 300, 512, 1024, 2, 4] for shape in range(1, 5)]
+    assert _child(stub, code % json.dumps(whole)) == [[0, 1]] * 5
+    assert _child(stub, code % json.dumps(parts)) == [[0, 2]] * 4
+    refused = [[0, 300, 512, 1024, 2, 4], [1, 300, 512, 1024, 2, 8], [4, 300, 512, 1024, 8, 2], [0, 300, 512, 1024, 2, 4, True],
+               [2, 300, 512, 1024, 2, 4, True], [3, 300, 512, 1024, 1, 8, True]]
+    got = _child(stub, code % json.dumps(refused))
+    assert all(rc != 0 and launched == 0 for rc, launched in got), got
