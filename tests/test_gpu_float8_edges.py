@@ -165,3 +165,107 @@ def test_no_columns_no_tokens_no_features(lead):
     assert out.codes.shape == h.shape == (*lead, 0)
     x, none = quantize_float8(torch.ones(*lead, 200, device="cuda")), quantize_float8(torch.zeros(0, 200, device="cuda"), block_rows=128)
     assert float8_linear(x, none).shape == (*lead, 0) and float8_swiglu(x, none, none).scales.shape == (*lead, 0)
+
+
+# ---- outputs in place ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,hidden,ld", [(1, 8, 8), (5, 1024, 1024), (3, 1000, 1003), (40, 4096, 4100), (2, 8192, 8200), (3, 16400, 16400)])
+@pytest.mark.parametrize("place", ["x", "residual"])
+def test_the_norms_stream_in_place(dtype, rows, hidden, ld, place):
+    """``h_out`` may be ``x`` or the residual: what comes of it is what comes of a stream of its own, and what lies between the rows is
+    left as it was."""
+    gen, lib, across = _gen(41), _lib.load_library(), -(-hidden // 128)
+    wide = [torch.randn(rows, ld, generator=gen, device="cuda").to(dtype) for _ in range(2)]
+    x, residual = (t[:, :hidden] for t in wide)
+    weight = (1 + 0.1 * torch.randn(hidden, generator=gen, device="cuda")).to(dtype)
+    want, stream = rmsnorm_float8(x, weight, 1e-5, residual=residual)
+    before = [t.clone() for t in wide]
+    h = wide[0] if place == "x" else wide[1]
+    codes = torch.empty(rows, hidden, dtype=F8, device="cuda")
+    scales = torch.empty(rows, across, dtype=E8, device="cuda")
+    _lib.call(lib.llmopt_f8_rmsnorm(x.data_ptr(), ld, residual.data_ptr(), ld, h.data_ptr(), ld, weight.data_ptr(), codes.data_ptr(),
+                                    hidden, scales.data_ptr(), across, rows, hidden, 1e-5, _lib.DTYPE_CODES[dtype], _stream()),
+              "llmopt_f8_rmsnorm")
+    assert torch.equal(_bits(codes), _bits(want.codes)) and torch.equal(_bits(scales), _bits(want.scales))
+    assert torch.equal(h[:, :hidden], stream)
+    assert all(torch.equal(t[:, hidden:], b[:, hidden:]) for t, b in zip(wide, before))
+    other = 1 if place == "x" else 0
+    assert torch.equal(wide[other], before[other])
+
+
+# ---- each kernel's typical error ------------------------------------------------------------------------
+
+
+def _near_product(x, w):
+    """``x w^T`` in 64 bits, and how far sums of products of either sign are off. Each of the seven smaller products of eight neighbouring ones
+    loses less than 2^-13 of the largest, in either direction: by Hoeffding's bound a sum is off by more than t 2^-13 root(7 times the
+    sum of the squares of the largest ones) in 2 exp(-t^2 / 2) of all cases, 5e-11 at t = 7; and the squares of all products are
+    no fewer. So 7 root 7 2^-13 = 2.3e-3 of the root of the sum of squares, a tenth more for the fp32 additions."""
+    return x @ w.t().contiguous(), 2.5e-3 * torch.sqrt((x * x) @ (w * w).t().contiguous())
+
+
+def _check_near(y, want, off):
+    half = torch.finfo(y.dtype).eps / 2
+    assert bool(((y.double() - want).abs() <= off + (want.abs() + off) * half + 2.0**-25).all())  # half of fp16's least step
+
+
+LINEAR = [
+    # the few-token kernel
+    (1, 6144, 4096), (4, 4096, 14336), (16, 1024, 4096), (17, 40, 16), (31, 300, 2064), (32, 1000, 4096), (33, 130, 4112), (150, 100, 2048),
+    # the tiles, whole and in parts of K
+    (1036, 16, 16), (8249, 16, 1968), (1036, 16, 1664), (1045, 16, 3680), (32, 4096, 14336), (130, 22445, 16), (8886, 261, 13728),
+    (8809, 16, 7456), (7202, 16, 5056), (130, 20409, 16), (130, 10691, 10160), (17, 15263, 2320), (133, 28530, 400), (66, 27201, 7936),
+    (65, 6387, 13952), (258, 22201, 16), (526, 21875, 272), (513, 14350, 6528), (261, 25258, 912), (534, 26166, 272),
+    # rows of any alignment
+    (70, 200, 1001), (1, 200, 77)]
+
+
+@pytest.mark.parametrize("m,n,k", LINEAR)
+def test_a_products_error_is_that_of_its_dropped_bits(m, n, k):
+    """Sixteen columns less would show, in any kernel: of 14336 they are 3 % of a typical sum."""
+    gen = _gen(42)
+    x, w = quantize_float8(torch.randn(m, k, generator=gen, device="cuda")), _weight(gen, n, k)
+    _check_near(float8_linear(x, w, dtype=torch.float16), *_near_product(_numbers(x), _numbers(w)))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 6144, 4096), (16, 4096, 14336), (32, 1536, 1024), (200, 3584, 4096), (777, 1536, 1040), (2000, 4096, 4096)])
+@pytest.mark.parametrize("share,gain", [(0.01, 8.0), (0.002, 100.0), (0.001, 1000.0)])
+def test_a_product_where_a_few_channels_are_strong(m, n, k, share, gain):
+    """A strong channel's product takes bits of the seven beside it: up to 1e-4 of a typical sum where it is all of it, a fifth of a
+    rounding to fp16. The largest products of eight are as independent as their signs, and a product's dropped bits spread
+    evenly up to 2^-13 of the largest: root(7 / 3) 2^-13 = 1.9e-4 of their root of squares, which the sums have for their own."""
+    gen = _gen(43)
+    x, w = quantize_float8(_strong(gen, m, k, share, gain)), quantize_float8(torch.randn(n, k, generator=gen, device="cuda") * 0.004, block_rows=128)
+    want, off = _near_product(_numbers(x), _numbers(w))
+    y = float8_linear(x, w, dtype=torch.float16)
+    _check_near(y, want, off)
+    err = (y.double() - want).norm()
+    assert float(err) <= float(want.norm()) * (2e-4 + 2.0**-11) + 2.0**-25 * want.numel() ** 0.5
+
+
+GATED = [
+    # the few-token kernel, the tiles, several one after the other, rows of any alignment
+    (1, 14336, 4096), (7, 2816, 1024), (32, 1000, 4096), (50, 260, 4112), (300, 1280, 2048), (200, 14336, 4096), (700, 130, 272),
+    (1035, 17, 400), (8262, 129, 272), (130, 16428, 400), (262, 12981, 928), (260, 16758, 400), (264, 22740, 272), (2048, 2816, 1024),
+    (70, 200, 1001)]
+
+
+@pytest.mark.parametrize("m,n,k", GATED)
+def test_the_gated_codes_are_the_nearest_but_for_dropped_bits(m, n, k):
+    """Sums are off by some 1e-4 of a number at most and a code's step is a twelfth of it, so one code in some hundreds is not the nearest to
+    the exact number: in no 16 tokens by 64 features more than 3 %. Without 16 columns of the product a third would be."""
+    gen = _gen(44)
+    x, gate, up = quantize_float8(torch.randn(m, k, generator=gen, device="cuda")), _weight(gen, n, k), _weight(gen, n, k)
+    out = float8_swiglu(x, gate, up)
+    (g, dg), (u, du) = (_near_product(_numbers(x), _numbers(w)) for w in (gate, up))
+    s = g * torch.sigmoid(g)
+    want = s * u
+    oracle.check_quantized(out.codes, out.scales, want, 1.1 * dg * (u.abs() + du) + s.abs() * du + want.abs() * (16 + 4 * g.abs()) * 2.0**-24)
+    v = want / oracle.spread(out.scales.double(), 1, want.shape)
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0**-6))) - 3)  # three fraction bits
+    other = (torch.round(v / step) * step).clamp(-448, 448) != out.codes.double()
+    other = torch.nn.functional.pad(other.double(), (0, -n % 64, 0, -m % 16))
+    share = other.view(-(-m // 16), 16, -(-n // 64), 64).sum((1, 3)) / (min(m, 16) * min(n, 64))
+    assert float(share.max()) <= 0.03 + 1 / (min(m, 16) * min(n, 64)) * 3, float(share.max())
