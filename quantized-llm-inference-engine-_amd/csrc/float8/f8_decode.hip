@@ -10,8 +10,10 @@
 //   (5.3 TB/s), 1536 x 1024 2.9 / 3.0 / 3.1 / 3.1.
 // Codes and scales loaded by each lane for itself: 10.2, 17.5 and 34.3 at one token, 14.7, 19.6 and 43.1 at 16.
 // The weight's codes into registers (HELD) instead of LDS: 8.4, 13.7, 24.2 and 3.3 at one token, but at more than four tokens, whose
-// LDS leaves room for fewer waves, faster from some 640 workgroups on (28672 x 4096 8 / 16 tokens 28.5 / 31.2 in LDS, 14336 x
-// 4096 16.9 / 18.4 against 15.7 / 17.4; 6144 x 4096 the same).
+// LDS leaves room for fewer waves, faster from some 640 workgroups on where a row has more than 16 steps, for eight waves (in LDS /
+// HELD, 8 and 16 tokens: 28672 x 4096 29.5 / 27.6 and 32.2 / 29.4, 16384 x 4096 18.3 / 17.1 and 19.6 / 18.6, 10240 x 4096 the
+// same; with 16 steps, for four waves: 28672 x 2048 13.6 / 14.7 and 15.8 / 16.2, 10240 x 2048 6.7 / 7.5 and 7.5 / 8.2, with eight
+// waves, half of which have none, 16.5 and 17.8, 8.2 and 8.4; 28672 x 1024 9.3 / 9.7 and 10.9 / 10.8).
 // More than 16 tokens go 32 at a time: their codes fill LDS with one workgroup a CU (two where a row has at most 16 steps), and the
 // weight's are HELD. 32 / 64 / 100 tokens, in brackets the best of the tiles: 1536 x 1024 3.9 / 3.9 / 4.5 (8.3), 4096 x 4096 8.6 (13.0) / 13.2 (13.2) / -,
 // 1024 x 2816 5.8 / 5.8 / 5.9 (9.4 - 10), 6144 x 4096 13.3 (14.0), 4096 x 14336 19.5 (18.6), 28672 x 4096 40 (30).
@@ -262,7 +264,7 @@ hipError_t launch_rows(const F8DecodeArgs& a, int out_dtype, hipStream_t stream)
     return one_group ? launch<XR, true, 8>(a, out_dtype, stream) : launch<XR, true, 4>(a, out_dtype, stream);
   } else {
     if constexpr (XR > 4) {
-      if (a.tiles * (a.w[1].codes ? 2 : 1) >= 640) return launch<XR, true, 8>(a, out_dtype, stream);
+      if (a.steps > 16 && a.tiles * (a.w[1].codes ? 2 : 1) >= 640) return launch<XR, true, 8>(a, out_dtype, stream);
     }
     return one_group ? launch<XR, false, 8>(a, out_dtype, stream) : launch<XR, false, 4>(a, out_dtype, stream);
   }

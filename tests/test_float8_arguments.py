@@ -20,6 +20,7 @@ import ctypes, json, struct, sys
 stub = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)
 lib = ctypes.CDLL(sys.argv[2])
 launches, attributes, refuse = (ctypes.c_int.in_dll(stub, "llmopt_stub_" + n) for n in ("launches", "attributes", "refuse"))
+block = (ctypes.c_uint * 3).in_dll(stub, "llmopt_stub_block")
 argument = (ctypes.c_ubyte * 96).in_dll(stub, "llmopt_stub_argument")
 i64, ptr, size = ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t
 P = ptr(1 << 20)  # never read: nothing is launched
@@ -110,3 +111,11 @@ def test_the_tiles_refuse_parts_of_k_that_they_have_no_kernel_for(stub):
                [2, 300, 512, 1024, 2, 4, True], [3, 300, 512, 1024, 1, 8, True]]
     got = _child(stub, code % json.dumps(refused))
     assert all(rc != 0 and launched == 0 for rc, launched in got), got
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 8, 9, 16])
+@pytest.mark.parametrize("n,k", [(128, 1024), (10240, 512), (28672, 2048), (28672, 4096)])
+def test_few_tokens_have_waves_by_their_steps(stub, tokens, n, k):
+    """A wave takes four steps of 128 columns at a time: up to 16 steps are for four waves at most, 32 for eight."""
+    got = _child(stub, f"rc = linear({tokens}, {n}, {k}); print(json.dumps([rc, launches.value, list(block)]))")
+    assert got == [0, 1, [256 if k <= 2048 else 512, 1, 1]]
