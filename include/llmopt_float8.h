@@ -48,8 +48,9 @@ size_t llmopt_f8_linear_workspace(int64_t M, int64_t N, int64_t K);
 /*
  * y [M, N] (F16 or BF16, row stride ldy elements; F32: LLMOPT_ERR_UNSUPPORTED) = x w^T + bias of x [M, K] quantized by rows
  * and a weight [N, K]; bias [N] of y's dtype, may be null. Products are exact, and added by the matrix cores in fp32 but for
- * this: of the products of eight neighbouring columns, what is below 2^-13 of the largest is dropped, so sums are off by
- * some 2.5e-5 of their typical size (hence no F32 output). Rounded once. Rows that are no multiples of 16 bytes, or not
+ * this: of the products of eight neighbouring columns, what is below 2^-13 of the largest is dropped, so sums are off by 1.5e-5 to
+ * 2.7e-5 of their typical size, up to 1e-4 where a few channels are 100 times as strong as the rest and more (hence no
+ * F32 output). Rounded once. Rows that are no multiples of 16 bytes, or not
  * aligned to them, run on a slower kernel. With less workspace than llmopt_f8_linear_workspace asks for, K is not split
  * (correct, slower for few tokens).
  */
@@ -62,7 +63,9 @@ size_t llmopt_f8_swiglu_workspace(int64_t M, int64_t N, int64_t K);
 
 /*
  * silu(x gate^T) * (x up^T), with silu(g) = g / (1 + exp(-g)) in fp32 on the fp32 sums, quantized by rows into codes [M, N]
- * and scales. x as in llmopt_f8_linear, gate and up weights [N, K]. With less workspace than llmopt_f8_swiglu_workspace
+ * and scales. A group's scale is that of exact sums, but where more than 16 different numbers that one wave holds are next to the
+ * same border of the scales (equal features): there it may be that of the matrix cores' sums. x as in llmopt_f8_linear, gate and up
+ * weights [N, K]. With less workspace than llmopt_f8_swiglu_workspace
  * asks for, another kernel runs (correct, slower).
  */
 int llmopt_f8_swiglu(const void* x, int64_t ldx, const void* x_scales, int64_t ldxs, int64_t M, int64_t K,

@@ -79,13 +79,15 @@ constexpr int64_t kSomeTokens = 1024;  // that it takes at most, 32 at a time
 // The decode kernel, or a tile's shape and the parts of K: the least of an estimate of the time. A workgroup's step of 128 columns takes
 // `alone` us where few workgroups run and `full` where every CU has its share; a round of workgroups (256 of them, or 512 where two
 // fit a CU) adds `round`, the first loads and the results; parts are written and read again at some 3 TB/s. Over 97 sizes, two
-// thirds of them drawn at random (17 to 1024 tokens, 128 to 10240 features and columns), the choice took 0.9 % more than the best of all on
-// average and 20 % at most.
-// Measured (MI355X, in a graph, us; the estimate's choice first): 4096 x 14336, 8192 tokens, 256 x 256 374, 256 x 128 472, 256 x
-// 64 637; 1024 tokens, 256 x 128 in two parts 74, 256 x 64 89, 256 x 256 160; 32 tokens, 128 x 64 in eight parts 18.6, whole 58, the
-// decode kernel 19.5; 6144 x 4096, 200 tokens, 128 x 64 20, 256 x 64 26, 256 x 256 53; 17 tokens, the decode kernel 12.5, 128 x 64 in eight
-// parts 14.0; 1536 x 1040, 777 tokens, 128 x 64 9.9, 128 x 128 13, 256 x 256 22; gate and up 2816 x 1024, 32 tokens, the decode
-// kernel 7.6, 256 x 64 10.0.
+// thirds of them drawn at random (17 to 1024 tokens, 128 to 10240 features and columns), the choice takes 0.8 % more than the best of all on
+// average and 17 % at most; over 120 of 1500 to 8192 tokens (1024 to 6144 features, 256 to 4096 columns) 1.4 % and 11 %, nearly all of
+// it at up to 1024 columns, where 128 x 128 is faster than 256 x 256; over 47 gated ones of 17 to 8192 tokens 0.8 %, and 32 % at
+// most (9000 x 3600, 25 tokens: 256 x 64 41, the decode kernel 31).
+// Measured (MI355X, in a graph, us; the estimate's choice first): 4096 x 14336, 8192 tokens, 256 x 256 377, 256 x 128 441, 256 x
+// 64 593; 1024 tokens, 256 x 128 in two parts 74, 256 x 64 88, 256 x 256 161; 32 tokens, 128 x 64 in eight parts 18.6, whole 57, the
+// decode kernel 19.6; 6144 x 4096, 200 tokens, 128 x 64 20, 256 x 64 27, 256 x 256 52; 17 tokens, the decode kernel 12.5, 128 x 64 in eight
+// parts 14.1; 1536 x 1040, 777 tokens, 128 x 64 9.8, 128 x 128 12, 256 x 256 21; 1536 x 1024, 8192 tokens, 256 x 256 25.3, 128 x
+// 128 23.9; gate and up 2816 x 1024, 32 tokens, the decode kernel 8.6, 256 x 64 12.1.
 struct Tile {
   F8Shape shape;
   int64_t n, m, per_cu;

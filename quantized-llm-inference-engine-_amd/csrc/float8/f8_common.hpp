@@ -180,9 +180,9 @@ __device__ __forceinline__ float f8_swiglu(float gate, float up) {
 // and 4096, 50,000 to 100,000 groups each): channels of like strength 1.3e-5 rms, 1 % of them 8 times as strong 2.5e-5, 0.2 % 100
 // times 8e-5, one or two 1000 times and more 1.2e-4; the largest of a million 8.6e-4. Without this 3 to 13 groups in 100,000
 // would be on the wrong side, with a window of 1e-4 none of the first, but up to 8 of the last.
-// Measured (MI355X, in a graph, us, without / with 1e-4 / with 2^-10; gate and up of 14336 x 4096): 4 tokens 24.1 / 24.3 / 25.1, 200
-// tokens 35 / 38 / 38, 8192 tokens 753 / 772 / 788; 2816 x 1024, 8192 tokens 58 / 65 / 70: half of that for the walks, of some 3 us
-// each, half for the registers that they take.
+// Measured (MI355X, in a graph, us, without / a window of 1e-4 with a walk for each number / as it is; gate and up of 14336 x 4096): 4
+// tokens 24.1 / 24.3 / 25.1, 200 tokens 35 / 38 / 38.5, 8192 tokens 750 / 772 / 797; 2816 x 1024, 8192 tokens 58 / 65 / 72: half of
+// that for the walks, of some 3 us each, half for the registers that they take.
 constexpr uint32_t kF8Near = 14336;  // in steps of the fraction's 23 bits
 __device__ __forceinline__ bool f8_near(uint32_t bits) {
   return bits < 0x7F800000u && ((bits - 0x600000u + kF8Near) & 0x7FFFFFu) < 2 * kF8Near;

@@ -1,7 +1,8 @@
 // Products of rows of any length, stride and alignment: the kernels of shapes that the others do not take. A wave multiplies 16
 // rows of the weight with 16 tokens, a group of 128 columns at a time, straight from memory. Bound by those loads, of which no two waves
-// share any: 4096 x 14336 takes 65.5 us at 32 tokens and 7.1 ms at 8192 (MI355X), 4 and 19 times what aligned rows do. A layer's weights
-// and activations are aligned.
+// share any, and of rows that start at any byte as pieces of several lines: 4096 x 14330 takes 87 us of one token, 149 of 32 and 18 ms of
+// 8192 (MI355X), 7, 9 and 47 times what rows of whole 16 bytes do (4096 x 14336 with the tokens' rows alone at an odd address 60, 65 and
+// 7.1 ms). A layer's weights and activations are aligned.
 #include "f8_common.hpp"
 #include "f8_mfma.hpp"
 

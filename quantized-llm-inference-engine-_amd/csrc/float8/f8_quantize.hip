@@ -6,7 +6,8 @@
 // is a power of two, so x / 2^e is exact and the only rounding is the conversion's, half a step of e4m3.
 //
 // Measured (MI355X, us; floor: the bytes at a large copy's 5.14 TB/s): a weight of 4096 x 14336 bf16 37.3 (34.3); residual and norm of
-// 8192 tokens of 4096 49.9 (45.7; with rows read a second time instead of held 53.0); 777 tokens of 1024 5.4, one token of 4096
+// 8192 tokens of 4096 49.9 (45.7; with rows read a second time instead of held 53.0); rows quantized, in a graph, 8192 of 4096 21.3
+// (19.6), 8192 of 1024 8.5 (4.9), 2048 of 4096 7.2 (4.9), 777 of 1024 2.7 (0.5); from Python 777 tokens of 1024 normed 5.5, one token of 4096
 // quantized 4.9 - 5.4 and normed 5.9, of which the kernels take 3.4, 1.8 and 3.5 and the call from Python the rest. Codes are
 // stored past the caches (a weight 39.6 us through them).
 #include "f8_common.hpp"

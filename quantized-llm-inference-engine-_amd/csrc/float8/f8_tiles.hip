@@ -4,8 +4,8 @@
 //
 // which the matrix core takes as it stands: a step of 128 columns has one scale for each of its rows, so no sum is rescaled and the
 // codes go from memory to the products through LDS only, never through a register that is not an operand. Bound by the matrix cores
-// from some 500 tokens on, at the clock that their power leaves (2.5 - 2.6 PFLOP/s against 3.7 from registers for microseconds, and
-// 2.67 - 2.94 of the library's product with one scale for all), below that by the weight's way from memory.
+// from some 500 tokens on, at the clock that their power leaves (2.55 PFLOP/s, gated 2.4, against 3.7 from registers for microseconds, and
+// 2.67 and 2.94 of the library's product with one scale for all), below that by the weight's way from memory.
 //
 // A workgroup holds a tile's sums in registers, a wave 128 weight rows x 16 TM tokens of them, and STAGES steps of both operands in
 // LDS, loaded past the registers as whole lines of 128 bytes and swizzled (no bank conflicts in any case). What was measured (MI355X, in
@@ -14,8 +14,8 @@
 //   256 x 256 in eight waves, one barrier a step: 445, 1067
 //   loads dealt among the products of two phases, scales of 32 steps at a time in LDS: 383, 765
 //   tiles one after the other, the next one's first stages beside the last products and the results' stores: 374, 737
-//   maxima next to a border of the scales summed again (f8_common.hpp): 374, 760
-//   the bias in LDS with the scales, stores of 16 bytes at any alignment: the same here; 1536 x 1024 with a bias 38 -> 26, 1536 x 1040 of
+//   maxima within 1e-4 of a border of the scales summed again (f8_common.hpp): 374, 760; within 2^-10, equal tokens once: 377, 782 - 797
+//   the bias in LDS with the scales, stores of 16 bytes at any alignment: the same at these sizes; 1536 x 1024 with a bias 38 -> 26, 1536 x 1040 of
 //   777 tokens with one 11.3 -> 8.9, 5225 x 2592 of 188 tokens 18.4 -> 13.4
 // Level or worse: products of 32 x 32 (387, 799 - 823), waves of 64 rows x 32 or 64 tokens in the smaller tiles (a fifth to a third
 // fewer LDS reads, all sizes within 2 %), a prefetch into L2 (443 for 421), waves of higher priority, 1 to 32 token tiles a sweep

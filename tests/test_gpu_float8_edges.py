@@ -233,8 +233,8 @@ def test_a_products_error_is_that_of_its_dropped_bits(m, n, k):
 @pytest.mark.parametrize("m,n,k", [(1, 6144, 4096), (16, 4096, 14336), (32, 1536, 1024), (200, 3584, 4096), (777, 1536, 1040), (2000, 4096, 4096)])
 @pytest.mark.parametrize("share,gain", [(0.01, 8.0), (0.002, 100.0), (0.001, 1000.0)])
 def test_a_product_where_a_few_channels_are_strong(m, n, k, share, gain):
-    """A strong channel's product takes bits of the seven beside it: up to 1e-4 of a typical sum where it is all of it, a fifth of a
-    rounding to fp16. The largest products of eight are as independent as their signs, and a product's dropped bits spread
+    """A strong channel's product takes bits of the seven beside it: up to 1e-4 of a typical sum where it is all of it, half of what
+    a rounding to fp16 brings. The largest products of eight are as independent as their signs, and a product's dropped bits spread
     evenly up to 2^-13 of the largest: root(7 / 3) 2^-13 = 1.9e-4 of their root of squares, which the sums have for their own."""
     gen = _gen(43)
     x, w = quantize_float8(_strong(gen, m, k, share, gain)), quantize_float8(torch.randn(n, k, generator=gen, device="cuda") * 0.004, block_rows=128)
