@@ -63,8 +63,9 @@ size_t llmopt_f8_swiglu_workspace(int64_t M, int64_t N, int64_t K);
 
 /*
  * silu(x gate^T) * (x up^T), with silu(g) = g / (1 + exp(-g)) in fp32 on the fp32 sums, quantized by rows into codes [M, N]
- * and scales. A group's scale is that of exact sums, but where more than 16 different numbers that one wave holds are next to the
- * same border of the scales (equal features): there it may be that of the matrix cores' sums. x as in llmopt_f8_linear, gate and up
+ * and scales. A group's largest magnitude is summed again in fp32 where a border of the scales is within 2^-10 of it, more
+ * than sums were found to be off by, so that its scale is that of exact sums; where more than 16 different numbers that one wave
+ * holds are next to a border (equal features), it may be that of the matrix cores' sums. x as in llmopt_f8_linear, gate and up
  * weights [N, K]. With less workspace than llmopt_f8_swiglu_workspace
  * asks for, another kernel runs (correct, slower).
  */
