@@ -165,7 +165,7 @@ __device__ __forceinline__ uint32_t f8_codes4(float a, float b, float c, float d
 }
 
 // silu(gate) * up in fp32, with the hardware's exponential and reciprocal (a step of fp32 each; 2^-22 |gate| of the
-// exponential's argument). Far below zero the exponential is infinite and the product 0.
+// exponential's argument). Below -87.3 the reciprocal is less than the least normal number and the product 0, which is off by 2^-119 |up|.
 __device__ __forceinline__ float f8_swiglu(float gate, float up) {
   return gate * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(gate * -1.44269504f)) * up;
 }

@@ -269,3 +269,45 @@ def test_the_gated_codes_are_the_nearest_but_for_dropped_bits(m, n, k):
     other = torch.nn.functional.pad(other.double(), (0, -n % 64, 0, -m % 16))
     share = other.view(-(-m // 16), 16, -(-n // 64), 64).sum((1, 3)) / (min(m, 16) * min(n, 64))
     assert float(share.max()) <= 0.03 + 1 / (min(m, 16) * min(n, 64)) * 3, float(share.max())
+
+
+# ---- layouts, and what is not finite --------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_operands_of_any_layout(m):
+    """Columns of a transposed tensor, one prompt expanded to two, tokens in front of prompts, a bias that is every other number."""
+    gen = _gen(51)
+    x, w = quantize_float8(torch.randn(m, 256, generator=gen, device="cuda")), _weight(gen, 384, 256)
+    y, act = float8_linear(x, w), float8_swiglu(x, w, w)
+    xt = Float8Tensor(x.codes.t().contiguous().t(), x.scales.t().contiguous().t())
+    wt = Float8Tensor(w.codes.t().contiguous().t(), w.scales.t().contiguous().t(), 128)
+    assert torch.equal(float8_linear(xt, wt), y)
+    assert torch.equal(_bits(float8_swiglu(xt, wt, w).codes), _bits(act.codes))
+    two = Float8Tensor(x.codes.expand(2, m, 256), x.scales.expand(2, m, 2))
+    want = float8_linear(Float8Tensor(two.codes.contiguous(), two.scales.contiguous()), w)
+    assert torch.equal(float8_linear(two, w), want)
+    swapped = Float8Tensor(two.codes.transpose(0, 1), two.scales.transpose(0, 1))
+    assert torch.equal(float8_linear(swapped, w), want.transpose(0, 1))
+    bias = torch.randn(768, generator=gen, device="cuda").bfloat16()[::2]
+    assert torch.equal(float8_linear(x, w, bias), float8_linear(x, w, bias.contiguous()))
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 300, 256), (40, 300, 1024), (300, 4000, 1024), (5, 50, 77), (700, 2816, 1024)])
+def test_what_is_not_finite_stays_in_its_groups_of_the_gated_product(m, n, k):
+    """A token's NaN scale, a feature's NaN code and a block's NaN scale: the groups that read as NaN are the host's, their codes 0."""
+    gen = _gen(52)
+    x, gate, up = quantize_float8(torch.randn(m, k, generator=gen, device="cuda")), _weight(gen, n, k), _weight(gen, n, k)
+    clean = float8_swiglu(x, gate, up)
+    _bits(x.scales)[m // 2, 0] = 255
+    _bits(up.codes)[17, 3] = 0x7F
+    if n > 256:
+        _bits(gate.scales)[1, 0] = 255
+    out = float8_swiglu(x, gate, up)
+    host = float8_swiglu(x.to("cpu"), gate.to("cpu"), up.to("cpu"))
+    bad = out.dequantize().isnan()
+    assert torch.equal(bad.cpu(), host.dequantize().isnan()) and not bool(_bits(out.codes)[bad].any())
+    assert torch.equal(_bits(out.codes)[~bad], _bits(clean.codes)[~bad])
+    large = quantize_float8(torch.full((m, 128), 1e20, device="cuda"))
+    w = quantize_float8(torch.full((200, 128), 1e20, device="cuda"), block_rows=128)
+    assert bool(float8_linear(large, w).isinf().all()) and bool(float8_swiglu(large, w, w).dequantize().isnan().all())
